@@ -44,29 +44,29 @@ def _balance(name, B, S, N, K, Ks=0, skew=0.5, dtype="bfloat16", per_sequence=Fa
 def listed():
     return [
         # one sequence being decoded: eight experts' weights stream, launches and host work show
-        _experts("experts, 1 token", 1, 2048, 768, 128, 8),
+        _experts("experts 1 token", 1, 2048, 768, 128, 8),
         # a decode batch: most experts hold one or two tokens
-        _experts("experts, 16 tokens", 16, 2048, 768, 128, 8),
+        _experts("experts 16 tokens", 16, 2048, 768, 128, 8),
         # a large decode batch or a short prompt, no multiple of anything: every expert's weights stream
-        _experts("experts, 131 tokens", 131, 2048, 768, 128, 8),
+        _experts("experts 131 tokens", 131, 2048, 768, 128, 8),
         # a prompt of ordinary length: between streaming and multiplying
-        _experts("experts, 1000 tokens", 1000, 2048, 768, 128, 8),
+        _experts("experts 1000 tokens", 1000, 2048, 768, 128, 8),
         # batched prefill: bound by the matrix products
-        _experts("experts, 8192 tokens", 8192, 2048, 768, 128, 8),
+        _experts("experts 8192 tokens", 8192, 2048, 768, 128, 8),
         # widths that are no power of two, K that does not divide N
-        _experts("experts, 7680 tokens, ragged", 7680, 2176, 1152, 64, 6),
+        _experts("experts 7680 tokens ragged", 7680, 2176, 1152, 64, 6),
         # few experts receive ten times the mean load and four see every token
-        _experts("experts, 16384 tokens, skewed", 16384, 2048, 1408, 64, 8, Ks=4, skew=1.8),
+        _experts("experts 16384 tokens skewed", 16384, 2048, 1408, 64, 8, Ks=4, skew=1.8),
         # a layer of a unit test or of a debugging run: launches only, widths below a block
-        _experts("experts, tiny", 128, 96, 64, 8, 2),
+        _experts("experts tiny", 128, 96, 64, 8, 2),
         # the loss beside a training step of that size: launches and host work only
-        _balance("balance, 128 tokens", 1, 128, 8, 2),
+        _balance("balance 128 tokens", 1, 128, 8, 2),
         # the loss beside the headline training layer, over the whole batch
-        _balance("balance, 8192 tokens", 4, 2048, 128, 8),
+        _balance("balance 8192 tokens", 4, 2048, 128, 8),
         # a padded batch, one loss a sequence, four shared experts that take no part, logits left in 32 bits
-        _balance("balance, 16 x 1000, padded", 16, 1000, 64, 8, Ks=4, dtype="float32", per_sequence=True, padded=True),
+        _balance("balance 16 x 1000 padded", 16, 1000, 64, 8, Ks=4, dtype="float32", per_sequence=True, padded=True),
         # the largest batch, 8 x 8192 tokens
-        _balance("balance, 65536 tokens", 8, 8192, 64, 8, per_sequence=True),
+        _balance("balance 65536 tokens", 8, 8192, 64, 8, per_sequence=True),
     ]
 
 
