@@ -413,6 +413,35 @@ int momoe_gate_dgrad(const void* Glogits_MN, const void* Wg_DN, const void* Gx_M
 int momoe_bias_update(const int64_t* sizes_N, float c_avg, float rate, int64_t N, float* biases_N,
                       void* stream);
 
+/* ---- balance loss of the router -----------------------------------------------
+ * No counterpart in the reference, whose only balancing is the selection bias (momoe/sample_moe.py:65-67).
+ * Tokens come in G groups of S consecutive ones, each balanced on its own (sequences, or G = 1: the whole batch).  Over the
+ * Ng = N - Ks routed experts p = softmax(logits); in a group with T tokens that count, c_i of them at expert i and
+ * P = the sum of c_i over the routed experts,
+ *   loss_g = Ng / (T P) * sum_i c_i * sum over those tokens of p_i,
+ * loss = the mean of loss_g over the groups with P > 0, zero if there are none.
+ * logits: [G * S, N] of logits_type, row pitch ld >= N elements.  mask_NM int32 0/1, element (i, m) at mask[i * stride_n + m * stride_m].
+ * valid_M (may be NULL: all count): one byte a token; what logits and mask hold of a token with zero there does not matter.  A
+ * token that counts and has no routed logit above -inf makes the loss NaN.
+ * Outputs: loss fp32[1]; counts_GN int64 [G, N], shared experts included; info fp32 [1 + G], what momoe_balance_bwd takes.
+ * workspace: momoe_balance_workspace_bytes(G, S, N) bytes of device memory on a 16-byte boundary (-1: sizes that it does not take).
+ */
+#define MOMOE_TYPE_BF16 0
+#define MOMOE_TYPE_F32 1
+#define MOMOE_TYPE_F16 2
+int64_t momoe_balance_workspace_bytes(int64_t G, int64_t S, int64_t N);
+int momoe_balance_fwd(const void* logits, int logits_type, int64_t ld, const int32_t* mask_NM, int64_t stride_n,
+                      int64_t stride_m, const uint8_t* valid_M, int64_t G, int64_t S, int64_t N, int64_t Ks,
+                      float* loss, int64_t* counts_GN, float* info, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* momoe_balance_bwd: G_loss[0] * d loss / d logits (the counts are constants) + add_MN, of grad_type (logits_type or
+ * MOMOE_TYPE_BF16), contiguous [G * S, N].  add_MN (may be NULL, or Glogits_MN itself): of grad_type, contiguous.  logits, valid_M,
+ * counts_GN and info as momoe_balance_fwd had and wrote them.
+ */
+int momoe_balance_bwd(const void* logits, int logits_type, int64_t ld, const uint8_t* valid_M, const int64_t* counts_GN,
+                      const float* info, const float* G_loss, const void* add_MN, void* Glogits_MN, int grad_type,
+                      int64_t G, int64_t S, int64_t N, int64_t Ks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,7 @@
 
 #include <atomic>
 #include <mutex>
+#include <optional>
 #include <string>
 #include <tuple>
 #include <utility>
@@ -453,8 +454,10 @@ std::tuple<Tensor, Tensor> experts(const Tensor& x, const Tensor& W1, const Tens
 // ---- router ------------------------------------------------------------------------------------
 struct Routed {
   Tensor x_MD, mask, s_MN, p_sel, norms;
+  Tensor logits;  // of `keep_logits`
 };
-Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biases, int64_t N, int64_t K, int64_t Ks) {
+Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biases, int64_t N, int64_t K, int64_t Ks,
+                      bool keep_logits = false) {
   const at::Device dev = Wg.device();
   const int64_t D = x_BSD.size(2), M = x_BSD.size(0) * x_BSD.size(1);
   const c10::DeviceGuard guard(dev);
@@ -463,7 +466,7 @@ Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biase
   // Few tokens: the product in the library's kernel, whose launch alone takes the host 18 us
   const int64_t ws_bytes = momoe_gate_router_workspace_bytes(M, D, N);
   const auto aligned = [](const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; };
-  const bool own = ws_bytes >= 0 && !at::autocast::is_autocast_enabled(at::kCUDA) && Wg.dim() == 2 && Wg.size(0) == D &&
+  const bool own = !keep_logits && ws_bytes >= 0 && !at::autocast::is_autocast_enabled(at::kCUDA) && Wg.dim() == 2 && Wg.size(0) == D &&
                    Wg.size(1) == N && Wg.is_contiguous() && aligned(Wg) && aligned(r.x_MD) && r.x_MD.stride(1) == 1 &&
                    r.x_MD.stride(0) >= D && r.x_MD.stride(0) % 8 == 0;
   // Other products come first of all: the GPU has work while the host allocates
@@ -493,6 +496,7 @@ Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biase
   }
   MOMOE_CALL(momoe_router_fwd, st, logits.data_ptr(), logits.scalar_type() == at::kFloat, bias.data_ptr<float>(), M, N, K, Ks,
              r.mask.data_ptr<int32_t>(), r.s_MN.data_ptr<float>(), r.p_sel.data_ptr<float>(), norms, norms + M);
+  if (keep_logits) r.logits = logits;
   return r;
 }
 
@@ -533,6 +537,37 @@ Tensor gate_input_gradient(const Tensor& G_x, const Tensor& G_logit, const Tenso
   return out;
 }
 
+// Gradient of the gate logits, bf16 [M, N], from that of the gate weights; `saved`: x, Wg, mask, p, s, norms
+Tensor router_gradient(const variable_list& saved, const at::Device& dev, const Tensor& G_s_NM, int64_t M, int64_t N, int64_t Ks) {
+  const Tensor& mask = as_saved(saved[2], "mask", dev, at::kInt, {N, M});
+  const Tensor& p_sel = as_saved(saved[3], "p", dev, at::kFloat, {M, N});
+  const Tensor& s_MN = as_saved(saved[4], "s", dev, at::kFloat, {M, N});
+  const Tensor& norms = as_saved(saved[5], "norms", dev, at::kFloat, {2, M});
+  const Tensor G_s = G_s_NM.to(dev, at::kFloat);
+  const Tensor G_logit = empty_bf16({M, N}, dev);
+  const float* nrm = norms.data_ptr<float>();
+  MOMOE_CALL(momoe_router_bwd, stream_of(dev), G_s.data_ptr<float>(), G_s.stride(0), G_s.stride(1),
+             p_sel.data_ptr<float>(), s_MN.data_ptr<float>(), nrm, nrm + M, mask.data_ptr<int32_t>(), M, N,
+             Ks, G_logit.data_ptr());
+  return G_logit;
+}
+// The gradients that go back through the gate product: of x to out[0] (G_x, what comes back past the gate, may be undefined), of
+// Wg to out[1]; without a gradient of the logits that of Wg is zero
+void gate_gradients(AutogradContext* ctx, const variable_list& saved, const at::Device& dev, Tensor G_x, const Tensor& G_logit,
+                    at::IntArrayRef x_sizes, int64_t N, variable_list& out) {
+  const int64_t M = x_sizes[0] * x_sizes[1], D = x_sizes[2];
+  const Tensor& x = as_saved(saved[0], "x", dev, at::kBFloat16, {M, D}, /*packed=*/false);
+  const Tensor& Wg = as_saved(saved[1], "Wg", dev, at::kBFloat16, {D, N}, /*packed=*/false);
+  const bool need_x = ctx->needs_input_grad(0), need_wg = ctx->needs_input_grad(1);
+  if (G_logit.defined()) {
+    if (need_x) G_x = gate_input_gradient(G_x, G_logit, Wg);
+    if (need_wg) out[1] = gate_gradient(x, G_logit);
+  } else if (need_wg) {
+    out[1] = at::zeros_like(Wg);
+  }
+  if (need_x && G_x.defined()) out[0] = G_x.reshape(x_sizes);
+}
+
 struct RouterFn : torch::autograd::Function<RouterFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& Wg, const Tensor& biases,
                                int64_t N, int64_t K, int64_t Ks) {
@@ -548,49 +583,231 @@ struct RouterFn : torch::autograd::Function<RouterFn> {
     const std::vector<int64_t> call_of = ctx->saved_data["call"].toIntVector();
     const at::Device dev(at::kCUDA, (at::DeviceIndex)call_of[2]);
     const int64_t Ks = call_of[0], N = call_of[1], M = call_of[3] * call_of[4], D = call_of[5];
-    const Tensor& x = as_saved(saved[0], "x", dev, at::kBFloat16, {M, D}, /*packed=*/false);
-    const Tensor& Wg = as_saved(saved[1], "Wg", dev, at::kBFloat16, {D, N}, /*packed=*/false);
-    const Tensor& mask = as_saved(saved[2], "mask", dev, at::kInt, {N, M});
-    const Tensor& p_sel = as_saved(saved[3], "p", dev, at::kFloat, {M, N});
-    const Tensor& s_MN = as_saved(saved[4], "s", dev, at::kFloat, {M, N});
-    const Tensor& norms = as_saved(saved[5], "norms", dev, at::kFloat, {2, M});
-    const bool need_x = ctx->needs_input_grad(0), need_wg = ctx->needs_input_grad(1);
     const c10::DeviceGuard guard(dev);
-    variable_list out(6);
     const Tensor &G_x_BSD = grads[0], &G_s_NM = grads[2];
-    Tensor G_x;
+    Tensor G_x, G_logit;
     if (G_x_BSD.defined()) G_x = G_x_BSD.reshape({M, D}).to(dev, at::kBFloat16);
-    if (G_s_NM.defined()) {
-      const Tensor G_s = G_s_NM.to(dev, at::kFloat);
-      const Tensor G_logit = empty_bf16({M, N}, dev);
-      const float* nrm = norms.data_ptr<float>();
-      MOMOE_CALL(momoe_router_bwd, stream_of(dev), G_s.data_ptr<float>(), G_s.stride(0), G_s.stride(1),
-                 p_sel.data_ptr<float>(), s_MN.data_ptr<float>(), nrm, nrm + M, mask.data_ptr<int32_t>(), M, N,
-                 Ks, G_logit.data_ptr());
-      if (need_x) G_x = gate_input_gradient(G_x, G_logit, Wg);
-      if (need_wg) out[1] = gate_gradient(x, G_logit);
-    } else if (need_wg) {
-      out[1] = at::zeros_like(Wg);
-    }
-    if (need_x && G_x.defined()) out[0] = G_x.reshape({call_of[3], call_of[4], D});
+    if (G_s_NM.defined()) G_logit = router_gradient(saved, dev, G_s_NM, M, N, Ks);
+    variable_list out(6);
+    gate_gradients(ctx, saved, dev, G_x, G_logit, {call_of[3], call_of[4], D}, N, out);
     return out;
   }
 };
+
+void check_router(const Tensor& x, const Tensor& Wg) {
+  if (Wg.scalar_type() != at::kBFloat16) throw_python(PyExc_AssertionError, "Wg_DN must be of type torch.bfloat16");
+  TORCH_CHECK(Wg.is_cuda(), "TopKRouter weights must live on the GPU: there is no CPU compute path");
+  TORCH_CHECK(x.dim() == 3, "x_BSD must be [B, S, D]");
+}
 
 std::tuple<Tensor, Tensor, Tensor> router(const Tensor& x, const Tensor& Wg, const Tensor& biases, int64_t N, int64_t K,
                                           int64_t Ks) {
   if (torch::jit::tracer::isTracing())
     return call_recorded<std::tuple<Tensor, Tensor, Tensor>, const Tensor&, const Tensor&, const Tensor&, int64_t,
                          int64_t, int64_t>("momoe::router", x, Wg, biases, N, K, Ks);
-  if (Wg.scalar_type() != at::kBFloat16) throw_python(PyExc_AssertionError, "Wg_DN must be of type torch.bfloat16");
-  TORCH_CHECK(Wg.is_cuda(), "TopKRouter weights must live on the GPU: there is no CPU compute path");
-  TORCH_CHECK(x.dim() == 3, "x_BSD must be [B, S, D]");
+  check_router(x, Wg);
   if (!wants_autograd({&x, &Wg})) {
     Routed r = router_forward(x, Wg, biases, N, K, Ks);
     return {x, r.mask, r.s_MN.t()};
   }
   variable_list r = RouterFn::apply(x, Wg, biases, N, K, Ks);
   return {r[0], r[1], r[2]};
+}
+
+// ---- balance loss ------------------------------------------------------------------------------
+int type_of(at::ScalarType t) {
+  return t == at::kBFloat16 ? MOMOE_TYPE_BF16 : t == at::kFloat ? MOMOE_TYPE_F32 : t == at::kHalf ? MOMOE_TYPE_F16 : -1;
+}
+
+// Rows that the kernels walk with one pitch: [M, N] of unit column stride
+bool has_rows(const Tensor& t) { return t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)); }
+Tensor rows_of(const Tensor& t, int64_t M, int64_t N) {
+  const Tensor rows = t.reshape({M, N});
+  return has_rows(rows) ? rows : rows.contiguous();
+}
+int64_t pitch_of(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+struct Balanced {
+  Tensor loss, counts;  // results: [], [groups, N]
+  Tensor valid, info;   // for the backward, with the logits; `valid` may be undefined
+};
+
+// logits [.., N] of one of the three types, `groups` of as many tokens each
+Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks, const std::optional<Tensor>& valid,
+                         int64_t groups) {
+  const at::Device dev = logits.device();
+  const int64_t N = logits.size(-1), M = logits.numel() / N;
+  const c10::DeviceGuard guard(dev);
+  Balanced b;
+  const Tensor rows = rows_of(logits, M, N);
+  const Tensor mask = mask_NM.to(dev, at::kInt);
+  TORCH_CHECK(mask.dim() == 2 && mask.size(0) == N && mask.size(1) == M, "mask_NM must be [", N, ", ", M, "]");
+  if (valid.has_value()) {
+    TORCH_CHECK(valid->scalar_type() == at::kBool && valid->numel() == M, "valid must be a bool tensor of ", M,
+                " elements, one for each token");
+    b.valid = valid->to(dev).reshape({M}).contiguous();
+  }
+  b.counts = at::empty({groups, N}, at::TensorOptions().dtype(at::kLong).device(dev));
+  b.loss = empty_f32({}, dev);
+  b.info = empty_f32({1 + groups}, dev);
+  if (M == 0) {
+    b.counts.zero_();
+    b.loss.zero_();
+    b.info.zero_();
+    return b;
+  }
+  const int64_t S = M / groups, ws_bytes = momoe_balance_workspace_bytes(groups, S, N);
+  TORCH_CHECK(ws_bytes >= 0, "balance loss: [", M, ", ", N, "] logits are past the sizes that it takes (N <= 512)");
+  const Tensor ws = empty_f32({ws_bytes / 4}, dev);
+  MOMOE_CALL(momoe_balance_fwd, stream_of(dev), rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
+             mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1),
+             b.valid.defined() ? (const uint8_t*)b.valid.data_ptr() : nullptr, groups, S, N, Ks, b.loss.data_ptr<float>(),
+             b.counts.data_ptr<int64_t>(), b.info.data_ptr<float>(), ws.data_ptr(), ws_bytes);
+  return b;
+}
+
+// d loss / d logits, of type `type`, + `add` in its place if that is defined
+Tensor balance_gradient(const Tensor& logits, const Tensor& valid, const Tensor& counts, const Tensor& info, const Tensor& G_loss,
+                        int64_t Ks, at::ScalarType type, const Tensor& add) {
+  const at::Device dev = logits.device();
+  const int64_t M = logits.size(0), N = logits.size(1), groups = counts.size(0);
+  const Tensor g = G_loss.to(dev, at::kFloat).contiguous();
+  Tensor out = add.defined() ? add : at::empty({M, N}, at::TensorOptions().dtype(type).device(dev));
+  if (M == 0) return out;
+  MOMOE_CALL(momoe_balance_bwd, stream_of(dev), logits.data_ptr(), type_of(logits.scalar_type()), pitch_of(logits),
+             valid.defined() ? (const uint8_t*)valid.data_ptr() : nullptr, counts.data_ptr<int64_t>(), info.data_ptr<float>(),
+             g.data_ptr<float>(), add.defined() ? (const void*)add.data_ptr() : nullptr, out.data_ptr(), type_of(type), groups,
+             M / groups, N, Ks);
+  return out;
+}
+
+// What the forward saved, as balance_gradient takes it: logits, valid, counts, info from `saved[at]` on
+struct BalanceSaved {
+  Tensor logits, valid, counts, info;
+  BalanceSaved(const variable_list& saved, size_t at, const at::Device& dev, at::ScalarType type, at::IntArrayRef sizes, int64_t M,
+               int64_t N, int64_t groups) {
+    logits = rows_of(as_saved(saved[at], "logits", dev, type, sizes, /*packed=*/false), M, N);
+    valid = saved[at + 1];
+    if (valid.defined()) {
+      as_saved(valid, "valid", dev, at::kBool, {M}, /*packed=*/false);
+      TORCH_CHECK(valid.is_contiguous(), "backward: the saved tensor valid came back from its hook with other strides");
+    }
+    counts = as_saved(saved[at + 2], "counts", dev, at::kLong, {groups, N});
+    info = as_saved(saved[at + 3], "info", dev, at::kFloat, {1 + groups});
+  }
+};
+
+struct BalanceFn : torch::autograd::Function<BalanceFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& mask, int64_t Ks,
+                               const std::optional<Tensor>& valid, int64_t groups) {
+    Balanced b = balance_forward(logits, mask, Ks, valid, groups);
+    // (the logits as they came: a view made here would hide from autograd that they changed since)
+    ctx->save_for_backward({logits, b.valid, b.counts, b.info});
+    ctx->saved_data["call"] = std::vector<int64_t>{Ks, groups, logits.device().index(), (int64_t)logits.scalar_type()};
+    ctx->saved_data["sizes"] = logits.sizes().vec();
+    ctx->mark_non_differentiable({b.counts});
+    ctx->set_materialize_grads(false);
+    return {b.loss, b.counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "balance_loss has no second derivative: call backward without create_graph");
+    const std::vector<int64_t> call_of = ctx->saved_data["call"].toIntVector();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const at::ScalarType type = (at::ScalarType)call_of[3];
+    const at::Device dev(at::kCUDA, (at::DeviceIndex)call_of[2]);
+    const c10::DeviceGuard guard(dev);
+    const BalanceSaved t(ctx->get_saved_variables(), 0, dev, type, sizes, c10::multiply_integers(sizes.begin(), sizes.end() - 1),
+                         sizes.back(), call_of[1]);
+    out[0] = balance_gradient(t.logits, t.valid, t.counts, t.info, grads[0], call_of[0], type, {}).view(sizes);
+    return out;
+  }
+};
+
+// Groups of a call: its sequences, or all of its tokens
+int64_t groups_of(at::IntArrayRef sizes, bool per_sequence) {
+  TORCH_CHECK(!per_sequence || sizes.size() == 3, "per_sequence takes [B, S, N] logits or [B, S, D] tokens");
+  return per_sequence && sizes[0] > 0 ? sizes[0] : 1;
+}
+
+std::tuple<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& mask, int64_t Ks, const std::optional<Tensor>& valid,
+                                        bool per_sequence) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<std::tuple<Tensor, Tensor>, const Tensor&, const Tensor&, int64_t, const std::optional<Tensor>&, bool>(
+        "momoe::balance_loss", logits, mask, Ks, valid, per_sequence);
+  TORCH_CHECK(logits.is_cuda(), "balance_loss needs logits on the GPU: there is no CPU compute path");
+  if (type_of(logits.scalar_type()) < 0)
+    throw_python(PyExc_AssertionError, std::string("the logits must be bfloat16, float32 or float16, got ") +
+                                           c10::toString(logits.scalar_type()));
+  TORCH_CHECK(logits.dim() == 2 || logits.dim() == 3, "logits must be [M, N] or [B, S, N]");
+  const int64_t N = logits.size(-1), groups = groups_of(logits.sizes(), per_sequence);
+  TORCH_CHECK(Ks >= 0 && Ks < N, "num_shared_experts must be between 0 and N - 1 = ", N - 1, ", got ", Ks);
+  TORCH_CHECK(N <= 512, "balance_loss takes up to 512 experts, got ", N);
+  Tensor loss, counts;
+  if (wants_autograd({&logits})) {
+    variable_list r = BalanceFn::apply(logits, mask, Ks, valid, groups);
+    loss = r[0], counts = r[1];
+  } else {
+    Balanced b = balance_forward(logits, mask, Ks, valid, groups);
+    loss = b.loss, counts = b.counts;
+  }
+  return {loss, per_sequence ? counts : counts.select(0, 0)};
+}
+
+// The router and, of its logits, the balance loss: one gradient of the logits goes back through the gate product
+struct BalancedRouterFn : torch::autograd::Function<BalancedRouterFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& Wg, const Tensor& biases, int64_t N, int64_t K,
+                               int64_t Ks, const std::optional<Tensor>& valid, int64_t groups) {
+    Routed r = router_forward(x, Wg, biases, N, K, Ks, /*keep_logits=*/true);
+    Balanced b = balance_forward(r.logits, r.mask, Ks, valid, groups);
+    ctx->save_for_backward({r.x_MD, Wg, r.mask, r.p_sel, r.s_MN, r.norms, r.logits, b.valid, b.counts, b.info});
+    ctx->saved_data["call"] = std::vector<int64_t>{Ks, N, Wg.device().index(), x.size(0), x.size(1), x.size(2), groups,
+                                                   (int64_t)r.logits.scalar_type()};
+    ctx->mark_non_differentiable({r.mask, b.counts});
+    ctx->set_materialize_grads(false);
+    return {x, r.mask, r.s_MN.t(), b.loss, b.counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const std::vector<int64_t> call_of = ctx->saved_data["call"].toIntVector();
+    const at::Device dev(at::kCUDA, (at::DeviceIndex)call_of[2]);
+    const c10::DeviceGuard guard(dev);
+    const int64_t Ks = call_of[0], N = call_of[1], M = call_of[3] * call_of[4], D = call_of[5];
+    const Tensor &G_x_BSD = grads[0], &G_s_NM = grads[2], &G_loss = grads[3];
+    Tensor G_x, G_logit;
+    if (G_x_BSD.defined()) G_x = G_x_BSD.reshape({M, D}).to(dev, at::kBFloat16);
+    if (G_s_NM.defined()) G_logit = router_gradient(saved, dev, G_s_NM, M, N, Ks);
+    if (G_loss.defined()) {
+      TORCH_CHECK(!at::GradMode::is_enabled(), "the balance loss has no second derivative: call backward without create_graph");
+      const BalanceSaved t(saved, 6, dev, (at::ScalarType)call_of[7], {M, N}, M, N, call_of[6]);
+      G_logit = balance_gradient(t.logits, t.valid, t.counts, t.info, G_loss, Ks, at::kBFloat16, G_logit);
+    }
+    variable_list out(8);
+    gate_gradients(ctx, saved, dev, G_x, G_logit, {call_of[3], call_of[4], D}, N, out);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> router_balanced(const Tensor& x, const Tensor& Wg, const Tensor& biases, int64_t N,
+                                                                   int64_t K, int64_t Ks, const std::optional<Tensor>& valid,
+                                                                   bool per_sequence) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>, const Tensor&, const Tensor&, const Tensor&, int64_t,
+                         int64_t, int64_t, const std::optional<Tensor>&, bool>("momoe::router_balanced", x, Wg, biases, N, K, Ks,
+                                                                               valid, per_sequence);
+  check_router(x, Wg);
+  TORCH_CHECK(Ks >= 0 && Ks < N, "the balance loss needs a routed expert: ", N, " experts, ", Ks, " of them shared");
+  const int64_t groups = groups_of(x.sizes(), per_sequence);
+  variable_list r;
+  if (wants_autograd({&x, &Wg})) {
+    r = BalancedRouterFn::apply(x, Wg, biases, N, K, Ks, valid, groups);
+  } else {
+    Routed t = router_forward(x, Wg, biases, N, K, Ks, /*keep_logits=*/true);
+    Balanced b = balance_forward(t.logits, t.mask, Ks, valid, groups);
+    r = {x, t.mask, t.s_MN.t(), b.loss, b.counts};
+  }
+  return {r[0], r[1], r[2], r[3], per_sequence ? r[4] : r[4].select(0, 0)};
 }
 
 // biases += rate * sign(c_avg - sizes), in place, in fp32
@@ -611,11 +828,18 @@ TORCH_LIBRARY(momoe, m) {
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts)));
   m.def("router(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks) -> (Tensor(a), Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(router)));
+  m.def("balance_loss(Tensor logits, Tensor mask_NM, int Ks, Tensor? valid, bool per_sequence) -> (Tensor, Tensor)",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(balance_loss)));
+  m.def("router_balanced(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks, Tensor? valid, bool per_sequence) "
+        "-> (Tensor(a), Tensor, Tensor, Tensor, Tensor)",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(router_balanced)));
 }
 
 PYBIND11_MODULE(_layer, m) {
   m.def("experts", &experts, py::call_guard<py::gil_scoped_release>());
   m.def("router", &router, py::call_guard<py::gil_scoped_release>());
+  m.def("balance_loss", &balance_loss, py::call_guard<py::gil_scoped_release>());
+  m.def("router_balanced", &router_balanced, py::call_guard<py::gil_scoped_release>());
   m.def("bias_update", &bias_update, py::call_guard<py::gil_scoped_release>());
   m.def("timing_start", &timing_start);
   m.def("timing_stop", &timing_stop);

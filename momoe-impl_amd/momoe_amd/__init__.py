@@ -1,9 +1,10 @@
 """MI355X-native MoMoE: SwiGLU mixture-of-experts layer on hand-written gfx950 kernels.
 
-Same public names as the reference package (momoe/__init__.py:1-5).
+The public names of the reference package (momoe/__init__.py:1-5), and `balance_loss`.
 """
 from .experts import MoMoE, MoEFunction
 from .router import TopKRouter, TopKRouterFunction
 from .moe import MoE
+from .balance import balance_loss
 
-__all__ = ["MoMoE", "MoE", "TopKRouter", "MoEFunction", "TopKRouterFunction"]
+__all__ = ["MoMoE", "MoE", "TopKRouter", "MoEFunction", "TopKRouterFunction", "balance_loss"]

@@ -82,6 +82,9 @@ _SIGNATURES = {
     "momoe_backward_tail": (_int, [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
                                    _p]),
     "momoe_gate_dgrad": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _p]),
+    "momoe_balance_workspace_bytes": (_i64, [_i64] * 3),
+    "momoe_balance_fwd": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    "momoe_balance_bwd": (_int, [_p, _int, _i64, _p, _p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p]),
     "momoe_bias_update": (_int, [_p, ctypes.c_float, ctypes.c_float, _i64, _p, _p]),
 }
 

@@ -1,4 +1,4 @@
-"""`MoE`: router -> experts -> auxiliary-loss-free bias update (momoe/sample_moe.py:16-68).
+"""`MoE`: router -> experts -> auxiliary-loss-free bias update (momoe/sample_moe.py:16-68), and on request a balance loss.
 
 Parameter names match the reference so state dicts interchange:
 `router.Wg_DN`, `momoe.Wl1_ND2H`, `momoe.Wl2_NHD`, `biases_N`.
@@ -14,8 +14,13 @@ from .router import TopKRouter
 class MoE(nn.Module):
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts,
                  num_shared_experts, save_percent=0, bias_update_rate=1e-4,
-                 Wg_DN=None, Wl1_ND2H=None, Wl2_NHD=None):
+                 Wg_DN=None, Wl1_ND2H=None, Wl2_NHD=None, balance=None):
+        """balance: None, "batch" or "sequence".  With one of the latter `forward` returns (y_BSD, loss), the
+        `balance_loss` over the whole batch or the mean of that of its sequences, to be weighed into the training loss."""
+        if balance not in (None, "batch", "sequence"):
+            raise ValueError(f'balance must be None, "batch" or "sequence", got {balance!r}')
         super().__init__()
+        self.balance = balance
         self.D = embedding_dim
         self.H = intermediate_dim
         self.N = num_experts
@@ -34,8 +39,18 @@ class MoE(nn.Module):
                        torch.full((self.Ks,), float("-inf"), device=dev, dtype=torch.float32)]),
             requires_grad=False)
 
-    def forward(self, x_BSD):
-        x_BSD, mask_NM, s_NM = self.router(x_BSD, self.biases_N)
+    def forward(self, x_BSD, valid=None):
+        """valid: bool [B, S], the tokens that count in the balance loss (all, if None)."""
+        if self.balance is None:
+            if valid is not None:
+                raise ValueError("valid is for the balance loss: build the MoE with balance=...")
+            x_BSD, mask_NM, s_NM = self.router(x_BSD, self.biases_N)
+            return self._experts(x_BSD, mask_NM, s_NM)
+        x_BSD, mask_NM, s_NM, loss, _ = self.router.with_balance_loss(x_BSD, self.biases_N, valid,
+                                                                      self.balance == "sequence")
+        return self._experts(x_BSD, mask_NM, s_NM), loss
+
+    def _experts(self, x_BSD, mask_NM, s_NM):
         y_BSD, sizes_N = self.momoe(x_BSD, mask_NM, s_NM)
         if self.bias_update_rate == 0.0:  # serving: the bias stays what it was trained to
             return y_BSD

@@ -23,6 +23,8 @@ reference, which has no tests, fixtures or golden vectors of its own):
 * `router_backward_closed_form` - pinned: autograd through a differentiable
                             restatement; finite differences
 * `bias_update`           - pinned: closed form on hand-computed cases
+* `balance_loss`          - pinned: autograd through the definition, hand-computed cases
+                            (tests/test_oracle_operators.py)
 
 The reference's intermediate bf16 rounding points, its autotune-dependent
 save/recompute tile boundary and its raced `which` order are NOT restated
@@ -44,3 +46,4 @@ from .moe_oracle import (  # noqa: F401
     OracleTopKRouter,
     OracleMoE,
 )
+from .operators import balance_loss  # noqa: F401
