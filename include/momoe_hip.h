@@ -442,6 +442,48 @@ int momoe_balance_bwd(const void* logits, int logits_type, int64_t ld, const uin
                       const float* info, const float* G_loss, const void* add_MN, void* Glogits_MN, int grad_type,
                       int64_t G, int64_t S, int64_t N, int64_t Ks, void* stream);
 
+/* ---- experts in 8-bit floating point, forward only --------------------------------
+ * No counterpart in the reference, whose weights are bf16.  e4m3 (largest value 448) with a scale for each 128 values:
+ *   rows     each 128 consecutive values of a row, scaled by the least power of two that leaves none above 448 (of magnitudes
+ *            below 2^-100: as if that were the largest).  q: momoe_fp8_row_bytes(cols) bytes a row, zeros past the last column;
+ *            codes: momoe_fp8_code_bytes(cols) bytes a row, of which the first ceil(cols / 128) are the scales, 2^(code - 127).  A NaN or an infinity among the 128 makes NaN of all results of that row.
+ *   weights  any fp32 scale for each block of 128 rows x 128 columns; of Wl1 the H columns of each half have blocks of their own:
+ *            Wl1_scale [N][ceil(D/128)][2][ceil(H/128)], Wl2_scale [N][ceil(H/128)][ceil(D/128)].  Kept in the order that the
+ *            kernels stream them in: [N][groups of 16 columns][ceil(rows/128)][2][64][16] bytes, byte b of piece (half h, lane l) the
+ *            k-value 64 h + 16 (l / 16) + b of column l % 16, zeros past the last row; the groups of the two halves in turn.
+ * A product is the sum over its blocks of (both scales) * (fp32 sum of the 128 products), in fp32.
+ */
+int64_t momoe_fp8_row_bytes(int64_t cols);
+int64_t momoe_fp8_code_bytes(int64_t cols);
+/* x: MOMOE_TYPE_*, row pitch ldx elements; cols and ldx multiples of 8; x and q on 16-byte boundaries, codes on a 4-byte one. */
+int momoe_fp8_quantize_rows(const void* x, int type, int64_t ldx, int64_t rows, int64_t cols, void* q, void* codes, void* stream);
+
+/* Weights [N][R][C] row-major, in `halves` (1 or 2) halves of C / halves columns, a multiple of 16: e4m3 to be laid out (quantized =
+ * 1; scale is not used), or bf16 (0) to be brought to e4m3 with scales by the rule for rows, written to
+ * scale [N][ceil(R/128)][halves][ceil(C/halves/128)].  packed: momoe_fp8_weight_bytes(N, R, C) bytes.  On 16-byte boundaries. */
+int64_t momoe_fp8_weight_bytes(int64_t N, int64_t R, int64_t C);
+int momoe_fp8_pack_weights(const void* W_NRC, int quantized, int64_t N, int64_t R, int64_t C, int halves, void* packed, float* scale,
+                           void* stream);
+
+/* Tile height of the table that suits both products below. */
+int momoe_fp8_tile_rows(int64_t Msum, int64_t N);
+/* momoe_fp8_lin1_swiglu_fwd: h = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i], brought to 8 bits from fp32.
+ * x_q, x_codes: rows of x [M][D]; h_q, h_codes: rows of h [Msum][H]; codes on 4-byte boundaries, the others on
+ * 16-byte ones.  tile_table: of momoe_index_build for
+ * momoe_fp8_tile_rows(Msum, N) rows. */
+int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, const void* Wl1_packed, const float* Wl1_scale,
+                              const int32_t* idx_Msum, const int32_t* tile_table, void* h_q, void* h_codes, int64_t M,
+                              int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);
+/* momoe_fp8_lin2_scale_fwd: ys[r] = (h[r] . Wl2[i]) * s[i, idx[r]], eight values in 16 bytes (15 bits each of the binade of the largest of
+ * the eight, in whose lowest bits lie those of its exponent): ys_packets Msum * D * 2 bytes on a 16-byte boundary, for
+ * momoe_fp8_combine: out_MD bf16 [M][D], out[m] = the sum of its experts' rows, in fp32, as momoe_combine. */
+int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, const void* Wl2_packed, const float* Wl2_scale,
+                             const float* s_NM, int64_t s_stride_n, int64_t s_stride_m, const int32_t* idx_Msum,
+                             const int32_t* tile_table, void* ys_packets, int64_t M, int64_t D, int64_t H, int64_t N,
+                             int64_t Msum, void* stream);
+int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K,
+                      int64_t Msum, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

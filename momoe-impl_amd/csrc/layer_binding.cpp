@@ -451,6 +451,80 @@ std::tuple<Tensor, Tensor> experts(const Tensor& x, const Tensor& W1, const Tens
   return {r[0], r[1]};
 }
 
+// ---- experts in 8-bit floating point ----------------------------------------------------------
+int type_of(at::ScalarType t) {
+  return t == at::kBFloat16 ? MOMOE_TYPE_BF16 : t == at::kFloat ? MOMOE_TYPE_F32 : t == at::kHalf ? MOMOE_TYPE_F16 : -1;
+}
+
+// x [B, S, D]; W1, W2 packed, S1, S2 their scales; forward only
+std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, const Tensor& S1, const Tensor& W2, const Tensor& S2,
+                                       const Tensor& mask_NM, const Tensor& s_NM, int64_t K, int64_t H, bool check) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<std::tuple<Tensor, Tensor>, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                         const Tensor&, const Tensor&, int64_t, int64_t, bool>("momoe::experts_fp8", x_BSD, W1, S1, W2, S2, mask_NM,
+                                                                              s_NM, K, H, check);
+  TORCH_CHECK(W1.is_cuda(), "MoMoEFP8 weights must live on the GPU: there is no CPU compute path");
+  TORCH_CHECK(!wants_autograd({&x_BSD, &s_NM}),
+              "MoMoEFP8 has no backward, and an input requires a gradient: call it under torch.no_grad()");
+  const at::Device dev = W1.device();
+  if (x_BSD.dim() != 3) throw_python(PyExc_AssertionError, "x_BSD must be [B, S, D]");
+  const int64_t B = x_BSD.size(0), S = x_BSD.size(1), D = x_BSD.size(2), M = B * S;
+  const int64_t N = S1.dim() == 4 ? S1.size(0) : 0, msum = M * K, DB = (D + 127) / 128, HB = (H + 127) / 128;
+  const auto held = [&](const Tensor& t, at::ScalarType type) {
+    return t.device() == dev && t.scalar_type() == type && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0;
+  };
+  const bool fit = S1.dim() == 4 && S2.dim() == 3 && S1.sizes() == at::IntArrayRef({N, DB, 2, HB}) &&
+                   S2.sizes() == at::IntArrayRef({N, HB, DB}) && W1.numel() == momoe_fp8_weight_bytes(N, D, 2 * H) &&
+                   W2.numel() == momoe_fp8_weight_bytes(N, H, D) && held(W1, at::kByte) && held(W2, at::kByte) && held(S1, at::kFloat) &&
+                   held(S2, at::kFloat);
+  if (!fit) throw_python(PyExc_AssertionError, "x_BSD [B,S,D] and the packed weights do not fit together");
+  const c10::DeviceGuard guard(dev);
+  const hipStream_t st = stream_of(dev);
+  const Tensor mask = mask_NM.to(dev, at::kInt), s = s_NM.to(dev, at::kFloat);
+  TORCH_CHECK(mask.dim() == 2 && mask.size(0) == N && mask.size(1) == M, "mask_NM must be [", N, ", ", M, "]");
+  TORCH_CHECK(s.dim() == 2 && s.size(0) == N && s.size(1) == M, "s_NM must be [", N, ", ", M, "]");
+  Tensor y = empty_bf16({B, S, D}, dev), sizes = at::empty({N}, at::TensorOptions().dtype(at::kLong).device(dev));
+  if (M == 0) return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes.zero_()};
+  // rows in 8 bits from the type they come in; any other type as bf16
+  Tensor x = x_BSD.reshape({M, D}).to(dev);
+  if (type_of(x.scalar_type()) < 0) x = x.to(at::kBFloat16);
+  x = x.contiguous();
+  if ((uintptr_t)x.data_ptr() % 16 != 0) x = x.clone();
+
+  Index ib(M, N, K, momoe_fp8_tile_rows(msum, N), false);
+  const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
+  const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
+  const int64_t xq_bytes = M * DB * 128, xs_bytes = M * momoe_fp8_code_bytes(D), hq_bytes = msum * HB * 128,
+                hs_bytes = msum * momoe_fp8_code_bytes(H);
+  Transients transients(dev, {index_bytes, scratch_bytes, xq_bytes, xs_bytes, hq_bytes, hs_bytes, msum * D * 2});
+  Tensor index_own, scratch, xq_own, xs_own, hq_own, hs_own, ys_own, counter;
+  ib.base = (int32_t*)transients.take(index_bytes, index_own);
+  int32_t* const build = (int32_t*)transients.take(scratch_bytes, scratch);
+  int32_t* violations = build;
+  if (check) {
+    counter = at::zeros({4}, at::TensorOptions().dtype(at::kInt).device(dev));
+    violations = counter.data_ptr<int32_t>();
+  }
+  MOMOE_CALL(momoe_index_build, st, mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), M, N, K, sizes.data_ptr<int64_t>(),
+             ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), (int)ib.tile_rows, (int32_t*)nullptr,
+             (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
+  void* const xq = transients.take(xq_bytes, xq_own);
+  void* const xs = transients.take(xs_bytes, xs_own);
+  MOMOE_CALL(momoe_fp8_quantize_rows, st, x.data_ptr(), type_of(x.scalar_type()), D, M, D, xq, xs);
+  void* const hq = transients.take(hq_bytes, hq_own);
+  void* const hs = transients.take(hs_bytes, hs_own);
+  MOMOE_CALL(momoe_fp8_lin1_swiglu_fwd, st, xq, xs, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(), hq, hs, M, D, H, N, msum);
+  void* const ys = transients.take(msum * D * 2, ys_own);
+  MOMOE_CALL(momoe_fp8_lin2_scale_fwd, st, hq, hs, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0), s.stride(1),
+             ib.idx(), ib.table(), ys, M, D, H, N, msum);
+  MOMOE_CALL(momoe_fp8_combine, st, ys, ib.inv(), y.data_ptr(), M, D, K, msum);
+  if (check) {
+    const int v = counter.narrow(0, 0, 1).item<int32_t>();
+    TORCH_CHECK(v == 0, "mask_NM: ", v, " tokens do not have exactly K = ", K, " experts (or the mask holds more than M*K pairs)");
+  }
+  return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes};
+}
+
 // ---- router ------------------------------------------------------------------------------------
 struct Routed {
   Tensor x_MD, mask, s_MN, p_sel, norms;
@@ -615,10 +689,6 @@ std::tuple<Tensor, Tensor, Tensor> router(const Tensor& x, const Tensor& Wg, con
 }
 
 // ---- balance loss ------------------------------------------------------------------------------
-int type_of(at::ScalarType t) {
-  return t == at::kBFloat16 ? MOMOE_TYPE_BF16 : t == at::kFloat ? MOMOE_TYPE_F32 : t == at::kHalf ? MOMOE_TYPE_F16 : -1;
-}
-
 // Rows that the kernels walk with one pitch: [M, N] of unit column stride
 bool has_rows(const Tensor& t) { return t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)); }
 Tensor rows_of(const Tensor& t, int64_t M, int64_t N) {
@@ -828,6 +898,9 @@ TORCH_LIBRARY(momoe, m) {
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts)));
   m.def("router(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks) -> (Tensor(a), Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(router)));
+  m.def("experts_fp8(Tensor x_BSD, Tensor Wl1, Tensor Wl1_scale, Tensor Wl2, Tensor Wl2_scale, Tensor mask_NM, Tensor s_NM, int K, "
+        "int H, bool check) -> (Tensor, Tensor)",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_fp8)));
   m.def("balance_loss(Tensor logits, Tensor mask_NM, int Ks, Tensor? valid, bool per_sequence) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(balance_loss)));
   m.def("router_balanced(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks, Tensor? valid, bool per_sequence) "
@@ -837,6 +910,7 @@ TORCH_LIBRARY(momoe, m) {
 
 PYBIND11_MODULE(_layer, m) {
   m.def("experts", &experts, py::call_guard<py::gil_scoped_release>());
+  m.def("experts_fp8", &experts_fp8, py::call_guard<py::gil_scoped_release>());
   m.def("router", &router, py::call_guard<py::gil_scoped_release>());
   m.def("balance_loss", &balance_loss, py::call_guard<py::gil_scoped_release>());
   m.def("router_balanced", &router_balanced, py::call_guard<py::gil_scoped_release>());

@@ -85,6 +85,15 @@ _SIGNATURES = {
     "momoe_balance_workspace_bytes": (_i64, [_i64] * 3),
     "momoe_balance_fwd": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
     "momoe_balance_bwd": (_int, [_p, _int, _i64, _p, _p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p]),
+    "momoe_fp8_row_bytes": (_i64, [_i64]),
+    "momoe_fp8_code_bytes": (_i64, [_i64]),
+    "momoe_fp8_quantize_rows": (_int, [_p, _int, _i64, _i64, _i64, _p, _p, _p]),
+    "momoe_fp8_weight_bytes": (_i64, [_i64] * 3),
+    "momoe_fp8_pack_weights": (_int, [_p, _int, _i64, _i64, _i64, _int, _p, _p, _p]),
+    "momoe_fp8_tile_rows": (_int, [_i64, _i64]),
+    "momoe_fp8_lin1_swiglu_fwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_fp8_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_bias_update": (_int, [_p, ctypes.c_float, ctypes.c_float, _i64, _p, _p]),
 }
 
@@ -445,3 +454,63 @@ def gate_dgrad(Glogits_MN, Wg_DN, Gx_MD, out_MD):
     (M, N), D = Glogits_MN.shape, Wg_DN.shape[0]
     assert all(t is None or t.is_contiguous() for t in (Glogits_MN, Wg_DN, Gx_MD, out_MD))
     _call("momoe_gate_dgrad", _ptr(Glogits_MN), _ptr(Wg_DN), _ptr(Gx_MD), _ptr(out_MD), M, D, N, _stream())
+
+
+# ---------------------------------------------------------------- 8-bit floating point
+_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def fp8_quantize_rows(x):
+    """x [rows, cols] -> (e4m3 [rows, padded cols], uint8 codes [rows, padded blocks]): the scale of a block is 2^(code - 127)."""
+    _need_cuda(x)
+    assert x.dim() == 2 and x.stride(1) == 1
+    rows, cols = x.shape
+    q = torch.empty((rows, _lib.momoe_fp8_row_bytes(cols)), dtype=torch.uint8, device=x.device)
+    codes = torch.empty((rows, _lib.momoe_fp8_code_bytes(cols)), dtype=torch.uint8, device=x.device)
+    _call("momoe_fp8_quantize_rows", _ptr(x), _TYPES[x.dtype], x.stride(0), rows, cols, _ptr(q), _ptr(codes), _stream())
+    return q.view(torch.float8_e4m3fn), codes
+
+
+def fp8_pack_weights(W_NRC, halves):
+    """Weights [N, R, C] in e4m3 -> packed bytes; in bf16 -> (packed bytes, scale [N, row blocks, halves, column blocks])."""
+    _need_cuda(W_NRC)
+    N, R, C = W_NRC.shape
+    quantized = W_NRC.dtype == torch.float8_e4m3fn
+    assert W_NRC.is_contiguous() and (quantized or W_NRC.dtype == torch.bfloat16)
+    nbytes = _lib.momoe_fp8_weight_bytes(N, R, C)
+    packed = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=W_NRC.device)
+    blocks = lambda n: -(-n // 128)
+    scale = None if quantized else torch.empty((N, blocks(R), halves, blocks(C // halves)), dtype=torch.float32, device=W_NRC.device)
+    with torch.cuda.device(W_NRC.device):
+        _call("momoe_fp8_pack_weights", _ptr(W_NRC), int(quantized), N, R, C, halves, _ptr(packed), _ptr(scale), _stream())
+    return packed if quantized else (packed, scale)
+
+
+def fp8_tile_rows(Msum, N):
+    return _lib.momoe_fp8_tile_rows(Msum, N)
+
+
+def fp8_lin1_swiglu_fwd(x_q, x_codes, Wl1_packed, Wl1_scale, idx, table, D, H):
+    """Rows of x as fp8_quantize_rows gives them -> those of h [Msum, H] (codes with their padding in both)."""
+    N, Msum, M = Wl1_scale.shape[0], idx.numel(), x_q.shape[0]
+    h_q = torch.empty((Msum, _lib.momoe_fp8_row_bytes(H)), dtype=torch.uint8, device=x_q.device)
+    h_codes = torch.empty((Msum, _lib.momoe_fp8_code_bytes(H)), dtype=torch.uint8, device=x_q.device)
+    _call("momoe_fp8_lin1_swiglu_fwd", _ptr(x_q), _ptr(x_codes), _ptr(Wl1_packed), _ptr(Wl1_scale), _ptr(idx), _ptr(table), _ptr(h_q),
+          _ptr(h_codes), M, D, H, N, Msum, _stream())
+    return h_q.view(torch.float8_e4m3fn), h_codes
+
+
+def fp8_lin2_scale_fwd(h_q, h_codes, Wl2_packed, Wl2_scale, s_NM, idx, table, D, H):
+    """The packets [Msum, D / 8, 4] (int32) of the second product."""
+    (N, M), Msum = s_NM.shape, idx.numel()
+    ys = torch.empty((Msum, D // 8, 4), dtype=torch.int32, device=h_q.device)
+    _call("momoe_fp8_lin2_scale_fwd", _ptr(h_q), _ptr(h_codes), _ptr(Wl2_packed), _ptr(Wl2_scale), _ptr(s_NM), s_NM.stride(0),
+          s_NM.stride(1), _ptr(idx), _ptr(table), _ptr(ys), M, D, H, N, Msum, _stream())
+    return ys
+
+
+def fp8_combine(ys, inv_MK, D):
+    M, K = inv_MK.shape
+    out = torch.empty((M, D), dtype=torch.bfloat16, device=ys.device)
+    _call("momoe_fp8_combine", _ptr(ys), _ptr(inv_MK), _ptr(out), M, D, K, ys.shape[0], _stream())
+    return out

@@ -8,6 +8,7 @@ import torch.nn as nn
 
 from . import _layer
 from .experts import MoMoE
+from .experts_fp8 import MoMoEFP8
 from .router import TopKRouter
 
 
@@ -38,6 +39,22 @@ class MoE(nn.Module):
             torch.cat([torch.zeros(self.N - self.Ks, device=dev, dtype=torch.float32),
                        torch.full((self.Ks,), float("-inf"), device=dev, dtype=torch.float32)]),
             requires_grad=False)
+
+    def to_fp8(self):
+        """A `MoE` for serving with the same router and selection bias and the experts in 8-bit floating point
+        (`MoMoEFP8.from_momoe`); forward only, under `torch.no_grad()`."""
+        return self.serving(self.router, self.biases_N, MoMoEFP8.from_momoe(self.momoe))
+
+    @classmethod
+    def serving(cls, router, biases_N, momoe):
+        """A `MoE` of a router, its selection bias and experts (`MoMoE` or `MoMoEFP8`) that leaves the bias as it is."""
+        self = cls.__new__(cls)
+        nn.Module.__init__(self)
+        self.D, self.H, self.N, self.K, self.Ks = router.D, momoe.H, router.N, router.K, router.Ks
+        assert (momoe.D, momoe.N, momoe.K) == (self.D, self.N, self.K), "router and experts of different sizes"
+        self.save_percent, self.bias_update_rate, self.balance = 0, 0.0, None
+        self.router, self.momoe, self.biases_N = router, momoe, biases_N
+        return self
 
     def forward(self, x_BSD, valid=None):
         """valid: bool [B, S], the tokens that count in the balance loss (all, if None)."""

@@ -25,6 +25,7 @@ reference, which has no tests, fixtures or golden vectors of its own):
 * `bias_update`           - pinned: closed form on hand-computed cases
 * `balance_loss`          - pinned: autograd through the definition, hand-computed cases
                             (tests/test_oracle_operators.py)
+* `experts_fp8`           - pinned: `e4m3` by torch's conversion, `experts_forward` where nothing is rounded
 
 The reference's intermediate bf16 rounding points, its autotune-dependent
 save/recompute tile boundary and its raced `which` order are NOT restated
@@ -46,4 +47,11 @@ from .moe_oracle import (  # noqa: F401
     OracleTopKRouter,
     OracleMoE,
 )
-from .operators import balance_loss  # noqa: F401
+from .operators import (  # noqa: F401
+    balance_loss,
+    block_weights,
+    e4m3,
+    experts_fp8,
+    rounded_rows,
+    rows_in_8_bits,
+)
