@@ -466,11 +466,11 @@ int momoe_fp8_pack_weights(const void* W_NRC, int quantized, int64_t N, int64_t 
                            void* stream);
 
 /* Tile height of the table that suits both products below. */
-int momoe_fp8_tile_rows(int64_t Msum, int64_t N);
+int momoe_fp8_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N);
 /* momoe_fp8_lin1_swiglu_fwd: h = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i], brought to 8 bits from fp32.
  * x_q, x_codes: rows of x [M][D]; h_q, h_codes: rows of h [Msum][H]; codes on 4-byte boundaries, the others on
  * 16-byte ones.  tile_table: of momoe_index_build for
- * momoe_fp8_tile_rows(Msum, N) rows. */
+ * momoe_fp8_tile_rows(Msum, D, H, N) rows. */
 int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, const void* Wl1_packed, const float* Wl1_scale,
                               const int32_t* idx_Msum, const int32_t* tile_table, void* h_q, void* h_codes, int64_t M,
                               int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);

@@ -50,17 +50,19 @@ __device__ __forceinline__ i32x8 weight_frag(const uint8_t* at) {
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
-// A row's columns 32 * pair + 4 * (lane / 16) .. +3 and those 16 further on, times s
-__device__ __forceinline__ void store_packet(const Fp8Args& p, int64_t row, int pair, int l, const f32x4& a, const f32x4& b, float s) {
-  const float v[8] = {a[0] * s, a[1] * s, a[2] * s, a[3] * s, b[0] * s, b[1] * s, b[2] * s, b[3] * s};
-  *(u32x4*)(p.out + row * p.D + 32 * pair + 8 * (l >> 4)) = Packet::of(v).w;
-}
-
 // the largest of the four lanes that hold a row
 __device__ __forceinline__ uint32_t top_of_rows(uint32_t v) {
   const auto larger = [](auto pair) { return (uint32_t)max((uint32_t)pair[0], (uint32_t)pair[1]); };
   v = larger(__builtin_amdgcn_permlane16_swap(v, v, false, false));
   return larger(__builtin_amdgcn_permlane32_swap(v, v, false, false));
+}
+
+// a * b * sigmoid(b)
+__device__ __forceinline__ f32x4 swiglu(const f32x4& a, const f32x4& b) {
+  f32x4 h;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) h[r] = a[r] * b[r] * sigmoidf_fast(b[r]);
+  return h;
 }
 
 // Tiles of up to 32 rows: a wavefront owns a pair of 16-column groups (of the first product one of each half) and streams
@@ -134,13 +136,8 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
       f32x4 h[FR];
 #pragma unroll
       for (int i = 0; i < FR; ++i) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          h[i][r] = real ? acc[0][i][r] * acc[1][i][r] * sigmoidf_fast(acc[1][i][r]) : 0.0f;
-          top = max(top, magnitude(h[i][r]));
-        }
-        top = top_of_rows(top);
+        h[i] = real ? swiglu(acc[0][i], acc[1][i]) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t top = top_of_rows(largest(h[i][0], h[i][1], h[i][2], h[i][3]));
         if (l < 16) top_lds[wave][16 * i + l] = top;
       }
       __syncthreads();
@@ -154,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
         if (r < tc.rows) {
           const int64_t row = tc.row0 + r;
           *(uint32_t*)(p.hq + (row * p.HB + tc.tn) * kFp8Block + wave * 16 + 4 * (l >> 4)) =
-              pack_e4m3(h[i][0] * s.inverse, h[i][1] * s.inverse, h[i][2] * s.inverse, h[i][3] * s.inverse);
+              pack_e4m3(h[i][0], h[i][1], h[i][2], h[i][3], s.scale);
           if (wave == 0 && l < 16) p.h_codes[row * fp8_code_bytes(p.HB) + tc.tn] = (uint8_t)s.code;
         }
       }
@@ -165,19 +162,24 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
         if (r >= tc.rows) continue;
         const int64_t row = tc.row0 + r;
         const float s = p.s[tc.expert * p.sn + p.idx[row] * p.sm];
-        store_packet(p, row, pair, l, acc[0][i], acc[1][i], s);
+        *(u32x4*)(p.out + row * p.D + 32 * pair + 8 * (l >> 4)) = Packet::of(acc[0][i], acc[1][i], s).w;
       }
     }
   }
 }
 
-// Tiles of up to 256 rows x 256 columns, a workgroup on a CU.  Each of its eight wavefronts owns 32 columns of all rows: it reads
-// their weights straight into registers, each byte once per workgroup, a stage of 128 k-values ahead and more; the rows of a stage
-// come to LDS by direct transfers, a stage ahead, in two slots.
-constexpr int kTileRows = 256, kTileChunk = 64;  // blocks of the contraction whose scales are held at a time
-constexpr int kTileSlot = kTileRows * kFp8Block;
-constexpr int kCodePitch = kTileChunk / 4 + 1;   // dwords; odd: sixteen rows read different banks
-constexpr int kTileLds = 2 * kTileSlot + kTileRows * kCodePitch * 4 + kWaves * kTileRows * 4;
+// Tiles of up to 256 rows x 256 columns, a persistent workgroup on a CU.  Each of its eight wavefronts owns 32 columns of all rows: it
+// reads their weights straight into registers, each byte once per workgroup; the rows come to LDS by direct transfers.  Both are
+// requested two stages of 128 k-values ahead, in three slots of LDS and two register sets, and the last two stages of a tile
+// request the first two of the next one.
+//
+// A stage: the fragments of 16 rows travel from LDS one ahead of the products, the fp32 sums follow one behind them.  Its barrier lies
+// behind the first rows, not at its end: by then the next stage's rows have landed for every wavefront, and the slot of the
+// last one is free.
+constexpr int kTileRows = 256, kTileBlocks = 64;  // most blocks of a contraction
+constexpr int kTileSlot = kTileRows * kFp8Block, kSlots = 3;
+constexpr int kTileCodes = kTileRows * kTileBlocks;  // bytes: [four blocks][row][block]
+constexpr int kTileLds = kSlots * kTileSlot + 2 * kTileCodes + 2 * kTileRows * 4 + 4 * kTileBlocks * 4 + kTileRows * 4;
 
 // `v` is in its registers here: what it is made of lies before this point, what it goes into behind it.  (Without, the compiler
 // forms all products of a stage first and keeps them.)
@@ -185,24 +187,54 @@ template <class T>
 __device__ __forceinline__ void keep(T& v) {
   asm volatile("" : "+v"(v));
 }
+// a value that is the same in every lane, as one that the compiler knows to be
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <class T>
+__device__ __forceinline__ const T* uniform(const T* p) {
+  const uint64_t v = (uint64_t)p;
+  return (const T*)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+// 4 bytes per lane, global -> LDS, as dma16: at a uniform base and an offset, or anywhere
+__device__ __forceinline__ void dma4(const void* from, uint32_t lds_wave_base) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(lds_wave_base)) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* uniform_base, uint32_t byte_offset, uint32_t lds_wave_base) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(byte_offset), "s"(uniform_base),
+               "s"(__builtin_amdgcn_readfirstlane(lds_wave_base))
+               : "memory");
+}
+// wavefronts meet: what they have read from or written to LDS is done with, what they have on the way stays there
+__device__ __forceinline__ void meet() {
+  wait_lgkm0();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
+// memory that stores at offsets of `bytes` and more do not reach
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)uniform((const char*)p), 0, uniform(bytes), 0x00027000);
+}
+
+// The rows of a tile, as a wavefront requests them
 template <bool FIRST>
 struct TileRows {
   static constexpr int DEP = kTileRows / (8 * kWaves);  // transfers of 8 rows each
   const uint8_t* base;
   uint32_t off[DEP];
-  __device__ __forceinline__ void init(const Fp8Args& p, const TileCoord& tc) {
-    const int l = threadIdx.x & 63;
-    base = FIRST ? p.rows : p.rows + (int64_t)tc.row0 * p.KB * kFp8Block;
+  // `idx`: the tokens of the tile's rows (of the first product, whose rows are gathered)
+  __device__ __forceinline__ void place(const Fp8Args& p, const TileCoord& tc, const int32_t* idx) {
+    const int l = fresh_lane();
+    base = FIRST ? p.rows : p.rows + (int64_t)uniform(tc.row0) * p.KB * kFp8Block;
 #pragma unroll
     for (int j = 0; j < DEP; ++j) {
-      const int r = (j * kWaves + wave_id()) * 8 + (l >> 3), have = min(r, tc.rows - 1);
-      const uint32_t src = FIRST ? p.idx[tc.row0 + have] : have;
+      const int r = (j * kWaves + wave_id()) * 8 + (l >> 3);
+      const uint32_t src = FIRST ? idx[r] : min(r, tc.rows - 1);
       off[j] = src * (uint32_t)(p.KB * kFp8Block) + (((l & 7) ^ ((r >> 1) & 7)) << 4);
     }
   }
   __device__ __forceinline__ void request(int kb, uint32_t slot) const {
-    const bf16* const b = (const bf16*)(base + (int64_t)kb * kFp8Block);
+    const bf16* const b = uniform((const bf16*)(base + (int64_t)kb * kFp8Block));
 #pragma unroll
     for (int j = 0; j < DEP; ++j) dma16(b, off[j], slot + (j * kWaves + wave_id()) * 1024);
   }
@@ -211,26 +243,81 @@ struct TileRows {
 template <bool FIRST>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   uint8_t* const lds = (uint8_t*)dyn_lds();
-  uint32_t* const codes_lds = (uint32_t*)(lds + 2 * kTileSlot);
-  uint32_t* const top_lds = codes_lds + kTileRows * kCodePitch;  // [wave][row]
-  float* const gate_lds = (float*)top_lds;  // of the second product
-  const uint32_t addr = lds_address(dyn_lds());
-  const int tid = threadIdx.x, l = tid & 63, wave = wave_id();
-  const int code_bytes = fp8_code_bytes(p.KB);
+  uint8_t* const codes_lds = lds + kSlots * kTileSlot;
+  uint32_t* const top_lds = (uint32_t*)(codes_lds + 2 * kTileCodes);  // [2][row]
+  float* const gate_lds = (float*)top_lds;                            // of the second product: [2][row]
+  float* const scales_lds = (float*)(top_lds + 2 * kTileRows);        // [2][set][block]
+  int32_t* const tokens_lds = (int32_t*)(scales_lds + 4 * kTileBlocks);
+  const uint32_t addr = lds_address(dyn_lds()), codes_addr = addr + kSlots * kTileSlot, gates_addr = codes_addr + 2 * kTileCodes;
+  const uint32_t scales_addr = gates_addr + 2 * kTileRows * 4, tokens_addr = scales_addr + 4 * kTileBlocks * 4;
+  const int wave = wave_id(), stages = max(p.KB, 2), code_bytes = fp8_code_bytes(p.KB);
   TileSchedT<1> sched(p.table, (p.pairs + kWaves - 1) / kWaves, kTileRows);
-  for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
-    const int pair = min(tc.tn * kWaves + wave, p.pairs - 1);
-    const bool real = tc.tn * kWaves + wave < p.pairs;
-    const uint8_t* const w0 = p.w + ((int64_t)tc.expert * p.pairs + pair) * 2 * p.KB * kFp8Frag;
-    const uint8_t* const w1 = w0 + (int64_t)p.KB * kFp8Frag;
-    TileRows<FIRST> rows;
-    rows.init(p, tc);
-    static_assert(2 * kTileRows == kThreads, "two threads a row");
-    const int my_row = tc.row0 + min(tid >> 1, tc.rows - 1), code_row = FIRST ? p.idx[my_row] : my_row;
-    if (!FIRST) {
-      __syncthreads();
-      gate_lds[tid >> 1] = p.s[tc.expert * p.sn + p.idx[my_row] * p.sm];
+  TileCoord cur = sched.next();
+  if (!cur.valid) return;
+
+  const auto pair_of = [&](const TileCoord& tc) { return min(tc.tn * kWaves + wave, p.pairs - 1); };
+  const auto weights_of = [&](const TileCoord& tc) { return p.w + ((int64_t)tc.expert * p.pairs + pair_of(tc)) * 2 * p.KB * kFp8Frag; };
+  // The scales of a tile's weights, block by block, one set of two a wavefront (and again by others): of the two halves; of the two
+  // blocks of columns
+  const auto request_weight_scales = [&](const TileCoord& tc, int to) {
+    const int set = wave & 1, k = min(fresh_lane(), p.KB - 1);
+    const float* const base = p.w_scale + (int64_t)uniform(tc.expert) * p.KB * (FIRST ? 2 * p.HB : p.DB) +
+                              (FIRST ? set * p.HB + uniform(tc.tn) : min(2 * uniform(tc.tn) + set, p.DB - 1));
+    dma4(uniform(base), k * (FIRST ? 2 * p.HB : p.DB) * 4, scales_addr + (2 * to + set) * (kTileBlocks * 4));
+  };
+  // the tokens of a tile's rows, the last one's for those that it does not have: 64 of them a wavefront, and again by another one
+  const auto request_tokens = [&](const TileCoord& tc) {
+    const int q = wave & 3, have = min(q * 64 + fresh_lane(), tc.rows - 1);
+    dma4(uniform(p.idx + tc.row0), have * 4, tokens_addr + q * 256);
+  };
+  // The codes of its rows: four blocks of 64 rows a transfer, as many transfers in every wavefront
+  const int dwords = code_bytes / 4;
+  const auto request_codes = [&](const TileCoord& tc, int to) {
+    const uint8_t* const base = FIRST ? p.codes : p.codes + (int64_t)uniform(tc.row0) * code_bytes;
+    const int q = wave & 3, r = q * 64 + fresh_lane();
+    const uint32_t src = FIRST ? tokens_lds[r] : min(r, tc.rows - 1);
+    for (int n = 0; n < dwords; n += 2) {
+      const int d = min(n + wave / 4, dwords - 1);
+      dma4(uniform(base + 4 * d), src * (uint32_t)code_bytes, codes_addr + to * kTileCodes + (d * kTileRows + q * 64) * 4);
     }
+  };
+  // the gate weights of its rows
+  const auto request_gates = [&](const TileCoord& tc, int to) {
+    const int q = wave & 3;
+    dma4(p.s + (tc.expert * p.sn + tokens_lds[q * 64 + fresh_lane()] * p.sm), gates_addr + (to * kTileRows + q * 64) * 4);
+  };
+
+  // the first tile's requests
+  i32x8 wf[2][2];
+  TileRows<FIRST> rows;
+  request_tokens(cur);
+  wait_vmcnt<0>();
+  meet();
+  rows.place(p, cur, tokens_lds);
+  rows.request(0, addr);
+  rows.request(min(1, p.KB - 1), addr + kTileSlot);
+  request_codes(cur, 0);
+  const uint8_t* w = weights_of(cur);
+  const auto weights = [&](i32x8 (&set)[2], int kb) {
+    set[0] = weight_frag(w + (int64_t)kb * kFp8Frag);
+    set[1] = weight_frag(w + (int64_t)(p.KB + kb) * kFp8Frag);
+  };
+  weights(wf[0], 0);
+  weights(wf[1], min(1, p.KB - 1));
+  request_weight_scales(cur, 0);
+  if (!FIRST) request_gates(cur, 0);
+  wait_vmcnt<0>();
+  meet();
+
+  uint32_t slot = 0, slot2 = 2 * kTileSlot;  // of the stage at hand, of the one two further on: byte offsets
+  int buffer = 0;                            // of the codes and gate weights
+  while (true) {
+    TileCoord nxt = sched.next();
+    const bool last = !nxt.valid;
+    if (last) nxt = cur;  // (requested again for nothing)
+    request_tokens(nxt);
+    // the largest of each row's values so far, for this tile's epilogue (the other buffer may still be read in the last one's)
+    if (FIRST) top_lds[buffer * kTileRows + wave * 32 + (fresh_lane() & 31)] = 0;
 
     const auto tile = [&](auto NAC) {
       constexpr int NA = decltype(NAC)::value;
@@ -239,150 +326,148 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < NA; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      for (int k0 = 0; k0 < p.KB; k0 += kTileChunk) {
-        const int blocks = min(kTileChunk, p.KB - k0);
-        __syncthreads();
-        rows.request(k0, addr);
-        // the scales of the chunk: the rows' in LDS, a row's by two threads, the weights' of block k0 + lane in a lane
-        {
-          constexpr int EACH = kTileChunk / 8;
-          const uint32_t* const from = (const uint32_t*)(p.codes + (int64_t)code_row * code_bytes + k0);
-          const int d0 = (tid & 1) * EACH, have = (blocks + 3) / 4;
-          uint32_t v[EACH];
-#pragma unroll
-          for (int d = 0; d < EACH; ++d) v[d] = from[min(d0 + d, have - 1)];
-#pragma unroll
-          for (int d = 0; d < EACH; ++d) codes_lds[(tid >> 1) * kCodePitch + d0 + d] = v[d];
+      const int end = stages - 2;
+      // Stage kb with register set B.  (The last two, which request the next tile's first ones, are not code of their own: apart, they
+      // cost the register allocation of the whole loop.)
+      const auto stage = [&](auto BC, int kb) {
+        constexpr int b = decltype(BC)::value;
+        if (kb == end) {  // `rows` and `w` are the next tile's from here on
+          if (end <= 1) {  // (later stages have met behind a wait of their own: the tokens are there)
+            wait_vmcnt<0>();
+            meet();
+          }
+          rows.place(p, nxt, tokens_lds);
+          w = weights_of(nxt);
         }
-        float ws[2];
-        {
-          const int64_t k = (int64_t)tc.expert * p.KB + k0 + min(l, blocks - 1);
-          ws[0] = FIRST ? p.w_scale[k * 2 * p.HB + pair / 8] : p.w_scale[k * p.DB + pair / 4];
-          ws[1] = FIRST ? p.w_scale[k * 2 * p.HB + p.HB + pair / 8] : ws[0];
-        }
-        i32x8 wf[2][2];
+        const int rk = min(kb < end ? kb + 2 : kb - end, p.KB - 1);
+        keep(wf[b][0]);
+        keep(wf[b][1]);
+        const int kc = min(kb, p.KB - 1);
+        // (a stage past the last block, where there is but one, counts for nothing)
+        const int live = kb < p.KB ? -1 : 0;
+        const float* const ws = scales_lds + 2 * buffer * kTileBlocks + kc;
+        const float s0 = __int_as_float(uniform(__float_as_int(ws[FIRST ? 0 : (wave >> 2) * kTileBlocks])) & live);
+        const float s1 = FIRST ? __int_as_float(uniform(__float_as_int(ws[kTileBlocks])) & live) : s0;
+        const uint8_t* const at = lds + slot;
+        const uint8_t* const my_codes = codes_lds + buffer * kTileCodes + (kc >> 2) * (kTileRows * 4) + (kc & 3) + (fresh_lane() & 15) * 4;
+        i32x8 rf[2];
+        int codes[2];
+        f32x4 t[2][2];
+        rf[0] = row_frag<kTileRows>(at, 0);
+        codes[0] = my_codes[0];
+        order_fence();
+        unrolled<0, NA>([&](auto IC) {
+          constexpr int i = decltype(IC)::value, c = i & 1;
+          keep(rf[c]);
+          if constexpr (i + 1 < NA) {
+            rf[c ^ 1] = row_frag<kTileRows>(at, i + 1);
+            codes[c ^ 1] = my_codes[64 * (i + 1)];
+          }
+          t[c][0] = mfma_e4m3<0>(wf[b][0], rf[c], codes[c]);
+          t[c][1] = mfma_e4m3<0>(wf[b][1], rf[c], codes[c]);
+          order_fence();
+          if constexpr (i > 0) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int64_t at = (int64_t)(k0 + min(b, blocks - 1)) * kFp8Frag;
-          wf[b][0] = weight_frag(w0 + at);
-          wf[b][1] = weight_frag(w1 + at);
-        }
-        wait_vmcnt<0>();
-        __syncthreads();
-        const uint32_t* const my_codes = codes_lds + (l & 15) * kCodePitch;
-        const auto stage = [&](auto BYTE, int kb) {
-          constexpr int byte = decltype(BYTE)::value, b = byte & 1;
-          if (kb > 0) {
-            // this stage's weights and rows have landed (what was requested after them: the weights of the next stage), for all
-            wait_vmcnt<4>();
+            for (int r = 0; r < 4; ++r) {
+              acc[0][i - 1][r] = fmaf(t[c ^ 1][0][r], s0, acc[0][i - 1][r]);
+              acc[1][i - 1][r] = fmaf(t[c ^ 1][1][r], s1, acc[1][i - 1][r]);
+            }
+            keep(acc[0][i - 1]);
+            keep(acc[1][i - 1]);
+          }
+          order_fence();
+          if constexpr (i == 1) {
+            // the rows of the next stage have landed (younger than they: its weights; of a tile's second stage they had
+            // before the last epilogue); every wavefront is past the stage before, whose slot the requests go to
+            if (kb > 0) wait_vmcnt<4>();
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
-          }
-          keep(wf[b][0]);
-          keep(wf[b][1]);
-          if (kb + 1 < blocks) rows.request(k0 + kb + 1, addr + (b ^ 1) * kTileSlot);
-          const float s0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws[0]), kb));
-          const float s1 = FIRST ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws[1]), kb)) : s0;
-          const uint8_t* const slot = lds + b * kTileSlot;
-          // row fragment i + 1 is on its way and the results of i - 1 are added while i is multiplied
-          i32x8 rf[2];
-          int codes[2];  // the four blocks' scales of the rows
-          f32x4 t[2][2];
-          int quad = kb / 4;
-          asm volatile("" : "+s"(quad));  // (read anew in each stage: kept, they were spilled)
-          rf[0] = row_frag<kTileRows>(slot, 0);
-          codes[0] = my_codes[quad];
-          order_fence();
-          unrolled<0, NA>([&](auto IC) {
-            constexpr int i = decltype(IC)::value, c = i & 1;
-            keep(rf[c]);
-            if constexpr (i + 1 < NA) {
-              rf[c ^ 1] = row_frag<kTileRows>(slot, i + 1);
-              codes[c ^ 1] = my_codes[16 * (i + 1) * kCodePitch + quad];
-            }
-            t[c][0] = mfma_e4m3<byte>(wf[b][0], rf[c], codes[c]);
-            t[c][1] = mfma_e4m3<byte>(wf[b][1], rf[c], codes[c]);
-            order_fence();
-            if constexpr (i > 0) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                acc[0][i - 1][r] = fmaf(t[c ^ 1][0][r], s0, acc[0][i - 1][r]);
-                acc[1][i - 1][r] = fmaf(t[c ^ 1][1][r], s1, acc[1][i - 1][r]);
-              }
-              keep(acc[0][i - 1]);
-              keep(acc[1][i - 1]);
+            rows.request(rk, addr + slot2);
+            if (kb == end) {
+              request_codes(nxt, buffer ^ 1);
+              request_weight_scales(nxt, buffer ^ 1);
+              if (!FIRST) request_gates(nxt, buffer ^ 1);
             }
             order_fence();
-          });
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            acc[0][NA - 1][r] = fmaf(t[(NA - 1) & 1][0][r], s0, acc[0][NA - 1][r]);
-            acc[1][NA - 1][r] = fmaf(t[(NA - 1) & 1][1][r], s1, acc[1][NA - 1][r]);
           }
-          const int64_t at = (int64_t)(k0 + min(kb + 2, blocks - 1)) * kFp8Frag;
-          wf[b][0] = weight_frag(w0 + at);
-          wf[b][1] = weight_frag(w1 + at);
-        };
-        // whole fours apart from the rest: behind a stage that may not run, the compiler waits for all that is on its way
-        int kb = 0;
+        });
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[0][NA - 1][r] = fmaf(t[(NA - 1) & 1][0][r], s0, acc[0][NA - 1][r]);
+          acc[1][NA - 1][r] = fmaf(t[(NA - 1) & 1][1][r], s1, acc[1][NA - 1][r]);
+        }
+        weights(wf[b], rk);
+        slot2 = slot;  // (free behind the next stage's barrier)
+        slot = slot == (kSlots - 1) * kTileSlot ? 0 : slot + kTileSlot;
+        order_fence();
+      };
+      int kb = 0;
 #pragma unroll 1
-        for (; kb + 4 <= blocks; kb += 4) {
-          stage(IntC<0>{}, kb);
-          stage(IntC<1>{}, kb + 1);
-          stage(IntC<2>{}, kb + 2);
-          stage(IntC<3>{}, kb + 3);
-        }
-        if (kb < blocks) {
-          stage(IntC<0>{}, kb);
-          if (kb + 1 < blocks) stage(IntC<1>{}, kb + 1);
-          if (kb + 2 < blocks) stage(IntC<2>{}, kb + 2);
-        }
+      for (; kb + 2 <= stages; kb += 2) {
+        stage(IntC<0>{}, kb);
+        stage(IntC<1>{}, kb + 1);
       }
-      const int l = fresh_lane();
+      if (kb < stages) stage(IntC<0>{}, kb);
+      wait_vmcnt<4>();  // the rows of the next tile's second stage
+      order_fence();
+
+      // Stores go at offsets from the tile's first row, and those past its last one are dropped.
+      const int l = fresh_lane(), r0 = l & 15, pair = cur.tn * kWaves + wave;
       if constexpr (FIRST) {
+        uint32_t* const top = top_lds + buffer * kTileRows + r0;
+        if (pair >= p.pairs) {  // columns past the last: zeros, up to a whole block
+#pragma unroll
+          for (int i = 0; i < NA; ++i) acc[0][i] = acc[1][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            acc[0][i][r] = real ? acc[0][i][r] * acc[1][i][r] * sigmoidf_fast(acc[1][i][r]) : 0.0f;
-            top = max(top, magnitude(acc[0][i][r]));
-          }
-          top = top_of_rows(top);
-          if (l < 16) top_lds[wave * kTileRows + 16 * i + l] = top;
+          acc[0][i] = swiglu(acc[0][i], acc[1][i]);
+          __hip_atomic_fetch_max(top + 16 * i, largest(acc[0][i][0], acc[0][i][1], acc[0][i][2], acc[0][i][3]), __ATOMIC_RELAXED,
+                                 __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-        __syncthreads();
+        meet();
+        const int row_bytes = p.HB * kFp8Block, code_row = fp8_code_bytes(p.HB);
+        const __amdgpu_buffer_rsrc_t h = buffer_of(p.hq + (int64_t)cur.row0 * row_bytes, cur.rows * row_bytes);
+        const __amdgpu_buffer_rsrc_t codes = buffer_of(p.h_codes + (int64_t)cur.row0 * code_row, wave == 0 ? cur.rows * code_row : 0);
+        int at = r0 * row_bytes + cur.tn * kFp8Block + wave * 16 + 4 * (l >> 4), code_at = r0 * code_row + cur.tn;
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-          const int r = 16 * i + (l & 15);
-          uint32_t top = 0;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) top = max(top, top_lds[w * kTileRows + r]);
-          const RowScale s(top);
-          if (r < tc.rows) {
-            const int64_t row = tc.row0 + r;
-            *(uint32_t*)(p.hq + (row * p.HB + tc.tn) * kFp8Block + wave * 16 + 4 * (l >> 4)) =
-                pack_e4m3(acc[0][i][0] * s.inverse, acc[0][i][1] * s.inverse, acc[0][i][2] * s.inverse, acc[0][i][3] * s.inverse);
-            if (wave == 0 && l < 16) p.h_codes[row * fp8_code_bytes(p.HB) + tc.tn] = (uint8_t)s.code;
-          }
+          const RowScale s(top[16 * i]);
+          __builtin_amdgcn_raw_buffer_store_b32(pack_e4m3(acc[0][i][0], acc[0][i][1], acc[0][i][2], acc[0][i][3], s.scale), h, at, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b8((uint8_t)s.code, codes, code_at, 0, 0);  // (the four lanes of a row the same)
+          at += 16 * row_bytes;
+          code_at += 16 * code_row;
         }
-      } else if (real) {
+      } else {
+        const __amdgpu_buffer_rsrc_t out = buffer_of(p.out + (int64_t)cur.row0 * p.D, pair < p.pairs ? cur.rows * p.D * 2 : 0);
+        int at = r0 * p.D * 2 + pair * 64 + 16 * (l >> 4);
+        const float* const gate = gate_lds + buffer * kTileRows + r0;
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-          const int r = 16 * i + (l & 15);
-          if (r >= tc.rows) continue;
-          const int64_t row = tc.row0 + r;
-          const float s = gate_lds[r];
-          store_packet(p, row, pair, l, acc[0][i], acc[1][i], s);
+          __builtin_amdgcn_raw_buffer_store_b128(Packet::of(acc[0][i], acc[1][i], gate[16 * i]).w, out, at, 0, 0);
+          at += 16 * p.D * 2;
         }
+        meet();  // (of two stages, the next tile's first one requests codes where this tile's have been read)
       }
     };
-    const int quads = __builtin_amdgcn_readfirstlane((tc.rows + 63) >> 6);
+    const int quads = __builtin_amdgcn_readfirstlane((cur.rows + 63) >> 6);
     if (quads == 4) tile(IntC<16>{});
     else if (quads == 3) tile(IntC<12>{});
     else if (quads == 2) tile(IntC<8>{});
     else tile(IntC<4>{});
+    if (last) break;
+    if (stages & 1) {  // the register sets have changed places
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const i32x8 other = wf[0][j];
+        wf[0][j] = wf[1][j];
+        wf[1][j] = other;
+      }
+    }
+    buffer ^= 1;
+    cur = nxt;
   }
+  wait_vmcnt<0>();  // nothing is on its way to LDS when the workgroup ends
 }
 
 // out[m] = the sum of its experts' rows, in fp32, in the order of the experts: packet 4 p + g of a row holds columns 32 p + 4 g .. +3
@@ -420,8 +505,11 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const u32x4* __restric
   }
 }
 
-// Whether a launch takes tiles of 256 rows: from an average of 48 rows an expert on (PROVISIONAL)
-bool takes_tiles(int64_t Msum, int64_t N) { return Msum >= 48 * N; }
+// Whether both products take tiles of 256 rows: from an average of 48 rows an expert on (PROVISIONAL), and for contractions of up
+// to kTileBlocks blocks
+bool takes_tiles(int64_t Msum, int64_t N, int64_t D, int64_t H) {
+  return Msum >= 48 * N && std::max(D, H) <= kTileBlocks * kFp8Block;
+}
 
 int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
   if (M <= 0 || D <= 0 || H <= 0 || N <= 0 || Msum <= 0) return MOMOE_ERR_BAD_ARG;
@@ -430,8 +518,8 @@ int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
   return MOMOE_OK;
 }
 template <bool FIRST>
-int launch_fp8(const Fp8Args& a, int64_t M, int64_t Msum, int64_t N, hipStream_t st) {
-  if (!takes_tiles(Msum, N)) {
+int launch_fp8(const Fp8Args& a, int64_t M, int64_t D, int64_t H, int64_t Msum, int64_t N, hipStream_t st) {
+  if (!takes_tiles(Msum, N, D, H)) {
     fp8_few_rows_kernel<FIRST><<<2 * persistent_grid(), kThreads, 0, st>>>(a);
     return launch_status();
   }
@@ -449,8 +537,8 @@ bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 using namespace momoe;
 
-extern "C" int momoe_fp8_tile_rows(int64_t Msum, int64_t N) {
-  return Msum <= 0 || N <= 0 ? 0 : takes_tiles(Msum, N) ? kTileRows : kFewRows;
+extern "C" int momoe_fp8_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N) {
+  return Msum <= 0 || D <= 0 || H <= 0 || N <= 0 ? 0 : takes_tiles(Msum, N, D, H) ? kTileRows : kFewRows;
 }
 
 extern "C" int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, const void* Wl1_packed, const float* Wl1_scale,
@@ -465,7 +553,7 @@ extern "C" int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, c
   a.h_codes = (uint8_t*)h_codes;
   a.HB = (int)fp8_blocks(H);
   a.msum = Msum;
-  return launch_fp8<true>(a, M, Msum, N, (hipStream_t)stream);
+  return launch_fp8<true>(a, M, D, H, Msum, N, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, const void* Wl2_packed, const float* Wl2_scale,
@@ -484,7 +572,7 @@ extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, co
   a.D = (int)D;
   a.DB = (int)fp8_blocks(D);
   a.msum = Msum;
-  return launch_fp8<false>(a, M, Msum, N, (hipStream_t)stream);
+  return launch_fp8<false>(a, M, D, H, Msum, N, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K,

@@ -27,16 +27,16 @@ __host__ __device__ inline int64_t fp8_blocks(int64_t n) { return (n + kFp8Block
 
 constexpr int fp8_code_bytes(int blocks) { return (blocks + 3) & ~3; }
 
-// The scale of values of which the largest has magnitude `amax`, as its code and its inverse; `amax` as bits, so that a NaN is the
-// largest of all.  NaN or infinity: the code of NaN, which makes NaN of every result that the values are part of.
+// The scale of values of which the largest has magnitude `amax`, and its code; `amax` as bits, so that a NaN is the largest of
+// all.  NaN or infinity: the code of NaN, which makes NaN of every result that the values are part of.
 struct RowScale {
   uint32_t code;
-  float inverse;
+  float scale;
   __device__ __forceinline__ explicit RowScale(uint32_t amax) {
     // 448 = 1.75 * 2^8: one binade more where the mantissa exceeds 1.75
     const uint32_t field = ((max(amax, kLeastAmax) + 0x1FFFFFu) >> 23) - 8;
     code = amax >= 0x7F800000u ? 255 : field;
-    inverse = __uint_as_float((254 - field) << 23);
+    scale = __uint_as_float(field << 23);
   }
 };
 __device__ __forceinline__ float scale_of_code(uint32_t code) { return __uint_as_float(code == 255 ? 0x7FC00000u : code << 23); }
@@ -47,9 +47,17 @@ struct LargerBits {
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
   }
 };
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+// the largest magnitude of four values, NaN if there is one, as bits: two instructions
+__device__ __forceinline__ uint32_t largest(float a, float b, float c, float d) {
+  const float three = __builtin_elementwise_maximum(__builtin_fabsf(a), __builtin_elementwise_maximum(__builtin_fabsf(b), __builtin_fabsf(c)));
+  return magnitude(__builtin_elementwise_maximum(three, __builtin_fabsf(d)));
+}
+// four values divided by `scale`, a power of two, and rounded to e4m3
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d, float scale) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  i16x2 v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, a, b, scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, v);
 }
 
 // first . second * the scales of the rows of `second`, byte BYTE of `codes` in the lanes of that row
@@ -77,19 +85,21 @@ __device__ __forceinline__ bf16x8 bf16_of_e4m3(uint32_t lo, uint32_t hi, float s
 // 2^-112 are zeros; an infinity or a NaN makes NaN of all eight.
 struct Packet {
   u32x4 w;
-  static __device__ __forceinline__ Packet of(const float (&v)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
-    uint32_t field = top >> 23;
-    const bool zero = field < 15, bad = field == 255;
-    const float unit = __uint_as_float((zero || bad ? 0 : 127 + 13 + 127 - field) << 23);  // 2^13 / 2^(field - 127)
-    field = zero ? 15 : field;
+  // of v * s
+  static __device__ __forceinline__ Packet of(const f32x4& a, const f32x4& b, float s) {
+    const uint32_t top = magnitude(__uint_as_float(max(largest(a[0], a[1], a[2], a[3]), largest(b[0], b[1], b[2], b[3]))) * s);
+    // (a value that would round up to 2^14 counts for the next binade)
+    const uint32_t binade = (top + 0x200) >> 23, field = max(binade, 15u);
+    // 2^13 / 2^(field - 127) * s; a sum with 1.5 * 2^23 has the rounded product in its lowest bits
+    const float unit = binade < 15 || binade == 255 ? 0.0f : __uint_as_float((127 + 13 + 127 - field) << 23) * s;
+    const auto rounded = [&](float v) { return __float_as_uint(fmaf(v, unit, 12582912.0f)); };
     Packet p;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int lo = min((int)rintf(v[2 * i] * unit), 16383), hi = min((int)rintf(v[2 * i + 1] * unit), 16383);
-      p.w[i] = (uint32_t)(lo << 1 & 0xFFFF) | (uint32_t)hi << 17 | (field >> i & 1) | (field >> (i + 4) & 1) << 16;
+      const f32x4& v = i < 2 ? a : b;
+      const uint32_t lo = rounded(v[2 * (i & 1)]), hi = rounded(v[2 * (i & 1) + 1]);
+      const uint32_t both = __builtin_amdgcn_perm(hi, lo, 0x05040100);  // the low half words of the two
+      p.w[i] = (both << 1 & 0xFFFEFFFEu) | (field >> i & 1) | (field >> (i + 4) & 1) << 16;
     }
     return p;
   }

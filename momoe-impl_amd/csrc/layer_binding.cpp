@@ -491,7 +491,7 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   x = x.contiguous();
   if ((uintptr_t)x.data_ptr() % 16 != 0) x = x.clone();
 
-  Index ib(M, N, K, momoe_fp8_tile_rows(msum, N), false);
+  Index ib(M, N, K, momoe_fp8_tile_rows(msum, D, H, N), false);
   const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
   const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
   const int64_t xq_bytes = M * DB * 128, xs_bytes = M * momoe_fp8_code_bytes(D), hq_bytes = msum * HB * 128,

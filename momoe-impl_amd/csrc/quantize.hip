@@ -34,9 +34,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     top = max(top, magnitude(v[i]));
   }
   const RowScale s(__float_as_uint(over_lanes<16>(__uint_as_float(top), LargerBits{})));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= s.inverse;
-  *(u32x2*)(q + row * (KB * kFp8Block) + c) = u32x2{pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7])};
+  *(u32x2*)(q + row * (KB * kFp8Block) + c) = u32x2{pack_e4m3(v[0], v[1], v[2], v[3], s.scale), pack_e4m3(v[4], v[5], v[6], v[7], s.scale)};
   if ((threadIdx.x & 15) == 0) code[row * fp8_code_bytes(KB) + kb] = (uint8_t)s.code;
 }
 
@@ -82,7 +80,7 @@ __global__ __launch_bounds__(256) void pack_weights_kernel(PackArgs p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *(uint32_t*)&tile[(tid >> 4) + 16 * i][c + 4 * h] =
-            pack_e4m3(v[i][4 * h] * s.inverse, v[i][4 * h + 1] * s.inverse, v[i][4 * h + 2] * s.inverse, v[i][4 * h + 3] * s.inverse);
+            pack_e4m3(v[i][4 * h], v[i][4 * h + 1], v[i][4 * h + 2], v[i][4 * h + 3], s.scale);
     if (tid == 0) p.scale[((e * KB + kb) * p.halves + half) * CB + cb] = scale_of_code(s.code);
   } else {
     const int c = (tid & 31) * 4;  // 32 lanes a row, four columns in each

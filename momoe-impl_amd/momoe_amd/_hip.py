@@ -90,7 +90,7 @@ _SIGNATURES = {
     "momoe_fp8_quantize_rows": (_int, [_p, _int, _i64, _i64, _i64, _p, _p, _p]),
     "momoe_fp8_weight_bytes": (_i64, [_i64] * 3),
     "momoe_fp8_pack_weights": (_int, [_p, _int, _i64, _i64, _i64, _int, _p, _p, _p]),
-    "momoe_fp8_tile_rows": (_int, [_i64, _i64]),
+    "momoe_fp8_tile_rows": (_int, [_i64] * 4),
     "momoe_fp8_lin1_swiglu_fwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
@@ -486,8 +486,8 @@ def fp8_pack_weights(W_NRC, halves):
     return packed if quantized else (packed, scale)
 
 
-def fp8_tile_rows(Msum, N):
-    return _lib.momoe_fp8_tile_rows(Msum, N)
+def fp8_tile_rows(Msum, D, H, N):
+    return _lib.momoe_fp8_tile_rows(Msum, D, H, N)
 
 
 def fp8_lin1_swiglu_fwd(x_q, x_codes, Wl1_packed, Wl1_scale, idx, table, D, H):

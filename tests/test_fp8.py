@@ -16,7 +16,10 @@ def test_sizes():
     assert [lib.momoe_fp8_code_bytes(n) for n in (0, 1, 512, 513, 2048)] == [-1, 4, 4, 8, 16]
     assert lib.momoe_fp8_weight_bytes(3, 200, 64) == 3 * 4 * 2 * 2048
     assert lib.momoe_fp8_weight_bytes(3, 200, 40) == lib.momoe_fp8_weight_bytes(0, 1, 16) == -1
-    assert lib.momoe_fp8_tile_rows(0, 8) == 0 and all(lib.momoe_fp8_tile_rows(m, 128) % 32 == 0 for m in (1, 1000, 10 ** 6))
+    rows = lib.momoe_fp8_tile_rows
+    assert rows(0, 64, 64, 8) == rows(1, 0, 64, 8) == rows(1, 64, 0, 8) == rows(1, 64, 64, 0) == 0
+    assert [rows(m, 2048, 768, 128) for m in (1, 8, 1000)] == [32] * 3 and rows(65536, 2048, 768, 128) == 256
+    assert rows(65536, 8224, 768, 128) == rows(65536, 768, 8224, 128) == 32  # contractions past what a tall tile holds the scales of
 
 
 def test_refusals_of_the_entry_points():
