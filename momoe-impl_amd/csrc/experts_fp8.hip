@@ -38,15 +38,15 @@ constexpr int kFewRows = 32, kFewChunk = 16;  // rows of a tile, blocks of the c
 // read cover all banks.
 __device__ __forceinline__ int row_piece_at(int r, int c) { return r * kFp8Block + ((c ^ ((r >> 1) & 7)) << 4); }
 
-// row fragment i of a block, lane l
-__device__ __forceinline__ i32x8 row_frag(const uint8_t* block, int l, int i) {
-  const int r = 16 * i + (l & 15), g = l >> 4;
+template <int ROWS>
+__device__ __forceinline__ i32x8 row_frag(const uint8_t* block, int i) {
+  const int l = threadIdx.x & 63, r = 16 * i + (l & 15), g = l >> 4;
   const u32x4 lo = *(const u32x4*)(block + row_piece_at(r, g)), hi = *(const u32x4*)(block + row_piece_at(r, 4 + g));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 __device__ __forceinline__ i32x8 weight_frag(const uint8_t* at) {
-  const uint32_t l = fresh_lane() * 16;  // (an offset beside a uniform address; hoisted, the sum takes registers of its own)
-  const u32x4 lo = *(const u32x4*)(at + l), hi = *(const u32x4*)(at + 1024 + l);
+  const uint32_t l = fresh_lane();  // (an offset beside a uniform address; hoisted, the sum takes registers of its own)
+  const u32x4 lo = *(const u32x4*)(at + l * 16), hi = *(const u32x4*)(at + (l * 16 + 1024));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
         }
 #pragma unroll
         for (int i = 0; i < FR; ++i) {
-          const i32x8 rq = row_frag(rows_lds + kb * (kFewRows * kFp8Block), l, i);
+          const i32x8 rq = row_frag<kFewRows>(rows_lds + kb * (kFewRows * kFp8Block), i);
           const float rs = scale_lds[kb][16 * i + (l & 15)];
           f32x4 t[2] = {};
 #pragma unroll
@@ -170,21 +170,16 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
 
 // Tiles of up to 256 rows x 256 columns, a persistent workgroup on a CU.  Each of its eight wavefronts owns 32 columns of all rows: it
 // reads their weights straight into registers, each byte once per workgroup; the rows come to LDS by direct transfers.  Both are
-// requested two stages of 128 k-values ahead, in four slots of LDS and two register sets, and the last two stages of a tile
+// requested two stages of 128 k-values ahead, in three slots of LDS and two register sets, and the last two stages of a tile
 // request the first two of the next one.
 //
-// A stage: the fragments of 16 rows travel from LDS one ahead of the products, the fp32 sums follow one behind them.  The two wavefronts
-// of a SIMD run half a stage apart, so that one multiplies while the other one is between stages: a barrier lies behind the first
-// rows of a stage of wavefronts 0 .. 3 and in the middle of the one before of wavefronts 4 .. 7.  With barrier n all rows of stage
-// n + 1 have landed, and the slot that those of stage n + 2 go to, that of stage n - 2, is free.
-constexpr int kTileRows = 256, kTileBlocks = 56;  // most blocks of a contraction: what is left of the LDS holds their codes
-constexpr int kTileSlot = kTileRows * kFp8Block, kSlots = 4;
-constexpr int kTileScales = (kTileBlocks + 63) / 64 * 64;  // of a set of the weights', whole transfers
-// The rows' codes come as [four blocks][row][block] bytes, a tile ahead, and are turned to [block][row % 16][row / 16]: those of a
-// lane's rows are then one read a stage, and its products take them from the bytes of four registers.
-constexpr int kTileCodes = kTileRows * kTileBlocks;
-constexpr int kTileLds = kSlots * kTileSlot + 2 * kTileCodes + 2 * kTileRows * 4 + 4 * kTileScales * 4 + kTileRows * 4;
-static_assert(kTileLds <= 160 << 10, "a CU's LDS");
+// A stage: the fragments of 16 rows travel from LDS one ahead of the products, the fp32 sums follow one behind them.  Its barrier lies
+// behind the first rows, not at its end: by then the next stage's rows have landed for every wavefront, and the slot of the
+// last one is free.
+constexpr int kTileRows = 256, kTileBlocks = 64;  // most blocks of a contraction
+constexpr int kTileSlot = kTileRows * kFp8Block, kSlots = 3;
+constexpr int kTileCodes = kTileRows * kTileBlocks;  // bytes: [four blocks][row][block]
+constexpr int kTileLds = kSlots * kTileSlot + 2 * kTileCodes + 2 * kTileRows * 4 + 4 * kTileBlocks * 4 + kTileRows * 4;
 
 // `v` is in its registers here: what it is made of lies before this point, what it goes into behind it.  (Without, the compiler
 // forms all products of a stage first and keeps them.)
@@ -238,14 +233,10 @@ struct TileRows {
       off[j] = src * (uint32_t)(p.KB * kFp8Block) + (((l & 7) ^ ((r >> 1) & 7)) << 4);
     }
   }
-  __device__ __forceinline__ const uint8_t* source(int kb) const { return uniform(base + (int64_t)kb * kFp8Block); }
-  template <int J>
-  __device__ __forceinline__ void request(const uint8_t* source, uint32_t slot) const {
-    dma16((const bf16*)source, off[J], slot + (J * kWaves + wave_id()) * 1024);
-  }
-  __device__ __forceinline__ void request_all(int kb, uint32_t slot) const {
-    const uint8_t* const from = source(kb);
-    unrolled<0, DEP>([&](auto JC) { request<decltype(JC)::value>(from, slot); });
+  __device__ __forceinline__ void request(int kb, uint32_t slot) const {
+    const bf16* const b = uniform((const bf16*)(base + (int64_t)kb * kFp8Block));
+#pragma unroll
+    for (int j = 0; j < DEP; ++j) dma16(b, off[j], slot + (j * kWaves + wave_id()) * 1024);
   }
 };
 
@@ -253,30 +244,26 @@ template <bool FIRST>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   uint8_t* const lds = (uint8_t*)dyn_lds();
   uint8_t* const codes_lds = lds + kSlots * kTileSlot;
-  uint8_t* const turned_lds = codes_lds + kTileCodes;
-  uint32_t* const top_lds = (uint32_t*)(turned_lds + kTileCodes);  // [2][row]
-  float* const gate_lds = (float*)top_lds;                         // of the second product: [2][row]
-  float* const scales_lds = (float*)(top_lds + 2 * kTileRows);     // [2][set][block]
-  int32_t* const tokens_lds = (int32_t*)(scales_lds + 4 * kTileScales);
+  uint32_t* const top_lds = (uint32_t*)(codes_lds + 2 * kTileCodes);  // [2][row]
+  float* const gate_lds = (float*)top_lds;                            // of the second product: [2][row]
+  float* const scales_lds = (float*)(top_lds + 2 * kTileRows);        // [2][set][block]
+  int32_t* const tokens_lds = (int32_t*)(scales_lds + 4 * kTileBlocks);
   const uint32_t addr = lds_address(dyn_lds()), codes_addr = addr + kSlots * kTileSlot, gates_addr = codes_addr + 2 * kTileCodes;
-  const uint32_t scales_addr = gates_addr + 2 * kTileRows * 4, tokens_addr = scales_addr + 4 * kTileScales * 4;
+  const uint32_t scales_addr = gates_addr + 2 * kTileRows * 4, tokens_addr = scales_addr + 4 * kTileBlocks * 4;
   const int wave = wave_id(), stages = max(p.KB, 2), code_bytes = fp8_code_bytes(p.KB);
   TileSchedT<1> sched(p.table, (p.pairs + kWaves - 1) / kWaves, kTileRows);
-  const bool second = wave >= 4;             // of the two wavefronts of a SIMD
   TileCoord cur = sched.next();
   if (!cur.valid) return;
-  auto entry = sched.fetch();  // (of the table, a tile ahead of its use)
 
   const auto pair_of = [&](const TileCoord& tc) { return min(tc.tn * kWaves + wave, p.pairs - 1); };
   const auto weights_of = [&](const TileCoord& tc) { return p.w + ((int64_t)tc.expert * p.pairs + pair_of(tc)) * 2 * p.KB * kFp8Frag; };
   // The scales of a tile's weights, block by block, one set of two a wavefront (and again by others): of the two halves; of the two
   // blocks of columns
   const auto request_weight_scales = [&](const TileCoord& tc, int to) {
-    const int set = wave & 1, pitch = FIRST ? 2 * p.HB : p.DB;
-    const float* const base = p.w_scale + (int64_t)uniform(tc.expert) * p.KB * pitch +
+    const int set = wave & 1, k = min(fresh_lane(), p.KB - 1);
+    const float* const base = p.w_scale + (int64_t)uniform(tc.expert) * p.KB * (FIRST ? 2 * p.HB : p.DB) +
                               (FIRST ? set * p.HB + uniform(tc.tn) : min(2 * uniform(tc.tn) + set, p.DB - 1));
-    for (int k = 0; k < p.KB; k += 64)
-      dma4(uniform(base), min(k + fresh_lane(), p.KB - 1) * pitch * 4, scales_addr + ((2 * to + set) * kTileScales + k) * 4);
+    dma4(uniform(base), k * (FIRST ? 2 * p.HB : p.DB) * 4, scales_addr + (2 * to + set) * (kTileBlocks * 4));
   };
   // the tokens of a tile's rows, the last one's for those that it does not have: 64 of them a wavefront, and again by another one
   const auto request_tokens = [&](const TileCoord& tc) {
@@ -285,22 +272,13 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   };
   // The codes of its rows: four blocks of 64 rows a transfer, as many transfers in every wavefront
   const int dwords = code_bytes / 4;
-  const auto request_codes = [&](const TileCoord& tc) {
+  const auto request_codes = [&](const TileCoord& tc, int to) {
     const uint8_t* const base = FIRST ? p.codes : p.codes + (int64_t)uniform(tc.row0) * code_bytes;
     const int q = wave & 3, r = q * 64 + fresh_lane();
     const uint32_t src = FIRST ? tokens_lds[r] : min(r, tc.rows - 1);
     for (int n = 0; n < dwords; n += 2) {
       const int d = min(n + wave / 4, dwords - 1);
-      dma4(uniform(base + 4 * d), src * (uint32_t)code_bytes, codes_addr + (d * kTileRows + q * 64) * 4);
-    }
-  };
-  const auto turn_codes = [&] {
-    const int tid = wave * 64 + fresh_lane(), r = tid & (kTileRows - 1);
-    for (int d = tid / kTileRows; d < dwords; d += 2) {
-      const uint32_t v = ((const uint32_t*)codes_lds)[d * kTileRows + r];
-      uint8_t* const to = turned_lds + 4 * d * kTileRows + (r & 15) * 16 + (r >> 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) to[e * kTileRows] = (uint8_t)(v >> (8 * e));
+      dma4(uniform(base + 4 * d), src * (uint32_t)code_bytes, codes_addr + to * kTileCodes + (d * kTileRows + q * 64) * 4);
     }
   };
   // the gate weights of its rows
@@ -316,64 +294,30 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   wait_vmcnt<0>();
   meet();
   rows.place(p, cur, tokens_lds);
-  rows.request_all(0, addr);
-  rows.request_all(min(1, p.KB - 1), addr + kTileSlot);
-  request_codes(cur);
-  const uint8_t* w = weights_of(cur);  // what is to be requested next
-  const int w_step = p.KB > 1 ? kFp8Frag : 0;
-  const int64_t w_second = (int64_t)p.KB * kFp8Frag;
-  const auto weights = [&](i32x8 (&set)[2]) {
-    set[0] = weight_frag(w);
-    set[1] = weight_frag(w + w_second);
-    w += w_step;
+  rows.request(0, addr);
+  rows.request(min(1, p.KB - 1), addr + kTileSlot);
+  request_codes(cur, 0);
+  const uint8_t* w = weights_of(cur);
+  const auto weights = [&](i32x8 (&set)[2], int kb) {
+    set[0] = weight_frag(w + (int64_t)kb * kFp8Frag);
+    set[1] = weight_frag(w + (int64_t)(p.KB + kb) * kFp8Frag);
   };
-  weights(wf[0]);
-  weights(wf[1]);
+  weights(wf[0], 0);
+  weights(wf[1], min(1, p.KB - 1));
   request_weight_scales(cur, 0);
   if (!FIRST) request_gates(cur, 0);
   wait_vmcnt<0>();
   meet();
-  turn_codes();
-  meet();
 
-  uint32_t slot = 0, slot2 = 2 * kTileSlot;  // of the stage at hand, of the next requests: byte offsets
-  const auto behind = [](uint32_t at) { return at + kTileSlot & (kSlots * kTileSlot - 1); };
+  uint32_t slot = 0, slot2 = 2 * kTileSlot;  // of the stage at hand, of the one two further on: byte offsets
   int buffer = 0;                            // of the codes and gate weights
   while (true) {
-    TileCoord nxt = sched.resolve(entry);
-    entry = sched.fetch();
+    TileCoord nxt = sched.next();
     const bool last = !nxt.valid;
     if (last) nxt = cur;  // (requested again for nothing)
     request_tokens(nxt);
     // the largest of each row's values so far, for this tile's epilogue (the other buffer may still be read in the last one's)
     if (FIRST) top_lds[buffer * kTileRows + wave * 32 + (fresh_lane() & 31)] = 0;
-
-    const int end = stages - 2;
-    if (end == 0) {  // (otherwise the tokens are there behind barrier 1, before they are wanted)
-      wait_vmcnt<0>();
-      meet();
-    }
-    // barrier n, and, in parts, what is requested behind it
-    const uint8_t* rows_from;
-    const auto step = [&](int n) {
-      if (n > 0) wait_vmcnt<4>();  // (younger than the rows: the next weights; those of barrier 0 had landed before the last epilogue)
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      if (n == end) {  // the last two stages' requests are the next tile's
-        rows.place(p, nxt, tokens_lds);
-        request_codes(nxt);
-        request_weight_scales(nxt, buffer ^ 1);
-        if (!FIRST) request_gates(nxt, buffer ^ 1);
-      }
-      rows_from = rows.source(min(n < end ? n + 2 : n - end, p.KB - 1));
-      order_fence();
-    };
-    const auto request = [&](auto JC) {
-      constexpr int j = decltype(JC)::value;
-      rows.template request<j>(rows_from, addr + slot2);
-      if constexpr (j + 1 == TileRows<FIRST>::DEP) slot2 = behind(slot2);
-      order_fence();
-    };
 
     const auto tile = [&](auto NAC) {
       constexpr int NA = decltype(NAC)::value;
@@ -382,77 +326,81 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < NA; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const int end = stages - 2;
       // Stage kb with register set B.  (The last two, which request the next tile's first ones, are not code of their own: apart, they
       // cost the register allocation of the whole loop.)
       const auto stage = [&](auto BC, int kb) {
         constexpr int b = decltype(BC)::value;
-        const int kc = min(kb, p.KB - 1), l = fresh_lane();
-        const float* const ws = scales_lds + 2 * buffer * kTileScales + kc;
-        const float v0 = ws[FIRST ? 0 : (wave >> 2) * kTileScales], v1 = FIRST ? ws[kTileScales] : 0.0f;
-        const uint8_t* const at = lds + slot;
-        // Row fragments travel two ahead of the products; a product's results are added behind the second one after it.
-        constexpr int RING = 3, LAG = 2, NM = 2 * NA;
-        i32x8 rf[RING];
-        f32x4 t[LAG + 1];
-        u32x4 codes = *(const u32x4*)(turned_lds + kc * kTileRows + (l & 15) * 16);
-        unrolled<0, RING - 1>([&](auto IC) { rf[decltype(IC)::value] = row_frag(at, l, decltype(IC)::value); });
+        if (kb == end) {  // `rows` and `w` are the next tile's from here on
+          if (end <= 1) {  // (later stages have met behind a wait of their own: the tokens are there)
+            wait_vmcnt<0>();
+            meet();
+          }
+          rows.place(p, nxt, tokens_lds);
+          w = weights_of(nxt);
+        }
+        const int rk = min(kb < end ? kb + 2 : kb - end, p.KB - 1);
         keep(wf[b][0]);
         keep(wf[b][1]);
+        const int kc = min(kb, p.KB - 1);
         // (a stage past the last block, where there is but one, counts for nothing)
         const int live = kb < p.KB ? -1 : 0;
-        float s0 = 0.0f, s1 = 0.0f;
-        const auto add = [&](auto MC) {
-          constexpr int m = decltype(MC)::value, i = m / 2, j = m % 2;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(t[m % (LAG + 1)][r], j ? s1 : s0, acc[j][i][r]);
-          keep(acc[j][i]);
-        };
-        keep(codes);
+        const float* const ws = scales_lds + 2 * buffer * kTileBlocks + kc;
+        const float s0 = __int_as_float(uniform(__float_as_int(ws[FIRST ? 0 : (wave >> 2) * kTileBlocks])) & live);
+        const float s1 = FIRST ? __int_as_float(uniform(__float_as_int(ws[kTileBlocks])) & live) : s0;
+        const uint8_t* const at = lds + slot;
+        const uint8_t* const my_codes = codes_lds + buffer * kTileCodes + (kc >> 2) * (kTileRows * 4) + (kc & 3) + (fresh_lane() & 15) * 4;
+        i32x8 rf[2];
+        int codes[2];
+        f32x4 t[2][2];
+        rf[0] = row_frag<kTileRows>(at, 0);
+        codes[0] = my_codes[0];
         order_fence();
         unrolled<0, NA>([&](auto IC) {
-          constexpr int i = decltype(IC)::value, g = i % RING;
-          keep(rf[g]);
-          if constexpr (i + RING - 1 < NA) rf[(i + RING - 1) % RING] = row_frag(at, l, i + RING - 1);
+          constexpr int i = decltype(IC)::value, c = i & 1;
+          keep(rf[c]);
+          if constexpr (i + 1 < NA) {
+            rf[c ^ 1] = row_frag<kTileRows>(at, i + 1);
+            codes[c ^ 1] = my_codes[64 * (i + 1)];
+          }
+          t[c][0] = mfma_e4m3<0>(wf[b][0], rf[c], codes[c]);
+          t[c][1] = mfma_e4m3<0>(wf[b][1], rf[c], codes[c]);
           order_fence();
-          unrolled<0, 2>([&](auto JC) {
-            constexpr int j = decltype(JC)::value, m = 2 * i + j;
-            t[m % (LAG + 1)] = mfma_e4m3<i % 4>(wf[b][j], rf[g], codes[i / 4]);
-            order_fence();
-            if constexpr (m >= LAG) add(IntC<m - LAG>{});
-            order_fence();
-          });
-          if constexpr (i == 0) {
-            s0 = __int_as_float(uniform(__float_as_int(v0)) & live);
-            s1 = FIRST ? __int_as_float(uniform(__float_as_int(v1)) & live) : s0;
-          }
-          // a transfer behind each of the rows that follow the barrier, as far as there are any
-          constexpr int A = 0, B = NA / 2;
-          if constexpr (i == A) {
-            if (!second) step(kb);
-          }
-          if constexpr (i == B) {
-            if (second && kb + 1 < stages) step(kb + 1);
-          }
-          unrolled<0, TileRows<FIRST>::DEP>([&](auto JC) {
-            constexpr int j = decltype(JC)::value, last_of = NA / 2 - 1;
-            if constexpr (i == A + (j + 1 < last_of ? j + 1 : last_of)) {
-              if (!second) request(JC);
+          if constexpr (i > 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[0][i - 1][r] = fmaf(t[c ^ 1][0][r], s0, acc[0][i - 1][r]);
+              acc[1][i - 1][r] = fmaf(t[c ^ 1][1][r], s1, acc[1][i - 1][r]);
             }
-            if constexpr (i == B + (j + 1 < last_of ? j + 1 : last_of)) {
-              if (second && kb + 1 < stages) request(JC);
+            keep(acc[0][i - 1]);
+            keep(acc[1][i - 1]);
+          }
+          order_fence();
+          if constexpr (i == 1) {
+            // the rows of the next stage have landed (younger than they: its weights; of a tile's second stage they had
+            // before the last epilogue); every wavefront is past the stage before, whose slot the requests go to
+            if (kb > 0) wait_vmcnt<4>();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            rows.request(rk, addr + slot2);
+            if (kb == end) {
+              request_codes(nxt, buffer ^ 1);
+              request_weight_scales(nxt, buffer ^ 1);
+              if (!FIRST) request_gates(nxt, buffer ^ 1);
             }
-          });
+            order_fence();
+          }
         });
-        unrolled<NM - LAG, NM>(add);
-        if (kb == end) w = weights_of(nxt);
-        weights(wf[b]);
-        slot = behind(slot);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[0][NA - 1][r] = fmaf(t[(NA - 1) & 1][0][r], s0, acc[0][NA - 1][r]);
+          acc[1][NA - 1][r] = fmaf(t[(NA - 1) & 1][1][r], s1, acc[1][NA - 1][r]);
+        }
+        weights(wf[b], rk);
+        slot2 = slot;  // (free behind the next stage's barrier)
+        slot = slot == (kSlots - 1) * kTileSlot ? 0 : slot + kTileSlot;
         order_fence();
       };
-      if (second) {
-        step(0);
-        unrolled<0, TileRows<FIRST>::DEP>(request);
-      }
       int kb = 0;
 #pragma unroll 1
       for (; kb + 2 <= stages; kb += 2) {
@@ -518,9 +466,6 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
     }
     buffer ^= 1;
     cur = nxt;
-    // (behind the epilogue's barrier the last tile's codes are done with; the next tile's had landed by then)
-    turn_codes();
-    meet();
   }
   wait_vmcnt<0>();  // nothing is on its way to LDS when the workgroup ends
 }

@@ -87,19 +87,22 @@ struct Packet {
   u32x4 w;
   // of v * s
   static __device__ __forceinline__ Packet of(const f32x4& a, const f32x4& b, float s) {
-    const uint32_t top = magnitude(__uint_as_float(max(largest(a[0], a[1], a[2], a[3]), largest(b[0], b[1], b[2], b[3]))) * s);
+    const auto larger = [](float x, float y, float z) {  // (NaN if there is one)
+      return __builtin_elementwise_maximum(__builtin_fabsf(x), __builtin_elementwise_maximum(__builtin_fabsf(y), __builtin_fabsf(z)));
+    };
+    const float all = __builtin_elementwise_maximum(larger(b[2], b[3], larger(a[0], a[1], a[2])), larger(a[3], b[0], b[1]));
     // (a value that would round up to 2^14 counts for the next binade)
-    const uint32_t binade = (top + 0x200) >> 23, field = max(binade, 15u);
+    const uint32_t binade = (magnitude(all * s) + 0x200) >> 23, field = max(binade, 15u);
     // 2^13 / 2^(field - 127) * s; a sum with 1.5 * 2^23 has the rounded product in its lowest bits
-    const float unit = binade < 15 || binade == 255 ? 0.0f : __uint_as_float((127 + 13 + 127 - field) << 23) * s;
+    const float unit = binade - 15 >= 255 - 15 ? 0.0f : __uint_as_float((127 + 13 + 127 - field) << 23) * s;
     const auto rounded = [&](float v) { return __float_as_uint(fmaf(v, unit, 12582912.0f)); };
+    const uint32_t spread = field | field << 12;  // bit i of the field in bit i, bit i + 4 in bit 16 + i
     Packet p;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const f32x4& v = i < 2 ? a : b;
-      const uint32_t lo = rounded(v[2 * (i & 1)]), hi = rounded(v[2 * (i & 1) + 1]);
-      const uint32_t both = __builtin_amdgcn_perm(hi, lo, 0x05040100);  // the low half words of the two
-      p.w[i] = (both << 1 & 0xFFFEFFFEu) | (field >> i & 1) | (field >> (i + 4) & 1) << 16;
+      const uint32_t both = __builtin_amdgcn_perm(rounded(v[2 * (i & 1) + 1]), rounded(v[2 * (i & 1)]), 0x05040100);  // the low half words
+      p.w[i] = (0x10001u & spread >> i) | (~0x10001u & both << 1);
     }
     return p;
   }

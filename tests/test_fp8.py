@@ -19,7 +19,7 @@ def test_sizes():
     rows = lib.momoe_fp8_tile_rows
     assert rows(0, 64, 64, 8) == rows(1, 0, 64, 8) == rows(1, 64, 0, 8) == rows(1, 64, 64, 0) == 0
     assert [rows(m, 2048, 768, 128) for m in (1, 8, 1000)] == [32] * 3 and rows(65536, 2048, 768, 128) == 256
-    assert rows(65536, 7200, 768, 128) == rows(65536, 768, 7200, 128) == 32  # contractions past what a tall tile holds the scales of
+    assert rows(65536, 8224, 768, 128) == rows(65536, 768, 8224, 128) == 32  # contractions past what a tall tile holds the scales of
 
 
 def test_refusals_of_the_entry_points():
