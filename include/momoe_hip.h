@@ -465,8 +465,21 @@ int64_t momoe_fp8_weight_bytes(int64_t N, int64_t R, int64_t C);
 int momoe_fp8_pack_weights(const void* W_NRC, int quantized, int64_t N, int64_t R, int64_t C, int halves, void* packed, float* scale,
                            void* stream);
 
-/* Tile height of the table that suits both products below. */
+/* Tile height of the table for both products, whichever suits the sizes: MOMOE_FP8_FEW_ROWS for the two entry points momoe_fp8_few_*,
+ * 256 for the other two, whose contractions are of up to 8192. */
+#define MOMOE_FP8_FEW_ROWS 32
 int momoe_fp8_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N);
+/* momoe_fp8_few_lin1_swiglu_fwd: h fp32 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i].  x: MOMOE_TYPE_*, row pitch ldx, a
+ * multiple of 8; its rows are brought to 8 bits on the way.
+ * momoe_fp8_few_lin2_scale_fwd: as momoe_fp8_lin2_scale_fwd, from that h, brought to 8 bits on the way.
+ * x, h, weights and packets on 16-byte boundaries. */
+int momoe_fp8_few_lin1_swiglu_fwd(const void* x, int type, int64_t ldx, const void* Wl1_packed, const float* Wl1_scale,
+                                  const int32_t* idx_Msum, const int32_t* tile_table, float* h_MsumH, int64_t M,
+                                  int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);
+int momoe_fp8_few_lin2_scale_fwd(const float* h_MsumH, const void* Wl2_packed, const float* Wl2_scale, const float* s_NM,
+                                 int64_t s_stride_n, int64_t s_stride_m, const int32_t* idx_Msum,
+                                 const int32_t* tile_table, void* ys_packets, int64_t M, int64_t D, int64_t H,
+                                 int64_t N, int64_t Msum, void* stream);
 /* momoe_fp8_lin1_swiglu_fwd: h = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i], brought to 8 bits from fp32.
  * x_q, x_codes: rows of x [M][D]; h_q, h_codes: rows of h [Msum][H]; codes on 4-byte boundaries, the others on
  * 16-byte ones.  tile_table: of momoe_index_build for

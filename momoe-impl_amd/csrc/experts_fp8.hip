@@ -32,15 +32,13 @@ struct Fp8Args {
   int64_t msum;
 };
 
-constexpr int kFewRows = 32, kFewChunk = 16;  // rows of a tile, blocks of the contraction whose rows are in LDS
-
-// LDS of a chunk: [block][row][128], the 16-byte piece c of row r at position c ^ ((r / 2) % 8): the 16 rows x 16 bytes that 16 lanes
-// read cover all banks.
+// LDS of a block's rows: [row][128], the 16-byte piece c of row r at position c ^ ((r / 2) % 8): the 16 rows x 16 bytes that 16 lanes
+// of a fragment read cover all banks.
 __device__ __forceinline__ int row_piece_at(int r, int c) { return r * kFp8Block + ((c ^ ((r >> 1) & 7)) << 4); }
 
-template <int ROWS>
-__device__ __forceinline__ i32x8 row_frag(const uint8_t* block, int i) {
-  const int l = threadIdx.x & 63, r = 16 * i + (l & 15), g = l >> 4;
+// row fragment i of a block, lane l
+__device__ __forceinline__ i32x8 row_frag(const uint8_t* block, int l, int i) {
+  const int r = 16 * i + (l & 15), g = l >> 4;
   const u32x4 lo = *(const u32x4*)(block + row_piece_at(r, g)), hi = *(const u32x4*)(block + row_piece_at(r, 4 + g));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
@@ -48,13 +46,6 @@ __device__ __forceinline__ i32x8 weight_frag(const uint8_t* at) {
   const uint32_t l = fresh_lane();  // (an offset beside a uniform address; hoisted, the sum takes registers of its own)
   const u32x4 lo = *(const u32x4*)(at + l * 16), hi = *(const u32x4*)(at + (l * 16 + 1024));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-}
-
-// the largest of the four lanes that hold a row
-__device__ __forceinline__ uint32_t top_of_rows(uint32_t v) {
-  const auto larger = [](auto pair) { return (uint32_t)max((uint32_t)pair[0], (uint32_t)pair[1]); };
-  v = larger(__builtin_amdgcn_permlane16_swap(v, v, false, false));
-  return larger(__builtin_amdgcn_permlane32_swap(v, v, false, false));
 }
 
 // a * b * sigmoid(b)
@@ -65,57 +56,103 @@ __device__ __forceinline__ f32x4 swiglu(const f32x4& a, const f32x4& b) {
   return h;
 }
 
-// Tiles of up to 32 rows: a wavefront owns a pair of 16-column groups (of the first product one of each half) and streams
-// their weights; the rows of the tile lie in LDS.
-template <bool FIRST>
-__global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
-  constexpr int FR = kFewRows / 16;
-  __shared__ __attribute__((aligned(16))) uint8_t rows_lds[kFewChunk * kFewRows * kFp8Block];
+// Tiles of up to 32 rows: launches that stream their weights.  A wavefront multiplies a pair of 16-column groups (of the first product
+// one of each half), their weights straight into registers, kFewAhead blocks of 128 k-values ahead.  KS wavefronts share a pair's
+// contraction, a block in KS each, and their sums meet in LDS: one token has few columns to spread over the CUs.  The tile's rows
+// are brought to 8 bits by the workgroup that multiplies them, which has the first weights on their way meanwhile: a few rows read
+// again for each block of columns, against a launch before either product.
+//
+// Products in bf16 (fp8.hpp): the conversions and the slower products hide behind the stream.
+constexpr int kFewRows = MOMOE_FP8_FEW_ROWS, kFewChunk = 16, kFewAhead = 4;  // rows of a tile; blocks whose rows are in LDS
+
+struct FewArgs {
+  const void* rows;      // [M or Msum][ld]
+  int64_t ld;
+  const uint8_t* w;
+  const float* w_scale;
+  const int32_t *idx, *table;
+  int K, KB, pairs;      // contraction, its blocks; pairs of 16-column groups
+  float* h;              // first product: [Msum][H]
+  int H, HB;
+  const float* s;        // second product
+  int64_t sn, sm;
+  uint16_t* out;         // [Msum][D / 8] packets
+  int D, DB;
+};
+
+template <bool FIRST, class X, int KS>
+__global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
+  constexpr int FR = kFewRows / 16, PW = kWaves / KS;
+  __shared__ __attribute__((aligned(16))) uint8_t rows_lds[kFewChunk * kFewRows * kFp8Block];  // then the sums of KS wavefronts
   __shared__ float scale_lds[kFewChunk][kFewRows];
-  __shared__ uint32_t top_lds[kWaves][kFewRows];
-  const int tid = threadIdx.x, l = tid & 63, wave = wave_id();
-  TileSchedT<1> sched(p.table, (p.pairs + kWaves - 1) / kWaves, kFewRows);
+  static_assert(kWaves * 64 * 4 * FR * 2 * 4 <= (int)sizeof(rows_lds), "16 sums a lane");
+  const int tid = threadIdx.x, l = tid & 63, wave = wave_id(), kw = wave % KS, cw = wave / KS;
+  TileSchedT<1> sched(p.table, (p.pairs + PW - 1) / PW, kFewRows);
   for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
-    const int pair = min(tc.tn * kWaves + wave, p.pairs - 1);
-    const bool real = tc.tn * kWaves + wave < p.pairs;
+    const int pair = min(tc.tn * PW + cw, p.pairs - 1);
+    const bool real = tc.tn * PW + cw < p.pairs, two = tc.rows > 16;
     const uint8_t* const w0 = p.w + ((int64_t)tc.expert * p.pairs + pair) * 2 * p.KB * kFp8Frag;
     const uint8_t* const w1 = w0 + (int64_t)p.KB * kFp8Frag;
     f32x4 acc[2][FR] = {};
     for (int k0 = 0; k0 < p.KB; k0 += kFewChunk) {
-      const int blocks = min(kFewChunk, p.KB - k0);
-      __syncthreads();
-      for (int q = tid; q < blocks * kFewRows * 8; q += kThreads) {
-        const int c = q & 7, r = (q >> 3) % kFewRows, kb = q / (8 * kFewRows);
-        const int row = tc.row0 + min(r, tc.rows - 1);
-        const int64_t src = FIRST ? p.idx[row] : row;
-        *(u32x4*)(rows_lds + kb * (kFewRows * kFp8Block) + row_piece_at(r, c)) =
-            *(const u32x4*)(p.rows + (src * p.KB + k0 + kb) * kFp8Block + c * 16);
+      const int blocks = min(kFewChunk, p.KB - k0), steps = (blocks - kw + KS - 1) / KS;  // (none for a wavefront past the last)
+      i32x8 wq[kFewAhead][2];
+      const auto load = [&](int q, int step) {
+        const int64_t at = (int64_t)(k0 + step * KS + kw) * kFp8Frag;
+        wq[q][0] = weight_frag(w0 + at);
+        wq[q][1] = weight_frag(w1 + at);
+      };
+      unrolled<0, kFewAhead>([&](auto QC) {
+        if (decltype(QC)::value < steps) load(decltype(QC)::value, decltype(QC)::value);
+      });
+      // the weights' scales, of block k0 + lane in a lane
+      float ws[2];
+      {
+        const int64_t k = (int64_t)tc.expert * p.KB + k0 + min(l, blocks - 1);
+        ws[0] = FIRST ? p.w_scale[k * 2 * p.HB + pair / 8] : p.w_scale[k * p.DB + pair / 4];
+        ws[1] = FIRST ? p.w_scale[k * 2 * p.HB + p.HB + pair / 8] : ws[0];
       }
-      for (int q = tid; q < blocks * kFewRows; q += kThreads) {
-        const int r = q % kFewRows, kb = q / kFewRows, row = tc.row0 + min(r, tc.rows - 1);
-        const int64_t src = FIRST ? p.idx[row] : row;
-        scale_lds[kb][r] = scale_of_code(p.codes[src * fp8_code_bytes(p.KB) + k0 + kb]);
+      __syncthreads();  // (the last rows, or sums, are done with)
+      // sixteen lanes a block of a row, two of them at once; rows that the tile does not have are its last one
+      const int have = min(kFewRows, (tc.rows + 15) & ~15), all = blocks * have;
+      for (int q0 = tid >> 4; q0 < all; q0 += 2 * (kThreads / 16)) {
+        constexpr int AT_ONCE = 2;
+        float v[AT_ONCE][8];
+#pragma unroll
+        for (int a = 0; a < AT_ONCE; ++a) {
+          const int q = min(q0 + a * (kThreads / 16), all - 1), r = q % have, c = (k0 + q / have) * kFp8Block + (l & 15) * 8;
+          const int row = tc.row0 + min(r, tc.rows - 1);
+          load8((const X*)p.rows + (int64_t)(FIRST ? p.idx[row] : row) * p.ld + min(c, p.K - 8), v[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < AT_ONCE; ++a) {
+          const int q = min(q0 + a * (kThreads / 16), all - 1), r = q % have, kb = q / have, c = (k0 + kb) * kFp8Block + (l & 15) * 8;
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[a][e] = c < p.K ? v[a][e] : 0.0f;
+            top = max(top, magnitude(v[a][e]));
+          }
+          const RowScale s(__float_as_uint(over_lanes<16>(__uint_as_float(top), LargerBits{})));
+          *(u32x2*)(rows_lds + kb * (kFewRows * kFp8Block) + row_piece_at(r, (l & 15) >> 1) + (l & 1) * 8) =
+              u32x2{pack_e4m3(v[a][0], v[a][1], v[a][2], v[a][3], s.scale), pack_e4m3(v[a][4], v[a][5], v[a][6], v[a][7], s.scale)};
+          if ((l & 15) == 0) scale_lds[kb][r] = scale_of_code(s.code);
+        }
       }
       __syncthreads();
-      for (int kb = 0; kb < blocks; ++kb) {
-        const int k = k0 + kb;
-        const i32x8 wq[2] = {weight_frag(w0 + (int64_t)k * kFp8Frag), weight_frag(w1 + (int64_t)k * kFp8Frag)};
+      const auto multiply = [&](int q, int step) {
+        const int kb = step * KS + kw;
+        const float s0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws[0]), kb));
+        const float s1 = FIRST ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws[1]), kb)) : s0;
         bf16x8 wf[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) wf[j][m] = bf16_of_e4m3(wq[j][2 * m], wq[j][2 * m + 1], 1.0f);
-        float ws[2];
-        if (FIRST) {
-          const float* at = p.w_scale + ((int64_t)tc.expert * p.KB + k) * 2 * p.HB + pair / 8;
-          ws[0] = load_uniform(at);
-          ws[1] = load_uniform(at + p.HB);
-        } else {
-          ws[0] = ws[1] = load_uniform(p.w_scale + ((int64_t)tc.expert * p.KB + k) * p.DB + pair / 4);
-        }
-#pragma unroll
-        for (int i = 0; i < FR; ++i) {
-          const i32x8 rq = row_frag<kFewRows>(rows_lds + kb * (kFewRows * kFp8Block), i);
+          for (int m = 0; m < 4; ++m) wf[j][m] = bf16_of_e4m3(wq[q][j][2 * m], wq[q][j][2 * m + 1], 1.0f);
+        unrolled<0, FR>([&](auto IC) {
+          constexpr int i = decltype(IC)::value;
+          if (i > 0 && !two) return;  // (wave-uniform)
+          const i32x8 rq = row_frag(rows_lds + kb * (kFewRows * kFp8Block), l, i);
           const float rs = scale_lds[kb][16 * i + (l & 15)];
           f32x4 t[2] = {};
 #pragma unroll
@@ -125,45 +162,54 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(Fp8Args p) {
             for (int j = 0; j < 2; ++j) t[j] = mfma16(wf[j][m], rf, t[j]);
           }
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int r = 0; r < 4; ++r) {
+            acc[0][i][r] = fmaf(t[0][r], s0, acc[0][i][r]);
+            acc[1][i][r] = fmaf(t[1][r], s1, acc[1][i][r]);
+          }
+        });
+      };
+      // what is multiplied last has nothing to request: apart, as behind a request that may not be made the compiler waits for all
+      int step = 0;
+#pragma unroll 1
+      for (; step + 2 * kFewAhead <= steps; step += kFewAhead)
+        unrolled<0, kFewAhead>([&](auto QC) {
+          constexpr int q = decltype(QC)::value;
+          multiply(q, step + q);
+          load(q, step + q + kFewAhead);
+        });
+      unrolled<0, kFewAhead>([&](auto QC) {
+        constexpr int q = decltype(QC)::value;
+        if (step + q < steps) multiply(q, step + q);
+        if (step + q + kFewAhead < steps) load(q, step + q + kFewAhead);
+      });
+      unrolled<0, kFewAhead>([&](auto QC) {
+        constexpr int q = decltype(QC)::value;
+        if (step + q + kFewAhead < steps) multiply(q, step + q + kFewAhead);
+      });
+    }
+    if constexpr (KS > 1) {
+      __syncthreads();
+      f32x4* const sums = (f32x4*)rows_lds + wave * (2 * FR) * 64 + l;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(t[j][r], ws[j], acc[j][i][r]);
-        }
+      for (int n = 0; n < 2 * FR; ++n) sums[n * 64] = acc[n / FR][n % FR];
+      __syncthreads();
+      if (kw == 0) {
+#pragma unroll
+        for (int n = 0; n < 2 * FR; ++n)
+#pragma unroll
+          for (int k = 1; k < KS; ++k) acc[n / FR][n % FR] += sums[(k * (2 * FR) + n) * 64];
       }
     }
-    if (FIRST) {
-      // h of 16 columns in each wavefront; the eight of a workgroup hold a block of 128
-      f32x4 h[FR];
+    if (!real || kw != 0) continue;
 #pragma unroll
-      for (int i = 0; i < FR; ++i) {
-        h[i] = real ? swiglu(acc[0][i], acc[1][i]) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const uint32_t top = top_of_rows(largest(h[i][0], h[i][1], h[i][2], h[i][3]));
-        if (l < 16) top_lds[wave][16 * i + l] = top;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < FR; ++i) {
-        const int r = 16 * i + (l & 15);
-        uint32_t top = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = max(top, top_lds[w][r]);
-        const RowScale s(top);
-        if (r < tc.rows) {
-          const int64_t row = tc.row0 + r;
-          *(uint32_t*)(p.hq + (row * p.HB + tc.tn) * kFp8Block + wave * 16 + 4 * (l >> 4)) =
-              pack_e4m3(h[i][0], h[i][1], h[i][2], h[i][3], s.scale);
-          if (wave == 0 && l < 16) p.h_codes[row * fp8_code_bytes(p.HB) + tc.tn] = (uint8_t)s.code;
-        }
-      }
-    } else if (real) {
-#pragma unroll
-      for (int i = 0; i < FR; ++i) {
-        const int r = 16 * i + (l & 15);
-        if (r >= tc.rows) continue;
-        const int64_t row = tc.row0 + r;
-        const float s = p.s[tc.expert * p.sn + p.idx[row] * p.sm];
-        *(u32x4*)(p.out + row * p.D + 32 * pair + 8 * (l >> 4)) = Packet::of(acc[0][i], acc[1][i], s).w;
-      }
+    for (int i = 0; i < FR; ++i) {
+      const int r = 16 * i + (l & 15);
+      if (r >= tc.rows) continue;
+      const int64_t row = tc.row0 + r;
+      if (FIRST)
+        *(f32x4*)(p.h + row * p.H + 16 * pair + 4 * (l >> 4)) = swiglu(acc[0][i], acc[1][i]);
+      else
+        *(u32x4*)(p.out + row * p.D + 32 * pair + 8 * (l >> 4)) = Packet::of(acc[0][i], acc[1][i], p.s[tc.expert * p.sn + p.idx[row] * p.sm]).w;
     }
   }
 }
@@ -348,19 +394,20 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
         const float* const ws = scales_lds + 2 * buffer * kTileBlocks + kc;
         const float s0 = __int_as_float(uniform(__float_as_int(ws[FIRST ? 0 : (wave >> 2) * kTileBlocks])) & live);
         const float s1 = FIRST ? __int_as_float(uniform(__float_as_int(ws[kTileBlocks])) & live) : s0;
+        const int l = fresh_lane();
         const uint8_t* const at = lds + slot;
-        const uint8_t* const my_codes = codes_lds + buffer * kTileCodes + (kc >> 2) * (kTileRows * 4) + (kc & 3) + (fresh_lane() & 15) * 4;
+        const uint8_t* const my_codes = codes_lds + buffer * kTileCodes + (kc >> 2) * (kTileRows * 4) + (kc & 3) + (l & 15) * 4;
         i32x8 rf[2];
         int codes[2];
         f32x4 t[2][2];
-        rf[0] = row_frag<kTileRows>(at, 0);
+        rf[0] = row_frag(at, l, 0);
         codes[0] = my_codes[0];
         order_fence();
         unrolled<0, NA>([&](auto IC) {
           constexpr int i = decltype(IC)::value, c = i & 1;
           keep(rf[c]);
           if constexpr (i + 1 < NA) {
-            rf[c ^ 1] = row_frag<kTileRows>(at, i + 1);
+            rf[c ^ 1] = row_frag(at, l, i + 1);
             codes[c ^ 1] = my_codes[64 * (i + 1)];
           }
           t[c][0] = mfma_e4m3<0>(wf[b][0], rf[c], codes[c]);
@@ -518,16 +565,22 @@ int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
   return MOMOE_OK;
 }
 template <bool FIRST>
-int launch_fp8(const Fp8Args& a, int64_t M, int64_t D, int64_t H, int64_t Msum, int64_t N, hipStream_t st) {
-  if (!takes_tiles(Msum, N, D, H)) {
-    fp8_few_rows_kernel<FIRST><<<2 * persistent_grid(), kThreads, 0, st>>>(a);
-    return launch_status();
-  }
+int launch_tiles(const Fp8Args& a, int64_t M, int64_t D, int64_t H, int64_t Msum, int64_t N, hipStream_t st) {
   // the rows of the first product are gathered at 32-bit offsets
-  if (FIRST && M * a.KB * kFp8Block >= (1ll << 32)) return MOMOE_ERR_UNSUPPORTED;
+  if (std::max(D, H) > kTileBlocks * kFp8Block || (FIRST && M * a.KB * kFp8Block >= (1ll << 32))) return MOMOE_ERR_UNSUPPORTED;
   static LdsLimit limit;
   if (!allow_lds(fp8_tile_kernel<FIRST>, kTileLds, limit)) return MOMOE_ERR_LAUNCH;
   fp8_tile_kernel<FIRST><<<persistent_grid(), kThreads, kTileLds, st>>>(a);
+  return launch_status();
+}
+// As many wavefronts to a pair's contraction as give every CU two workgroups, had each expert that may hold a row one tile
+template <bool FIRST, class X>
+int launch_few(const FewArgs& a, int64_t Msum, int64_t N, hipStream_t st) {
+  const int64_t experts = std::min(N, Msum), wanted = 2 * persistent_grid();
+  const auto enough = [&](int ks) { return a.KB < 2 * ks || experts * cdiv64(a.pairs, kWaves / ks) >= wanted; };
+  auto kernel = enough(1) ? fp8_few_rows_kernel<FIRST, X, 1> : enough(2) ? fp8_few_rows_kernel<FIRST, X, 2>
+              : enough(4) ? fp8_few_rows_kernel<FIRST, X, 4> : fp8_few_rows_kernel<FIRST, X, 8>;
+  kernel<<<(unsigned)wanted, kThreads, 0, st>>>(a);
   return launch_status();
 }
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -553,7 +606,7 @@ extern "C" int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, c
   a.h_codes = (uint8_t*)h_codes;
   a.HB = (int)fp8_blocks(H);
   a.msum = Msum;
-  return launch_fp8<true>(a, M, D, H, Msum, N, (hipStream_t)stream);
+  return launch_tiles<true>(a, M, D, H, Msum, N, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, const void* Wl2_packed, const float* Wl2_scale,
@@ -572,7 +625,43 @@ extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, co
   a.D = (int)D;
   a.DB = (int)fp8_blocks(D);
   a.msum = Msum;
-  return launch_fp8<false>(a, M, D, H, Msum, N, (hipStream_t)stream);
+  return launch_tiles<false>(a, M, D, H, Msum, N, (hipStream_t)stream);
+}
+
+extern "C" int momoe_fp8_few_lin1_swiglu_fwd(const void* x, int type, int64_t ldx, const void* Wl1_packed, const float* Wl1_scale,
+                                             const int32_t* idx_Msum, const int32_t* tile_table, float* h_MsumH, int64_t M,
+                                             int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream) {
+  if (!x || !Wl1_packed || !Wl1_scale || !idx_Msum || !tile_table || !h_MsumH || ldx < D) return MOMOE_ERR_BAD_ARG;
+  if (type != MOMOE_TYPE_BF16 && type != MOMOE_TYPE_F32 && type != MOMOE_TYPE_F16) return MOMOE_ERR_BAD_ARG;
+  const int st = check_fp8(M, D, H, N, Msum);
+  if (st != MOMOE_OK) return st;
+  if (unaligned16(x) || unaligned16(Wl1_packed) || unaligned16(h_MsumH)) return MOMOE_ERR_BAD_ARG;
+  if (ldx % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
+  FewArgs a{x, ldx, (const uint8_t*)Wl1_packed, Wl1_scale, idx_Msum, tile_table, (int)D, (int)fp8_blocks(D), (int)(H / 16)};
+  a.h = h_MsumH;
+  a.H = (int)H;
+  a.HB = (int)fp8_blocks(H);
+  hipStream_t to = (hipStream_t)stream;
+  return type == MOMOE_TYPE_BF16 ? launch_few<true, bf16>(a, Msum, N, to)
+         : type == MOMOE_TYPE_F32 ? launch_few<true, float>(a, Msum, N, to) : launch_few<true, _Float16>(a, Msum, N, to);
+}
+
+extern "C" int momoe_fp8_few_lin2_scale_fwd(const float* h_MsumH, const void* Wl2_packed, const float* Wl2_scale, const float* s_NM,
+                                            int64_t s_stride_n, int64_t s_stride_m, const int32_t* idx_Msum,
+                                            const int32_t* tile_table, void* ys_packets, int64_t M, int64_t D, int64_t H,
+                                            int64_t N, int64_t Msum, void* stream) {
+  if (!h_MsumH || !Wl2_packed || !Wl2_scale || !s_NM || !idx_Msum || !tile_table || !ys_packets) return MOMOE_ERR_BAD_ARG;
+  const int st = check_fp8(M, D, H, N, Msum);
+  if (st != MOMOE_OK) return st;
+  if (unaligned16(h_MsumH) || unaligned16(Wl2_packed) || unaligned16(ys_packets)) return MOMOE_ERR_BAD_ARG;
+  FewArgs a{h_MsumH, H, (const uint8_t*)Wl2_packed, Wl2_scale, idx_Msum, tile_table, (int)H, (int)fp8_blocks(H), (int)(D / 32)};
+  a.s = s_NM;
+  a.sn = s_stride_n;
+  a.sm = s_stride_m;
+  a.out = (uint16_t*)ys_packets;
+  a.D = (int)D;
+  a.DB = (int)fp8_blocks(D);
+  return launch_few<false, float>(a, Msum, N, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K,

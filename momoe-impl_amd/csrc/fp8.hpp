@@ -41,6 +41,18 @@ struct RowScale {
 };
 __device__ __forceinline__ float scale_of_code(uint32_t code) { return __uint_as_float(code == 255 ? 0x7FC00000u : code << 23); }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// eight consecutive values on a 16-byte boundary
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  struct alignas(16) Vec { T t[16 / sizeof(T)]; };
+#pragma unroll
+  for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) {
+    const Vec w = ((const Vec*)p)[i];
+#pragma unroll
+    for (int e = 0; e < (int)(16 / sizeof(T)); ++e) v[i * (16 / sizeof(T)) + e] = (float)w.t[e];
+  }
+}
+
 // the larger of two magnitudes, for reductions over lanes
 struct LargerBits {
   __device__ __forceinline__ float operator()(float a, float b) const {

@@ -492,12 +492,13 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   if ((uintptr_t)x.data_ptr() % 16 != 0) x = x.clone();
 
   Index ib(M, N, K, momoe_fp8_tile_rows(msum, D, H, N), false);
+  const bool few = ib.tile_rows == MOMOE_FP8_FEW_ROWS;  // the products bring their rows to 8 bits themselves
   const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
   const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
-  const int64_t xq_bytes = M * DB * 128, xs_bytes = M * momoe_fp8_code_bytes(D), hq_bytes = msum * HB * 128,
-                hs_bytes = msum * momoe_fp8_code_bytes(H);
-  Transients transients(dev, {index_bytes, scratch_bytes, xq_bytes, xs_bytes, hq_bytes, hs_bytes, msum * D * 2});
-  Tensor index_own, scratch, xq_own, xs_own, hq_own, hs_own, ys_own, counter;
+  const int64_t xq_bytes = few ? 0 : M * DB * 128, xs_bytes = few ? 0 : M * momoe_fp8_code_bytes(D);
+  const int64_t h_bytes = few ? msum * H * 4 : msum * HB * 128, hs_bytes = few ? 0 : msum * momoe_fp8_code_bytes(H);
+  Transients transients(dev, {index_bytes, scratch_bytes, xq_bytes, xs_bytes, h_bytes, hs_bytes, msum * D * 2});
+  Tensor index_own, scratch, xq_own, xs_own, h_own, hs_own, ys_own, counter;
   ib.base = (int32_t*)transients.take(index_bytes, index_own);
   int32_t* const build = (int32_t*)transients.take(scratch_bytes, scratch);
   int32_t* violations = build;
@@ -508,15 +509,26 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   MOMOE_CALL(momoe_index_build, st, mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), M, N, K, sizes.data_ptr<int64_t>(),
              ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), (int)ib.tile_rows, (int32_t*)nullptr,
              (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
-  void* const xq = transients.take(xq_bytes, xq_own);
-  void* const xs = transients.take(xs_bytes, xs_own);
-  MOMOE_CALL(momoe_fp8_quantize_rows, st, x.data_ptr(), type_of(x.scalar_type()), D, M, D, xq, xs);
-  void* const hq = transients.take(hq_bytes, hq_own);
-  void* const hs = transients.take(hs_bytes, hs_own);
-  MOMOE_CALL(momoe_fp8_lin1_swiglu_fwd, st, xq, xs, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(), hq, hs, M, D, H, N, msum);
-  void* const ys = transients.take(msum * D * 2, ys_own);
-  MOMOE_CALL(momoe_fp8_lin2_scale_fwd, st, hq, hs, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0), s.stride(1),
-             ib.idx(), ib.table(), ys, M, D, H, N, msum);
+  void *h, *ys;
+  const int type = type_of(x.scalar_type());
+  if (few) {
+    h = transients.take(h_bytes, h_own);
+    MOMOE_CALL(momoe_fp8_few_lin1_swiglu_fwd, st, x.data_ptr(), type, D, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(),
+               (float*)h, M, D, H, N, msum);
+    ys = transients.take(msum * D * 2, ys_own);
+    MOMOE_CALL(momoe_fp8_few_lin2_scale_fwd, st, (const float*)h, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0),
+               s.stride(1), ib.idx(), ib.table(), ys, M, D, H, N, msum);
+  } else {
+    void* const xq = transients.take(xq_bytes, xq_own);
+    void* const xs = transients.take(xs_bytes, xs_own);
+    MOMOE_CALL(momoe_fp8_quantize_rows, st, x.data_ptr(), type, D, M, D, xq, xs);
+    h = transients.take(h_bytes, h_own);
+    void* const hs = transients.take(hs_bytes, hs_own);
+    MOMOE_CALL(momoe_fp8_lin1_swiglu_fwd, st, xq, xs, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(), h, hs, M, D, H, N, msum);
+    ys = transients.take(msum * D * 2, ys_own);
+    MOMOE_CALL(momoe_fp8_lin2_scale_fwd, st, h, hs, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0), s.stride(1),
+               ib.idx(), ib.table(), ys, M, D, H, N, msum);
+  }
   MOMOE_CALL(momoe_fp8_combine, st, ys, ib.inv(), y.data_ptr(), M, D, K, msum);
   if (check) {
     const int v = counter.narrow(0, 0, 1).item<int32_t>();

@@ -6,17 +6,6 @@ namespace {
 
 typedef _Float16 f16;
 
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  struct alignas(16) Vec { T t[16 / sizeof(T)]; };
-#pragma unroll
-  for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) {
-    const Vec w = ((const Vec*)p)[i];
-#pragma unroll
-    for (int e = 0; e < (int)(16 / sizeof(T)); ++e) v[i * (16 / sizeof(T)) + e] = (float)w.t[e];
-  }
-}
-
 // Sixteen lanes a block of 128 values, eight in each.  Bound by HBM, the values read once.
 template <class T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int KB,

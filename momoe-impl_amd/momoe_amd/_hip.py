@@ -93,6 +93,8 @@ _SIGNATURES = {
     "momoe_fp8_tile_rows": (_int, [_i64] * 4),
     "momoe_fp8_lin1_swiglu_fwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_fp8_few_lin1_swiglu_fwd": (_int, [_p, _int, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_fp8_few_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_bias_update": (_int, [_p, ctypes.c_float, ctypes.c_float, _i64, _p, _p]),
 }
@@ -506,6 +508,26 @@ def fp8_lin2_scale_fwd(h_q, h_codes, Wl2_packed, Wl2_scale, s_NM, idx, table, D,
     ys = torch.empty((Msum, D // 8, 4), dtype=torch.int32, device=h_q.device)
     _call("momoe_fp8_lin2_scale_fwd", _ptr(h_q), _ptr(h_codes), _ptr(Wl2_packed), _ptr(Wl2_scale), _ptr(s_NM), s_NM.stride(0),
           s_NM.stride(1), _ptr(idx), _ptr(table), _ptr(ys), M, D, H, N, Msum, _stream())
+    return ys
+
+
+def fp8_few_lin1_swiglu_fwd(x, Wl1_packed, Wl1_scale, idx, table, H):
+    """x [M, D] -> h fp32 [Msum, H], by tiles of MOMOE_FP8_FEW_ROWS rows."""
+    assert x.dim() == 2 and x.stride(1) == 1
+    (M, D), N, Msum = x.shape, Wl1_scale.shape[0], idx.numel()
+    h = torch.empty((Msum, H), dtype=torch.float32, device=x.device)
+    _call("momoe_fp8_few_lin1_swiglu_fwd", _ptr(x), _TYPES[x.dtype], x.stride(0), _ptr(Wl1_packed), _ptr(Wl1_scale), _ptr(idx),
+          _ptr(table), _ptr(h), M, D, H, N, Msum, _stream())
+    return h
+
+
+def fp8_few_lin2_scale_fwd(h, Wl2_packed, Wl2_scale, s_NM, idx, table, D):
+    """As fp8_lin2_scale_fwd, from that h."""
+    (N, M), (Msum, H) = s_NM.shape, h.shape
+    assert h.is_contiguous()
+    ys = torch.empty((Msum, D // 8, 4), dtype=torch.int32, device=h.device)
+    _call("momoe_fp8_few_lin2_scale_fwd", _ptr(h), _ptr(Wl2_packed), _ptr(Wl2_scale), _ptr(s_NM), s_NM.stride(0), s_NM.stride(1),
+          _ptr(idx), _ptr(table), _ptr(ys), M, D, H, N, Msum, _stream())
     return ys
 
 

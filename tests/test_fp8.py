@@ -43,6 +43,16 @@ def test_refusals_of_the_entry_points():
     assert all(lin2(**{k: None}) == 1 for k in ("h", "hc", "W", "S", "s", "idx", "table", "ys"))
     assert all(lin2(**{k: 0}) == 1 for k in ("M", "D", "H", "N", "Msum")) and all(lin2(**{k: P + 8}) == 1 for k in ("h", "W", "ys"))
     assert lin2(hc=P + 2) == 1 and lin2(D=48) == lin2(H=40) == 2
+    few1 = dict(x=P, t=0, ld=64, W=P, S=P, idx=P, table=P, h=P, M=16, D=64, H=32, N=8, Msum=32)
+    lin1 = lambda **c: lib.momoe_fp8_few_lin1_swiglu_fwd(*{**few1, **c}.values(), None)
+    assert all(lin1(**{k: None}) == 1 for k in ("x", "W", "S", "idx", "table", "h"))
+    assert all(lin1(**{k: 0}) == 1 for k in ("M", "D", "H", "N", "Msum")) and all(lin1(**{k: P + 8}) == 1 for k in ("x", "W", "h"))
+    assert lin1(t=3) == lin1(t=-1) == lin1(ld=56) == 1 and lin1(ld=68) == lin1(D=48) == lin1(H=40) == lin1(Msum=1 << 31) == 2
+    few2 = {k: v for k, v in two.items() if k != "hc"}
+    lin2 = lambda **c: lib.momoe_fp8_few_lin2_scale_fwd(*{**few2, **c}.values(), None)
+    assert all(lin2(**{k: None}) == 1 for k in ("h", "W", "S", "s", "idx", "table", "ys"))
+    assert all(lin2(**{k: 0}) == 1 for k in ("M", "D", "H", "N", "Msum")) and all(lin2(**{k: P + 8}) == 1 for k in ("h", "W", "ys"))
+    assert lin2(D=48) == lin2(H=40) == 2
     c = lambda **k: lib.momoe_fp8_combine(*{**dict(ys=P, inv=P, out=P, M=4, D=64, K=2, Msum=8), **k}.values(), None)
     assert all(c(**{k: None}) == 1 for k in ("ys", "inv", "out")) and all(c(**{k: 0}) == 1 for k in ("M", "D", "K", "Msum"))
     assert c(ys=P + 8) == c(out=P + 8) == 1 and c(D=48) == c(M=1 << 31) == 2

@@ -107,7 +107,7 @@ SIZES = [
     (64, 64, 2208, 2, 2, 1, 0), (200, 128, 128, 16, 2, 0, 1.5),
     (300, 96, 64, 4, 2, 0, 0), (517, 288, 160, 5, 2, 1, 0), (700, 128, 416, 4, 3, 1, 2.0), (900, 640, 96, 3, 1, 0, 0),
     (150, 8320, 32, 2, 1, 0, 0), (140, 32, 8320, 2, 1, 0, 0), (150, 8192, 384, 2, 1, 0, 0), (200, 384, 1056, 3, 1, 0, 0), (700, 4224, 4192, 3, 2, 0, 0), (130, 7200, 64, 2, 1, 0, 0),
-    (60, 128, 8192, 1, 1, 0, 0), (9000, 64, 1280, 6, 2, 0, 0.5), (7000, 512, 288, 20, 2, 0, 0.5),
+    (60, 128, 8192, 1, 1, 0, 0), (2, 8224, 2112, 12, 3, 0, 0), (90, 1056, 1024, 40, 4, 0, 0), (33, 2080, 160, 1, 1, 0, 0), (9000, 64, 1280, 6, 2, 0, 0.5), (7000, 512, 288, 20, 2, 0, 0.5),
 ]
 
 
@@ -139,12 +139,18 @@ def test_products(M, D, H, N, K, Ks, skew):
     assert torch.equal(index["idx_Msum"].cpu().long(), tok)
     xq, xc = _hip.fp8_quantize_rows(_x(M, D).to(DEV))
     p1, p2 = _hip.fp8_pack_weights(W1.to(DEV), 2), _hip.fp8_pack_weights(W2.to(DEV), 1)
-    hq, hc = _hip.fp8_lin1_swiglu_fwd(xq, xc, p1, S1.to(DEV), index["idx_Msum"], index["tile_table"], D, H)
+    at = index["idx_Msum"], index["tile_table"]
+    sd = s.T.contiguous().to(DEV).T
+    if tile_rows == 32:  # the products bring their rows to 8 bits themselves
+        h32 = _hip.fp8_few_lin1_swiglu_fwd(_x(M, D).to(DEV), p1, S1.to(DEV), *at, H)
+        hq, hc = _hip.fp8_quantize_rows(h32)
+        ys = _hip.fp8_few_lin2_scale_fwd(h32, p2, S2.to(DEV), sd, *at, D)
+    else:
+        hq, hc = _hip.fp8_lin1_swiglu_fwd(xq, xc, p1, S1.to(DEV), *at, D, H)
+        ys = _hip.fp8_lin2_scale_fwd(hq, hc, p2, S2.to(DEV), sd, *at, D, H)
     assert torch.equal(hq.view(torch.uint8)[:, H:], torch.zeros_like(hq.view(torch.uint8)[:, H:]))
     xv, hv = _dequantized(xq, xc, D)[tok], _dequantized(hq, hc, H)
     codes = hc.cpu().long()[:, :hq.shape[1] // 128].repeat_interleave(128, 1)[:, :H]
-    sd = s.T.contiguous().to(DEV).T
-    ys = _hip.fp8_lin2_scale_fwd(hq, hc, p2, S2.to(DEV), sd, index["idx_Msum"], index["tile_table"], D, H)
     y = _hip.fp8_combine(ys, index["inv_MK"], D).cpu().double()
     tiles = tile_rows == 256
     total, slack = torch.zeros(M, D, dtype=torch.float64), torch.zeros(M, D, dtype=torch.float64)
