@@ -42,9 +42,10 @@ __device__ __forceinline__ i32x8 row_frag(const uint8_t* block, int l, int i) {
   const u32x4 lo = *(const u32x4*)(block + row_piece_at(r, g)), hi = *(const u32x4*)(block + row_piece_at(r, 4 + g));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
+template <bool ONCE>
 __device__ __forceinline__ i32x8 weight_frag(const uint8_t* at) {
   const uint32_t l = fresh_lane();  // (an offset beside a uniform address; hoisted, the sum takes registers of its own)
-  const u32x4 lo = *(const u32x4*)(at + l * 16), hi = *(const u32x4*)(at + (l * 16 + 1024));
+  const u32x4 lo = load_maybe_once<ONCE>((const u32x4*)(at + l * 16)), hi = load_maybe_once<ONCE>((const u32x4*)(at + (l * 16 + 1024)));
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
@@ -63,7 +64,7 @@ __device__ __forceinline__ f32x4 swiglu(const f32x4& a, const f32x4& b) {
 // again for each block of columns, against a launch before either product.
 //
 // Products in bf16 (fp8.hpp): the conversions and the slower products hide behind the stream.
-constexpr int kFewRows = MOMOE_FP8_FEW_ROWS, kFewChunk = 16, kFewAhead = 4;  // rows of a tile; blocks whose rows are in LDS
+constexpr int kFewRows = MOMOE_FP8_FEW_ROWS, kFewChunk = 16, kFewAhead = 4, kRowsAtOnce = 2;
 
 struct FewArgs {
   const void* rows;      // [M or Msum][ld]
@@ -80,7 +81,7 @@ struct FewArgs {
   int D, DB;
 };
 
-template <bool FIRST, class X, int KS>
+template <bool FIRST, bool ONCE, class X, int KS>
 __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
   constexpr int FR = kFewRows / 16, PW = kWaves / KS;
   __shared__ __attribute__((aligned(16))) uint8_t rows_lds[kFewChunk * kFewRows * kFp8Block];  // then the sums of KS wavefronts
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
       i32x8 wq[kFewAhead][2];
       const auto load = [&](int q, int step) {
         const int64_t at = (int64_t)(k0 + step * KS + kw) * kFp8Frag;
-        wq[q][0] = weight_frag(w0 + at);
-        wq[q][1] = weight_frag(w1 + at);
+        wq[q][0] = weight_frag<ONCE>(w0 + at);
+        wq[q][1] = weight_frag<ONCE>(w1 + at);
       };
       unrolled<0, kFewAhead>([&](auto QC) {
         if (decltype(QC)::value < steps) load(decltype(QC)::value, decltype(QC)::value);
@@ -113,20 +114,26 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
         ws[1] = FIRST ? p.w_scale[k * 2 * p.HB + p.HB + pair / 8] : ws[0];
       }
       __syncthreads();  // (the last rows, or sums, are done with)
-      // sixteen lanes a block of a row, two of them at once; rows that the tile does not have are its last one
-      const int have = min(kFewRows, (tc.rows + 15) & ~15), all = blocks * have;
-      for (int q0 = tid >> 4; q0 < all; q0 += 2 * (kThreads / 16)) {
-        constexpr int AT_ONCE = 2;
-        float v[AT_ONCE][8];
+      // sixteen lanes a block of a row.  (What is left in LDS for rows that the tile does not have meets columns that nobody reads.)
+      const int all = blocks * tc.rows;
+      for (int q0 = tid >> 4; q0 < all; q0 += kRowsAtOnce * (kThreads / 16)) {
+        float v[kRowsAtOnce][8];
+        const auto place = [&](int a, int& r, int& kb) {
+          const int q = min(q0 + a * (kThreads / 16), all - 1);
+          kb = q / tc.rows;
+          r = q - kb * tc.rows;
+          return (k0 + kb) * kFp8Block + (l & 15) * 8;
+        };
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-          const int q = min(q0 + a * (kThreads / 16), all - 1), r = q % have, c = (k0 + q / have) * kFp8Block + (l & 15) * 8;
-          const int row = tc.row0 + min(r, tc.rows - 1);
+        for (int a = 0; a < kRowsAtOnce; ++a) {
+          int r, kb;
+          const int c = place(a, r, kb), row = tc.row0 + r;
           load8((const X*)p.rows + (int64_t)(FIRST ? p.idx[row] : row) * p.ld + min(c, p.K - 8), v[a]);
         }
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-          const int q = min(q0 + a * (kThreads / 16), all - 1), r = q % have, kb = q / have, c = (k0 + kb) * kFp8Block + (l & 15) * 8;
+        for (int a = 0; a < kRowsAtOnce; ++a) {
+          int r, kb;
+          const int c = place(a, r, kb);
           uint32_t top = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -286,7 +293,7 @@ struct TileRows {
   }
 };
 
-template <bool FIRST>
+template <bool FIRST, bool ONCE>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   uint8_t* const lds = (uint8_t*)dyn_lds();
   uint8_t* const codes_lds = lds + kSlots * kTileSlot;
@@ -345,8 +352,8 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Fp8Args p) {
   request_codes(cur, 0);
   const uint8_t* w = weights_of(cur);
   const auto weights = [&](i32x8 (&set)[2], int kb) {
-    set[0] = weight_frag(w + (int64_t)kb * kFp8Frag);
-    set[1] = weight_frag(w + (int64_t)(p.KB + kb) * kFp8Frag);
+    set[0] = weight_frag<ONCE>(w + (int64_t)kb * kFp8Frag);
+    set[1] = weight_frag<ONCE>(w + (int64_t)(p.KB + kb) * kFp8Frag);
   };
   weights(wf[0], 0);
   weights(wf[1], min(1, p.KB - 1));
@@ -552,10 +559,11 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const u32x4* __restric
   }
 }
 
-// Whether both products take tiles of 256 rows: from an average of 48 rows an expert on (PROVISIONAL), and for contractions of up
-// to kTileBlocks blocks
+// Whether both products take tiles of 256 rows: from an average of 20 rows an expert on, and for contractions of up to kTileBlocks
+// blocks.  Both products of 128 experts of 2048 x 768 at 8, 16, 32, 62 rows each: 115, 119, 118, 123 us by tiles of 256 rows, and 4 for
+// bringing the rows to 8 bits before; 104, 119, 141, 217 by tiles of 32.
 bool takes_tiles(int64_t Msum, int64_t N, int64_t D, int64_t H) {
-  return Msum >= 48 * N && std::max(D, H) <= kTileBlocks * kFp8Block;
+  return Msum >= 20 * N && std::max(D, H) <= kTileBlocks * kFp8Block;
 }
 
 int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
@@ -564,24 +572,41 @@ int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
     return MOMOE_ERR_UNSUPPORTED;
   return MOMOE_OK;
 }
-template <bool FIRST>
-int launch_tiles(const Fp8Args& a, int64_t M, int64_t D, int64_t H, int64_t Msum, int64_t N, hipStream_t st) {
-  // the rows of the first product are gathered at 32-bit offsets
-  if (std::max(D, H) > kTileBlocks * kFp8Block || (FIRST && M * a.KB * kFp8Block >= (1ll << 32))) return MOMOE_ERR_UNSUPPORTED;
+// Whether the weights, each read by one tile, do better past the last-level cache.  128 experts of 2048 x 768: the first product's,
+// 384 MiB, with the hint take 64 us instead of 78 for 16 tokens and 77 instead of 80 for 1000; the second's, 192 MiB, 44 instead of 41
+// and 57 instead of 49.
+template <class A>
+bool read_once(const A& a, int64_t Msum, int64_t N, int64_t tile_rows) {
+  return Msum <= tile_rows * N && std::min(N, Msum) * a.pairs * 2 * a.KB * kFp8Frag >= kBeyondCache;
+}
+
+template <bool FIRST, bool ONCE>
+int launch_tiles(const Fp8Args& a, hipStream_t st) {
   static LdsLimit limit;
-  if (!allow_lds(fp8_tile_kernel<FIRST>, kTileLds, limit)) return MOMOE_ERR_LAUNCH;
-  fp8_tile_kernel<FIRST><<<persistent_grid(), kThreads, kTileLds, st>>>(a);
+  if (!allow_lds(fp8_tile_kernel<FIRST, ONCE>, kTileLds, limit)) return MOMOE_ERR_LAUNCH;
+  fp8_tile_kernel<FIRST, ONCE><<<persistent_grid(), kThreads, kTileLds, st>>>(a);
   return launch_status();
 }
+template <bool FIRST>
+int launch_tiles(const Fp8Args& a, int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, hipStream_t st) {
+  // the rows of the first product are gathered at 32-bit offsets
+  if (std::max(D, H) > kTileBlocks * kFp8Block || (FIRST && M * a.KB * kFp8Block >= (1ll << 32))) return MOMOE_ERR_UNSUPPORTED;
+  return read_once(a, Msum, N, kTileRows) ? launch_tiles<FIRST, true>(a, st) : launch_tiles<FIRST, false>(a, st);
+}
 // As many wavefronts to a pair's contraction as give every CU two workgroups, had each expert that may hold a row one tile
-template <bool FIRST, class X>
-int launch_few(const FewArgs& a, int64_t Msum, int64_t N, hipStream_t st) {
-  const int64_t experts = std::min(N, Msum), wanted = 2 * persistent_grid();
+template <bool FIRST, bool ONCE, class X>
+int launch_few(const FewArgs& a, int64_t experts, hipStream_t st) {
+  const int64_t wanted = 2 * persistent_grid();
   const auto enough = [&](int ks) { return a.KB < 2 * ks || experts * cdiv64(a.pairs, kWaves / ks) >= wanted; };
-  auto kernel = enough(1) ? fp8_few_rows_kernel<FIRST, X, 1> : enough(2) ? fp8_few_rows_kernel<FIRST, X, 2>
-              : enough(4) ? fp8_few_rows_kernel<FIRST, X, 4> : fp8_few_rows_kernel<FIRST, X, 8>;
+  auto kernel = enough(1) ? fp8_few_rows_kernel<FIRST, ONCE, X, 1> : enough(2) ? fp8_few_rows_kernel<FIRST, ONCE, X, 2>
+              : enough(4) ? fp8_few_rows_kernel<FIRST, ONCE, X, 4> : fp8_few_rows_kernel<FIRST, ONCE, X, 8>;
   kernel<<<(unsigned)wanted, kThreads, 0, st>>>(a);
   return launch_status();
+}
+template <bool FIRST, class X>
+int launch_few(const FewArgs& a, int64_t Msum, int64_t N, hipStream_t st) {
+  const int64_t experts = std::min(N, Msum);
+  return read_once(a, Msum, N, kFewRows) ? launch_few<FIRST, true, X>(a, experts, st) : launch_few<FIRST, false, X>(a, experts, st);
 }
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
@@ -606,7 +631,7 @@ extern "C" int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, c
   a.h_codes = (uint8_t*)h_codes;
   a.HB = (int)fp8_blocks(H);
   a.msum = Msum;
-  return launch_tiles<true>(a, M, D, H, Msum, N, (hipStream_t)stream);
+  return launch_tiles<true>(a, M, D, H, N, Msum, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, const void* Wl2_packed, const float* Wl2_scale,
@@ -625,7 +650,7 @@ extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, co
   a.D = (int)D;
   a.DB = (int)fp8_blocks(D);
   a.msum = Msum;
-  return launch_tiles<false>(a, M, D, H, Msum, N, (hipStream_t)stream);
+  return launch_tiles<false>(a, M, D, H, N, Msum, (hipStream_t)stream);
 }
 
 extern "C" int momoe_fp8_few_lin1_swiglu_fwd(const void* x, int type, int64_t ldx, const void* Wl1_packed, const float* Wl1_scale,

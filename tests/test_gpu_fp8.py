@@ -107,7 +107,8 @@ SIZES = [
     (64, 64, 2208, 2, 2, 1, 0), (200, 128, 128, 16, 2, 0, 1.5),
     (300, 96, 64, 4, 2, 0, 0), (517, 288, 160, 5, 2, 1, 0), (700, 128, 416, 4, 3, 1, 2.0), (900, 640, 96, 3, 1, 0, 0),
     (150, 8320, 32, 2, 1, 0, 0), (140, 32, 8320, 2, 1, 0, 0), (150, 8192, 384, 2, 1, 0, 0), (200, 384, 1056, 3, 1, 0, 0), (700, 4224, 4192, 3, 2, 0, 0), (130, 7200, 64, 2, 1, 0, 0),
-    (60, 128, 8192, 1, 1, 0, 0), (2, 8224, 2112, 12, 3, 0, 0), (90, 1056, 1024, 40, 4, 0, 0), (33, 2080, 160, 1, 1, 0, 0), (9000, 64, 1280, 6, 2, 0, 0.5), (7000, 512, 288, 20, 2, 0, 0.5),
+    (60, 128, 8192, 1, 1, 0, 0), (2, 8224, 2112, 12, 3, 0, 0), (90, 1056, 1024, 40, 4, 0, 0), (18, 2080, 160, 1, 1, 0, 0), (300, 128, 96, 40, 2, 0, 2.0),
+    (9, 1056, 512, 8, 2, 0, 0), (9000, 64, 1280, 6, 2, 0, 0.5), (7000, 512, 288, 20, 2, 0, 0.5),
 ]
 
 
