@@ -367,7 +367,7 @@ Plan fwd_plan(int64_t G, int64_t S) { return G > 64 || G * S <= 256 ? Plan{1, S}
 
 int check_balance(int64_t G, int64_t S, int64_t N, int64_t Ks, int64_t ld) {
   if (G <= 0 || S <= 0 || N <= 0 || Ks < 0 || Ks >= N || ld < N) return MOMOE_ERR_BAD_ARG;
-  return N > kMaxExperts || G >= (1ll << 31) || S >= (1ll << 31) || G * S >= (1ll << 31) - 4 ? MOMOE_ERR_UNSUPPORTED : MOMOE_OK;
+  return N > kMaxExperts || G > (1ll << 30) || S > (1ll << 30) || G * S > (1ll << 30) ? MOMOE_ERR_UNSUPPORTED : MOMOE_OK;
 }
 bool type_ok(int t) { return t == MOMOE_TYPE_BF16 || t == MOMOE_TYPE_F32 || t == MOMOE_TYPE_F16; }
 int64_t type_bytes(int t) { return t == MOMOE_TYPE_F32 ? 4 : 2; }

@@ -456,7 +456,7 @@ int type_of(at::ScalarType t) {
   return t == at::kBFloat16 ? MOMOE_TYPE_BF16 : t == at::kFloat ? MOMOE_TYPE_F32 : t == at::kHalf ? MOMOE_TYPE_F16 : -1;
 }
 
-// x [B, S, D]; W1, W2 packed, S1, S2 their scales; forward only
+// x [B, S, D]; W1, W2 packed, S1, S2 the bits of their scales, int32 (a trace cannot hold the view between the two); forward only
 std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, const Tensor& S1, const Tensor& W2, const Tensor& S2,
                                        const Tensor& mask_NM, const Tensor& s_NM, int64_t K, int64_t H, bool check) {
   if (torch::jit::tracer::isTracing())
@@ -469,14 +469,15 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   const at::Device dev = W1.device();
   if (x_BSD.dim() != 3) throw_python(PyExc_AssertionError, "x_BSD must be [B, S, D]");
   const int64_t B = x_BSD.size(0), S = x_BSD.size(1), D = x_BSD.size(2), M = B * S;
+  TORCH_CHECK(K >= 1, "K, the experts of a token, must be at least 1, got ", K);
   const int64_t N = S1.dim() == 4 ? S1.size(0) : 0, msum = M * K, DB = (D + 127) / 128, HB = (H + 127) / 128;
   const auto held = [&](const Tensor& t, at::ScalarType type) {
     return t.device() == dev && t.scalar_type() == type && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0;
   };
   const bool fit = S1.dim() == 4 && S2.dim() == 3 && S1.sizes() == at::IntArrayRef({N, DB, 2, HB}) &&
                    S2.sizes() == at::IntArrayRef({N, HB, DB}) && W1.numel() == momoe_fp8_weight_bytes(N, D, 2 * H) &&
-                   W2.numel() == momoe_fp8_weight_bytes(N, H, D) && held(W1, at::kByte) && held(W2, at::kByte) && held(S1, at::kFloat) &&
-                   held(S2, at::kFloat);
+                   W2.numel() == momoe_fp8_weight_bytes(N, H, D) && held(W1, at::kByte) && held(W2, at::kByte) && held(S1, at::kInt) &&
+                   held(S2, at::kInt);
   if (!fit) throw_python(PyExc_AssertionError, "x_BSD [B,S,D] and the packed weights do not fit together");
   const c10::DeviceGuard guard(dev);
   const hipStream_t st = stream_of(dev);
@@ -513,10 +514,10 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   const int type = type_of(x.scalar_type());
   if (few) {
     h = transients.take(h_bytes, h_own);
-    MOMOE_CALL(momoe_fp8_few_lin1_swiglu_fwd, st, x.data_ptr(), type, D, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(),
+    MOMOE_CALL(momoe_fp8_few_lin1_swiglu_fwd, st, x.data_ptr(), type, D, W1.data_ptr(), (const float*)S1.data_ptr(), ib.idx(), ib.table(),
                (float*)h, M, D, H, N, msum);
     ys = transients.take(msum * D * 2, ys_own);
-    MOMOE_CALL(momoe_fp8_few_lin2_scale_fwd, st, (const float*)h, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0),
+    MOMOE_CALL(momoe_fp8_few_lin2_scale_fwd, st, (const float*)h, W2.data_ptr(), (const float*)S2.data_ptr(), s.data_ptr<float>(), s.stride(0),
                s.stride(1), ib.idx(), ib.table(), ys, M, D, H, N, msum);
   } else {
     void* const xq = transients.take(xq_bytes, xq_own);
@@ -524,9 +525,9 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
     MOMOE_CALL(momoe_fp8_quantize_rows, st, x.data_ptr(), type, D, M, D, xq, xs);
     h = transients.take(h_bytes, h_own);
     void* const hs = transients.take(hs_bytes, hs_own);
-    MOMOE_CALL(momoe_fp8_lin1_swiglu_fwd, st, xq, xs, W1.data_ptr(), S1.data_ptr<float>(), ib.idx(), ib.table(), h, hs, M, D, H, N, msum);
+    MOMOE_CALL(momoe_fp8_lin1_swiglu_fwd, st, xq, xs, W1.data_ptr(), (const float*)S1.data_ptr(), ib.idx(), ib.table(), h, hs, M, D, H, N, msum);
     ys = transients.take(msum * D * 2, ys_own);
-    MOMOE_CALL(momoe_fp8_lin2_scale_fwd, st, h, hs, W2.data_ptr(), S2.data_ptr<float>(), s.data_ptr<float>(), s.stride(0), s.stride(1),
+    MOMOE_CALL(momoe_fp8_lin2_scale_fwd, st, h, hs, W2.data_ptr(), (const float*)S2.data_ptr(), s.data_ptr<float>(), s.stride(0), s.stride(1),
                ib.idx(), ib.table(), ys, M, D, H, N, msum);
   }
   MOMOE_CALL(momoe_fp8_combine, st, ys, ib.inv(), y.data_ptr(), M, D, K, msum);
@@ -707,11 +708,12 @@ Tensor rows_of(const Tensor& t, int64_t M, int64_t N) {
   const Tensor rows = t.reshape({M, N});
   return has_rows(rows) ? rows : rows.contiguous();
 }
+Tensor flags_of(const Tensor& valid, int64_t M) { return valid.reshape({M}).contiguous(); }
 int64_t pitch_of(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
 struct Balanced {
   Tensor loss, counts;  // results: [], [groups, N]
-  Tensor valid, info;   // for the backward, with the logits; `valid` may be undefined
+  Tensor valid, info;   // for the backward, with the logits; `valid` may be undefined, and has the shape that it came in
 };
 
 // logits [.., N] of one of the three types, `groups` of as many tokens each
@@ -724,10 +726,12 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   const Tensor rows = rows_of(logits, M, N);
   const Tensor mask = mask_NM.to(dev, at::kInt);
   TORCH_CHECK(mask.dim() == 2 && mask.size(0) == N && mask.size(1) == M, "mask_NM must be [", N, ", ", M, "]");
+  Tensor flags;
   if (valid.has_value()) {
     TORCH_CHECK(valid->scalar_type() == at::kBool && valid->numel() == M, "valid must be a bool tensor of ", M,
                 " elements, one for each token");
-    b.valid = valid->to(dev).reshape({M}).contiguous();
+    b.valid = valid->to(dev);
+    flags = flags_of(b.valid, M);
   }
   b.counts = at::empty({groups, N}, at::TensorOptions().dtype(at::kLong).device(dev));
   b.loss = empty_f32({}, dev);
@@ -743,7 +747,7 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   const Tensor ws = empty_f32({ws_bytes / 4}, dev);
   MOMOE_CALL(momoe_balance_fwd, stream_of(dev), rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
              mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1),
-             b.valid.defined() ? (const uint8_t*)b.valid.data_ptr() : nullptr, groups, S, N, Ks, b.loss.data_ptr<float>(),
+             flags.defined() ? (const uint8_t*)flags.data_ptr() : nullptr, groups, S, N, Ks, b.loss.data_ptr<float>(),
              b.counts.data_ptr<int64_t>(), b.info.data_ptr<float>(), ws.data_ptr(), ws_bytes);
   return b;
 }
@@ -769,10 +773,10 @@ struct BalanceSaved {
   BalanceSaved(const variable_list& saved, size_t at, const at::Device& dev, at::ScalarType type, at::IntArrayRef sizes, int64_t M,
                int64_t N, int64_t groups) {
     logits = rows_of(as_saved(saved[at], "logits", dev, type, sizes, /*packed=*/false), M, N);
-    valid = saved[at + 1];
-    if (valid.defined()) {
-      as_saved(valid, "valid", dev, at::kBool, {M}, /*packed=*/false);
-      TORCH_CHECK(valid.is_contiguous(), "backward: the saved tensor valid came back from its hook with other strides");
+    if (saved[at + 1].defined()) {
+      const Tensor& v = saved[at + 1];
+      TORCH_CHECK(v.numel() == M, "backward: the saved tensor valid came back from its hook in another size");
+      valid = flags_of(as_saved(v, "valid", dev, at::kBool, v.sizes(), /*packed=*/false), M);
     }
     counts = as_saved(saved[at + 2], "counts", dev, at::kLong, {groups, N});
     info = as_saved(saved[at + 3], "info", dev, at::kFloat, {1 + groups});
@@ -783,7 +787,7 @@ struct BalanceFn : torch::autograd::Function<BalanceFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& mask, int64_t Ks,
                                const std::optional<Tensor>& valid, int64_t groups) {
     Balanced b = balance_forward(logits, mask, Ks, valid, groups);
-    // (the logits as they came: a view made here would hide from autograd that they changed since)
+    // (logits and valid as they came: a view made here would hide from autograd that they changed since)
     ctx->save_for_backward({logits, b.valid, b.counts, b.info});
     ctx->saved_data["call"] = std::vector<int64_t>{Ks, groups, logits.device().index(), (int64_t)logits.scalar_type()};
     ctx->saved_data["sizes"] = logits.sizes().vec();
@@ -810,7 +814,7 @@ struct BalanceFn : torch::autograd::Function<BalanceFn> {
 // Groups of a call: its sequences, or all of its tokens
 int64_t groups_of(at::IntArrayRef sizes, bool per_sequence) {
   TORCH_CHECK(!per_sequence || sizes.size() == 3, "per_sequence takes [B, S, N] logits or [B, S, D] tokens");
-  return per_sequence && sizes[0] > 0 ? sizes[0] : 1;
+  return per_sequence ? sizes[0] : 1;
 }
 
 std::tuple<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& mask, int64_t Ks, const std::optional<Tensor>& valid,
@@ -910,7 +914,7 @@ TORCH_LIBRARY(momoe, m) {
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts)));
   m.def("router(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks) -> (Tensor(a), Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(router)));
-  m.def("experts_fp8(Tensor x_BSD, Tensor Wl1, Tensor Wl1_scale, Tensor Wl2, Tensor Wl2_scale, Tensor mask_NM, Tensor s_NM, int K, "
+  m.def("experts_fp8(Tensor x_BSD, Tensor Wl1, Tensor Wl1_scale_bits, Tensor Wl2, Tensor Wl2_scale_bits, Tensor mask_NM, Tensor s_NM, int K, "
         "int H, bool check) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_fp8)));
   m.def("balance_loss(Tensor logits, Tensor mask_NM, int Ks, Tensor? valid, bool per_sequence) -> (Tensor, Tensor)",

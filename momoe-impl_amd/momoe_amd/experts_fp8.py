@@ -25,7 +25,8 @@ class MoMoEFP8(nn.Module):
         Wl1_scale, Wl2_scale: fp32, [N, ceil(D/128), 2, ceil(H/128)] (the two halves have blocks of their own) and
         [N, ceil(H/128), ceil(D/128)]: a weight is its e4m3 value times the scale of its 128 x 128 block.
     D and H must be multiples of 32.  Each 128 consecutive values of a token (and of its h) are scaled by the least
-    power of two that leaves none above 448, e4m3's largest; NaN or infinity among them make NaN of the token.
+    power of two that leaves none above 448, e4m3's largest (values below 2^-100 by one of 2^-108); NaN or infinity among
+    them make NaN of the token.  A call takes tokens of up to 4 GiB in 8 bits.
 
     The weights are laid out once, in the order that the kernels read them in; `weights()` gives them back.
     `from_momoe` quantizes the weights of a `MoMoE`.
@@ -57,6 +58,7 @@ class MoMoEFP8(nn.Module):
 
     def _set_sizes(self, D, H, N, K):
         assert D % 32 == 0 and H % 32 == 0, f"D and H must be multiples of 32, got {D} and {H}"
+        assert 1 <= K <= N, f"num_chosen_experts must be between 1 and {N}, got {K}"
         self.D, self.H, self.N, self.K = D, H, N, K
 
     def _hold(self, W1, S1, W2, S2):
@@ -86,5 +88,5 @@ class MoMoEFP8(nn.Module):
 
     def forward(self, x_BSD, mask_NM, s_NM):
         """As `MoMoE.forward`: (y_BSD bf16, tokens per expert int64 [N]).  Nothing may require a gradient."""
-        return _layer.experts_fp8(x_BSD, self.Wl1_packed, self.Wl1_scale, self.Wl2_packed, self.Wl2_scale, mask_NM, s_NM, self.K,
-                                  self.H, experts.CHECK_ROUTING)
+        return _layer.experts_fp8(x_BSD, self.Wl1_packed, self.Wl1_scale_bits, self.Wl2_packed, self.Wl2_scale_bits, mask_NM, s_NM,
+                                  self.K, self.H, experts.CHECK_ROUTING)

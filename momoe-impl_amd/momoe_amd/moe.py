@@ -13,6 +13,8 @@ from .router import TopKRouter
 
 
 class MoE(nn.Module):
+    balance = None  # of layers pickled before they had one
+
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts,
                  num_shared_experts, save_percent=0, bias_update_rate=1e-4,
                  Wg_DN=None, Wl1_ND2H=None, Wl2_NHD=None, balance=None):

@@ -21,7 +21,7 @@ def test_refusals_of_the_entry_points():
     assert all(fwd(type=t) == 1 for t in (-1, 3))
     assert fwd(ld=63) == fwd(G=0) == fwd(S=0) == fwd(N=0) == fwd(Ks=-1) == fwd(Ks=64) == 1
     assert fwd(ws=p + 8) == fwd(bytes=0) == 1
-    assert fwd(N=513, ld=513) == fwd(G=1 << 20, S=1 << 12) == fwd(S=1 << 31) == 2
+    assert fwd(N=513, ld=513) == fwd(G=1 << 20, S=1 << 12) == fwd(S=1 << 31) == fwd(G=1, S=(1 << 30) + 1) == 2
     back = dict(logits=p, type=1, ld=64, valid=None, counts=p, info=p, g=p, add=None, out=p, gtype=1, G=2, S=64, N=64, Ks=0)
 
     def bwd(**changed):

@@ -65,6 +65,9 @@ def test_constructor_refusals():
                       ("Wl1_scale", good["Wl1_scale"].double()), ("Wl2_NHD", e4(2, 160, 64)), ("Wl2_scale", torch.ones(2, 2, 1))):
         with pytest.raises(AssertionError, match=name):
             momoe_amd.MoMoEFP8(160, 64, 2, 1, **{**good, name: bad})
+    for k in (0, 3):
+        with pytest.raises(AssertionError, match="num_chosen_experts"):
+            momoe_amd.MoMoEFP8(160, 64, 2, k, **good)
     with pytest.raises(AssertionError, match="multiples of 32"):
         momoe_amd.MoMoEFP8(160, 48, 2, 1, **good)
     with pytest.raises(RuntimeError, match="no CPU compute path"):

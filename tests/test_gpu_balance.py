@@ -152,6 +152,43 @@ def test_gradient_against_differences():
         assert abs((f(up) - f(down)) / (2 * h) - grad[b, s, n].item()) < 1e-8
 
 
+@pytest.mark.parametrize("size", [(2, 30), (60,)])
+def test_flags_that_changed_since_the_forward_are_refused(size):
+    N = 16
+    l = torch.randn(2, 30, N, device=DEV, requires_grad=True)
+    mask = (torch.rand(N, 60, device=DEV) < 0.3).int()
+    valid = torch.ones(size, dtype=torch.bool, device=DEV)
+    loss, _ = momoe_amd.balance_loss(l, mask, valid=valid)
+    valid.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("B,S", [(0, 5), (3, 0)])
+def test_counts_of_no_tokens(B, S):
+    loss, counts = momoe_amd.balance_loss(torch.zeros(B, S, 8, device=DEV), torch.zeros(8, 0, dtype=torch.int32, device=DEV),
+                                          per_sequence=True)
+    assert loss == 0 and counts.shape == (B, 8) and counts.sum() == 0
+
+
+def test_traced_modules_with_a_balance_loss():
+    """A graph of torch.jit.trace does on inputs of other sizes what the module does."""
+    D, H, N, K, Ks = 64, 32, 8, 3, 1
+    torch.manual_seed(4)
+    moe = momoe_amd.MoE(D, H, N, K, Ks, bias_update_rate=0.0, balance="sequence")
+    x = torch.randn(2, 20, D, device=DEV, dtype=torch.bfloat16)
+    traced = torch.jit.trace(moe, x)
+    for B, S in ((2, 20), (3, 31)):
+        results = []
+        for module in (moe, traced):
+            moe.zero_grad(set_to_none=True)
+            xr = torch.randn(B, S, D, device=DEV, dtype=torch.bfloat16, generator=torch.Generator(DEV).manual_seed(B)).requires_grad_()
+            y, loss = module(xr)
+            torch.autograd.backward([y, loss], [torch.ones_like(y), torch.full_like(loss, 3.0)])
+            results.append([y, loss, xr.grad, moe.router.Wg_DN.grad])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_refusals():
     logits, mask = _inputs(2, 10, 8, 2, 0, torch.float32)
     l, m = logits.to(DEV), mask.to(DEV)

@@ -267,6 +267,15 @@ def test_routing_that_is_not_k_of_n(M, monkeypatch):
             layer(x.view(1, M, D).to(DEV), m.to(DEV), s.to(DEV))
 
 
+def test_traced_layer():
+    layer, _ = _layer(96, 64, 4, 2)
+    args = lambda M: (_x(M, 96).view(1, M, 96).to(DEV), *[t.to(DEV) for t in make_routing(M, 4, 2, seed=M)])
+    traced = torch.jit.trace(layer, args(10))
+    for M in (10, 3, 300):
+        a = args(M)
+        assert all(torch.equal(u, v) for u, v in zip(layer(*a), traced(*a)))
+
+
 def test_refusals():
     D, H, N, K, M = 96, 64, 4, 2, 10
     layer, _ = _layer(D, H, N, K)
@@ -280,6 +289,10 @@ def test_refusals():
     for a in ((x, mask[:3], s), (x, mask[:, :9], s), (x, mask, s[:3]), (x, mask, s[:, :9])):
         with pytest.raises(RuntimeError, match="must be"):
             layer(*a)
+    held = layer.Wl1_packed, layer.Wl1_scale_bits, layer.Wl2_packed, layer.Wl2_scale_bits
+    for k in (0, -1):
+        with pytest.raises(RuntimeError, match="at least 1"):
+            torch.ops.momoe.experts_fp8(x, *held, mask, s, k, H, False)
     for bad in (x[0], x[:, :, :64], torch.cat([x, x, x], -1)):
         with pytest.raises(AssertionError):
             layer(bad, mask, s)
