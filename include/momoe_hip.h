@@ -446,7 +446,8 @@ int momoe_balance_bwd(const void* logits, int logits_type, int64_t ld, const uin
  * No counterpart in the reference, whose weights are bf16.  e4m3 (largest value 448) with a scale for each 128 values:
  *   rows     each 128 consecutive values of a row, scaled by the least power of two that leaves none above 448 (of magnitudes
  *            below 2^-100: as if that were the largest).  q: momoe_fp8_row_bytes(cols) bytes a row, zeros past the last column;
- *            codes: momoe_fp8_code_bytes(cols) bytes a row, of which the first ceil(cols / 128) are the scales, 2^(code - 127).  A NaN or an infinity among the 128 makes NaN of all results of that row.
+ *            codes: momoe_fp8_code_bytes(cols) bytes a row, of which the first ceil(cols / 128) are the scales,
+ *            2^(code - 127).  A NaN or an infinity among the 128 makes NaN of all results of that row.
  *   weights  any fp32 scale for each block of 128 rows x 128 columns; of Wl1 the H columns of each half have blocks of their own:
  *            Wl1_scale [N][ceil(D/128)][2][ceil(H/128)], Wl2_scale [N][ceil(H/128)][ceil(D/128)].  Kept in the order that the
  *            kernels stream them in: [N][groups of 16 columns][ceil(rows/128)][2][64][16] bytes, byte b of piece (half h, lane l) the

@@ -12,7 +12,8 @@
 // wavefront a token, as in the router, costs ten times the instructions for 64 experts: its reductions take as many
 // steps for two elements a lane as for sixteen.)
 //
-// Bound by launches up to some ten thousand tokens, then by the reads of the mask, four bytes an element.
+// Bound by launches up to some ten thousand tokens, then by the reads of the mask, four bytes an element.  Pieces, their sum, gradient:
+// 8, 6, 6 us for 8192 x 128 bf16 logits, 14, 6, 9 us for 65536 x 64 (25 MB forward, 16 backward: 1.8 TB/s each).
 // No atomics: the column sums of a workgroup's tokens go to the workspace and one workgroup adds them in a fixed order.
 #include "lanes.hpp"
 
