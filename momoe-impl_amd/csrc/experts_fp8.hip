@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
 // 1.78 GHz with the matrix cores half busy; the same with zeros for data takes 216 and 146, and without the fp32 sums 209 and 146.  A
 // library's plain product of 8192^3 reaches 2.98 PFLOP/s, with neither block scales nor an epilogue.  Two wavefronts of a SIMD half a stage
 // apart: 274 to 277 and 180.  128 rows x 64 columns a wavefront, half the reads of LDS: 306 and 256, with spills.  The tile's end (h, its
-// largest, packing; packets of 15 bits) is 10 to 18 thousand clocks of some 45 thousand for six blocks.
+// largest, packing; packets of 15 bits) is 10 to 18 thousand clocks, a stage 3400.
 constexpr int kTileRows = 256, kTileBlocks = 64;  // most blocks of a contraction
 constexpr int kTileSlot = kTileRows * kFp8Block, kSlots = 3;
 constexpr int kTileCodes = kTileRows * kTileBlocks;  // bytes: [four blocks][row][block]
