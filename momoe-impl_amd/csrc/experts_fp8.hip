@@ -64,11 +64,12 @@ __device__ __forceinline__ f32x4 swiglu(const f32x4& a, const f32x4& b) {
 // again for each block of columns, against a launch before either product.
 //
 // Products in bf16 (fp8.hpp): the conversions and the slower products hide behind the stream.  Bound by HBM: of 128 experts of
-// 2048 x 768, one row each, x . Wl1 64 us, 6.3 TB/s, h . Wl2 38 us, 5.3 TB/s (contractions of six blocks: a tile's start counts); of one
-// token, 8 experts, 11 and 6 us, of which the weights alone are 4 and 2: its chain of table, token, row, product and sum.  Two rows at a
-// time are as fast as four; each wavefront's blocks in another order, against all of them at the same place of a row's
-// stretch, changed nothing.
-constexpr int kFewRows = MOMOE_FP8_FEW_ROWS, kFewChunk = 16, kFewAhead = 4, kRowsAtOnce = 2;
+// 2048 x 768, one row each, x . Wl1 64 us, 6.3 TB/s, h . Wl2 30 us, 6.6 TB/s; 19 rows each 72 and 37.  Two workgroups share a CU, so
+// that one streams while the other starts or ends a tile: with four blocks ahead, the registers of which leave room for one, it is
+// 63 and 37, at 19 rows 78 and 48.  One token, 8 experts: 11 and 6 us, of which the weights alone are 4 and 2: its chain of table, token,
+// row, product and sum.  Two rows at a time are as fast as four; each wavefront's blocks in another order, against all of them
+// at the same place of a row's stretch, changed nothing.
+constexpr int kFewRows = MOMOE_FP8_FEW_ROWS, kFewChunk = 16, kFewAhead = 2, kRowsAtOnce = 2;
 
 struct FewArgs {
   const void* rows;      // [M or Msum][ld]
@@ -86,7 +87,7 @@ struct FewArgs {
 };
 
 template <bool FIRST, bool ONCE, class X, int KS>
-__global__ __launch_bounds__(kThreads) void fp8_few_rows_kernel(FewArgs p) {
+__global__ __launch_bounds__(kThreads, 4) void fp8_few_rows_kernel(FewArgs p) {
   constexpr int FR = kFewRows / 16, PW = kWaves / KS;
   __shared__ __attribute__((aligned(16))) uint8_t rows_lds[kFewChunk * kFewRows * kFp8Block];  // then the sums of KS wavefronts
   __shared__ float scale_lds[kFewChunk][kFewRows];
@@ -570,8 +571,9 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const u32x4* __restric
 }
 
 // Whether both products take tiles of 256 rows: from an average of 20 rows an expert on, and for contractions of up to kTileBlocks
-// blocks.  Both products of 128 experts of 2048 x 768 at 8, 16, 32, 62 rows each: 115, 119, 118, 123 us by tiles of 256 rows, and 4 for
-// bringing the rows to 8 bits before; 104, 119, 141, 217 by tiles of 32.
+// blocks.  Both products of 128 experts of 2048 x 768 at 8, 16, 25, 32 rows each: 111, 116, 115, 114 us by tiles of 256 rows, and 4 for
+// bringing the rows to 8 bits before; 98, 106, 117, 123 by tiles of 32, and twice as much past 32 rows, which some experts hold before
+// the average does.  8 experts of 1408 x 2048 at 20, 32 rows each: 31, 32 and 4 more; 33, 40.
 bool takes_tiles(int64_t Msum, int64_t N, int64_t D, int64_t H) {
   return Msum >= 20 * N && std::max(D, H) <= kTileBlocks * kFp8Block;
 }
@@ -583,7 +585,7 @@ int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
   return MOMOE_OK;
 }
 // Whether the weights, each read by one tile, do better past the last-level cache.  128 experts of 2048 x 768: the first product's,
-// 384 MiB, with the hint take 64 us instead of 78 for 16 tokens and 77 instead of 80 for 1000; the second's, 192 MiB, 44 instead of 41
+// 384 MiB, with the hint take 71 us instead of 79 for 16 tokens and 77 instead of 80 for 1000; the second's, 192 MiB, 44 instead of 41
 // and 57 instead of 49.
 template <class A>
 bool read_once(const A& a, int64_t Msum, int64_t N, int64_t tile_rows) {
