@@ -171,6 +171,29 @@ def test_counts_of_no_tokens(B, S):
     assert loss == 0 and counts.shape == (B, 8) and counts.sum() == 0
 
 
+def test_logits_past_32_bit_offsets():
+    """Tokens behind 2^31 logits: their counts, and their gradient against the formula."""
+    M, N = 4_300_000, 512
+    logits = torch.zeros(M, N, device=DEV, dtype=torch.bfloat16)
+    mask = torch.zeros(N, M, dtype=torch.int32, device=DEV)
+    logits[-3:] = torch.randn(3, N, device=DEV).bfloat16()
+    mask[7, -3:] = mask[500, -1] = mask[1, 0] = 1
+    logits.requires_grad_()
+    loss, counts = momoe_amd.balance_loss(logits, mask)
+    want = torch.zeros(N, dtype=torch.int64)
+    want[7], want[500], want[1] = 3, 1, 1
+    assert torch.equal(counts.cpu(), want)
+    (loss * 2.0 ** 30).backward()
+    p = torch.softmax(logits.detach()[-3:].cpu().double(), -1)
+    c = want.double()
+    g = 2.0 ** 30 * N / (M * 5.0) * p * (c - p @ c[:, None])
+    got = logits.grad[-3:].cpu().double()
+    # the sum over c in fp32, and one rounding to bf16
+    assert ((got - g).abs() <= g.abs() * (2.0 ** -8 + 2.0 ** -14) + 2.0 ** 30 * N / (M * 5.0) * p * 5 * 2.0 ** -18).all()
+    # nearly all tokens are even: p = 1 / N, and with it the loss is 1, but for three tokens of M
+    assert abs(loss.item() - 1) <= 3 * N / M + 2.0 ** -10
+
+
 def test_traced_modules_with_a_balance_loss():
     """A graph of torch.jit.trace does on inputs of other sizes what the module does."""
     D, H, N, K, Ks = 64, 32, 8, 3, 1

@@ -185,6 +185,27 @@ def test_products(M, D, H, N, K, Ks, skew):
     assert torch.isfinite(y).all() and ((y - total).abs() <= slack).all(), ((y - total).abs() / slack).max()
 
 
+@pytest.mark.parametrize("M", [1, 1000])
+def test_weights_past_32_bit_offsets(M):
+    """The last of 40 experts, behind 5 GiB of others' weights, does what it does alone."""
+    N, D, H = 40, 8192, 8192
+    w = _weights(1, D, H)
+    alone = momoe_amd.MoMoEFP8(D, H, 1, 1, *[t.to(DEV) for t in w])
+    many = []
+    for t in w:
+        big = torch.zeros(N, *t.shape[1:], dtype=t.dtype, device=DEV)
+        big[-1] = t[0].to(DEV)
+        many.append(big)
+    last = momoe_amd.MoMoEFP8(D, H, N, 1, *many)
+    del many
+    x, s = _x(M, D).view(1, M, D).to(DEV), torch.rand(1, M, device=DEV) + 0.5
+    mask = torch.zeros(N, M, dtype=torch.int32, device=DEV)
+    mask[-1] = 1
+    y, sizes = last(x, mask, s.expand(N, M))
+    want, _ = alone(x, mask[-1:], s)
+    assert sizes[-1] == M and want.norm() > 0 and torch.equal(y, want)
+
+
 def _layer(D, H, N, K, seed=0):
     w = _weights(N, D, H, seed)
     return momoe_amd.MoMoEFP8(D, H, N, K, *[t.to(DEV) for t in w]), _values(*w)
