@@ -103,8 +103,9 @@ struct Packet {
       return __builtin_elementwise_maximum(__builtin_fabsf(x), __builtin_elementwise_maximum(__builtin_fabsf(y), __builtin_fabsf(z)));
     };
     const float all = __builtin_elementwise_maximum(larger(b[2], b[3], larger(a[0], a[1], a[2])), larger(a[3], b[0], b[1]));
-    // (a value that would round up to 2^14 counts for the next binade)
-    const uint32_t binade = (magnitude(all * s) + 0x200) >> 23, field = max(binade, 15u);
+    // (a value that would round up to 2^14 counts for the next binade; of a NaN with nearly all bits set that would be one past
+    // the last, of which eight bits hold nothing)
+    const uint32_t binade = min((magnitude(all * s) + 0x200) >> 23, 255u), field = max(binade, 15u);
     // 2^13 / 2^(field - 127) * s; a sum with 1.5 * 2^23 has the rounded product in its lowest bits
     const float unit = binade - 15 >= 255 - 15 ? 0.0f : __uint_as_float((127 + 13 + 127 - field) << 23) * s;
     const auto rounded = [&](float v) { return __float_as_uint(fmaf(v, unit, 12582912.0f)); };

@@ -387,3 +387,49 @@ def test_trained_with_a_balance_loss_then_served_in_8_bits():
     assert (got.float() - ref.float()).norm() <= 0.1 * ref.float().norm()
     with pytest.raises(RuntimeError, match="no_grad"):
         served(x)
+
+
+@pytest.mark.parametrize("bits", [0x7FC00000, 0x7FFFFFFF, -1])
+@pytest.mark.parametrize("M", [12, 400])
+def test_nan_of_any_bits_in_gate_weights_and_scales(M, bits):
+    """A NaN stays one whatever its payload, and stays with the results that it is part of."""
+    D, H, N, K, e = 288, 160, 4, 2, 1
+    w = [t.to(DEV) for t in _weights(N, D, H)]
+    mask, s = [t.to(DEV) for t in make_routing(M, N, K, seed=2)]
+    x = _x(M, D).view(1, M, D).to(DEV)
+    layer = lambda *held: momoe_amd.MoMoEFP8(D, H, N, K, *held)
+    ref, _ = layer(*w)(x, mask, s)
+    held = mask[e].bool()
+    rows, cols = held[:, None].expand(M, D), torch.arange(D, device=DEV) // 128
+
+    def poisoned(t, at):
+        t = t.clone(memory_format=torch.contiguous_format)
+        t.view(torch.int32)[at] = bits
+        return t
+
+    def check(y, nan):
+        assert torch.equal(y[0].isnan(), nan) and torch.equal(y[0][~nan], ref[0][~nan])
+
+    m = held.nonzero()[3, 0]
+    check(layer(*w)(x, mask, poisoned(s, (e, m)))[0], (torch.arange(M, device=DEV) == m)[:, None].expand(M, D))
+    check(layer(w[0], w[1], w[2], poisoned(w[3], (e, 1, 1)))(x, mask, s)[0], rows & (cols == 1))
+    for half in range(2):  # h is brought to 8 bits again: all that follows from it
+        check(layer(w[0], poisoned(w[1], (e, 2, half, 1)), w[2], w[3])(x, mask, s)[0], rows)
+
+
+@pytest.mark.parametrize("byte", [0x7F, 0xFF])
+@pytest.mark.parametrize("M", [12, 400])
+def test_nan_among_the_weights(M, byte):
+    """Of Wl1: all results of the expert's tokens.  Of Wl2: the eight columns that share a packet with its own."""
+    D, H, N, K, e = 288, 160, 4, 2, 1
+    w = [t.to(DEV) for t in _weights(N, D, H)]
+    mask, s = [t.to(DEV) for t in make_routing(M, N, K, seed=2)]
+    x = _x(M, D).view(1, M, D).to(DEV)
+    ref, _ = momoe_amd.MoMoEFP8(D, H, N, K, *w)(x, mask, s)
+    rows, col = mask[e].bool()[:, None].expand(M, D), torch.arange(D, device=DEV)
+    for which, at, nan in ((0, (e, 200, 70), rows), (0, (e, 31, H + 150), rows),
+                           (2, (e, 150, 201), rows & (col // 32 == 201 // 32) & (col % 16 // 4 == 201 % 16 // 4))):
+        bad = [t.clone() for t in w]
+        bad[which].view(torch.uint8)[at] = byte
+        y, _ = momoe_amd.MoMoEFP8(D, H, N, K, *bad)(x, mask, s)
+        assert torch.equal(y[0].isnan(), nan) and torch.equal(y[0][~nan], ref[0][~nan])
