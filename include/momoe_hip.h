@@ -433,6 +433,12 @@ int64_t momoe_balance_workspace_bytes(int64_t G, int64_t S, int64_t N);
 int momoe_balance_fwd(const void* logits, int logits_type, int64_t ld, const int32_t* mask_NM, int64_t stride_n,
                       int64_t stride_m, const uint8_t* valid_M, int64_t G, int64_t S, int64_t N, int64_t Ks,
                       float* loss, int64_t* counts_GN, float* info, void* workspace, int64_t workspace_bytes, void* stream);
+/* momoe_balance_fwd_kept: the same, and the counts once more to kept_GN (may be NULL), for a caller that hands counts_GN on to
+ * somebody who may change them before momoe_balance_bwd has read them. */
+int momoe_balance_fwd_kept(const void* logits, int logits_type, int64_t ld, const int32_t* mask_NM, int64_t stride_n,
+                           int64_t stride_m, const uint8_t* valid_M, int64_t G, int64_t S, int64_t N, int64_t Ks,
+                           float* loss, int64_t* counts_GN, int64_t* kept_GN, float* info, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /* momoe_balance_bwd: G_loss[0] * d loss / d logits (the counts are constants) + add_MN, of grad_type (logits_type or
  * MOMOE_TYPE_BF16), contiguous [G * S, N].  add_MN (may be NULL, or Glogits_MN itself): of grad_type, contiguous.  logits, valid_M,

@@ -40,6 +40,7 @@ struct BalanceArgs {
   float* group_p;        // [G][N]
   float* group_loss;     // [G]
   int64_t* counts;       // [G][N]
+  int64_t* kept;         // the same once more, or NULL
   float* info;           // [0]: 1 / groups with pairs (0: there are none), [1 + g]: Ng / (T P) (0: none)
   float* loss;
 };
@@ -81,6 +82,11 @@ struct Columns {
     for (int i = 0; i < kColsPerLane; ++i) p[i] *= scale;
   }
 };
+
+__device__ __forceinline__ void store_count(const BalanceArgs& p, int64_t at, int64_t count) {
+  p.counts[at] = count;
+  if (p.kept != nullptr) p.kept[at] = count;
+}
 
 // The sum of one value a thread over the workgroup, in every thread; `room` holds a value per wavefront
 template <int THREADS>
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(kThreadsFwd) void balance_piece_kernel(BalanceArgs 
   }
   float pairs = 0.0f, dot = 0.0f;
   for (int j = threadIdx.x; j < p.N; j += kThreadsFwd) {
-    p.counts[(int64_t)g * p.N + j] = count_of[j];
+    store_count(p, (int64_t)g * p.N + j, count_of[j]);
     if (j < p.Ng) {
       pairs += (float)count_of[j];
       dot += (float)count_of[j] * sum_at(j);
@@ -250,7 +256,7 @@ __global__ __launch_bounds__(kThreadsSum) void balance_sum_kernel(BalanceArgs p)
           count += some_c[s * items + item];
         }
         p.group_p[q] = sum;
-        p.counts[q] = count;
+        store_count(p, q, count);
       }
       __syncthreads();
     }
@@ -405,6 +411,14 @@ extern "C" int momoe_balance_fwd(const void* logits, int logits_type, int64_t ld
                                  int64_t stride_m, const uint8_t* valid_M, int64_t G, int64_t S, int64_t N, int64_t Ks,
                                  float* loss, int64_t* counts_GN, float* info, void* workspace, int64_t workspace_bytes,
                                  void* stream) {
+  return momoe_balance_fwd_kept(logits, logits_type, ld, mask_NM, stride_n, stride_m, valid_M, G, S, N, Ks, loss, counts_GN, nullptr,
+                                info, workspace, workspace_bytes, stream);
+}
+
+extern "C" int momoe_balance_fwd_kept(const void* logits, int logits_type, int64_t ld, const int32_t* mask_NM, int64_t stride_n,
+                                      int64_t stride_m, const uint8_t* valid_M, int64_t G, int64_t S, int64_t N, int64_t Ks,
+                                      float* loss, int64_t* counts_GN, int64_t* kept_GN, float* info, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
   if (!logits || !mask_NM || !loss || !counts_GN || !info || !workspace || !type_ok(logits_type)) return MOMOE_ERR_BAD_ARG;
   const int status = check_balance(G, S, N, Ks, ld);
   if (status != MOMOE_OK) return status;
@@ -412,6 +426,7 @@ extern "C" int momoe_balance_fwd(const void* logits, int logits_type, int64_t ld
   const Plan plan = fwd_plan(G, S);
   BalanceArgs a{logits, ld, mask_NM, stride_n, stride_m, valid_M, (int)S, (int)G, (int)N, (int)(N - Ks), (int)plan.C, (int)plan.TB};
   a.counts = counts_GN;
+  a.kept = kept_GN;
   a.info = info;
   a.loss = loss;
   char* at = (char*)workspace;

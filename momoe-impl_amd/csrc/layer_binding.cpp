@@ -713,12 +713,14 @@ int64_t pitch_of(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride
 
 struct Balanced {
   Tensor loss, counts;  // results: [], [groups, N]
-  Tensor valid, info;   // for the backward, with the logits; `valid` may be undefined, and has the shape that it came in
+  // For the backward, with the logits.  `valid` may be undefined, and has the shape that it came in.  `kept`: the counts once more:
+  // the others are the caller's, who may sum them over ranks before the backward, which autograd does not see.
+  Tensor valid, kept, info;
 };
 
 // logits [.., N] of one of the three types, `groups` of as many tokens each
 Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks, const std::optional<Tensor>& valid,
-                         int64_t groups) {
+                         int64_t groups, bool for_backward) {
   const at::Device dev = logits.device();
   const int64_t N = logits.size(-1), M = logits.numel() / N;
   const c10::DeviceGuard guard(dev);
@@ -734,10 +736,12 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
     flags = flags_of(b.valid, M);
   }
   b.counts = at::empty({groups, N}, at::TensorOptions().dtype(at::kLong).device(dev));
+  if (for_backward) b.kept = at::empty_like(b.counts);
   b.loss = empty_f32({}, dev);
   b.info = empty_f32({1 + groups}, dev);
   if (M == 0) {
     b.counts.zero_();
+    if (for_backward) b.kept.zero_();
     b.loss.zero_();
     b.info.zero_();
     return b;
@@ -745,10 +749,11 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   const int64_t S = M / groups, ws_bytes = momoe_balance_workspace_bytes(groups, S, N);
   TORCH_CHECK(ws_bytes >= 0, "balance loss: [", M, ", ", N, "] logits are past the sizes that it takes (N <= 512)");
   const Tensor ws = empty_f32({ws_bytes / 4}, dev);
-  MOMOE_CALL(momoe_balance_fwd, stream_of(dev), rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
+  MOMOE_CALL(momoe_balance_fwd_kept, stream_of(dev), rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
              mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1),
              flags.defined() ? (const uint8_t*)flags.data_ptr() : nullptr, groups, S, N, Ks, b.loss.data_ptr<float>(),
-             b.counts.data_ptr<int64_t>(), b.info.data_ptr<float>(), ws.data_ptr(), ws_bytes);
+             b.counts.data_ptr<int64_t>(), for_backward ? b.kept.data_ptr<int64_t>() : nullptr, b.info.data_ptr<float>(), ws.data_ptr(),
+             ws_bytes);
   return b;
 }
 
@@ -786,9 +791,9 @@ struct BalanceSaved {
 struct BalanceFn : torch::autograd::Function<BalanceFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& mask, int64_t Ks,
                                const std::optional<Tensor>& valid, int64_t groups) {
-    Balanced b = balance_forward(logits, mask, Ks, valid, groups);
+    Balanced b = balance_forward(logits, mask, Ks, valid, groups, /*for_backward=*/true);
     // (logits and valid as they came: a view made here would hide from autograd that they changed since)
-    ctx->save_for_backward({logits, b.valid, b.counts, b.info});
+    ctx->save_for_backward({logits, b.valid, b.kept, b.info});
     ctx->saved_data["call"] = std::vector<int64_t>{Ks, groups, logits.device().index(), (int64_t)logits.scalar_type()};
     ctx->saved_data["sizes"] = logits.sizes().vec();
     ctx->mark_non_differentiable({b.counts});
@@ -835,7 +840,7 @@ std::tuple<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& mask
     variable_list r = BalanceFn::apply(logits, mask, Ks, valid, groups);
     loss = r[0], counts = r[1];
   } else {
-    Balanced b = balance_forward(logits, mask, Ks, valid, groups);
+    Balanced b = balance_forward(logits, mask, Ks, valid, groups, /*for_backward=*/false);
     loss = b.loss, counts = b.counts;
   }
   return {loss, per_sequence ? counts : counts.select(0, 0)};
@@ -846,8 +851,8 @@ struct BalancedRouterFn : torch::autograd::Function<BalancedRouterFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& Wg, const Tensor& biases, int64_t N, int64_t K,
                                int64_t Ks, const std::optional<Tensor>& valid, int64_t groups) {
     Routed r = router_forward(x, Wg, biases, N, K, Ks, /*keep_logits=*/true);
-    Balanced b = balance_forward(r.logits, r.mask, Ks, valid, groups);
-    ctx->save_for_backward({r.x_MD, Wg, r.mask, r.p_sel, r.s_MN, r.norms, r.logits, b.valid, b.counts, b.info});
+    Balanced b = balance_forward(r.logits, r.mask, Ks, valid, groups, /*for_backward=*/true);
+    ctx->save_for_backward({r.x_MD, Wg, r.mask, r.p_sel, r.s_MN, r.norms, r.logits, b.valid, b.kept, b.info});
     ctx->saved_data["call"] = std::vector<int64_t>{Ks, N, Wg.device().index(), x.size(0), x.size(1), x.size(2), groups,
                                                    (int64_t)r.logits.scalar_type()};
     ctx->mark_non_differentiable({r.mask, b.counts});
@@ -890,7 +895,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> router_balanced(const Tensor&
     r = BalancedRouterFn::apply(x, Wg, biases, N, K, Ks, valid, groups);
   } else {
     Routed t = router_forward(x, Wg, biases, N, K, Ks, /*keep_logits=*/true);
-    Balanced b = balance_forward(t.logits, t.mask, Ks, valid, groups);
+    Balanced b = balance_forward(t.logits, t.mask, Ks, valid, groups, /*for_backward=*/false);
     r = {x, t.mask, t.s_MN.t(), b.loss, b.counts};
   }
   return {r[0], r[1], r[2], r[3], per_sequence ? r[4] : r[4].select(0, 0)};

@@ -84,6 +84,7 @@ _SIGNATURES = {
     "momoe_gate_dgrad": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _p]),
     "momoe_balance_workspace_bytes": (_i64, [_i64] * 3),
     "momoe_balance_fwd": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    "momoe_balance_fwd_kept": (_int, [_p, _int, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
     "momoe_balance_bwd": (_int, [_p, _int, _i64, _p, _p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_row_bytes": (_i64, [_i64]),
     "momoe_fp8_code_bytes": (_i64, [_i64]),

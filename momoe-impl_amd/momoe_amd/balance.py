@@ -16,7 +16,8 @@ def balance_loss(logits, mask_NM, num_shared_experts=0, valid=None, per_sequence
         loss = (N - Ks) * sum_i (c_i / sum_j c_j) * (sum over tokens of p_i / T)
 
     which is 1 where both are even.  The counts are constants of the gradient, which goes to the logits; those of shared experts
-    and of tokens that do not count get zeros.
+    and of tokens that do not count get zeros.  The tensor of counts is the caller's own: summing it over ranks before the backward
+    changes no gradient.
 
     valid: bool [M] or [B, S], False for the tokens that do not count (padding); what their logits hold does not matter.
     per_sequence: the loss is taken for each of the B sequences and averaged over those in which a routed expert holds a token;

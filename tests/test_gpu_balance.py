@@ -338,3 +338,29 @@ def test_moe_trains_with_a_balance_loss():
     assert isinstance(plain(x), torch.Tensor)
     with pytest.raises(ValueError, match="valid"):
         plain(x, valid)
+
+
+@pytest.mark.parametrize("per_sequence", [False, True])
+def test_counts_are_the_callers_own(per_sequence):
+    """Summed over ranks or added up in place between the forward and the backward: the gradient stays what it is.  (A collective
+    changes a tensor without autograd's knowledge, as `.data` does.)"""
+    B, S, N, K, D = 3, 200, 24, 3, 64
+    logits, mask = _inputs(B, S, N, K, 0, torch.float32)
+    want = _run(logits, mask, 0, None, per_sequence)
+    leaf = logits.to(DEV).requires_grad_()
+    router = momoe_amd.TopKRouter(D, N, K, 0, Wg_DN=torch.randn(D, N, generator=torch.Generator().manual_seed(1)).to(DEV))
+    x = torch.randn(B, S, D, generator=torch.Generator().manual_seed(2)).to(DEV, torch.bfloat16)
+    bias = torch.zeros(N, device=DEV)
+    loss, _ = router.with_balance_loss(x, bias, None, per_sequence)[3:]
+    through_gate, = torch.autograd.grad(1e3 * loss, router.Wg_DN)
+    for change in (lambda c: c.data.add_(1000), lambda c: c.add_(1000), lambda c: c.data.zero_()):
+        leaf.grad = None
+        loss, counts = momoe_amd.balance_loss(leaf, mask.to(DEV), 0, None, per_sequence)
+        assert torch.equal(counts, want[1])
+        change(counts)
+        loss.backward()
+        assert torch.equal(leaf.grad, want[2])
+        loss, counts = router.with_balance_loss(x, bias, None, per_sequence)[3:]
+        change(counts)
+        got, = torch.autograd.grad(1e3 * loss, router.Wg_DN)
+        assert torch.equal(got, through_gate)
