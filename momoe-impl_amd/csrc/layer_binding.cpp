@@ -718,7 +718,7 @@ struct Balanced {
   Tensor valid, kept, info;
 };
 
-// logits [.., N] of one of the three types, `groups` of as many tokens each
+// logits [.., N] of one of the three types, `groups` of as many tokens each; `valid` as check_valid takes it
 Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks, const std::optional<Tensor>& valid,
                          int64_t groups, bool for_backward) {
   const at::Device dev = logits.device();
@@ -730,8 +730,6 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   TORCH_CHECK(mask.dim() == 2 && mask.size(0) == N && mask.size(1) == M, "mask_NM must be [", N, ", ", M, "]");
   Tensor flags;
   if (valid.has_value()) {
-    TORCH_CHECK(valid->scalar_type() == at::kBool && valid->numel() == M, "valid must be a bool tensor of ", M,
-                " elements, one for each token");
     b.valid = valid->to(dev);
     flags = flags_of(b.valid, M);
   }
@@ -822,6 +820,17 @@ int64_t groups_of(at::IntArrayRef sizes, bool per_sequence) {
   return per_sequence ? sizes[0] : 1;
 }
 
+// One flag a token, in their order: as many in another shape would be those of other tokens.  `sizes`: of the tokens and their
+// logits or values, [M, ..] or [B, S, ..]
+void check_valid(const std::optional<Tensor>& valid, at::IntArrayRef sizes) {
+  if (!valid.has_value()) return;
+  const at::IntArrayRef tokens = sizes.slice(0, sizes.size() - 1);
+  const int64_t M = c10::multiply_integers(tokens);
+  const bool shape = valid->dim() == 1 || (valid->dim() == 2 && (tokens.size() == 1 || valid->sizes() == tokens));
+  TORCH_CHECK(valid->scalar_type() == at::kBool && shape && valid->numel() == M, "valid must be a bool tensor with a flag for each of the ",
+              tokens, " tokens, in that shape or in one dimension, got ", valid->scalar_type(), " ", valid->sizes());
+}
+
 std::tuple<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& mask, int64_t Ks, const std::optional<Tensor>& valid,
                                         bool per_sequence) {
   if (torch::jit::tracer::isTracing())
@@ -835,6 +844,7 @@ std::tuple<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& mask
   const int64_t N = logits.size(-1), groups = groups_of(logits.sizes(), per_sequence);
   TORCH_CHECK(Ks >= 0 && Ks < N, "num_shared_experts must be between 0 and N - 1 = ", N - 1, ", got ", Ks);
   TORCH_CHECK(N <= 512, "balance_loss takes up to 512 experts, got ", N);
+  check_valid(valid, logits.sizes());
   Tensor loss, counts;
   if (wants_autograd({&logits})) {
     variable_list r = BalanceFn::apply(logits, mask, Ks, valid, groups);
@@ -890,6 +900,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> router_balanced(const Tensor&
   check_router(x, Wg);
   TORCH_CHECK(Ks >= 0 && Ks < N, "the balance loss needs a routed expert: ", N, " experts, ", Ks, " of them shared");
   const int64_t groups = groups_of(x.sizes(), per_sequence);
+  check_valid(valid, x.sizes());
   variable_list r;
   if (wants_autograd({&x, &Wg})) {
     r = BalancedRouterFn::apply(x, Wg, biases, N, K, Ks, valid, groups);

@@ -19,7 +19,8 @@ def balance_loss(logits, mask_NM, num_shared_experts=0, valid=None, per_sequence
     and of tokens that do not count get zeros.  The tensor of counts is the caller's own: summing it over ranks before the backward
     changes no gradient.
 
-    valid: bool [M] or [B, S], False for the tokens that do not count (padding); what their logits hold does not matter.
+    valid: bool [M] or [B, S] (for [M, N] logits any two dimensions that hold M flags in order), False for the tokens that do
+    not count (padding); what their logits hold does not matter.
     per_sequence: the loss is taken for each of the B sequences and averaged over those in which a routed expert holds a token;
     counts are then [B, N].  Without any such token the loss is zero.
     A token that counts and has no routed logit above -inf makes the loss NaN.

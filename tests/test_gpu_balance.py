@@ -364,3 +364,28 @@ def test_counts_are_the_callers_own(per_sequence):
         change(counts)
         got, = torch.autograd.grad(1e3 * loss, router.Wg_DN)
         assert torch.equal(got, through_gate)
+
+
+def test_flags_of_other_shapes_are_refused():
+    """As many flags as tokens, but in another order than theirs."""
+    B, S, N, K, D = 3, 20, 8, 2, 32
+    logits, mask = _inputs(B, S, N, K, 0, torch.float32)
+    l, m = logits.to(DEV), mask.to(DEV)
+    flags = torch.ones(B * S, dtype=torch.bool, device=DEV)
+    flags[50:] = False
+    want, _ = momoe_amd.balance_loss(l, m, valid=flags)
+    moe = momoe_amd.MoE(D, 32, N, K, 0, bias_update_rate=0.0, balance="batch")
+    x = torch.randn(B, S, D, device=DEV, dtype=torch.bfloat16)
+    _, through_moe = moe(x, flags)
+    for good in (flags.view(B, S), flags):
+        assert torch.equal(momoe_amd.balance_loss(l, m, valid=good)[0], want)
+        assert torch.equal(momoe_amd.balance_loss(l.view(B * S, N), m, valid=good)[0], want)
+        assert torch.equal(moe(x, good)[1], through_moe)
+    for bad in (flags.view(S, B), flags.view(B, S).T, flags.view(1, B * S), flags.view(B, S, 1), flags.view(2, B, S // 2)):
+        for per_sequence in (False, True):
+            with pytest.raises(RuntimeError, match="valid must be"):
+                momoe_amd.balance_loss(l, m, valid=bad, per_sequence=per_sequence)
+        with pytest.raises(RuntimeError, match="valid must be"):
+            moe(x, bad)
+    with pytest.raises(RuntimeError, match="valid must be"):
+        momoe_amd.balance_loss(l.view(B * S, N), m, valid=flags.view(B, S, 1))
