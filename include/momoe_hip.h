@@ -380,6 +380,11 @@ int momoe_gate_router_fwd(const void* x_MD, int64_t ldx, const void* Wg_DN, cons
                           int64_t M, int64_t D, int64_t N, int64_t K, int64_t Ks,
                           int32_t* mask_NM, float* s_MN, float* p_sel_MN, float* Ng_M, float* Ks_M,
                           void* workspace, int64_t workspace_bytes, void* stream);
+/* momoe_gate_router_fwd_logits: the same, and the logits to logits_MN bf16 [M,N] (may be NULL). */
+int momoe_gate_router_fwd_logits(const void* x_MD, int64_t ldx, const void* Wg_DN, const float* biases_N,
+                                 int64_t M, int64_t D, int64_t N, int64_t K, int64_t Ks,
+                                 int32_t* mask_NM, float* s_MN, float* p_sel_MN, float* Ng_M, float* Ks_M,
+                                 void* logits_MN, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* momoe_router_bwd replaces normalize_backward_kernel (momoe/topk_router.py:11-56):
  * gradient w.r.t. the gate logits, bf16 [M,N] row-major.  Gs_NM fp32, element (i,m) at

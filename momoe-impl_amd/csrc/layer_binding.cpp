@@ -553,7 +553,7 @@ Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biase
   // Few tokens: the product in the library's kernel, whose launch alone takes the host 18 us
   const int64_t ws_bytes = momoe_gate_router_workspace_bytes(M, D, N);
   const auto aligned = [](const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; };
-  const bool own = !keep_logits && ws_bytes >= 0 && !at::autocast::is_autocast_enabled(at::kCUDA) && Wg.dim() == 2 && Wg.size(0) == D &&
+  const bool own = ws_bytes >= 0 && !at::autocast::is_autocast_enabled(at::kCUDA) && Wg.dim() == 2 && Wg.size(0) == D &&
                    Wg.size(1) == N && Wg.is_contiguous() && aligned(Wg) && aligned(r.x_MD) && r.x_MD.stride(1) == 1 &&
                    r.x_MD.stride(0) >= D && r.x_MD.stride(0) % 8 == 0;
   // Other products come first of all: the GPU has work while the host allocates
@@ -576,9 +576,10 @@ Routed router_forward(const Tensor& x_BSD, const Tensor& Wg, const Tensor& biase
   const hipStream_t st = stream_of(dev);
   if (own) {
     const Tensor ws = empty_f32({ws_bytes / 4}, dev);
-    MOMOE_CALL(momoe_gate_router_fwd, st, r.x_MD.data_ptr(), r.x_MD.stride(0), Wg.data_ptr(), bias.data_ptr<float>(), M, D, N, K,
-               Ks, r.mask.data_ptr<int32_t>(), r.s_MN.data_ptr<float>(), r.p_sel.data_ptr<float>(), norms, norms + M,
-               ws.data_ptr(), ws_bytes);
+    if (keep_logits) r.logits = empty_bf16({M, N}, dev);
+    call("momoe_gate_router_fwd", st, momoe_gate_router_fwd_logits, r.x_MD.data_ptr(), r.x_MD.stride(0), Wg.data_ptr(),
+         bias.data_ptr<float>(), M, D, N, K, Ks, r.mask.data_ptr<int32_t>(), r.s_MN.data_ptr<float>(), r.p_sel.data_ptr<float>(), norms,
+         norms + M, keep_logits ? r.logits.data_ptr() : nullptr, ws.data_ptr(), ws_bytes);
     return r;
   }
   MOMOE_CALL(momoe_router_fwd, st, logits.data_ptr(), logits.scalar_type() == at::kFloat, bias.data_ptr<float>(), M, N, K, Ks,
@@ -747,11 +748,10 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   const int64_t S = M / groups, ws_bytes = momoe_balance_workspace_bytes(groups, S, N);
   TORCH_CHECK(ws_bytes >= 0, "balance loss: [", M, ", ", N, "] logits are past the sizes that it takes (N <= 512)");
   const Tensor ws = empty_f32({ws_bytes / 4}, dev);
-  MOMOE_CALL(momoe_balance_fwd_kept, stream_of(dev), rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
-             mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1),
-             flags.defined() ? (const uint8_t*)flags.data_ptr() : nullptr, groups, S, N, Ks, b.loss.data_ptr<float>(),
-             b.counts.data_ptr<int64_t>(), for_backward ? b.kept.data_ptr<int64_t>() : nullptr, b.info.data_ptr<float>(), ws.data_ptr(),
-             ws_bytes);
+  call("momoe_balance_fwd", stream_of(dev), momoe_balance_fwd_kept, rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
+       mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), flags.defined() ? (const uint8_t*)flags.data_ptr() : nullptr, groups, S,
+       N, Ks, b.loss.data_ptr<float>(), b.counts.data_ptr<int64_t>(), for_backward ? b.kept.data_ptr<int64_t>() : nullptr,
+       b.info.data_ptr<float>(), ws.data_ptr(), ws_bytes);
   return b;
 }
 

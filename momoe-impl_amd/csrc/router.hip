@@ -136,6 +136,7 @@ struct RouterFwdArgs {
   float* psel;
   float* ng;
   float* ks;
+  bf16* sums;  // PARTS: the logits [M][N], for who needs them later; or NULL
 };
 
 // A workgroup handles kTok consecutive tokens.  The mask is [N, M] (token fastest)
@@ -185,6 +186,7 @@ __global__ __launch_bounds__(THREADS) void router_fwd_kernel(RouterFwdArgs p) {
           for (int q = 0; q < AT_ONCE; ++q) sum += q0 + q < p.parts ? t[q] : 0.0f;
         }
         v[c] = (float)(bf16)sum;
+        if (p.sums != nullptr && lane + 64 * c < N) p.sums[(int64_t)m * N + jc] = (bf16)sum;
       } else {
         v[c] = p.logits_f32 ? ((const float*)p.logits)[(int64_t)m * N + jc] : (float)((const bf16*)p.logits)[(int64_t)m * N + jc];
       }
@@ -433,6 +435,14 @@ extern "C" int64_t momoe_gate_router_workspace_bytes(int64_t M, int64_t D, int64
 extern "C" int momoe_gate_router_fwd(const void* x_MD, int64_t ldx, const void* Wg_DN, const float* biases_N, int64_t M, int64_t D,
                                      int64_t N, int64_t K, int64_t Ks, int32_t* mask_NM, float* s_MN, float* p_sel_MN, float* Ng_M,
                                      float* Ks_M, void* workspace, int64_t workspace_bytes, void* stream) {
+  return momoe_gate_router_fwd_logits(x_MD, ldx, Wg_DN, biases_N, M, D, N, K, Ks, mask_NM, s_MN, p_sel_MN, Ng_M, Ks_M, nullptr,
+                                      workspace, workspace_bytes, stream);
+}
+
+extern "C" int momoe_gate_router_fwd_logits(const void* x_MD, int64_t ldx, const void* Wg_DN, const float* biases_N, int64_t M,
+                                            int64_t D, int64_t N, int64_t K, int64_t Ks, int32_t* mask_NM, float* s_MN,
+                                            float* p_sel_MN, float* Ng_M, float* Ks_M, void* logits_MN, void* workspace,
+                                            int64_t workspace_bytes, void* stream) {
   if (!x_MD || !Wg_DN || !biases_N || !mask_NM || !s_MN || !p_sel_MN || !Ng_M || !Ks_M || !workspace) return MOMOE_ERR_BAD_ARG;
   const int status = check_router_fwd(M, N, K, Ks);
   if (status != MOMOE_OK) return status;
@@ -447,7 +457,8 @@ extern "C" int momoe_gate_router_fwd(const void* x_MD, int64_t ldx, const void* 
   gate_logits_kernel<<<grid, GateStage::THREADS, 0, st>>>(g);
   const int launched = launch_status();
   if (launched != MOMOE_OK) return launched;
-  return launch_router_fwd({workspace, 1, (int)grid.x, biases_N, (int)M, (int)N, (int)K, (int)Ks, mask_NM, s_MN, p_sel_MN, Ng_M, Ks_M},
+  return launch_router_fwd({workspace, 1, (int)grid.x, biases_N, (int)M, (int)N, (int)K, (int)Ks, mask_NM, s_MN, p_sel_MN, Ng_M, Ks_M,
+                            (bf16*)logits_MN},
                            st);
 }
 

@@ -76,6 +76,7 @@ _SIGNATURES = {
     "momoe_router_bwd": (_int, [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p]),
     "momoe_gate_router_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "momoe_gate_router_fwd": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "momoe_gate_router_fwd_logits": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "momoe_gate_wgrad_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "momoe_gate_wgrad": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _p]),
     "momoe_backward_tail_fits": (_int, [_i64] * 5),

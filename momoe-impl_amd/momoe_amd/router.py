@@ -42,6 +42,6 @@ class TopKRouter(nn.Module):
         return TopKRouterFunction.apply(x_BSD, self.Wg_DN, biases_N, self.N, self.K, self.Ks)
 
     def with_balance_loss(self, x_BSD, biases_N, valid=None, per_sequence=False):
-        """(x_BSD, mask_NM, s_NM, loss, counts): the router's results and, of the same gate logits, those of
-        `balance_loss`, with one gradient of the logits through the gate product."""
+        """(x_BSD, mask_NM, s_NM, loss, counts): the router's results, bit by bit those of `forward`, and, of the same gate logits,
+        those of `balance_loss`, with one gradient of the logits through the gate product."""
         return _layer.router_balanced(x_BSD, self.Wg_DN, biases_N, self.N, self.K, self.Ks, valid, per_sequence)

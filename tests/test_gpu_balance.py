@@ -389,3 +389,29 @@ def test_flags_of_other_shapes_are_refused():
             moe(x, bad)
     with pytest.raises(RuntimeError, match="valid must be"):
         momoe_amd.balance_loss(l.view(B * S, N), m, valid=flags.view(B, S, 1))
+
+
+@pytest.mark.parametrize("M,D,N,K,Ks", [(1, 64, 8, 2, 0), (128, 256, 16, 2, 0), (300, 512, 64, 6, 2), (1000, 1024, 128, 8, 0), (3000, 128, 60, 4, 0)])
+def test_the_loss_leaves_the_routing_as_it_is(M, D, N, K, Ks):
+    """Mask, gate weights, their gradients and the layer's result, bit by bit those without the loss."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(1, M, D, generator=g).to(DEV, torch.bfloat16)
+    router = momoe_amd.TopKRouter(D, N, K, Ks, Wg_DN=(torch.randn(D, N, generator=g) / D ** 0.5).to(DEV))
+    bias = torch.cat([torch.zeros(N - Ks), torch.full((Ks,), float("-inf"))]).to(DEV)
+    Gs = torch.randn(N, M, generator=g).to(DEV)
+    with torch.no_grad():
+        _, mask, s = router(x, bias)
+        _, mask1, s1, _, counts = router.with_balance_loss(x, bias)
+    assert torch.equal(mask, mask1) and torch.equal(s, s1) and torch.equal(counts, mask.sum(1))
+    results = []
+    for with_loss in (False, True):
+        xr = x.clone().requires_grad_()
+        _, mask1, s1 = (router.with_balance_loss if with_loss else router)(xr, bias)[:3]
+        assert torch.equal(mask, mask1) and torch.equal(s, s1)
+        results.append(torch.autograd.grad((s1 * Gs).sum(), [xr, router.Wg_DN]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    plain = momoe_amd.MoE(D, 32, N, K, Ks, bias_update_rate=0.0)
+    balanced = momoe_amd.MoE(D, 32, N, K, Ks, bias_update_rate=0.0, balance="batch")
+    balanced.load_state_dict(plain.state_dict())
+    with torch.no_grad():
+        assert torch.equal(plain(x), balanced(x)[0])
