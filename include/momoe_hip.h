@@ -478,7 +478,8 @@ int momoe_fp8_pack_weights(const void* W_NRC, int quantized, int64_t N, int64_t 
                            void* stream);
 
 /* Tile height of the table for both products, whichever suits the sizes: MOMOE_FP8_FEW_ROWS for the two entry points momoe_fp8_few_*,
- * 256 for the other two, whose contractions are of up to 8192. */
+ * 256 for the other two, whose contractions are of up to 8192 and whose rows of x take less than 4 GiB in 8 bits: a call of more
+ * (M * momoe_fp8_row_bytes(D) >= 2^32) takes the first two and their height whatever this returns. */
 #define MOMOE_FP8_FEW_ROWS 32
 int momoe_fp8_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N);
 /* momoe_fp8_few_lin1_swiglu_fwd: h fp32 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i].  x: MOMOE_TYPE_*, row pitch ldx, a

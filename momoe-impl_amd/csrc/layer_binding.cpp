@@ -492,7 +492,9 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   x = x.contiguous();
   if ((uintptr_t)x.data_ptr() % 16 != 0) x = x.clone();
 
-  Index ib(M, N, K, momoe_fp8_tile_rows(msum, D, H, N), false);
+  // (the tall tiles gather their rows in 8 bits at 32-bit offsets)
+  const bool far = M * DB * 128 >= (1ll << 32);
+  Index ib(M, N, K, far ? MOMOE_FP8_FEW_ROWS : momoe_fp8_tile_rows(msum, D, H, N), false);
   const bool few = ib.tile_rows == MOMOE_FP8_FEW_ROWS;  // the products bring their rows to 8 bits themselves
   const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
   const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;

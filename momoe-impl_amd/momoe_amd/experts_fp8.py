@@ -26,7 +26,7 @@ class MoMoEFP8(nn.Module):
         [N, ceil(H/128), ceil(D/128)]: a weight is its e4m3 value times the scale of its 128 x 128 block.
     D and H must be multiples of 32.  Each 128 consecutive values of a token (and of its h) are scaled by the least
     power of two that leaves none above 448, e4m3's largest (values below 2^-100 by one of 2^-108); NaN or infinity among
-    them make NaN of the token.  A call takes tokens of up to 4 GiB in 8 bits.
+    them make NaN of the token.
 
     The weights are laid out once, in the order that the kernels read them in; `weights()` gives them back.
     `from_momoe` quantizes the weights of a `MoMoE`.

@@ -433,3 +433,17 @@ def test_nan_among_the_weights(M, byte):
         bad[which].view(torch.uint8)[at] = byte
         y, _ = momoe_amd.MoMoEFP8(D, H, N, K, *bad)(x, mask, s)
         assert torch.equal(y[0].isnan(), nan) and torch.equal(y[0][~nan], ref[0][~nan])
+
+
+@pytest.mark.parametrize("M", [300_000, 540_000])
+def test_tokens_past_32_bit_offsets(M):
+    """Tokens of 2.3 GiB and of 4.1 GiB in 8 bits: the last of them against 64 bits."""
+    D, H = 8192, 32
+    layer, (V1, V2) = _layer(D, H, 1, 1)
+    x = torch.randn(1, M, D, device=DEV, dtype=torch.bfloat16)
+    s = torch.rand(1, M, device=DEV) + 0.5
+    mask = torch.ones(1, M, dtype=torch.int32, device=DEV)
+    y, sizes = layer(x, mask, s)
+    assert sizes.item() == M
+    for at in (slice(0, 8), slice(M // 2, M // 2 + 8), slice(M - 8, M)):
+        _close(y[0, at], oracle.experts_fp8(x[0, at].cpu().double(), V1, V2, mask[:, at].cpu(), s[:, at].cpu()))
