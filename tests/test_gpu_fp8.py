@@ -447,3 +447,10 @@ def test_tokens_past_32_bit_offsets(M):
     assert sizes.item() == M
     for at in (slice(0, 8), slice(M // 2, M // 2 + 8), slice(M - 8, M)):
         _close(y[0, at], oracle.experts_fp8(x[0, at].cpu().double(), V1, V2, mask[:, at].cpu(), s[:, at].cpu()))
+
+
+@pytest.mark.parametrize("M,D,H,N,K", [(700, 8224, 288, 3, 2), (600, 160, 8320, 2, 2), (2000, 8224, 64, 40, 2)])
+def test_many_rows_in_tiles_of_few(M, D, H, N, K):
+    """Contractions past what the tall tiles take: more tiles than experts."""
+    assert _hip.fp8_tile_rows(M * K, D, H, N) == 32 and M * K > 32 * N
+    test_products(M, D, H, N, K, 0, 0.5)
