@@ -116,29 +116,38 @@ __global__ __launch_bounds__(kThreadsFwd) void balance_piece_kernel(BalanceArgs 
   if (threadIdx.x == 0) tokens_of = 0;
   __syncthreads();
 
-  // p summed over the tokens
+  // p summed over the tokens, in chains of 256 at the most and then the chains: over some thousand equal terms the roundings of one
+  // chain go one way
+  constexpr int STEP = kWavesFwd * TPW * AHEAD, CHAIN = 256 / AHEAD * STEP;
   const int j0 = (lane % LPT) * kColsPerLane;
   float sum[kColsPerLane];
 #pragma unroll
   for (int i = 0; i < kColsPerLane; ++i) sum[i] = 0.0f;
-  for (int base = t0 + wave * TPW; base < t1; base += kWavesFwd * TPW * AHEAD) {
-    Columns<T, VEC> col[AHEAD];
-    bool on[AHEAD];
+  for (int from = t0; from < t1; from += CHAIN) {
+    float part[kColsPerLane];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int t = base + a * kWavesFwd * TPW + lane / LPT;
-      const int64_t m = m0 + min(t, t1 - 1);
-      col[a].load((const T*)p.logits + m * p.ld, j0, p.N);
-      on[a] = t < t1 && (p.valid == nullptr || p.valid[m] != 0);
+    for (int i = 0; i < kColsPerLane; ++i) part[i] = 0.0f;
+    for (int base = from + wave * TPW; base < min(t1, from + CHAIN); base += STEP) {
+      Columns<T, VEC> col[AHEAD];
+      bool on[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int t = base + a * kWavesFwd * TPW + lane / LPT;
+        const int64_t m = m0 + min(t, t1 - 1);
+        col[a].load((const T*)p.logits + m * p.ld, j0, p.N);
+        on[a] = t < t1 && (p.valid == nullptr || p.valid[m] != 0);
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        float pr[kColsPerLane];
+        col[a].template softmax<LPT>(j0, p.Ng, pr);
+        // (a token that does not count may hold anything, NaN too)
+#pragma unroll
+        for (int i = 0; i < kColsPerLane; ++i) part[i] += on[a] ? pr[i] : 0.0f;
+      }
     }
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      float pr[kColsPerLane];
-      col[a].template softmax<LPT>(j0, p.Ng, pr);
-      // (a token that does not count may hold anything, NaN too)
-#pragma unroll
-      for (int i = 0; i < kColsPerLane; ++i) sum[i] += on[a] ? pr[i] : 0.0f;
-    }
+    for (int i = 0; i < kColsPerLane; ++i) sum[i] += part[i];
   }
 #pragma unroll
   for (int i = 0; i < kColsPerLane; ++i) {

@@ -415,3 +415,16 @@ def test_the_loss_leaves_the_routing_as_it_is(M, D, N, K, Ks):
     balanced.load_state_dict(plain.state_dict())
     with torch.no_grad():
         assert torch.equal(plain(x), balanced(x)[0])
+
+
+def test_sums_over_many_tokens():
+    """2^27 tokens of the same logits: column sums whose terms would all be rounded the same way."""
+    M, N = 1 << 27, 2
+    logits = torch.tensor([0.0, 0.84375], device=DEV, dtype=torch.bfloat16).repeat(M, 1)
+    mask = torch.zeros(N, M, dtype=torch.int32, device=DEV)
+    mask[0] = 1
+    loss, counts = momoe_amd.balance_loss(logits, mask)
+    assert torch.equal(counts.cpu(), torch.tensor([M, 0]))
+    want = 2 * torch.softmax(torch.tensor([0.0, 0.84375], dtype=torch.float64), 0)[0].item()
+    # the bound of _check: 512 half steps, of p and of chains of some hundred terms at each level of the sums
+    assert abs(loss.item() - want) <= 512 * E * want
