@@ -481,6 +481,8 @@ def fp8_pack_weights(W_NRC, halves):
     N, R, C = W_NRC.shape
     quantized = W_NRC.dtype == torch.float8_e4m3fn
     assert W_NRC.is_contiguous() and (quantized or W_NRC.dtype == torch.bfloat16)
+    if W_NRC.data_ptr() % 16:  # a view into a buffer that holds other things: the kernels read 16 bytes at a time
+        W_NRC = W_NRC.clone()
     nbytes = _lib.momoe_fp8_weight_bytes(N, R, C)
     packed = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=W_NRC.device)
     blocks = lambda n: -(-n // 128)

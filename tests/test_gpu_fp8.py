@@ -454,3 +454,28 @@ def test_many_rows_in_tiles_of_few(M, D, H, N, K):
     """Contractions past what the tall tiles take: more tiles than experts."""
     assert _hip.fp8_tile_rows(M * K, D, H, N) == 32 and M * K > 32 * N
     test_products(M, D, H, N, K, 0, 0.5)
+
+
+def test_weights_anywhere_in_memory():
+    """Views into one buffer, off the boundaries that the kernels read by."""
+    D, H, N, K, M = 96, 64, 4, 2, 30
+    w = _weights(N, D, H)
+    mask, s = [t.to(DEV) for t in make_routing(M, N, K, seed=2)]
+    x = _x(M, D).view(1, M, D).to(DEV)
+    ref, _ = momoe_amd.MoMoEFP8(D, H, N, K, *[t.to(DEV) for t in w])(x, mask, s)
+    placed = []
+    for t in w:
+        raw = torch.empty(t.numel() * t.element_size() + 4, dtype=torch.uint8, device=DEV)[4:]
+        raw.copy_(t.contiguous().view(torch.uint8).reshape(-1))
+        placed.append(raw.view(t.dtype).view(t.shape))
+        assert placed[-1].data_ptr() % 16 == 4
+    assert torch.equal(momoe_amd.MoMoEFP8(D, H, N, K, *placed)(x, mask, s)[0], ref)
+    momoe = momoe_amd.MoMoE(D, H, N, K)
+    ref = momoe_amd.MoMoEFP8.from_momoe(momoe).weights()
+    for name in ("Wl1_ND2H", "Wl2_NHD"):
+        p = getattr(momoe, name)
+        off = torch.empty(p.numel() + 2, dtype=p.dtype, device=DEV)[2:].view(p.shape)
+        p.data = off.copy_(p.data)
+        assert p.data_ptr() % 16 == 4
+    for a, b in zip(momoe_amd.MoMoEFP8.from_momoe(momoe).weights(), ref):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
