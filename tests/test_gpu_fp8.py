@@ -479,3 +479,30 @@ def test_weights_anywhere_in_memory():
         assert p.data_ptr() % 16 == 4
     for a, b in zip(momoe_amd.MoMoEFP8.from_momoe(momoe).weights(), ref):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("M,D,H", [
+    *[(9000, 2080, H) for H in (96, 256, 384, 512, 640)],  # the second product's tiles, of 1 to 5 blocks of its contraction
+    *[(9000, D, 1120) for D in (96, 256, 384, 512, 640)],  # the first one's
+    (9000, 1120, 1120),
+])
+def test_tiles_one_behind_the_other(M, D, H):
+    """Two tiles and more a workgroup do what they do in calls of fewer tokens, a tile a workgroup: a row's results are its own."""
+    N, K = 6, 2
+    layer, (V1, V2) = _layer(D, H, N, K)
+    mask, s = make_routing(M, N, K, seed=2, skew=0.5)
+    x = _x(M, D)
+    row_tiles = lambda m: ((m.sum(1) + 255) // 256).sum().item()
+    blocks = {"first": -(-H // 128), "second": -(-D // 256)}
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert max(blocks.values()) * row_tiles(mask) > 2 * cus
+    assert _hip.fp8_tile_rows(M * K, D, H, N) == _hip.fp8_tile_rows(500 * K, D, H, N) == 256
+    y, sizes = layer(x.view(1, M, D).to(DEV), mask.to(DEV), s.to(DEV))
+    assert torch.equal(sizes.cpu(), mask.sum(1))
+    for at in range(0, M, 500):
+        part = slice(at, at + 500)
+        assert max(blocks.values()) * row_tiles(mask[:, part]) <= cus
+        few, _ = layer(x[part].view(1, -1, D).to(DEV), mask[:, part].contiguous().to(DEV), s[:, part].to(DEV))
+        assert torch.equal(few[0], y[0, part])
+    at = slice(M - 200, M)
+    _close(y[0, at], oracle.experts_fp8(x[at], V1, V2, mask[:, at], s[:, at]))
