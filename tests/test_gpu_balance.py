@@ -428,3 +428,12 @@ def test_sums_over_many_tokens():
     want = 2 * torch.softmax(torch.tensor([0.0, 0.84375], dtype=torch.float64), 0)[0].item()
     # the bound of _check: 512 half steps, of p and of chains of some hundred terms at each level of the sums
     assert abs(loss.item() - want) <= 512 * E * want
+
+
+@pytest.mark.parametrize("B,S,N,K", [(65, 500, 64, 4), (70, 1000, 33, 2), (130, 910, 16, 2), (130, 911, 16, 2), (260, 2000, 8, 1)])
+@pytest.mark.parametrize("padded", [False, True])
+def test_many_long_sequences(B, S, N, K, padded):
+    """More than 64 sequences, on both sides of the line from which each is cut into pieces."""
+    logits, mask = _inputs(B, S, N, K, 0, torch.bfloat16)
+    valid = torch.arange(S)[None] < torch.arange(0, B * 37, 37)[:, None] % (S + 1) if padded else None
+    _check(logits, mask, 0, valid, True, *_run(logits, mask, 0, valid, True, 0.01), 0.01)
