@@ -716,10 +716,14 @@ int64_t pitch_of(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride
 
 struct Balanced {
   Tensor loss, counts;  // results: [], [groups, N]
-  // For the backward, with the logits.  `valid` may be undefined, and has the shape that it came in.  `kept`: the counts once more:
-  // the others are the caller's, who may sum them over ranks before the backward, which autograd does not see.
-  Tensor valid, kept, info;
+  // For the backward, with the logits.  `valid` may be undefined, and has the shape that it came in.  `kept`: info, and behind it the
+  // counts once more: the others are the caller's, who may sum them over ranks before the backward, which autograd does not see.
+  // (One tensor: each takes the host 1.5 us to make, save and find.)
+  Tensor valid, kept;
 };
+// int64 places of info, of which it takes half of one for each group and one for all; kept_of: those of `kept`
+int64_t info_of(int64_t groups) { return groups / 2 + 1; }
+int64_t kept_of(int64_t groups, int64_t N) { return info_of(groups) + groups * N; }
 
 // logits [.., N] of one of the three types, `groups` of as many tokens each; `valid` as check_valid takes it
 Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks, const std::optional<Tensor>& valid,
@@ -737,14 +741,12 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
     flags = flags_of(b.valid, M);
   }
   b.counts = at::empty({groups, N}, at::TensorOptions().dtype(at::kLong).device(dev));
-  if (for_backward) b.kept = at::empty_like(b.counts);
+  b.kept = at::empty({for_backward ? kept_of(groups, N) : info_of(groups)}, b.counts.options());
   b.loss = empty_f32({}, dev);
-  b.info = empty_f32({1 + groups}, dev);
   if (M == 0) {
     b.counts.zero_();
-    if (for_backward) b.kept.zero_();
+    b.kept.zero_();
     b.loss.zero_();
-    b.info.zero_();
     return b;
   }
   const int64_t S = M / groups, ws_bytes = momoe_balance_workspace_bytes(groups, S, N);
@@ -752,48 +754,48 @@ Balanced balance_forward(const Tensor& logits, const Tensor& mask_NM, int64_t Ks
   const Tensor ws = empty_f32({ws_bytes / 4}, dev);
   call("momoe_balance_fwd", stream_of(dev), momoe_balance_fwd_kept, rows.data_ptr(), type_of(rows.scalar_type()), pitch_of(rows),
        mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), flags.defined() ? (const uint8_t*)flags.data_ptr() : nullptr, groups, S,
-       N, Ks, b.loss.data_ptr<float>(), b.counts.data_ptr<int64_t>(), for_backward ? b.kept.data_ptr<int64_t>() : nullptr,
-       b.info.data_ptr<float>(), ws.data_ptr(), ws_bytes);
+       N, Ks, b.loss.data_ptr<float>(), b.counts.data_ptr<int64_t>(), for_backward ? b.kept.data_ptr<int64_t>() + info_of(groups) : nullptr,
+       (float*)b.kept.data_ptr(), ws.data_ptr(), ws_bytes);
   return b;
 }
 
-// d loss / d logits, of type `type`, + `add` in its place if that is defined
-Tensor balance_gradient(const Tensor& logits, const Tensor& valid, const Tensor& counts, const Tensor& info, const Tensor& G_loss,
-                        int64_t Ks, at::ScalarType type, const Tensor& add) {
-  const at::Device dev = logits.device();
-  const int64_t M = logits.size(0), N = logits.size(1), groups = counts.size(0);
-  const Tensor g = G_loss.to(dev, at::kFloat).contiguous();
-  Tensor out = add.defined() ? add : at::empty({M, N}, at::TensorOptions().dtype(type).device(dev));
-  if (M == 0) return out;
-  MOMOE_CALL(momoe_balance_bwd, stream_of(dev), logits.data_ptr(), type_of(logits.scalar_type()), pitch_of(logits),
-             valid.defined() ? (const uint8_t*)valid.data_ptr() : nullptr, counts.data_ptr<int64_t>(), info.data_ptr<float>(),
-             g.data_ptr<float>(), add.defined() ? (const void*)add.data_ptr() : nullptr, out.data_ptr(), type_of(type), groups,
-             M / groups, N, Ks);
-  return out;
-}
-
-// What the forward saved, as balance_gradient takes it: logits, valid, counts, info from `saved[at]` on
+// What the forward saved, as balance_gradient takes it: logits, valid, kept from `saved[at]` on
 struct BalanceSaved {
-  Tensor logits, valid, counts, info;
+  Tensor logits, valid, kept;
+  int64_t groups;
   BalanceSaved(const variable_list& saved, size_t at, const at::Device& dev, at::ScalarType type, at::IntArrayRef sizes, int64_t M,
-               int64_t N, int64_t groups) {
+               int64_t N, int64_t groups_)
+      : groups(groups_) {
     logits = rows_of(as_saved(saved[at], "logits", dev, type, sizes, /*packed=*/false), M, N);
     if (saved[at + 1].defined()) {
       const Tensor& v = saved[at + 1];
       TORCH_CHECK(v.numel() == M, "backward: the saved tensor valid came back from its hook in another size");
       valid = flags_of(as_saved(v, "valid", dev, at::kBool, v.sizes(), /*packed=*/false), M);
     }
-    counts = as_saved(saved[at + 2], "counts", dev, at::kLong, {groups, N});
-    info = as_saved(saved[at + 3], "info", dev, at::kFloat, {1 + groups});
+    kept = as_saved(saved[at + 2], "counts", dev, at::kLong, {kept_of(groups, N)});
   }
 };
+
+// d loss / d logits, of type `type`, + `add` in its place if that is defined
+Tensor balance_gradient(const BalanceSaved& t, const Tensor& G_loss, int64_t Ks, at::ScalarType type, const Tensor& add) {
+  const at::Device dev = t.logits.device();
+  const int64_t M = t.logits.size(0), N = t.logits.size(1);
+  const Tensor g = G_loss.to(dev, at::kFloat).contiguous();
+  Tensor out = add.defined() ? add : at::empty({M, N}, at::TensorOptions().dtype(type).device(dev));
+  if (M == 0) return out;
+  MOMOE_CALL(momoe_balance_bwd, stream_of(dev), t.logits.data_ptr(), type_of(t.logits.scalar_type()), pitch_of(t.logits),
+             t.valid.defined() ? (const uint8_t*)t.valid.data_ptr() : nullptr, t.kept.data_ptr<int64_t>() + info_of(t.groups),
+             (const float*)t.kept.data_ptr(), g.data_ptr<float>(), add.defined() ? (const void*)add.data_ptr() : nullptr, out.data_ptr(),
+             type_of(type), t.groups, M / t.groups, N, Ks);
+  return out;
+}
 
 struct BalanceFn : torch::autograd::Function<BalanceFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& mask, int64_t Ks,
                                const std::optional<Tensor>& valid, int64_t groups) {
     Balanced b = balance_forward(logits, mask, Ks, valid, groups, /*for_backward=*/true);
     // (logits and valid as they came: a view made here would hide from autograd that they changed since)
-    ctx->save_for_backward({logits, b.valid, b.kept, b.info});
+    ctx->save_for_backward({logits, b.valid, b.kept});
     ctx->saved_data["call"] = std::vector<int64_t>{Ks, groups, logits.device().index(), (int64_t)logits.scalar_type()};
     ctx->saved_data["sizes"] = logits.sizes().vec();
     ctx->mark_non_differentiable({b.counts});
@@ -811,7 +813,7 @@ struct BalanceFn : torch::autograd::Function<BalanceFn> {
     const c10::DeviceGuard guard(dev);
     const BalanceSaved t(ctx->get_saved_variables(), 0, dev, type, sizes, c10::multiply_integers(sizes.begin(), sizes.end() - 1),
                          sizes.back(), call_of[1]);
-    out[0] = balance_gradient(t.logits, t.valid, t.counts, t.info, grads[0], call_of[0], type, {}).view(sizes);
+    out[0] = balance_gradient(t, grads[0], call_of[0], type, {}).view(sizes);
     return out;
   }
 };
@@ -864,7 +866,7 @@ struct BalancedRouterFn : torch::autograd::Function<BalancedRouterFn> {
                                int64_t Ks, const std::optional<Tensor>& valid, int64_t groups) {
     Routed r = router_forward(x, Wg, biases, N, K, Ks, /*keep_logits=*/true);
     Balanced b = balance_forward(r.logits, r.mask, Ks, valid, groups, /*for_backward=*/true);
-    ctx->save_for_backward({r.x_MD, Wg, r.mask, r.p_sel, r.s_MN, r.norms, r.logits, b.valid, b.kept, b.info});
+    ctx->save_for_backward({r.x_MD, Wg, r.mask, r.p_sel, r.s_MN, r.norms, r.logits, b.valid, b.kept});
     ctx->saved_data["call"] = std::vector<int64_t>{Ks, N, Wg.device().index(), x.size(0), x.size(1), x.size(2), groups,
                                                    (int64_t)r.logits.scalar_type()};
     ctx->mark_non_differentiable({r.mask, b.counts});
@@ -884,7 +886,8 @@ struct BalancedRouterFn : torch::autograd::Function<BalancedRouterFn> {
     if (G_loss.defined()) {
       TORCH_CHECK(!at::GradMode::is_enabled(), "the balance loss has no second derivative: call backward without create_graph");
       const BalanceSaved t(saved, 6, dev, (at::ScalarType)call_of[7], {M, N}, M, N, call_of[6]);
-      G_logit = balance_gradient(t.logits, t.valid, t.counts, t.info, G_loss, Ks, at::kBFloat16, G_logit);
+      // (where both come back the router's is rounded to bf16 first, as without the loss, and their sum again: two half steps)
+      G_logit = balance_gradient(t, G_loss, Ks, at::kBFloat16, G_logit);
     }
     variable_list out(8);
     gate_gradients(ctx, saved, dev, G_x, G_logit, {call_of[3], call_of[4], D}, N, out);
