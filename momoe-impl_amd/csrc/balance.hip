@@ -14,7 +14,8 @@
 //
 // Bound by launches up to some ten thousand tokens, then by the reads of the mask, four bytes an element.  Pieces, their sum, gradient:
 // 8, 6, 6 us for 8192 x 128 bf16 logits, 14, 6, 9 us for 65536 x 64 (25 MB forward, 16 backward: 1.8 TB/s each).
-// No atomics: the column sums of a workgroup's tokens go to the workspace and one workgroup adds them in a fixed order.
+// The column sums of a workgroup's tokens go to the workspace and one workgroup adds them in a fixed order: the same bits each time.
+// (Atomics count tokens only, whole numbers in LDS.)
 #include "lanes.hpp"
 
 namespace momoe {
@@ -322,9 +323,10 @@ __global__ __launch_bounds__(kThreadsFwd) void balance_bwd_kernel(BalanceBwdArgs
   const int j0 = (lane % LPT) * kColsPerLane;
   const float per_group = p.info[1 + g], weight = *p.g_loss * p.info[0] * per_group;
   const bool any = per_group != 0.0f;
-  float c[kColsPerLane];
+  int64_t count[kColsPerLane];
 #pragma unroll
-  for (int i = 0; i < kColsPerLane; ++i) c[i] = j0 + i < p.Ng ? (float)p.counts[(int64_t)g * p.N + j0 + i] : 0.0f;
+  for (int i = 0; i < kColsPerLane; ++i) count[i] = p.counts[(int64_t)g * p.N + min(j0 + i, p.Ng - 1)];
+  float c[kColsPerLane];
   for (int base = t0 + wave * TPW; base < t1; base += kWavesFwd * TPW * AHEAD) {
     Columns<T, VEC> col[AHEAD];
     Columns<U, VEC> add[AHEAD];
@@ -336,6 +338,16 @@ __global__ __launch_bounds__(kThreadsFwd) void balance_bwd_kernel(BalanceBwdArgs
       col[a].load((const T*)p.logits + m * p.ld, j0, p.N);
       if (p.add != nullptr) add[a].load((const U*)p.add + m * p.N, j0, p.N);
       on[a] = any && (p.valid == nullptr || p.valid[m] != 0);
+    }
+    if (base == t0 + wave * TPW) {  // (behind the first tokens' requests)
+      // Counts from their mean on: the p add up to one, so that all may be less by the same, and of an even load nothing but the
+      // differences is left of them.
+      float all = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kColsPerLane; ++i) all += j0 + i < p.Ng ? (float)count[i] : 0.0f;
+      const int64_t mean = (int64_t)(sum_over_lanes<LPT>(all) / (float)p.Ng);
+#pragma unroll
+      for (int i = 0; i < kColsPerLane; ++i) c[i] = j0 + i < p.Ng ? (float)(count[i] - mean) : 0.0f;
     }
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {

@@ -29,7 +29,6 @@ struct Fp8Args {
   int64_t sn, sm;
   uint16_t* out;           // [Msum][D / 8] packets
   int D, DB;
-  int64_t msum;
 };
 
 // LDS of a block's rows: [row][128], the 16-byte piece c of row r at position c ^ ((r / 2) % 8): the 16 rows x 16 bytes that 16 lanes
@@ -235,11 +234,13 @@ __global__ __launch_bounds__(kThreads, 4) void fp8_few_rows_kernel(FewArgs p) {
 // behind the first rows, not at its end: by then the next stage's rows have landed for every wavefront, and the slot of the
 // last one is free.
 //
-// Bound by power.  8192 tokens, 2048 x 768, 8 of 128 experts: x . Wl1 235 to 265 us (1.6 to 1.75 PFLOP/s), h . Wl2 165 to 177, at
-// 1.78 GHz with the matrix cores half busy; the same with zeros for data takes 216 and 146, and without the fp32 sums 209 and 146.  A
-// library's plain product of 8192^3 reaches 2.98 PFLOP/s, with neither block scales nor an epilogue.  Two wavefronts of a SIMD half a stage
-// apart: 274 to 277 and 180.  128 rows x 64 columns a wavefront, half the reads of LDS: 306 and 256, with spills.  The tile's end (h, its
-// largest, packing; packets of 15 bits) is 10 to 18 thousand clocks, a stage 3400.
+// Bound by the issue of what is not a product, and by the clock.  8192 tokens, 2048 x 768, 8 of 128 experts: x . Wl1 235 to 265 us (1.6 to
+// 1.75 PFLOP/s), h . Wl2 165 to 177.  A stage takes 3400 clocks, of which the 64 matrix instructions of a SIMD's two wavefronts
+// are some 2050; the fp32 sums are part of the rest (without them 209 and 146 us).  The clock is 1.78 GHz under this data: with zeros the same
+// takes 216 and 146.  A tile's end (h, its largest, packing; packets of 15 bits) is 10 to 18 thousand clocks with no product beside
+// it: in h . Wl2, whose six stages are 20 thousand, a third to nearly half of the tile.  A library's plain product of 8192^3 reaches 2.98
+// PFLOP/s, with neither block scales nor such an end.  Two wavefronts of a SIMD half a stage apart: 274 to 277 and 180.  128 rows x 64
+// columns a wavefront, half the reads of LDS: 306 and 256, with spills.
 constexpr int kTileRows = 256, kTileBlocks = 64;  // most blocks of a contraction
 constexpr int kTileSlot = kTileRows * kFp8Block, kSlots = 3;
 constexpr int kTileCodes = kTileRows * kTileBlocks;  // bytes: [four blocks][row][block]
@@ -584,9 +585,11 @@ int check_fp8(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum) {
     return MOMOE_ERR_UNSUPPORTED;
   return MOMOE_OK;
 }
-// Whether the weights, each read by one tile, do better past the last-level cache.  128 experts of 2048 x 768: the first product's,
-// 384 MiB, with the hint take 71 us instead of 79 for 16 tokens and 77 instead of 80 for 1000; the second's, 192 MiB, 44 instead of 41
-// and 57 instead of 49.
+// Whether the weights, each read by one tile, go past the last-level cache: those that do not fit it.  With the hint | without, us between
+// events, calls one behind the other.  128 experts of 2048 x 768, the first product's 384 MiB: 16 tokens 43 | 46, 131 69 | 75, 1000
+// 80 | 85.  64 experts of 1024 x 768, which stay in the cache from call to call, 96 and 48 MiB: 16 tokens 19.0 | 18.8 and 13.4 | 12.8, 500 33.2 | 32.2
+// and 21.5 | 18.4.  (In between, and where other layers' data pass through the cache before the next call, the hint would win
+// below the line, too: the second product's 192 MiB of the 128 experts 26 | 28 at 16 tokens, 37 | 43 at 131, 58 | 59 at 1000.)
 template <class A>
 bool read_once(const A& a, int64_t Msum, int64_t N, int64_t tile_rows) {
   return Msum <= tile_rows * N && std::min(N, Msum) * a.pairs * 2 * a.KB * kFp8Frag >= kBeyondCache;
@@ -646,7 +649,6 @@ extern "C" int momoe_fp8_lin1_swiglu_fwd(const void* x_q, const void* x_codes, c
   a.hq = (uint8_t*)h_q;
   a.h_codes = (uint8_t*)h_codes;
   a.HB = (int)fp8_blocks(H);
-  a.msum = Msum;
   return launch_tiles<true>(a, M, D, H, N, Msum, (hipStream_t)stream);
 }
 
@@ -665,7 +667,6 @@ extern "C" int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, co
   a.out = (uint16_t*)ys_packets;
   a.D = (int)D;
   a.DB = (int)fp8_blocks(D);
-  a.msum = Msum;
   return launch_tiles<false>(a, M, D, H, N, Msum, (hipStream_t)stream);
 }
 

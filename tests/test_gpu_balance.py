@@ -437,3 +437,31 @@ def test_many_long_sequences(B, S, N, K, padded):
     logits, mask = _inputs(B, S, N, K, 0, torch.bfloat16)
     valid = torch.arange(S)[None] < torch.arange(0, B * 37, 37)[:, None] % (S + 1) if padded else None
     _check(logits, mask, 0, valid, True, *_run(logits, mask, 0, valid, True, 0.01), 0.01)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("per_sequence", [False, True])
+def test_gradient_of_an_even_load(dtype, per_sequence):
+    """Counts that are all the same: none.  Counts of half a million that differ by a few: as exact as their differences, which is what
+    the loss is there for."""
+    B, S, N, Ks = 2, 1 << 18, 5, 1
+    logits = torch.randn(B, S, N, generator=torch.Generator().manual_seed(3)).to(dtype)
+    mask = torch.ones(N, B * S, dtype=torch.int32)
+    _, _, grad = _run(logits, mask, Ks, None, per_sequence, 1e6)
+    assert (grad == 0).all()
+    mask[1, [0, S + 7]] = 0
+    mask[2, [5, 9, S, S + 1]] = 0
+    loss, counts, grad = _run(logits, mask, Ks, None, per_sequence, 1e6)
+    _check(logits, mask, Ks, None, per_sequence, loss, counts, grad, 1e6)
+    groups = B if per_sequence else 1
+    _, n, g = oracle.balance_loss(logits.reshape(-1, N), mask, Ks, None, groups, 1e6)
+    n, p = n[:, :N - Ks].double(), torch.softmax(logits.reshape(-1, N)[:, :N - Ks].double(), -1)
+    # Written with the counts' distances from their whole mean, which changes nothing as the p add up to one, the two terms of the
+    # difference are p_j |c_j - mean| and p_j sum_i p_i |c_i - mean|: with every p good to 64 + 8 half steps as in _check, 128 of
+    # these bound it.
+    apart = (n - n.mean(1, keepdim=True).floor()).abs().repeat_interleave(B * S // groups, 0)
+    scale = 1e6 * (N - Ks) / (B * S // groups) / n.sum(1).repeat_interleave(B * S // groups)[:, None] / groups
+    bound = 128 * E * scale * p * (apart + (apart * p).sum(-1, keepdim=True))
+    bound += g[:, :N - Ks].abs() * torch.finfo(dtype).eps / 2
+    off = (grad.cpu().reshape(-1, N).double() - g)[:, :N - Ks].abs()
+    assert (off <= bound).all(), (off / bound).max()
