@@ -13,7 +13,7 @@
 // steps for two elements a lane as for sixteen.)
 //
 // Bound by launches up to some ten thousand tokens, then by the reads of the mask, four bytes an element.  Pieces, their sum, gradient:
-// 8, 6, 6 us for 8192 x 128 bf16 logits, 14, 6, 9 us for 65536 x 64 (25 MB forward, 16 backward: 1.8 TB/s each).
+// 8, 6, 6 us for 8192 x 128 bf16 logits, 15, 6, 9 us for 65536 x 64 (25 MB forward, 16 backward: 1.7 and 1.8 TB/s).
 // The column sums of a workgroup's tokens go to the workspace and one workgroup adds them in a fixed order: the same bits each time.
 // (Atomics count tokens only, whole numbers in LDS.)
 #include "lanes.hpp"
