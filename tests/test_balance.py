@@ -46,3 +46,16 @@ def test_host_checks():
         momoe_amd.balance_loss(torch.zeros(4, 8), torch.zeros(8, 4, dtype=torch.int32))
     with pytest.raises(ValueError, match="balance must be"):
         momoe_amd.MoE(32, 32, 4, 2, 0, balance="tokens")
+
+
+def test_refusals_of_the_entry_points_with_another_output():
+    """As those without: before any launch."""
+    p, lib = 4096, _hip._lib
+    good = dict(logits=p, type=0, ld=64, mask=p, sn=128, sm=1, valid=None, G=2, S=64, N=64, Ks=4, loss=p, counts=p, kept=p, info=p, ws=p, bytes=1 << 20)
+    kept = lambda **c: lib.momoe_balance_fwd_kept(*{**good, **c}.values(), None)
+    assert all(kept(**{k: None}) == 1 for k in ("logits", "mask", "loss", "counts", "info", "ws"))
+    assert kept(type=3) == kept(ld=63) == kept(Ks=64) == kept(ws=p + 8) == kept(bytes=0) == 1 and kept(N=513, ld=513) == 2
+    gate = dict(x=p, ldx=64, Wg=p, bias=p, M=4, D=64, N=8, K=2, Ks=0, mask=p, s=p, psel=p, ng=p, ks=p, logits=p, ws=p, bytes=1 << 20)
+    route = lambda **c: lib.momoe_gate_router_fwd_logits(*{**gate, **c}.values(), None)
+    assert all(route(**{k: None}) == 1 for k in ("x", "Wg", "bias", "mask", "s", "psel", "ng", "ks", "ws"))
+    assert route(M=0) == route(K=9) == route(ldx=56) == route(x=p + 8) == route(bytes=0) == 1 and route(N=12) == route(ldx=68) == 2
