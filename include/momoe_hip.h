@@ -510,6 +510,45 @@ int momoe_fp8_lin2_scale_fwd(const void* h_q, const void* h_codes, const void* W
 int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K,
                       int64_t Msum, void* stream);
 
+/* ---- SwiGLU blocks with weights in 4 bits, forward only -------------------------------
+ * No counterpart in the reference, whose weights are bf16.  A weight is (code - zero) * scale: a 4-bit code, and for each `group`
+ * (32, 64 or 128) consecutive k-values of a column a zero from 0 to 15 and a scale in bf16 or fp16.  Rows are bf16, sums fp32; h is
+ * rounded to bf16.  A NaN or an infinity in a row of x makes NaN of all its results (so may one above 2^113, whose products with
+ * codes can be infinite on the way).
+ * momoe_int4_pack_weights: codes_NRC [N][R / 2][C] bytes, k-value 2 r of column c in the low half of byte (r, c), 2 r + 1 in the high
+ * one; scale (scale_type: MOMOE_TYPE_BF16 or _F16) and zero (one byte each, of which the low four bits count; NULL: 8 throughout)
+ * [N][ceil(R / group)][C]; `halves` 2 for Wl1, whose columns are the linear half and that of the SiLU, 1 for Wl2; R a multiple of 32, C of
+ * 16 * halves.  packed: momoe_int4_weight_bytes(N, R, C) bytes, words: momoe_int4_scale_words(N, R, C, group) 32-bit words, both on
+ * 16-byte boundaries, in the order that the kernels read them in:
+ *   packed [N][groups of 16 columns][ceil(R / 128)][64][4] words: word m of piece l holds the codes of k-values 32 m + 8 (l / 16) .. +7
+ *          of column l % 16, k-value 2 i in bits 4 i .. +3, 2 i + 1 in bits 16 + 4 i .. +3; the groups of the two halves in turn
+ *   words  [N][groups of 16 columns][ceil(R / 128)][16][128 / group]: the bits of the scale as fp32, the zero in the low four
+ */
+int64_t momoe_int4_weight_bytes(int64_t N, int64_t R, int64_t C);
+int64_t momoe_int4_scale_words(int64_t N, int64_t R, int64_t C, int group);
+int momoe_int4_pack_weights(const void* codes_NRC, const void* scale, int scale_type, const void* zero, int64_t N, int64_t R, int64_t C,
+                            int halves, int group, void* packed, void* words, void* stream);
+
+/* The experts.  tile_table: of momoe_index_build for tile_rows = momoe_int4_tile_rows(Msum, N) rows.
+ * momoe_int4_lin1_swiglu_fwd: h bf16 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i]; x bf16 with row pitch ldx, a multiple of 8.
+ * momoe_int4_lin2_scale_fwd: ys fp32 [Msum][D], ys[r] = (h[r] . Wl2[i]) * s[i, idx[r]].
+ * momoe_int4_combine: out_MD bf16 [M][D], out[m] = the sum of its experts' rows, in fp32, rounded once.
+ * Pointers to rows, weights and results on 16-byte boundaries. */
+int momoe_int4_tile_rows(int64_t Msum, int64_t N);
+int momoe_int4_lin1_swiglu_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, int group,
+                               const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH, int64_t M, int64_t D,
+                               int64_t H, int64_t N, int64_t Msum, void* stream);
+int momoe_int4_lin2_scale_fwd(const void* h_MsumH, const void* Wl2_packed, const void* Wl2_words, int group, const float* s_NM,
+                              int64_t s_stride_n, int64_t s_stride_m, const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows,
+                              float* ys_MsumD, int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);
+int momoe_int4_combine(const float* ys_MsumD, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K, int64_t Msum,
+                       void* stream);
+
+/* A dense block: y = (a * b * sigmoid(b)) . Wl2, a | b = x . Wl1, weights as of one expert.  x bf16 with row pitch ldx, a multiple of 8;
+ * h_MH bf16 [M][H] scratch; y bf16 [M][D].  All on 16-byte boundaries. */
+int momoe_int4_ffn_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, const void* Wl2_packed,
+                       const void* Wl2_words, int group, void* h_MH, void* y_MD, int64_t M, int64_t D, int64_t H, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -540,6 +540,102 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes};
 }
 
+// ---- blocks with weights in 4 bits --------------------------------------------------------------
+// [M, D] bf16 rows on a 16-byte boundary, of the device the weights are on; any other type is rounded to bf16
+Tensor rows_in_bf16(const Tensor& x, int64_t M, int64_t D, const at::Device& dev) {
+  Tensor rows = x.reshape({M, D}).to(dev, at::kBFloat16);
+  if (rows.stride(1) != 1 || (M > 1 && (rows.stride(0) < D || rows.stride(0) % 8 != 0))) rows = rows.contiguous();
+  if ((uintptr_t)rows.data_ptr() % 16 != 0) rows = rows.clone(at::MemoryFormat::Contiguous);
+  return rows;
+}
+bool held_int4(const Tensor& W, const Tensor& S, const at::Device& dev, int64_t N, int64_t R, int64_t C, int64_t group) {
+  const auto held = [&](const Tensor& t, at::ScalarType type, int64_t n) {
+    return t.device() == dev && t.scalar_type() == type && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 && t.numel() == n;
+  };
+  return held(W, at::kByte, momoe_int4_weight_bytes(N, R, C)) && held(S, at::kInt, momoe_int4_scale_words(N, R, C, (int)group));
+}
+
+// x [B, S, D]; W1, W2 packed, S1, S2 words of their scales and zeros; forward only
+std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, const Tensor& S1, const Tensor& W2, const Tensor& S2,
+                                        const Tensor& mask_NM, const Tensor& s_NM, int64_t K, int64_t H, int64_t group, bool check) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<std::tuple<Tensor, Tensor>, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                         const Tensor&, const Tensor&, int64_t, int64_t, int64_t, bool>("momoe::experts_int4", x_BSD, W1, S1, W2, S2,
+                                                                                       mask_NM, s_NM, K, H, group, check);
+  TORCH_CHECK(W1.is_cuda(), "MoMoEInt4 weights must live on the GPU: there is no CPU compute path");
+  TORCH_CHECK(!wants_autograd({&x_BSD, &s_NM}),
+              "MoMoEInt4 has no backward, and an input requires a gradient: call it under torch.no_grad()");
+  const at::Device dev = W1.device();
+  if (x_BSD.dim() != 3) throw_python(PyExc_AssertionError, "x_BSD must be [B, S, D]");
+  const int64_t B = x_BSD.size(0), S = x_BSD.size(1), D = x_BSD.size(2), M = B * S;
+  TORCH_CHECK(K >= 1, "K, the experts of a token, must be at least 1, got ", K);
+  const int64_t N = mask_NM.dim() == 2 ? mask_NM.size(0) : 0, msum = M * K;
+  if (!held_int4(W1, S1, dev, N, D, 2 * H, group) || !held_int4(W2, S2, dev, N, H, D, group))
+    throw_python(PyExc_AssertionError, "x_BSD [B,S,D], mask_NM [N,M] and the packed weights do not fit together");
+  const c10::DeviceGuard guard(dev);
+  const hipStream_t st = stream_of(dev);
+  const Tensor mask = mask_NM.to(dev, at::kInt), s = s_NM.to(dev, at::kFloat);
+  TORCH_CHECK(mask.size(1) == M, "mask_NM must be [", N, ", ", M, "]");
+  TORCH_CHECK(s.dim() == 2 && s.size(0) == N && s.size(1) == M, "s_NM must be [", N, ", ", M, "]");
+  Tensor y = empty_bf16({B, S, D}, dev), sizes = at::empty({N}, at::TensorOptions().dtype(at::kLong).device(dev));
+  if (M == 0) return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes.zero_()};
+  const Tensor x = rows_in_bf16(x_BSD, M, D, dev);
+
+  const int tile_rows = momoe_int4_tile_rows(msum, N);
+  Index ib(M, N, K, tile_rows, false);
+  const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
+  const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
+  Transients transients(dev, {index_bytes, scratch_bytes, msum * H * 2, msum * D * 4});
+  Tensor index_own, scratch, h_own, ys_own, counter;
+  ib.base = (int32_t*)transients.take(index_bytes, index_own);
+  int32_t* const build = (int32_t*)transients.take(scratch_bytes, scratch);
+  int32_t* violations = build;
+  if (check) {
+    counter = at::zeros({4}, at::TensorOptions().dtype(at::kInt).device(dev));
+    violations = counter.data_ptr<int32_t>();
+  }
+  MOMOE_CALL(momoe_index_build, st, mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), M, N, K, sizes.data_ptr<int64_t>(),
+             ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), tile_rows, (int32_t*)nullptr,
+             (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
+  void* const h = transients.take(msum * H * 2, h_own);
+  MOMOE_CALL(momoe_int4_lin1_swiglu_fwd, st, x.data_ptr(), M > 1 ? x.stride(0) : D, W1.data_ptr(), S1.data_ptr(), (int)group,
+             (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, h, M, D, H, N, msum);
+  float* const ys = (float*)transients.take(msum * D * 4, ys_own);
+  MOMOE_CALL(momoe_int4_lin2_scale_fwd, st, h, W2.data_ptr(), S2.data_ptr(), (int)group, (const float*)s.data_ptr<float>(), s.stride(0),
+             s.stride(1), (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, ys, M, D, H, N, msum);
+  MOMOE_CALL(momoe_int4_combine, st, (const float*)ys, (const int32_t*)ib.inv(), y.data_ptr(), M, D, K, msum);
+  if (check) {
+    const int v = counter.narrow(0, 0, 1).item<int32_t>();
+    TORCH_CHECK(v == 0, "mask_NM: ", v, " tokens do not have exactly K = ", K, " experts (or the mask holds more than M*K pairs)");
+  }
+  return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes};
+}
+
+// x [.., D]; a dense block
+Tensor feed_forward_int4(const Tensor& x, const Tensor& W1, const Tensor& S1, const Tensor& W2, const Tensor& S2, int64_t H,
+                         int64_t group) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<Tensor, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t>(
+        "momoe::feed_forward_int4", x, W1, S1, W2, S2, H, group);
+  TORCH_CHECK(W1.is_cuda(), "FeedForwardInt4 weights must live on the GPU: there is no CPU compute path");
+  TORCH_CHECK(!wants_autograd({&x}), "FeedForwardInt4 has no backward, and x requires a gradient: call it under torch.no_grad()");
+  const at::Device dev = W1.device();
+  if (x.dim() < 1) throw_python(PyExc_AssertionError, "x must be [.., D]");
+  const int64_t D = x.size(-1);
+  if (!held_int4(W1, S1, dev, 1, D, 2 * H, group) || !held_int4(W2, S2, dev, 1, H, D, group))
+    throw_python(PyExc_AssertionError, "x [.., D] and the packed weights do not fit together");
+  const int64_t M = x.numel() / D;
+  const c10::DeviceGuard guard(dev);
+  const hipStream_t st = stream_of(dev);
+  Tensor y = empty_bf16(x.sizes(), dev);
+  if (M > 0) {
+    const Tensor rows = rows_in_bf16(x, M, D, dev), h = empty_bf16({M, H}, dev);
+    MOMOE_CALL(momoe_int4_ffn_fwd, st, rows.data_ptr(), M > 1 ? rows.stride(0) : D, W1.data_ptr(), S1.data_ptr(), W2.data_ptr(),
+               S2.data_ptr(), (int)group, h.data_ptr(), y.data_ptr(), M, D, H);
+  }
+  return x.device() == dev ? y : y.to(x.device());
+}
+
 // ---- router ------------------------------------------------------------------------------------
 struct Routed {
   Tensor x_MD, mask, s_MN, p_sel, norms;
@@ -938,6 +1034,11 @@ TORCH_LIBRARY(momoe, m) {
   m.def("experts_fp8(Tensor x_BSD, Tensor Wl1, Tensor Wl1_scale_bits, Tensor Wl2, Tensor Wl2_scale_bits, Tensor mask_NM, Tensor s_NM, int K, "
         "int H, bool check) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_fp8)));
+  m.def("experts_int4(Tensor x_BSD, Tensor Wl1, Tensor Wl1_words, Tensor Wl2, Tensor Wl2_words, Tensor mask_NM, Tensor s_NM, int K, int H, "
+        "int group, bool check) -> (Tensor, Tensor)",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_int4)));
+  m.def("feed_forward_int4(Tensor x, Tensor Wl1, Tensor Wl1_words, Tensor Wl2, Tensor Wl2_words, int H, int group) -> Tensor",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(feed_forward_int4)));
   m.def("balance_loss(Tensor logits, Tensor mask_NM, int Ks, Tensor? valid, bool per_sequence) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(balance_loss)));
   m.def("router_balanced(Tensor(a) x_BSD, Tensor Wg_DN, Tensor biases_N, int N, int K, int Ks, Tensor? valid, bool per_sequence) "
@@ -948,6 +1049,8 @@ TORCH_LIBRARY(momoe, m) {
 PYBIND11_MODULE(_layer, m) {
   m.def("experts", &experts, py::call_guard<py::gil_scoped_release>());
   m.def("experts_fp8", &experts_fp8, py::call_guard<py::gil_scoped_release>());
+  m.def("experts_int4", &experts_int4, py::call_guard<py::gil_scoped_release>());
+  m.def("feed_forward_int4", &feed_forward_int4, py::call_guard<py::gil_scoped_release>());
   m.def("router", &router, py::call_guard<py::gil_scoped_release>());
   m.def("balance_loss", &balance_loss, py::call_guard<py::gil_scoped_release>());
   m.def("router_balanced", &router_balanced, py::call_guard<py::gil_scoped_release>());

@@ -98,6 +98,14 @@ _SIGNATURES = {
     "momoe_fp8_few_lin1_swiglu_fwd": (_int, [_p, _int, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_few_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_weight_bytes": (_i64, [_i64] * 3),
+    "momoe_int4_scale_words": (_i64, [_i64] * 3 + [_int]),
+    "momoe_int4_pack_weights": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _int, _int, _p, _p, _p]),
+    "momoe_int4_tile_rows": (_int, [_i64] * 2),
+    "momoe_int4_lin1_swiglu_fwd": (_int, [_p, _i64, _p, _p, _int, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_lin2_scale_fwd": (_int, [_p, _p, _p, _int, _p, _i64, _i64, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_ffn_fwd": (_int, [_p, _i64, _p, _p, _p, _p, _int, _p, _p, _i64, _i64, _i64, _p]),
     "momoe_bias_update": (_int, [_p, ctypes.c_float, ctypes.c_float, _i64, _p, _p]),
 }
 
@@ -540,3 +548,22 @@ def fp8_combine(ys, inv_MK, D):
     out = torch.empty((M, D), dtype=torch.bfloat16, device=ys.device)
     _call("momoe_fp8_combine", _ptr(ys), _ptr(inv_MK), _ptr(out), M, D, K, ys.shape[0], _stream())
     return out
+
+
+# ---------------------------------------------------------------- 4-bit weights
+def int4_pack_weights(codes_NRC, scale, zero, halves, group):
+    """Codes [N, R / 2, C], two to a byte, scale and zero (or None) [N, groups, C] -> (packed bytes, int32 words of scale and zero)."""
+    _need_cuda(codes_NRC, scale, zero)
+    N, R, C = codes_NRC.shape[0], 2 * codes_NRC.shape[1], codes_NRC.shape[2]
+    assert codes_NRC.is_contiguous() and scale.is_contiguous() and (zero is None or zero.is_contiguous())
+    dev = codes_NRC.device
+    packed = torch.empty(max(_lib.momoe_int4_weight_bytes(N, R, C), 0), dtype=torch.uint8, device=dev)
+    words = torch.empty(max(_lib.momoe_int4_scale_words(N, R, C, group), 0), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _call("momoe_int4_pack_weights", _ptr(codes_NRC), _ptr(scale), _TYPES[scale.dtype], _ptr(zero), N, R, C, halves, group, _ptr(packed),
+              _ptr(words), _stream())
+    return packed, words
+
+
+def int4_tile_rows(Msum, N):
+    return _lib.momoe_int4_tile_rows(Msum, N)

@@ -9,6 +9,7 @@ import torch.nn as nn
 from . import _layer
 from .experts import MoMoE
 from .experts_fp8 import MoMoEFP8
+from .int4 import MoMoEInt4
 from .router import TopKRouter
 
 
@@ -47,9 +48,13 @@ class MoE(nn.Module):
         (`MoMoEFP8.from_momoe`); forward only, under `torch.no_grad()`."""
         return self.serving(self.router, self.biases_N, MoMoEFP8.from_momoe(self.momoe))
 
+    def to_int4(self, group_size=128):
+        """The same with the experts' weights in 4 bits (`MoMoEInt4.from_momoe`)."""
+        return self.serving(self.router, self.biases_N, MoMoEInt4.from_momoe(self.momoe, group_size))
+
     @classmethod
     def serving(cls, router, biases_N, momoe):
-        """A `MoE` of a router, its selection bias and experts (`MoMoE` or `MoMoEFP8`) that leaves the bias as it is."""
+        """A `MoE` of a router, its selection bias and experts (`MoMoE`, `MoMoEFP8` or `MoMoEInt4`) that leaves the bias as it is."""
         self = cls.__new__(cls)
         nn.Module.__init__(self)
         self.D, self.H, self.N, self.K, self.Ks = router.D, momoe.H, router.N, router.K, router.Ks

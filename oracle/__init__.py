@@ -26,6 +26,8 @@ reference, which has no tests, fixtures or golden vectors of its own):
 * `balance_loss`          - pinned: autograd through the definition, hand-computed cases
                             (tests/test_oracle_operators.py)
 * `experts_fp8`           - pinned: `e4m3` by torch's conversion, `experts_forward` where nothing is rounded
+* `swiglu_block`, `swiglu_block_gradients` - pinned: `experts_forward` of one expert, autograd, differences
+* `int4_weights`          - pinned: hand-computed case, loops
 
 The reference's intermediate bf16 rounding points, its autotune-dependent
 save/recompute tile boundary and its raced `which` order are NOT restated
@@ -52,6 +54,9 @@ from .operators import (  # noqa: F401
     block_weights,
     e4m3,
     experts_fp8,
+    int4_weights,
     rounded_rows,
     rows_in_8_bits,
+    swiglu_block,
+    swiglu_block_gradients,
 )

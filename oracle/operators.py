@@ -79,3 +79,30 @@ def experts_fp8(x_MD, W1, W2, mask_NM, s_NM):
             h = z[:, :H] * z[:, H:] * torch.sigmoid(z[:, H:])
             y[rows] += s_NM[i, rows].double()[:, None] * (rounded_rows(h) @ W2[i])
     return y
+
+
+# ---- 4-bit weights with a scale and a zero for each group of k-values ---------------------------------------------------------
+def int4_weights(codes, scale, zero, group):
+    """The values, in 64 bits, of codes [.., R / 2, C] (two to a byte) with scale and zero (None: 8) [.., groups, C]."""
+    R = 2 * codes.shape[-2]
+    q = torch.stack([codes & 15, codes >> 4], -2).reshape(*codes.shape[:-2], R, codes.shape[-1]).double()
+    z = torch.full_like(scale, 8, dtype=torch.float64) if zero is None else (zero & 15).double()
+    return (q - z.repeat_interleave(group, -2)[..., :R, :]) * scale.double().repeat_interleave(group, -2)[..., :R, :]
+
+
+def swiglu_block(x, W1, W2):
+    """(a, b, h, y) in 64 bits of rows x through one block."""
+    H = W2.shape[0]
+    z = x.double() @ W1
+    a, b = z[:, :H], z[:, H:]
+    h = a * b * torch.sigmoid(b)
+    return a, b, h, h @ W2
+
+
+def swiglu_block_gradients(x, W1, W2, Gy):
+    """(Gx, GW1, GW2) in 64 bits, from the formulas."""
+    a, b, h, _ = swiglu_block(x, W1, W2)
+    sig = torch.sigmoid(b)
+    u = Gy.double() @ W2.T
+    gz = torch.cat([u * b * sig, u * a * sig * (1 + b * (1 - sig))], -1)
+    return gz @ W1.T, x.double().T @ gz, h.T @ Gy.double()
