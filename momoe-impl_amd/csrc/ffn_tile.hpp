@@ -1,0 +1,163 @@
+// Products of a dense SwiGLU block in tiles of BM x 128: a workgroup a tile, 64 k-values a stage, any contraction of a multiple of 32.
+//
+// For launches of few tiles, short contractions, few rows; the large ones run in the loop of gemm_span.hpp, whose operands and fragment
+// layout these are (the first input of the MFMA is the weight side: a lane holds, for one tile row (lane % 16), four consecutive
+// columns).  4 waves, 2 x 2; three stages in LDS, two of them on the way; with 72 or 96 KiB a workgroup two of them, or one and the
+// next one's start, share a CU.
+#pragma once
+#include "gemm_span.hpp"
+
+namespace momoe {
+
+constexpr int kFfnCols = 128, kFfnStages = 3;
+
+// Rows of a matrix at any pitch, k-contiguous, rows past the last one repeat it.  `K`: of 32 k-values the stage's first half is all
+// there is, and stands in the second, too.
+template <int ROWS>
+struct FfnRows : SpanGatheredRows<ROWS> {
+  using Base = SpanGatheredRows<ROWS>;
+  using L = SpanRowsLayout<ROWS>;
+  __device__ __forceinline__ void init(const bf16* mat, int64_t ld, int64_t row0, int rows, int K) {
+    Base::base = mat + row0 * ld;
+    const int l = fresh_lane();
+    const uint32_t piece = L::piece_bytes(l) & (K == 32 ? 0x3Fu : ~0u);
+#pragma unroll
+    for (int j = 0; j < L::DEP; ++j) Base::off[j] = (uint32_t)min(32 * j + L::first_row(l), rows - 1) * (uint32_t)(2 * ld) + piece;
+  }
+};
+// Rows of a k-blocked matrix [K / 32][ldm][32]
+template <int ROWS>
+struct FfnBlockedRows : SpanBlockedRows<ROWS> {
+  using Base = SpanBlockedRows<ROWS>;
+  int64_t far;  // elements to the second half of a stage
+  __device__ __forceinline__ void init(const bf16* mat, int64_t ldm, int64_t row0, int rows, int K) {
+    Base::init(mat, ldm, row0, rows);
+    far = K == 32 ? 0 : ldm * kHalf;
+  }
+  template <int j>
+  __device__ __forceinline__ void deposit(const bf16* src, uint32_t slot) const {
+    constexpr int h = j / Base::PER_HALF, q = j % Base::PER_HALF;
+    dma16_at<h * (ROWS * kHalf * 2) + q * kSpanWaves * 1024>(h ? src + far : src, Base::off[q], slot);
+  }
+};
+
+// k-strided columns ([k][n] weights), as SpanCols.  PAIRED: a wave's second half of fragments are the columns 64 further on.
+template <bool PAIRED>
+struct FfnCols {
+  static constexpr int COLS = kFfnCols, DEP = COLS / 32, FN = COLS / 32;
+  static constexpr int ELEMS = COLS * kSpan;
+  static constexpr int PIECES = COLS / 8, RPD = 64 / PIECES, STEP = RPD * kSpanWaves;
+  static_assert(STEP == 16, "one pattern of swizzles in all deposits, two deposits a half stage");
+  static __device__ __forceinline__ int swz(int k) { return 2 * (k & 3) + 8 * ((k >> 3) & 1); }
+  const bf16* base;
+  uint32_t off, pitch, wrap;  // bytes; wrap: of the k-rows that a stage's second half lies behind the first
+  template <class ColOff>
+  __device__ __forceinline__ void init(const bf16* base_, int ld, int K, ColOff coloff) {
+    base = base_;
+    pitch = (uint32_t)ld * 2;
+    wrap = K == 32 ? 0 : 2 * STEP * pitch;
+    const int l = fresh_lane(), krow = wave_id() * RPD + l / PIECES;
+    off = (uint32_t)krow * pitch + (uint32_t)coloff(((l % PIECES) ^ swz(krow)) * 8) * 2;
+  }
+  __device__ __forceinline__ const bf16* source(int k) const { return (const bf16*)((const char*)base + (uint32_t)k * pitch); }
+  template <int j>
+  __device__ __forceinline__ void deposit(const bf16* src, uint32_t slot) const {
+    dma16_at<j * kSpanWaves * 1024>((const char*)src + (uint32_t)(STEP * (j % 2)) * pitch + (j / 2 ? wrap : 0u), off, slot);
+  }
+  struct Lane {
+    int o;  // first fragment, in bytes
+    __device__ __forceinline__ explicit Lane(int org) {
+      const int l = fresh_lane(), krow = 8 * (l >> 4) + ((l & 15) >> 2), col = org + 4 * (l & 3);
+      o = (krow * COLS + (((col >> 3) ^ swz(krow)) << 3) + (col & 7)) * 2;
+    }
+  };
+  static __device__ __forceinline__ bf16x8 frag(const bf16* slot, const Lane& ln, int i, int h) {
+    // (pieces 1 to 3 bits up are permuted, so what is added to a column there is an exclusive or)
+    const int add = PAIRED ? 32 * (i % (FN / 2)) ^ (i >= FN / 2 ? COLS : 0) : 32 * i;
+    const bf16* p = (const bf16*)((const char*)slot + (ln.o ^ add)) + h * (kHalf * COLS);
+    const bf16x4 lo = lds_read_tr4(p), hi = lds_read_tr4(p + 4 * COLS);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+// rows at a fixed pitch (k-contiguous weights): a multiple of 32 of them, the last 32 repeated where the tile sticks out
+struct FfnWeightRows : SpanPitchedRows<kFfnCols> {
+  using Base = SpanPitchedRows<kFfnCols>;
+  __device__ __forceinline__ void init(const bf16* mat, int K, int row0, int nrows) {
+    Base::init(mat, K, row0, nrows);
+    if (K == 32) {
+      const int l = fresh_lane();
+      off = (uint32_t)L::first_row(l) * pitch + (L::piece_bytes(l) & 0x3F);
+    }
+  }
+};
+
+// A tile program P: P::Rows, P::Weights, FM; K, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column of a wave's
+// fragments in the tile; epilogue(row0, rows, tn, wm, wn, acc).
+template <class P>
+__device__ __forceinline__ void run_ffn_tile(const P& prog) {
+  using Rows = typename P::Rows;
+  using Weights = typename P::Weights;
+  constexpr int FM = P::FM, FN = 4, BM = 32 * FM;
+  constexpr int LOADS = Rows::DEP + Weights::DEP;
+  // An XCD has a contiguous eighth of the tiles, row tiles fastest: those that share weights meet in one L2
+  const int total = prog.row_tiles * prog.col_tiles, chunk = (total + 7) >> 3;
+  const int t = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= chunk || t >= total) return;
+  const int tn = t / prog.row_tiles;
+  const int64_t row0 = (int64_t)(t - tn * prog.row_tiles) * BM;
+  const int rows = (int)min((int64_t)BM, prog.rows - row0);
+  Rows A;
+  Weights W;
+  prog.setup(row0, rows, tn, A, W);
+  bf16* const lds = dyn_lds();
+  constexpr int STAGE = Rows::ELEMS + Weights::ELEMS;  // elements
+  const uint32_t addr = lds_address(lds) + wave_id() * 1024;
+  const int wn = wave_id() & 1, wm = wave_id() >> 1;
+  const SpanStages st(prog.K);
+  const int count = st.count;
+  int k = 0, put = 0, got = 0;
+  auto request = [&] {
+    const bf16 *asrc = A.source(k), *wsrc = W.source(k);
+    const uint32_t to = addr + (uint32_t)put * (STAGE * 2);
+    unrolled<0, Rows::DEP>([&](auto D) { A.template deposit<decltype(D)::value>(asrc, to); });
+    unrolled<0, Weights::DEP>([&](auto D) { W.template deposit<decltype(D)::value>(wsrc, to + Rows::ELEMS * 2); });
+    k = max(0, st.after(k));
+    put = put + 1 == kFfnStages ? 0 : put + 1;
+  };
+  request();
+  if (count > 1) request();
+  f32x4 acc[FN][FM] = {};
+  const typename Rows::Lane alane(wm * 16 * FM);
+  const typename Weights::Lane wlane(prog.n_org(wn));
+  for (int s = 0; s < count; ++s) {
+    if (s + 1 < count) wait_vmcnt<LOADS>();
+    else wait_vmcnt<0>();
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    order_fence();
+    if (s + 2 < count) request();
+    const bf16 *sa = lds + got * STAGE, *sw = sa + Rows::ELEMS;
+    auto half = [&](auto H) {
+      bf16x8 wf[FN], af[FM];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) wf[j] = Weights::frag(sw, wlane, j, decltype(H)::value);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) af[i] = Rows::frag(sa, alane, i, decltype(H)::value);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[j][i] = mfma16(wf[j], af[i], acc[j][i]);
+    };
+    // a last stage that is not whole starts at K - 64: its first half has been multiplied (of 32 k-values the first is all)
+    const bool part = s + 1 == count && st.tail;
+    if (!part || prog.K == 32) half(IntC<0>{});
+    if (!part) half(IntC<1>{});
+    else if (prog.K != 32) half(IntC<1>{});
+    got = got + 1 == kFfnStages ? 0 : got + 1;
+  }
+  prog.epilogue(row0, rows, tn, wm, wn, acc);
+}
+template <class P>
+constexpr size_t kFfnLds = (size_t)kFfnStages * (P::Rows::ELEMS + P::Weights::ELEMS) * sizeof(bf16);
+
+}  // namespace momoe

@@ -540,14 +540,139 @@ std::tuple<Tensor, Tensor> experts_fp8(const Tensor& x_BSD, const Tensor& W1, co
   return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes};
 }
 
-// ---- blocks with weights in 4 bits --------------------------------------------------------------
+// ---- dense block ---------------------------------------------------------------------------------
 // [M, D] bf16 rows on a 16-byte boundary, of the device the weights are on; any other type is rounded to bf16
 Tensor rows_in_bf16(const Tensor& x, int64_t M, int64_t D, const at::Device& dev) {
   Tensor rows = x.reshape({M, D}).to(dev, at::kBFloat16);
-  if (rows.stride(1) != 1 || (M > 1 && (rows.stride(0) < D || rows.stride(0) % 8 != 0))) rows = rows.contiguous();
+  // (pitches that the kernels take, and momoe_wgrad of a gradient)
+  const int64_t ld = M > 1 ? rows.stride(0) : D;
+  if (rows.stride(1) != 1 || ld < D || ld % 8 != 0 || ld >= (1 << 22) || (ld > D && M * ld * 2 >= (1ll << 32))) rows = rows.contiguous();
   if ((uintptr_t)rows.data_ptr() % 16 != 0) rows = rows.clone(at::MemoryFormat::Contiguous);
   return rows;
 }
+int64_t pitch_of_rows(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+// a weight as the kernels read it
+Tensor packed_bf16(const Tensor& W) {
+  const Tensor w = W.to(at::kBFloat16).contiguous();
+  return (uintptr_t)w.data_ptr() % 16 != 0 ? w.clone() : w;
+}
+Tensor fragments(int64_t rows, int64_t cols, const at::Device& dev) { return empty_f32({momoe_ffn_fragment_floats(rows, cols)}, dev); }
+
+struct FeedForward {
+  Tensor y;
+  Tensor x, W1, W2, ab;  // for the backward
+};
+
+// a | b of the first `msave` rows are kept
+FeedForward feed_forward_forward(const Tensor& x, const Tensor& W1, const Tensor& W2, int64_t msave) {
+  const at::Device dev = W1.device();
+  const int64_t D = W1.size(0), H = W2.size(0), M = x.numel() / D;
+  const c10::DeviceGuard guard(dev);
+  const hipStream_t st = stream_of(dev);
+  FeedForward f;
+  f.y = empty_bf16(x.sizes(), dev);
+  f.x = rows_in_bf16(x, M, D, dev);
+  f.W1 = packed_bf16(W1);
+  f.W2 = packed_bf16(W2);
+  if (M > 0) {
+    if (msave > 0) f.ab = fragments(msave, 2 * H, dev);
+    const Tensor h = empty_bf16({M * H}, dev);
+    MOMOE_CALL(momoe_ffn_lin1_fwd, st, f.x.data_ptr(), pitch_of_rows(f.x), f.W1.data_ptr(), h.data_ptr(),
+               msave > 0 ? f.ab.data_ptr<float>() : nullptr, (msave + 31) / 32 * 32, M, M, D, H);
+    MOMOE_CALL(momoe_ffn_lin2_fwd, st, h.data_ptr(), f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H);
+  }
+  if (x.device() != dev) f.y = f.y.to(x.device());
+  return f;
+}
+
+struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& W1, const Tensor& W2, int64_t msave) {
+    FeedForward f = feed_forward_forward(x, W1, W2, msave);
+    ctx->save_for_backward({f.x, f.W1, f.W2, f.ab});
+    ctx->saved_data["call"] = std::vector<int64_t>{msave, f.W1.device().index(), f.x.size(0), W1.size(0), W2.size(0)};
+    return {f.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "FeedForward has no second derivative: call backward without create_graph");
+    const std::vector<int64_t> call_of = ctx->saved_data["call"].toIntVector();
+    const int64_t msave = call_of[0], M = call_of[2], D = call_of[3], H = call_of[4];
+    const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(1), need_w2 = ctx->needs_input_grad(2);
+    const at::Device dev(at::kCUDA, (at::DeviceIndex)call_of[1]);
+    const c10::DeviceGuard guard(dev);
+    const hipStream_t st = stream_of(dev);
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor& W1 = as_saved(saved[1], "Wl1", dev, at::kBFloat16, {D, 2 * H});
+    const Tensor& W2 = as_saved(saved[2], "Wl2", dev, at::kBFloat16, {H, D});
+    // (a hook may have brought x back with other strides)
+    const Tensor x = rows_in_bf16(as_saved(saved[0], "x", dev, at::kBFloat16, {M, D}, /*packed=*/false), M, D, dev);
+    if (msave > 0) as_saved(saved[3], "a|b", dev, at::kFloat, {momoe_ffn_fragment_floats(msave, 2 * H)});
+    if (need_w1) out[1] = empty_bf16({D, 2 * H}, dev);
+    if (need_w2) out[2] = empty_bf16({H, D}, dev);
+    if (M == 0) {
+      if (need_x) out[0] = at::empty(grads[0].sizes(), grads[0].options().dtype(at::kBFloat16));
+      if (need_w1) out[1].zero_();
+      if (need_w2) out[2].zero_();
+      return out;
+    }
+    const Tensor Gy = rows_in_bf16(grads[0], M, D, dev);
+    const int64_t ldx = pitch_of_rows(x), ldgy = pitch_of_rows(Gy);
+    Tensor gz = empty_bf16({2 * H * M}, dev), hT, counts = empty_i32(4, dev);
+    if (need_w2) hT = empty_bf16({momoe_padded_rows(M, 1) * H}, dev);
+    // what lies behind row `at`, a multiple of 32
+    const auto rows_at = [](const Tensor& t, int64_t at, int64_t pitch) { return (void*)((char*)t.data_ptr() + at * pitch * 2); };
+    void* const ht = need_w2 ? hT.data_ptr() : nullptr;
+    if (msave > 0)
+      MOMOE_CALL(momoe_ffn_dgrad_h_saved, st, Gy.data_ptr(), ldgy, W2.data_ptr(), (const float*)saved[3].data_ptr<float>(), gz.data_ptr(), ht,
+                 counts.data_ptr<int32_t>(), msave, M, D, H);
+    if (msave < M) {
+      const Tensor u = fragments(M - msave, H, dev);
+      MOMOE_CALL(momoe_ffn_dgrad_h, st, rows_at(Gy, msave, ldgy), ldgy, W2.data_ptr(), u.data_ptr<float>(), M - msave, D, H);
+      MOMOE_CALL(momoe_ffn_swiglu_bwd, st, rows_at(x, msave, ldx), ldx, W1.data_ptr(), (const float*)u.data_ptr<float>(), rows_at(gz, msave, 32),
+                 need_w2 ? rows_at(hT, msave, H) : nullptr, counts.data_ptr<int32_t>(), M - msave, M, D, H);
+    }
+    const auto weight_gradient = [&](const void* A, int64_t lda, int a_layout, const void* B, int64_t ldb, int b_layout, const Tensor& G) {
+      const int64_t X = G.size(0), Y = G.size(1), bytes = std::min(M * H * 8, momoe_wgrad_workspace_bytes(1, X, Y, M));
+      const Tensor ws = empty_f32({bytes / 4}, dev);
+      MOMOE_CALL(momoe_wgrad, st, A, lda, a_layout, (const int32_t*)nullptr, B, ldb, b_layout, (const int32_t*)nullptr,
+                 (const int32_t*)counts.data_ptr<int32_t>(), G.data_ptr(), M, (int64_t)1, X, Y, M, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
+    };
+    if (need_w2) weight_gradient(ht, H, MOMOE_LAYOUT_TRANSPOSED, Gy.data_ptr(), ldgy, MOMOE_LAYOUT_ROWS, out[2]);
+    hT.reset();
+    if (need_w1) weight_gradient(x.data_ptr(), ldx, MOMOE_LAYOUT_ROWS, gz.data_ptr(), M, MOMOE_LAYOUT_KBLOCKED, out[1]);
+    if (need_x) {
+      const Tensor Gx = empty_bf16({M, D}, dev);
+      MOMOE_CALL(momoe_ffn_dgrad_x, st, gz.data_ptr(), W1.data_ptr(), Gx.data_ptr(), M, D, H);
+      out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
+    }
+    return out;
+  }
+};
+
+Tensor feed_forward(const Tensor& x, const Tensor& W1, const Tensor& W2, double save_percent) {
+  if (torch::jit::tracer::isTracing())
+    return call_recorded<Tensor, const Tensor&, const Tensor&, const Tensor&, double>("momoe::feed_forward", x, W1, W2, save_percent);
+  if (W1.device() != W2.device())
+    throw_python(PyExc_AssertionError, "All weights must be on the same device, but got: Wl1_D2H.device = " + W1.device().str() +
+                                           ", Wl2_HD.device = " + W2.device().str());
+  TORCH_CHECK(W1.is_cuda(), "FeedForward weights must live on the GPU: there is no CPU compute path");
+  if (x.dim() < 1 || W1.dim() != 2 || W2.dim() != 2 || W1.size(0) != x.size(-1) || W2.size(1) != x.size(-1) || W1.size(1) != 2 * W2.size(0))
+    throw_python(PyExc_AssertionError, "x [.., D], Wl1_D2H [D,2H] and Wl2_HD [H,D] do not fit together");
+  const int64_t D = W1.size(0), H = W2.size(0);
+  TORCH_CHECK(D > 0 && H > 0 && D % 32 == 0 && H % 32 == 0 && D * H * 4 < (1ll << 32),
+              "FeedForward takes D and H that are multiples of 32 with weights below 4 GiB, got ", D, " and ", H);
+  TORCH_CHECK(save_percent >= 0 && save_percent <= 100, "save_percent must be between 0 and 100, got ", save_percent);
+  const int64_t M = x.numel() / D;
+  if (!wants_autograd({&x, &W1, &W2})) return feed_forward_forward(x, W1, W2, 0).y;
+  // the gradients of the weights address tokens at 32-bit offsets (momoe_wgrad): say so now rather than in the backward
+  TORCH_CHECK(!(W1.requires_grad() || W2.requires_grad()) || (M * D * 2 < (1ll << 32) && 8 * M * 64 < (1ll << 32)),
+              "FeedForward backward supports batches of less than 4 GiB and 8388608 tokens per call, got ", M, " tokens: split the batch");
+  const int64_t part = (int64_t)((double)M * save_percent / 100.0), msave = part == M ? M : part / 32 * 32;
+  return FeedForwardFn::apply(x, W1, W2, msave)[0];
+}
+
+// ---- blocks with weights in 4 bits --------------------------------------------------------------
 bool held_int4(const Tensor& W, const Tensor& S, const at::Device& dev, int64_t N, int64_t R, int64_t C, int64_t group) {
   const auto held = [&](const Tensor& t, at::ScalarType type, int64_t n) {
     return t.device() == dev && t.scalar_type() == type && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 && t.numel() == n;
@@ -598,7 +723,7 @@ std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, c
              ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), tile_rows, (int32_t*)nullptr,
              (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
   void* const h = transients.take(msum * H * 2, h_own);
-  MOMOE_CALL(momoe_int4_lin1_swiglu_fwd, st, x.data_ptr(), M > 1 ? x.stride(0) : D, W1.data_ptr(), S1.data_ptr(), (int)group,
+  MOMOE_CALL(momoe_int4_lin1_swiglu_fwd, st, x.data_ptr(), pitch_of_rows(x), W1.data_ptr(), S1.data_ptr(), (int)group,
              (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, h, M, D, H, N, msum);
   float* const ys = (float*)transients.take(msum * D * 4, ys_own);
   MOMOE_CALL(momoe_int4_lin2_scale_fwd, st, h, W2.data_ptr(), S2.data_ptr(), (int)group, (const float*)s.data_ptr<float>(), s.stride(0),
@@ -630,7 +755,7 @@ Tensor feed_forward_int4(const Tensor& x, const Tensor& W1, const Tensor& S1, co
   Tensor y = empty_bf16(x.sizes(), dev);
   if (M > 0) {
     const Tensor rows = rows_in_bf16(x, M, D, dev), h = empty_bf16({M, H}, dev);
-    MOMOE_CALL(momoe_int4_ffn_fwd, st, rows.data_ptr(), M > 1 ? rows.stride(0) : D, W1.data_ptr(), S1.data_ptr(), W2.data_ptr(),
+    MOMOE_CALL(momoe_int4_ffn_fwd, st, rows.data_ptr(), pitch_of_rows(rows), W1.data_ptr(), S1.data_ptr(), W2.data_ptr(),
                S2.data_ptr(), (int)group, h.data_ptr(), y.data_ptr(), M, D, H);
   }
   return x.device() == dev ? y : y.to(x.device());
@@ -1034,6 +1159,8 @@ TORCH_LIBRARY(momoe, m) {
   m.def("experts_fp8(Tensor x_BSD, Tensor Wl1, Tensor Wl1_scale_bits, Tensor Wl2, Tensor Wl2_scale_bits, Tensor mask_NM, Tensor s_NM, int K, "
         "int H, bool check) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_fp8)));
+  m.def("feed_forward(Tensor x, Tensor Wl1_D2H, Tensor Wl2_HD, float save_percent) -> Tensor",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(feed_forward)));
   m.def("experts_int4(Tensor x_BSD, Tensor Wl1, Tensor Wl1_words, Tensor Wl2, Tensor Wl2_words, Tensor mask_NM, Tensor s_NM, int K, int H, "
         "int group, bool check) -> (Tensor, Tensor)",
         torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(experts_int4)));
@@ -1049,6 +1176,7 @@ TORCH_LIBRARY(momoe, m) {
 PYBIND11_MODULE(_layer, m) {
   m.def("experts", &experts, py::call_guard<py::gil_scoped_release>());
   m.def("experts_fp8", &experts_fp8, py::call_guard<py::gil_scoped_release>());
+  m.def("feed_forward", &feed_forward, py::call_guard<py::gil_scoped_release>());
   m.def("experts_int4", &experts_int4, py::call_guard<py::gil_scoped_release>());
   m.def("feed_forward_int4", &feed_forward_int4, py::call_guard<py::gil_scoped_release>());
   m.def("router", &router, py::call_guard<py::gil_scoped_release>());

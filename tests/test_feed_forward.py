@@ -1,0 +1,46 @@
+"""CPU: what the dense block refuses, before any launch."""
+import pytest
+import torch
+
+import momoe_amd
+from momoe_amd import _hip
+
+lib, P = _hip._lib, 4096
+
+
+def test_sizes():
+    assert [lib.momoe_ffn_fragment_floats(r, 64) for r in (0, 1, 16, 17)] == [0, 1024, 1024, 2048]
+    assert lib.momoe_ffn_fragment_floats(-1, 64) == lib.momoe_ffn_fragment_floats(1, 24) == lib.momoe_ffn_fragment_floats(1, 0) == -1
+
+
+def _refuses(fn, good, pointers, aligned, optional=()):
+    call = lambda **c: fn(*{**good, **c}.values(), None)
+    assert all(call(**{k: None}) == 1 for k in pointers) and all(call(**{k: P + 8}) == 1 for k in aligned)
+    assert all(call(**{k: 0}) == 1 for k in ("rows", "D", "H")) and call(D=48) == call(H=40) == 2
+    assert call(D=1 << 16, H=1 << 16, **{k: 1 << 17 for k in good if k.startswith("ld") and k != "ldm"}) == 2
+    return call
+
+
+def test_refusals_of_the_entry_points():
+    sizes = dict(rows=40, ldm=40, D=64, H=32)
+    c = _refuses(lib.momoe_ffn_lin1_fwd, dict(x=P, ldx=64, W=P, h=P, ab=None, ab_rows=0, **sizes), ("x", "W", "h"), ("x", "W", "h"))
+    assert c(ldx=56) == c(ldm=39) == c(ab_rows=32) == c(ab=P, ab_rows=-32) == c(ab=P, ab_rows=96) == c(ab=P + 4, ab_rows=32) == 1
+    assert c(ldx=68) == c(ab=P, ab_rows=40) == c(ldx=1 << 22) == 2
+    c = _refuses(lib.momoe_ffn_lin2_fwd, dict(h=P, W=P, y=P, **sizes), ("h", "W", "y"), ("h", "W", "y"))
+    assert c(ldm=39) == 1 and c(ldm=1 << 31) == 2
+    c = _refuses(lib.momoe_ffn_dgrad_h, dict(Gy=P, ldgy=64, W=P, u=P, rows=40, D=64, H=32), ("Gy", "W", "u"), ("Gy", "W", "u"))
+    assert c(ldgy=56) == 1 and c(ldgy=68) == 2
+    c = _refuses(lib.momoe_ffn_swiglu_bwd, dict(x=P, ldx=64, W=P, u=P, gz=P, hT=None, counts=None, **sizes), ("x", "W", "u", "gz"), ("x", "W", "u", "gz", "hT"))
+    assert c(ldx=56) == c(ldm=39) == 1 and c(ldx=68) == 2
+    c = _refuses(lib.momoe_ffn_dgrad_h_saved, dict(Gy=P, ldgy=64, W=P, ab=P, gz=P, hT=None, counts=None, **sizes), ("Gy", "W", "ab", "gz"), ("Gy", "W", "ab", "gz", "hT"))
+    assert c(ldgy=56) == c(ldm=39) == 1 and c(ldgy=68) == 2
+    _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, rows=40, D=64, H=32), ("gz", "W", "Gx"), ("gz", "W", "Gx"))
+
+
+def test_module_refusals():
+    W1, W2 = torch.zeros(32, 64), torch.zeros(32, 32)
+    for save in (-1, 101):
+        with pytest.raises(AssertionError, match="save_percent"):
+            momoe_amd.FeedForward(32, 32, save, W1, W2)
+    with pytest.raises(RuntimeError, match="no CPU compute path"):
+        momoe_amd.FeedForward(32, 32, 0, W1, W2)(torch.zeros(4, 32))

@@ -1,0 +1,312 @@
+"""GPU: the dense SwiGLU block, forward and backward, against the formulas in 64 bits."""
+import copy
+
+import pytest
+import torch
+
+import momoe_amd
+import oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E, B = 2.0 ** -24, 2.0 ** -8  # half a step of fp32, of bf16
+
+
+def _inputs(M, D, H, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *size: torch.randn(*size, generator=g)
+    lift = torch.exp2(torch.randint(-3, 4, (M, 1), generator=g).float())
+    return [t.to(torch.bfloat16) for t in (r(M, D) * lift, r(D, 2 * H) * 2 / D ** 0.5, r(H, D) / H ** 0.5, r(M, D))]
+
+
+def _block(W1, W2, save=0):
+    return momoe_amd.FeedForward(W2.shape[1], W2.shape[0], save, Wl1_D2H=W1.to(DEV), Wl2_HD=W2.to(DEV))
+
+
+def _bounds(x, W1, W2, Gy):
+    """[(value, how far it may be off)] of y, Gx, GW1, GW2, the last rounding included.  A sum of n products is off by 2 (n + 8) E of their
+    magnitudes at most; h and gz are rounded to bf16 before they are multiplied."""
+    x, W1, W2, Gy = [t.double() for t in (x, W1, W2, Gy)]
+    H = W2.shape[0]
+    sums = lambda a, b: a.abs() @ b.abs() * 2 * (a.shape[1] + 8) * E
+    a, b, h, y = oracle.swiglu_block(x, W1, W2)
+    d = sums(x, W1)
+    da, db = d[:, :H], d[:, H:]
+    sig = torch.sigmoid(b)
+    silu, slope = b * sig, sig * (1 + b * (1 - sig))
+    # |silu'| <= 1.1, |silu''| <= 0.5; exp and reciprocal of the sigmoid, the products: some 16 + |b| roundings
+    few = (16 + b.abs()) * 2 * E
+    dsilu, dslope = 1.1 * db + silu.abs() * few, 0.5 * db + (slope.abs() + silu.abs() + 1) * few
+    rounded = lambda v, dv: dv + (v.abs() + dv) * B
+    dh = rounded(h, da * (silu.abs() + dsilu) + a.abs() * dsilu + h.abs() * 8 * E)
+    u, du = Gy @ W2.T, sums(Gy, W2.T)
+    ga, gb = u * silu, u * a * slope
+    dga = rounded(ga, du * (silu.abs() + dsilu) + u.abs() * dsilu + ga.abs() * 8 * E)
+    dgb = rounded(gb, (du * (a.abs() + da) + u.abs() * da) * (slope.abs() + dslope) + (u * a).abs() * dslope + gb.abs() * 8 * E)
+    gz, dgz = torch.cat([ga, gb], 1), torch.cat([dga, dgb], 1)
+    Gx, GW1, GW2 = oracle.swiglu_block_gradients(x, W1, W2, Gy)
+    out = [(y, dh @ W2.abs() + sums(h.abs() + dh, W2)), (Gx, dgz @ W1.abs().T + sums(gz.abs() + dgz, W1.T)),
+           (GW1, x.abs().T @ dgz + sums(x.T, gz.abs() + dgz)), (GW2, dh.T @ Gy.abs() + sums((h.abs() + dh).T, Gy))]
+    return [(v, dv + (v.abs() + dv) * B + 1e-37) for v, dv in out]
+
+
+def _check(got, bounds):
+    for name, t, (v, off) in zip(("y", "Gx", "GW1", "GW2"), got, bounds):
+        t = t.detach().cpu().double().reshape(v.shape)
+        assert torch.isfinite(t).all() and ((t - v).abs() <= off).all(), (name, ((t - v).abs() / off).max())
+
+
+def _step(block, x, Gy):
+    block.zero_grad()
+    x = x.detach().requires_grad_()
+    y = block(x)
+    y.backward(Gy)
+    return y.detach(), x.grad, block.Wl1_D2H.grad, block.Wl2_HD.grad
+
+
+# M, D, H: one row, ends of groups of 16 and 32 rows, of tiles of 64, 128 and 256; contractions of one, one and a half, two halves of a
+# stage, odd and even; columns short of a tile and past it
+SIZES = [
+    (1, 32, 32), (1, 2048, 96), (3, 96, 2080), (16, 64, 64), (17, 160, 32), (31, 32, 288), (33, 288, 96), (64, 128, 128), (65, 96, 64), (128, 96, 64),
+    (130, 224, 160), (257, 416, 352), (300, 640, 96), (513, 128, 1056), (700, 1056, 128), (1025, 320, 576), (2000, 96, 32), (5000, 64, 160),
+]
+
+
+@pytest.mark.parametrize("M,D,H", SIZES)
+def test_values_and_gradients(M, D, H):
+    x, W1, W2, Gy = _inputs(M, D, H)
+    bounds = _bounds(x, W1, W2, Gy)
+    for save in (0, 50, 100):
+        got = _step(_block(W1, W2, save), x.to(DEV), Gy.to(DEV))
+        assert all(t.dtype == torch.bfloat16 for t in got)
+        _check(got, bounds)
+        with torch.no_grad():
+            assert torch.equal(_block(W1, W2, save)(x.to(DEV)), got[0])
+
+
+def test_gradients_by_differences():
+    """v = sum(y * G_y) at two points of a line through each input: v(p + d) - v(p - d) = 2 g . d + r, where r, what the definition in 64 bits
+    has beyond its own derivative on so long a step, is computed from it.  The left side is off by the bounds of y at the two points
+    times |G_y|, the right by those of g times |d|."""
+    M, D, H = 64, 96, 64
+    x, W1, W2, Gy = _inputs(M, D, H)
+    grads = _step(_block(W1, W2), x.to(DEV), Gy.to(DEV))[1:]
+    bounds = _bounds(x, W1, W2, Gy)[1:]
+    for i, (g, (exact, off)) in enumerate(zip(grads, bounds)):
+        step = (g.cpu().float() * ((x, W1, W2)[i].float().norm() / g.float().norm().item())).to(torch.bfloat16)  # as long as the input itself
+        value, true, slack, points = [], [], 0.0, []
+        for sign in (1, -1):
+            p = [x, W1, W2]
+            p[i] = (p[i].float() + sign * step.float()).to(torch.bfloat16)
+            y = _block(p[1], p[2])(p[0].to(DEV)).cpu().double()
+            want, dy = _bounds(*p, Gy)[0]
+            value.append((y * Gy.double()).sum().item())
+            true.append((want * Gy.double()).sum().item())
+            slack += (dy * Gy.double().abs()).sum().item()
+            points.append(p[i].double())
+        d = points[0] - points[1]
+        r = true[0] - true[1] - (exact * d).sum().item()
+        slack += (off * d.abs()).sum().item()
+        along = (g.cpu().double() * d).sum().item()
+        assert slack < 0.3 * abs(along) and abs(value[0] - value[1] - along - r) <= slack, (i, slack, along, r)
+
+
+@pytest.mark.parametrize("save", [0, 50, 100])
+def test_only_the_gradients_that_are_wanted(save):
+    M, D, H = 100, 96, 160
+    x, W1, W2, Gy = _inputs(M, D, H)
+    ref = _step(_block(W1, W2, save), x.to(DEV), Gy.to(DEV))[1:]
+    for wanted in range(1, 8):
+        block, xd = _block(W1, W2, save), x.to(DEV)
+        leaves = [xd, block.Wl1_D2H, block.Wl2_HD]
+        for i, t in enumerate(leaves):
+            t.requires_grad_(bool(wanted >> i & 1))
+        block(xd).backward(Gy.to(DEV))
+        for i, (t, r) in enumerate(zip(leaves, ref)):
+            assert (t.grad is None) if not wanted >> i & 1 else torch.equal(t.grad, r)
+
+
+def test_strides_types_shapes_and_places():
+    M, D, H = 60, 96, 64
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(M, D, H)]
+    ref = _step(_block(W1, W2), x, Gy)
+    wide = torch.zeros(2 * M, D + 24, device=DEV, dtype=torch.bfloat16)
+    for at in (0, 3, 8):
+        wide[::2, at:at + D] = x
+        gwide = torch.zeros_like(wide)
+        gwide[::2, at:at + D] = Gy
+        got = _step(_block(W1, W2), wide[::2, at:at + D], gwide[::2, at:at + D])
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    for f in (torch.float32, torch.float64):
+        y, Gx, G1, G2 = _step(_block(W1, W2), x.to(f), Gy)
+        assert y.dtype == torch.bfloat16 and Gx.dtype == f and all(torch.equal(a.to(torch.bfloat16), b) for a, b in zip((y, Gx, G1, G2), ref))
+    got = _step(_block(W1, W2), x.view(3, 5, 4, D), Gy.view(3, 5, 4, D))
+    assert got[0].shape == got[1].shape == (3, 5, 4, D) and all(torch.equal(a.reshape(b.shape), b) for a, b in zip(got, ref))
+    got = _step(_block(W1, W2), x.T.contiguous().T, Gy.T.contiguous().T)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    # a broadcast input: its gradient is the sum over the rows, of bf16 rows
+    one = x[:1].detach().requires_grad_()
+    _block(W1, W2)(one.expand(M, D)).backward(Gy)
+    rows = _step(_block(W1, W2), x[:1].repeat(M, 1), Gy)[1].float()
+    assert one.grad.shape == (1, D) and ((one.grad.float() - rows.sum(0)).abs() <= 2 * B * rows.sum(0).abs() + M * B * rows.abs().amax(0)).all()
+    # a vector, a tensor on the host, a broadcast gradient, no rows
+    assert torch.equal(_block(W1, W2)(x[0]), _block(W1, W2)(x[:1])[0])
+    host = x.cpu().requires_grad_()
+    y = _block(W1, W2)(host)
+    y.backward(Gy.cpu())
+    assert y.device.type == "cpu" and torch.equal(y, ref[0].cpu()) and torch.equal(host.grad, ref[1].cpu())
+    a = _step(_block(W1, W2), x, torch.ones(1, 1, device=DEV, dtype=torch.bfloat16).expand(M, D))
+    b = _step(_block(W1, W2), x, torch.ones(M, D, device=DEV, dtype=torch.bfloat16))
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    for save in (0, 100):
+        y, Gx, G1, G2 = _step(_block(W1, W2, save), x[:0], Gy[:0])
+        assert y.shape == Gx.shape == (0, D) and (G1 == 0).all() and (G2 == 0).all()
+
+
+@pytest.mark.parametrize("save", [0, 100])
+@pytest.mark.parametrize("M", [40, 600])
+def test_rows_of_nan_and_infinity_stay_with_themselves(M, save):
+    D, H = 160, 288
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(M, D, H)]
+    ref = _step(_block(W1, W2, save), x, Gy)
+    bad, gbad = x.clone(), Gy.clone()
+    bad[3, 100], bad[17, 20], bad[M - 1, 0], gbad[20, 5], gbad[M - 2, 0] = float("nan"), float("inf"), float("-inf"), float("nan"), float("inf")
+    keep = torch.ones(M, dtype=torch.bool, device=DEV)
+    keep[[3, 17, 20, M - 1, M - 2]] = False
+    got = _step(_block(W1, W2, save), bad, gbad)
+    assert torch.equal(got[0][keep], ref[0][keep]) and torch.equal(got[1][keep], ref[1][keep])
+    assert not got[0][3].isfinite().any() and not got[1][20].isfinite().any()
+    # of the gradient of W2 column d sees G_y[:, d] alone: those without a bad value in it or a bad h
+    ok = _step(_block(W1, W2, save), x, gbad)[3]
+    cols = torch.ones(D, dtype=torch.bool, device=DEV)
+    cols[[5, 0]] = False
+    assert torch.equal(ok[:, cols], ref[3][:, cols]) and not ok[:, 5].isfinite().any() and not ok[:, 0].isfinite().any()
+
+
+def test_rows_behind_the_last_stay_as_they_are():
+    """Results lie in a larger buffer of the allocator's: what is behind them keeps its bits."""
+    D, H = 96, 64
+    for M in (1, 31, 33, 100):
+        x, W1, W2, Gy = [t.to(DEV) for t in _inputs(M, D, H)]
+        y = torch.full((M + 40, D), 7.0, device=DEV, dtype=torch.bfloat16)
+        h = torch.full((H // 32, M, 32), 7.0, device=DEV, dtype=torch.bfloat16)
+        guard = torch.full((4096,), 7.0, device=DEV, dtype=torch.bfloat16)
+        lib, st = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream
+        assert lib.momoe_ffn_lin1_fwd(x.data_ptr(), D, W1.data_ptr(), h.data_ptr(), None, 0, M, M, D, H, st) == 0
+        assert lib.momoe_ffn_lin2_fwd(h.data_ptr(), W2.data_ptr(), y.data_ptr(), M, M, D, H, st) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y[:M], _block(W1, W2)(x)) and (y[M:] == 7).all() and (guard == 7).all()
+
+
+@pytest.mark.parametrize("M,save", [(40, 0), (300, 50), (700, 100)])
+def test_streams_and_replayed_graphs(M, save):
+    D, H = 160, 288
+    ins = [[t.to(DEV) for t in _inputs(M, D, H, seed=i)] for i in range(3)]
+    block = _block(ins[0][1], ins[0][2], save)
+
+    def step(x, Gy):
+        y = block(x)
+        return (y, *torch.autograd.grad(y, (x, block.Wl1_D2H, block.Wl2_HD), Gy))
+    leaf = lambda i: (ins[i][0].detach().requires_grad_(), ins[i][3])
+    ref = [[t.detach().clone() for t in step(*leaf(i))] for i in range(3)]
+    torch.cuda.synchronize()
+    streams, out = [torch.cuda.Stream() for _ in ins], []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            out.append([t.detach() for t in step(*leaf(i))])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for u, v in zip(out, ref) for a, b in zip(u, v))
+    del out
+    x, Gy = leaf(0)
+    x = x.detach().clone().requires_grad_()
+    Gy = Gy.clone()
+    with torch.cuda.stream(streams[0]):
+        step(x, Gy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, Gy)
+    got = [t.detach() for t in got]
+    for i in (1, 2, 0, 1):
+        with torch.no_grad():
+            x.copy_(ins[i][0])
+            Gy.copy_(ins[i][3])
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref[i]))
+        eager = step(*leaf(i))
+        assert all(torch.equal(a, b) for a, b in zip(eager, ref[i]))
+        torch.cuda.synchronize()
+
+
+def test_beside_a_mixture():
+    """As a model has it: a dense layer, then a mixture, one backward through both; and a step of an optimizer."""
+    D, H, N, K, S = 64, 96, 4, 2, 50
+    g = torch.Generator().manual_seed(1)
+    r = lambda *size: (torch.randn(*size, generator=g) * 0.1).to(DEV)
+    dense = momoe_amd.FeedForward(D, H, 100, r(D, 2 * H), r(H, D))
+    moe = momoe_amd.MoE(D, H, N, K, 0, Wg_DN=r(D, N), Wl1_ND2H=r(N, D, 2 * H), Wl2_NHD=r(N, H, D))
+    x = r(2, S, D).to(torch.bfloat16).requires_grad_()
+    mid = x + dense(x)
+    mid.retain_grad()
+    y = mid + moe(mid)
+    y.float().square().sum().backward()
+    want = _step(copy.deepcopy(dense), x, mid.grad)
+    assert torch.equal(dense.Wl1_D2H.grad, want[2]) and torch.equal(dense.Wl2_HD.grad, want[3])
+    assert ((x.grad - (mid.grad.float() + want[1].float())).abs() <= B * (mid.grad.float() + want[1].float()).abs() + 1e-30).all()
+    before = dense.Wl1_D2H.detach().clone()
+    torch.optim.SGD(dense.parameters(), lr=0.1).step()
+    assert not torch.equal(before, dense.Wl1_D2H)
+    with torch.no_grad():
+        served = dense.to_int4(32)
+        y4, ref = served(x), dense(x)
+    W = [oracle.int4_weights(*[t.cpu() for t in q], 32) for q in ((w[0], w[1], w[4]) if i == 0 else (w[2], w[3], w[5])
+                                                               for i, w in ((0, served.weights()), (1, served.weights())))]
+    want4 = oracle.swiglu_block(x.detach().cpu().reshape(-1, D), *W)[3]
+    assert (y4.cpu().double().reshape(want4.shape) - want4).norm() <= 2 * B * want4.norm()
+    assert (y4 - ref).norm() < 0.5 * ref.norm()
+
+
+def test_traced_block():
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(40, 96, 64)]
+    block = _block(W1, W2, 50)
+    traced = torch.jit.trace(block, (x,))
+    for M in (40, 7, 300):
+        xs, _, _, g = [t.to(DEV) for t in _inputs(M, 96, 64, seed=M)]
+        a, b = _step(block, xs, g), None
+        leaf = xs.detach().requires_grad_()
+        block.zero_grad()
+        y = traced(leaf)
+        y.backward(g)
+        b = y.detach(), leaf.grad, block.Wl1_D2H.grad, block.Wl2_HD.grad
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_refusals():
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(10, 96, 64)]
+    f = momoe_amd.FeedForwardFunction.apply
+    for bad in ((x[:, :64], W1, W2), (x, W1[:64], W2), (x, W1[:, :64], W2), (x, W1, W2[:32]), (x, W1, W2[:, :64]), (x[0, 0], W1, W2), (x, W1, W2.cpu())):
+        with pytest.raises(AssertionError):
+            f(*bad)
+    for bad in ((x, W1[:, :96].contiguous(), W2[:48]), (x[:, :48], W1[:48], W2[:, :48])):
+        with pytest.raises(RuntimeError, match="multiples of 32"):
+            f(*bad)
+    for save in (-1, 101, float("nan")):
+        with pytest.raises(RuntimeError, match="save_percent"):
+            f(x, W1, W2, save)
+    block, leaf = _block(W1, W2), x.clone().requires_grad_()
+    y = block(leaf)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y, leaf, Gy, create_graph=True)
+    huge = torch.empty(1, 1, device=DEV, dtype=torch.bfloat16).expand(1 << 23, 32)
+    with pytest.raises(RuntimeError, match="split the batch"):
+        _block(torch.zeros(32, 64), torch.zeros(32, 32))(huge)
+    with torch.no_grad():
+        block.Wl1_D2H.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(Gy)
+    for shape in ((10, 96), (2, 5, 96)):
+        changed = x.clone().view(shape)
+        y = _block(W1, W2)(changed)
+        changed.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(Gy.view(shape))
