@@ -528,7 +528,9 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * momoe_ffn_dgrad_h_saved: gz and hT from the a | b that were kept, u on the way.
  * Both write {0, ldm} to counts2 (may be NULL).
  * momoe_ffn_dgrad_x: Gx [rows][D].
+ * momoe_ffn_wgrad_workspace_bytes: what to give momoe_wgrad for a gradient [X][Y] of one expert with all rows (any other size will do).
  */
+int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y);
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);

@@ -33,6 +33,7 @@ struct FfnArgs {
   bf16* ht;
   bf16* out;       // y or G_x, row-major, D columns
   int32_t* counts; // {0, ldm}: what momoe_wgrad takes as the rows of its one expert
+  unsigned long long* clk = clock_trace_buffer();
 };
 
 // fragment (row / 16, column / 16) of a matrix of `cols` columns, this lane's four values
@@ -235,6 +236,321 @@ template <int FM> using Lin1Bwd = FfnLin1<FM, true>;
 template <int FM> using DhPlain = FfnDh<FM, false>;
 template <int FM> using DhSaved = FfnDh<FM, true>;
 
+// ---- large launches: the loop of gemm_span.hpp ------------------------------------------------------------------------------------
+// Its tiles of a dense block: as SpanSched deals those of one expert that holds all rows, without a table.
+struct DenseSpanSched {
+  using Tiles = TileSchedT<WideSpan::WROWS, WideSpan::MAX_ROWS, kSpanWaves>;
+  static constexpr int kBand = Tiles::kBandTiles;
+  struct Raw {
+    int q;
+    bool any, piece;
+  };
+  int rows, nb, nt, begin, limit, pos, stride, rest, cut;
+  __device__ __forceinline__ DenseSpanSched(int rows_, int nb_) : rows(rows_), nb(nb_), nt((rows_ + WideSpan::MAX_ROWS - 1) / WideSpan::MAX_ROWS) {
+    const int total = nt * nb, chunk = (total + 7) >> 3;
+    begin = (int)(blockIdx.x & 7) * chunk;
+    limit = max(0, min(chunk, total - begin));
+    pos = blockIdx.x >> 3;
+    stride = gridDim.x >> 3;
+    rest = limit % stride;
+    cut = 8 * rest <= stride ? 8 : 4 * rest <= stride ? 4 : 2;
+    if (2 * rest > stride || rest == 0) cut = 0;
+    else limit -= rest;
+  }
+  __device__ __forceinline__ int order() const { return blockIdx.x >> 3; }
+  __device__ __forceinline__ Raw fetch() {
+    const bool whole = pos < limit;
+    Raw r;
+    r.piece = !whole && cut > 0 && order() < rest * cut;
+    r.any = whole || r.piece;
+    r.q = begin + (whole ? pos : limit + order() / max(cut, 1));
+    if (!whole) rest = 0;
+    pos += stride;
+    return r;
+  }
+  __device__ __forceinline__ TileCoord resolve(const Raw& r) const {
+    TileCoord tc;
+    tc.valid = r.any;
+    if (!r.any) return tc;
+    const int nfe = (rows + 31) >> 5, fbase = nfe / nt, fextra = nfe - fbase * nt;
+    const int band = r.q / (kBand * nb), in_band = r.q - band * (kBand * nb), band_rows = min(kBand, nt - band * kBand);
+    const int tl = band * kBand + in_band % band_rows;
+    tc.tn = in_band / band_rows;
+    int f0 = tl * fbase + min(tl, fextra), nf = fbase + (tl < fextra ? 1 : 0);
+    if (r.piece) {
+      const int part = order() % cut, base = nf / cut, extra = nf - base * cut;
+      f0 += part * base + min(part, extra);
+      nf = base + (part < extra ? 1 : 0);
+    }
+    tc.expert = 0;
+    tc.row0 = tc.prow0 = 32 * f0;
+    tc.rows = min(32 * nf, rows - 32 * f0);
+    tc.alone = false;
+    tc.valid = tc.rows > 0;
+    Tiles::deal(tc);
+    return tc;
+  }
+  __device__ __forceinline__ TileCoord next() { return resolve(fetch()); }
+};
+
+struct DenseSpan {
+  using G = WideSpan;
+  static constexpr bool EXCHANGE = false;
+  struct Ids {};
+  struct Late {};
+  const FfnArgs& p;
+  const int K;
+  int n_org;
+  __device__ __forceinline__ DenseSpan(const FfnArgs& p_, int K_, int width) : p(p_), K(K_), n_org(wave_id() % G::WCOLS * width) {}
+  __device__ __forceinline__ void gather(const TileCoord&, Ids&) const {}
+  __device__ __forceinline__ void late(const TileCoord&, const Ids&, Late&) const {}
+  __device__ __forceinline__ void settle(Ids&) const {}
+  __device__ __forceinline__ void settle(Late&) const {}
+  __device__ __forceinline__ void finish(const TileCoord&, bf16*) const {}
+  template <int NA>
+  __device__ __forceinline__ void store_out(const TileCoord& tc, f32x4 (&acc)[G::FN][NA], bf16* staging) const {
+    store_rows(acc, staging, p.out, (int64_t)tc.row0 + tc.mbase, tc.rows - tc.mbase, p.D, tc.tn * G::COLS + n_org, fresh_lane(),
+               [](int) { return 1.0f; });
+  }
+};
+
+// gz and hT of the 64 hidden columns from j0 of a wave's rows.  load(i): the values of fragment row i that come from memory are asked for;
+// values(i, f, a, b, u): all of fragment (i, f).  Staging areas: 0 G_a, 1 G_b, 2 and 3 h of 32 rows.
+template <int NA, class Load, class Values>
+__device__ __forceinline__ void store_gradients(const FfnArgs& p, const TileCoord& tc, int j0, bf16* staging, Load load, Values values) {
+  constexpr int HF = 4;
+  using Stager = SpanStager<16 * HF>;
+  static_assert(4 * Stager::ELEMS <= kStagingElems && NA % 2 == 0, "four areas; groups of 32 rows");
+  const int H = p.H, l = fresh_lane(), rows = tc.rows - tc.mbase;
+  const Stager stager(staging, l);
+  const int64_t r0 = (int64_t)tc.row0 + tc.mbase;
+  bf16* const gza = p.gz + ((int64_t)(j0 >> 5) * p.ldm + r0) * 32;  // uniform
+  const int64_t to_b = (int64_t)(H >> 5) * p.ldm * 32;
+  const uint32_t off = (stager.block_row() * 32 + stager.block_col()) * 2;
+  bf16x8 v[2][2][Stager::PASSES];
+  auto store_gz = [&](int i) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int q = 0; q < Stager::PASSES; ++q)
+        store16(gza + half * to_b + ((int64_t)q * p.ldm + 16 * i) * 32, off, 16 * i + stager.block_row() < rows && j0 + 32 * q < H, v[i & 1][half][q]);
+  };
+  bf16* const ht = p.ht + ((r0 >> 5) * H + j0) * 32;  // uniform
+  const uint32_t hoff = (l & 15) * 64 + (l >> 4) * 16;
+  bf16x8 hv[HF];
+  auto store_h = [&](int i) {
+    if (!p.ht) return;
+#pragma unroll
+    for (int q = 0; q < HF; ++q) store16(ht + ((int64_t)(i / 2) * H + 16 * q) * 32, hoff, j0 + 16 * q < H, hv[q]);
+  };
+  load(0);
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    if (i + 1 < NA) load(i + 1);
+    const bool some = 16 * i + (l & 15) < rows;
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+      f32x4 a, b, u;
+      values(i, f, a, b, u);
+      float va[4], vb[4], vh[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const SwigluGrad g(a[e], b[e], u[e]);
+        va[e] = g.a, vb[e] = g.b, vh[e] = some ? g.h : 0.0f;
+      }
+      stager.put(0, f, pack_bf16x4(va[0], va[1], va[2], va[3]));
+      stager.put(1, f, pack_bf16x4(vb[0], vb[1], vb[2], vb[3]));
+      stager.put(2 + (i & 1), f, pack_bf16x4(vh[0], vh[1], vh[2], vh[3]));
+    }
+    if (i > 0) store_gz(i - 1);
+    if (i > 0 && i % 2 == 0) store_h(i - 1);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int q = 0; q < Stager::PASSES; ++q) v[i & 1][half][q] = stager.get_block(half, q);
+    if (i % 2 == 1) {
+#pragma unroll
+      for (int q = 0; q < HF; ++q) hv[q] = stager.get_rows(2, q);
+    }
+    order_fence();  // (loads of several rounds ahead were spilled)
+  }
+  store_gz(NA - 1);
+  store_h(NA - 1);
+}
+// where fragment row i of a wave's lies among the fragments of a matrix of `cols` columns, from column col; past the last row or column
+// (of which nothing is used) at one that exists
+__device__ __forceinline__ const float* fragment_of(const float* m, const FfnArgs& p, const TileCoord& tc, int i, int cols, int col, bool in) {
+  const int64_t rf = min((int64_t)tc.row0 + tc.mbase + 16 * i, p.rows - 1) >> 4;
+  return m + ((rf * (cols >> 4) + (in ? col >> 4 : 0)) << 8);
+}
+
+template <bool BWD>
+struct Lin1DenseSpan : DenseSpan {
+  static constexpr int BNH = G::COLS / 2, WIDTH = 8 * G::FN, HF = G::FN / 2;  // hidden columns of a tile, of a wave
+  using Rows = FfnRows<256>;
+  using Weights = SpanCols<true>;
+  __device__ __forceinline__ explicit Lin1DenseSpan(const FfnArgs& p_) : DenseSpan(p_, p_.D, WIDTH) {}
+  __device__ __forceinline__ void setup(const TileCoord& t, const Ids&, Rows& A, Weights& W) const {
+    const int H = p.H, j0 = t.tn * BNH;
+    A.init(p.x, p.ldx, t.row0, t.rows, K);
+    W.init(p.w, 2 * H, [&](int c) { return (c / BNH) * H + min(j0 + (c % BNH), H - 8); });
+  }
+  template <int NA>
+  __device__ __forceinline__ void epilogue(const TileCoord& tc, f32x4 (&acc)[G::FN][NA], const Ids&, const Late&, bf16* staging) const {
+    const int H = p.H, j0 = tc.tn * BNH + n_org;  // first hidden column of this wave
+    if constexpr (BWD) {
+      f32x4 uq[2][HF];
+      const int l = fresh_lane();
+      store_gradients<NA>(
+          p, tc, j0, staging,
+          [&](int i) {
+#pragma unroll
+            for (int f = 0; f < HF; ++f) uq[i & 1][f] = *(const f32x4*)(fragment_of(p.u, p, tc, i, H, j0 + 16 * f, j0 + 16 * f < H) + 4 * l);
+          },
+          [&](int i, int f, f32x4& a, f32x4& b, f32x4& u) { a = acc[f][i], b = acc[HF + f][i], u = uq[i & 1][f]; });
+    } else {
+      using Stager = SpanStager<WIDTH>;
+      const Stager stager(staging, fresh_lane());
+      const int rows = tc.rows - tc.mbase;
+      const int64_t r0 = (int64_t)tc.row0 + tc.mbase;
+      keep_in_place(acc);
+      bf16* const first = p.h + ((int64_t)(j0 >> 5) * p.ldm + r0) * 32;  // uniform
+      const uint32_t off = (stager.block_row() * 32 + stager.block_col()) * 2;
+      bf16x8 v[2][Stager::PASSES];
+      auto store = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < Stager::PASSES; ++q)
+          store16(first + ((int64_t)q * p.ldm + 16 * i) * 32, off, 16 * i + stager.block_row() < rows && j0 + 32 * q < H, v[i & 1][q]);
+      };
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+#pragma unroll
+        for (int f = 0; f < HF; ++f) {
+          float hv[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hv[e] = swiglu(acc[f][i][e], acc[HF + f][i][e]);
+          stager.put(i & 1, f, pack_bf16x4(hv[0], hv[1], hv[2], hv[3]));
+        }
+        if (i > 0) store(i - 1);
+#pragma unroll
+        for (int q = 0; q < Stager::PASSES; ++q) v[i & 1][q] = stager.get_block(i & 1, q);
+      }
+      store(NA - 1);
+      if (r0 < p.ab_rows) {
+        keep_in_place(acc);
+        const int l = fresh_lane();
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+          if (r0 + 16 * i >= p.ab_rows) break;
+#pragma unroll
+          for (int f = 0; f < G::FN; ++f) {
+            const int col = j0 + 16 * (f % HF);
+            if (col >= H) continue;
+            float* const to = p.ab + ((((r0 >> 4) + i) * (2 * H >> 4) + ((f / HF * H + col) >> 4)) << 8);
+            *(f32x4*)(to + 4 * l) = acc[f][i];
+          }
+        }
+      }
+    }
+  }
+};
+
+struct Lin2DenseSpan : DenseSpan {
+  using Rows = SpanBlockedRows<256>;
+  using Weights = SpanCols<>;
+  __device__ __forceinline__ explicit Lin2DenseSpan(const FfnArgs& p_) : DenseSpan(p_, p_.H, 16 * G::FN) {}
+  __device__ __forceinline__ void setup(const TileCoord& t, const Ids&, Rows& A, Weights& W) const {
+    const int D = p.D, d0 = t.tn * G::COLS;
+    A.init(p.h, p.ldm, t.row0, t.rows);
+    W.init(p.w, D, [&](int c) { return min(d0 + c, D - 8); });
+  }
+  template <int NA>
+  __device__ __forceinline__ void epilogue(const TileCoord& tc, f32x4 (&acc)[G::FN][NA], const Ids&, const Late&, bf16* staging) const {
+    store_out(tc, acc, staging);
+  }
+};
+
+template <bool SAVED>
+struct DhDenseSpan : DenseSpan {
+  using Rows = FfnRows<256>;
+  using Weights = SpanPitchedRows<G::COLS>;
+  __device__ __forceinline__ explicit DhDenseSpan(const FfnArgs& p_) : DenseSpan(p_, p_.D, 16 * G::FN) {}
+  __device__ __forceinline__ void setup(const TileCoord& t, const Ids&, Rows& A, Weights& W) const {
+    A.init(p.x, p.ldx, t.row0, t.rows, K);
+    W.init(p.w, p.D, t.tn * G::COLS, p.H);
+  }
+  template <int NA>
+  __device__ __forceinline__ void epilogue(const TileCoord& tc, f32x4 (&acc)[G::FN][NA], const Ids&, const Late&, bf16* staging) const {
+    const int H = p.H, j0 = tc.tn * G::COLS + n_org, l = fresh_lane();
+    if constexpr (SAVED) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int jh = j0 + 64 * half;
+        f32x4 ab[2][4][2];
+        store_gradients<NA>(
+            p, tc, jh, staging,
+            [&](int i) {
+#pragma unroll
+              for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                  ab[i & 1][f][q] = *(const f32x4*)(fragment_of(p.ab, p, tc, i, 2 * H, q * H + jh + 16 * f, jh + 16 * f < H) + 4 * l);
+            },
+            [&](int i, int f, f32x4& a, f32x4& b, f32x4& u) { a = ab[i & 1][f][0], b = ab[i & 1][f][1], u = acc[4 * half + f][i]; });
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        if (16 * i >= tc.rows - tc.mbase) break;
+#pragma unroll
+        for (int f = 0; f < G::FN; ++f)
+          if (j0 + 16 * f < H)
+            *(f32x4*)(const_cast<float*>(fragment_of(p.u, p, tc, i, H, j0 + 16 * f, true)) + 4 * l) = acc[f][i];
+      }
+    }
+  }
+};
+
+struct DxDenseSpan : DenseSpan {
+  using Rows = SpanBlockedRows<256>;
+  using Weights = SpanPitchedRows<G::COLS>;
+  __device__ __forceinline__ explicit DxDenseSpan(const FfnArgs& p_) : DenseSpan(p_, 2 * p_.H, 16 * G::FN) {}
+  __device__ __forceinline__ void setup(const TileCoord& t, const Ids&, Rows& A, Weights& W) const {
+    A.init(p.gz, p.ldm, t.row0, t.rows);
+    W.init(p.w, K, t.tn * G::COLS, p.D);
+  }
+  template <int NA>
+  __device__ __forceinline__ void epilogue(const TileCoord& tc, f32x4 (&acc)[G::FN][NA], const Ids&, const Late&, bf16* staging) const {
+    store_out(tc, acc, staging);
+  }
+};
+
+template <class P>
+__global__ __launch_bounds__(kSpanThreads, 1) void ffn_span_kernel(FfnArgs p, int nb) {
+  const ClockTrace trace(p.clk);
+  if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.ldm : 0;
+  run_span_tiles_of<P>(p, DenseSpanSched((int)p.rows, nb));
+  trace.finish();
+}
+
+// ---- which of the two -----------------------------------------------------------------------------------------------------------
+// 256 x 256 tiles where they are half a round of one a CU at least (and there are two stages of k-values)
+inline bool takes_span(int64_t rows, int64_t cols, int64_t contraction) {
+  return contraction >= WideSpan::AHEAD * kSpan && 2 * cdiv64(rows, WideSpan::MAX_ROWS) * cdiv64(cols, WideSpan::COLS) >= persistent_grid();
+}
+template <class P>
+int launch_dense_span(const FfnArgs& a, int64_t cols, hipStream_t st) {
+  static LdsLimit lds;
+  if (!allow_lds(ffn_span_kernel<P>, kSpanLds, lds)) return MOMOE_ERR_LAUNCH;
+  ffn_span_kernel<P><<<persistent_grid(), kSpanThreads, kSpanLds, st>>>(a, (int)cdiv64(cols, WideSpan::COLS));
+  return launch_status();
+}
+// cols, contraction: of the product (of x W1 both halves' columns)
+template <class Span, template <int> class P>
+int launch(const FfnArgs& a, int64_t cols, int64_t contraction, int64_t col_tiles, hipStream_t st) {
+  return takes_span(a.rows, cols, contraction) ? launch_dense_span<Span>(a, cols, st) : launch_by_rows<P>(a, col_tiles, st);
+}
+
 int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
   if (rows <= 0 || D <= 0 || H <= 0 || ldm < rows) return MOMOE_ERR_BAD_ARG;
   // 32-bit byte offsets into a weight matrix, and from a k-blocked tile's first row
@@ -254,6 +570,16 @@ extern "C" int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols) {
   return rows < 0 || cols <= 0 || cols % 16 != 0 ? -1 : (rows + 15) / 16 * 16 * cols;
 }
 
+// An expert of all rows is cut along them, through the workspace, where its tiles leave CUs idle in their last round; tiles that fill 5 of 6
+// are done whole, which saves the partial sums' way through memory.  Us, 8192 tokens, D = 2048, H = 8192 (256 and 512 tiles of 256 x 256), cut |
+// whole: W2 335 | 256, W1 640 | 470.
+extern "C" int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y) {
+  const int64_t bytes = momoe_wgrad_workspace_bytes(1, X, Y, rows);
+  if (bytes <= 0) return bytes;
+  const int64_t tiles = cdiv64(X, 256) * cdiv64(Y, 256), grid = persistent_grid(), rounds = cdiv64(tiles, grid);
+  return 6 * tiles >= 5 * rounds * grid ? 0 : bytes;
+}
+
 extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                                   int64_t ldm, int64_t D, int64_t H, void* stream) {
   if (!x || !W1_D2H || !h_blocked || (ab_rows > 0 && !ab) || ab_rows < 0 || ab_rows > (rows + 31) / 32 * 32 || ldx < D) return MOMOE_ERR_BAD_ARG;
@@ -265,7 +591,7 @@ extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H
   a.h = (bf16*)h_blocked;
   a.ab = ab;
   a.ab_rows = std::min((rows + 15) / 16 * 16, ab_rows);
-  return launch_by_rows<Lin1Fwd>(a, cdiv64(H, 64), (hipStream_t)stream);
+  return launch<Lin1DenseSpan<false>, Lin1Fwd>(a, 2 * H, D, cdiv64(H, 64), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H,
@@ -277,7 +603,7 @@ extern "C" int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void
   FfnArgs a{nullptr, 0, (const bf16*)W2_HD, rows, ldm, (int)D, (int)H};
   a.h = (bf16*)h_blocked;
   a.out = (bf16*)y;
-  return launch_by_rows<FfnLin2>(a, cdiv64(D, kFfnCols), (hipStream_t)stream);
+  return launch<Lin2DenseSpan, FfnLin2>(a, D, H, cdiv64(D, kFfnCols), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_dgrad_h(const void* Gy, int64_t ldgy, const void* W2_HD, float* u, int64_t rows, int64_t D, int64_t H, void* stream) {
@@ -288,7 +614,7 @@ extern "C" int momoe_ffn_dgrad_h(const void* Gy, int64_t ldgy, const void* W2_HD
   if (ldgy % 8 != 0 || ldgy >= (1 << 22)) return MOMOE_ERR_UNSUPPORTED;
   FfnArgs a{(const bf16*)Gy, ldgy, (const bf16*)W2_HD, rows, rows, (int)D, (int)H};
   a.u = u;
-  return launch_by_rows<DhPlain>(a, cdiv64(H, kFfnCols), (hipStream_t)stream);
+  return launch<DhDenseSpan<false>, DhPlain>(a, H, D, cdiv64(H, kFfnCols), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D2H, const float* u, void* gz_blocked, void* hT, int32_t* counts2,
@@ -303,7 +629,7 @@ extern "C" int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D
   a.gz = (bf16*)gz_blocked;
   a.ht = (bf16*)hT;
   a.counts = counts2;
-  return launch_by_rows<Lin1Bwd>(a, cdiv64(H, 64), (hipStream_t)stream);
+  return launch<Lin1DenseSpan<true>, Lin1Bwd>(a, 2 * H, D, cdiv64(H, 64), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void* W2_HD, const float* ab, void* gz_blocked, void* hT,
@@ -318,7 +644,7 @@ extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void*
   a.gz = (bf16*)gz_blocked;
   a.ht = (bf16*)hT;
   a.counts = counts2;
-  return launch_by_rows<DhSaved>(a, cdiv64(H, kFfnCols), (hipStream_t)stream);
+  return launch<DhDenseSpan<true>, DhSaved>(a, H, D, cdiv64(H, kFfnCols), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H,
@@ -330,5 +656,5 @@ extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, voi
   FfnArgs a{nullptr, 0, (const bf16*)W1_D2H, rows, rows, (int)D, (int)H};
   a.gz = (bf16*)const_cast<void*>(gz_blocked);
   a.out = (bf16*)Gx;
-  return launch_by_rows<FfnDx>(a, cdiv64(D, kFfnCols), (hipStream_t)stream);
+  return launch<DxDenseSpan, FfnDx>(a, D, 2 * H, cdiv64(D, kFfnCols), (hipStream_t)stream);
 }

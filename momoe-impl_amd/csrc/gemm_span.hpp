@@ -424,12 +424,10 @@ __device__ __forceinline__ void settle(T& v) {
 // not see the transfers, so its wait for any load is a wait for every transfer older than the
 // youngest few, which cost a memory latency per tile in the middle of a stage; there the transfers
 // have had the epilogue to arrive.
-// The launch has `nb` column blocks; `first`: row tiles left out.
-template <class P, class Args>
-__device__ __forceinline__ void run_span_tiles(const Args& args, int nb, int max_tile_rows, int first = 0) {
+// `sched`: SpanSched, or one of its interface.
+template <class P, class Args, class Sched>
+__device__ __forceinline__ void run_span_tiles_of(const Args& args, Sched sched) {
   using G = typename P::G;
-  using Sched = SpanSched<G>;
-  Sched sched(args.table, nb, max_tile_rows, first);
   P prog(args);
   using Rows = typename P::Rows;
   using Weights = typename P::Weights;
@@ -573,6 +571,12 @@ __device__ __forceinline__ void run_span_tiles(const Args& args, int nb, int max
     l0 = l1;
   }
   wait_vmcnt<0>();  // no transfer may outlive the workgroup's LDS
+}
+
+// The launch has `nb` column blocks; `first`: row tiles left out.
+template <class P, class Args>
+__device__ __forceinline__ void run_span_tiles(const Args& args, int nb, int max_tile_rows, int first = 0) {
+  run_span_tiles_of<P>(args, SpanSched<typename P::G>(args.table, nb, max_tile_rows, first));
 }
 
 // Whether a launch over `cols` output columns takes these tiles rather than those of gemm_tile.hpp.  Not

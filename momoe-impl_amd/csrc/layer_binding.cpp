@@ -633,7 +633,7 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
                  need_w2 ? rows_at(hT, msave, H) : nullptr, counts.data_ptr<int32_t>(), M - msave, M, D, H);
     }
     const auto weight_gradient = [&](const void* A, int64_t lda, int a_layout, const void* B, int64_t ldb, int b_layout, const Tensor& G) {
-      const int64_t X = G.size(0), Y = G.size(1), bytes = std::min(M * H * 8, momoe_wgrad_workspace_bytes(1, X, Y, M));
+      const int64_t X = G.size(0), Y = G.size(1), bytes = momoe_ffn_wgrad_workspace_bytes(M, X, Y);
       const Tensor ws = empty_f32({bytes / 4}, dev);
       MOMOE_CALL(momoe_wgrad, st, A, lda, a_layout, (const int32_t*)nullptr, B, ldb, b_layout, (const int32_t*)nullptr,
                  (const int32_t*)counts.data_ptr<int32_t>(), G.data_ptr(), M, (int64_t)1, X, Y, M, bytes > 0 ? ws.data_ptr() : nullptr, bytes);

@@ -99,6 +99,7 @@ _SIGNATURES = {
     "momoe_fp8_few_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_fragment_floats": (_i64, [_i64] * 2),
+    "momoe_ffn_wgrad_workspace_bytes": (_i64, [_i64] * 3),
     "momoe_ffn_lin1_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_lin2_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_dgrad_h": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _p]),

@@ -69,6 +69,8 @@ def _step(block, x, Gy):
 SIZES = [
     (1, 32, 32), (1, 2048, 96), (3, 96, 2080), (16, 64, 64), (17, 160, 32), (31, 32, 288), (33, 288, 96), (64, 128, 128), (65, 96, 64), (128, 96, 64),
     (130, 224, 160), (257, 416, 352), (300, 640, 96), (513, 128, 1056), (700, 1056, 128), (1025, 320, 576), (2000, 96, 32), (5000, 64, 160),
+    # large launches: of x W1 and G_y W2^T, of h W2 and gz W1^T; contractions of an odd number of 32
+    (8200, 160, 1056), (8200, 1056, 160), (17000, 128, 544),
 ]
 
 
