@@ -528,19 +528,24 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * momoe_ffn_dgrad_h_saved: gz and hT from the a | b that were kept, u on the way.
  * Both write {0, ldm} to counts2 (may be NULL).
  * momoe_ffn_dgrad_x: Gx [rows][D].
+ * These two take scratch (of at least momoe_ffn_workspace_bytes(rows, D, H, or 2H); 0, NULL: none is needed) for the sums of a contraction
+ * that is cut because the launch has few tiles.
  * momoe_ffn_wgrad_workspace_bytes: what to give momoe_wgrad for a gradient [X][Y] of one expert with all rows (any other size will do).
  */
 int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y);
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);
-int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
+int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction);
+int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 int momoe_ffn_dgrad_h(const void* Gy, int64_t ldgy, const void* W2_HD, float* u, int64_t rows, int64_t D, int64_t H, void* stream);
 int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D2H, const float* u, void* gz_blocked, void* hT, int32_t* counts2,
                          int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
 int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void* W2_HD, const float* ab, void* gz_blocked, void* hT, int32_t* counts2,
                             int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
-int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H, void* stream);
+int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 /* ---- SwiGLU blocks with weights in 4 bits, forward only -------------------------------
  * No counterpart in the reference, whose weights are bf16.  A weight is (code - zero) * scale: a 4-bit code, and for each `group`

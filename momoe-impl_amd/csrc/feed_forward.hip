@@ -32,6 +32,8 @@ struct FfnArgs {
   bf16* gz;
   bf16* ht;
   bf16* out;       // y or G_x, row-major, D columns
+  float* part;     // its sums by slices of the contraction, [slices][rows][D], where there are several
+  int slices = 1;
   int32_t* counts; // {0, ldm}: what momoe_wgrad takes as the rows of its one expert
   unsigned long long* clk = clock_trace_buffer();
 };
@@ -57,12 +59,12 @@ template <int FM_>
 struct FfnProg {
   static constexpr int FM = FM_;
   const FfnArgs& p;
-  int K, row_tiles, col_tiles;
+  int K, slices, row_tiles, col_tiles;
   int64_t rows;
-  __device__ __forceinline__ FfnProg(const FfnArgs& p_, int K_, int col_tiles_)
-      : p(p_), K(K_), row_tiles((int)((p_.rows + 32 * FM - 1) / (32 * FM))), col_tiles(col_tiles_), rows(p_.rows) {}
+  __device__ __forceinline__ FfnProg(const FfnArgs& p_, int K_, int col_tiles_, int slices_ = 1)
+      : p(p_), K(K_), slices(slices_), row_tiles((int)((p_.rows + 32 * FM - 1) / (32 * FM))), col_tiles(col_tiles_), rows(p_.rows) {}
   // rows as they come out of the accumulators
-  __device__ __forceinline__ void store_rows_plain(int64_t row0, int rows_, int col0, f32x4 (&acc)[4][FM], int wm) const {
+  __device__ __forceinline__ void store_rows_plain(int64_t row0, int rows_, int slice, int col0, f32x4 (&acc)[4][FM], int wm) const {
     const int l = lane_id();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -71,7 +73,9 @@ struct FfnProg {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int r = 16 * (wm * FM + i) + (l & 15);
-        if (r < rows_) *(bf16x4*)(p.out + (row0 + r) * p.D + col) = pack_bf16x4(acc[j][i], 1.0f);
+        if (r >= rows_) continue;
+        if (slices > 1) *(f32x4*)(p.part + (slice * rows + row0 + r) * p.D + col) = acc[j][i];
+        else *(bf16x4*)(p.out + (row0 + r) * p.D + col) = pack_bf16x4(acc[j][i], 1.0f);
       }
     }
   }
@@ -105,7 +109,7 @@ struct FfnLin1 : FfnProg<FM> {
     A.init(p.x, p.ldx, row0, rows, p.D);
     W.init(p.w, 2 * H, p.D, [&](int c) { return (c / 64) * H + min(j0 + c % 64, H - 8); });
   }
-  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int wm, int wn, f32x4 (&acc)[4][FM]) const {
+  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int slice, int wm, int wn, f32x4 (&acc)[4][FM]) const {
     const int l = lane_id(), j0 = tn * 64 + wn * 32;
     if (j0 >= p.H) return;
 #pragma unroll
@@ -142,15 +146,15 @@ struct FfnLin2 : FfnProg<FM> {
   using Rows = FfnBlockedRows<32 * FM>;
   using Weights = FfnCols<false>;
   using Base::p;
-  __device__ __forceinline__ explicit FfnLin2(const FfnArgs& p_) : Base(p_, p_.H, (p_.D + kFfnCols - 1) / kFfnCols) {}
+  __device__ __forceinline__ explicit FfnLin2(const FfnArgs& p_) : Base(p_, p_.H, (p_.D + kFfnCols - 1) / kFfnCols, p_.slices) {}
   __device__ __forceinline__ int n_org(int wn) const { return wn * 64; }
   __device__ __forceinline__ void setup(int64_t row0, int rows, int tn, Rows& A, Weights& W) const {
     const int D = p.D, d0 = tn * kFfnCols;
     A.init(p.h, p.ldm, row0, rows, p.H);
     W.init(p.w, D, p.H, [&](int c) { return min(d0 + c, D - 8); });
   }
-  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int wm, int wn, f32x4 (&acc)[4][FM]) const {
-    Base::store_rows_plain(row0, rows, tn * kFfnCols + wn * 64, acc, wm);
+  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int slice, int wm, int wn, f32x4 (&acc)[4][FM]) const {
+    Base::store_rows_plain(row0, rows, slice, tn * kFfnCols + wn * 64, acc, wm);
   }
 };
 
@@ -167,7 +171,7 @@ struct FfnDh : FfnProg<FM> {
     A.init(p.x, p.ldx, row0, rows, p.D);
     W.init(p.w, p.D, tn * kFfnCols, p.H);
   }
-  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int wm, int wn, f32x4 (&acc)[4][FM]) const {
+  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int slice, int wm, int wn, f32x4 (&acc)[4][FM]) const {
     const int l = lane_id(), j0 = tn * kFfnCols + wn * 64;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -199,37 +203,69 @@ struct FfnDx : FfnProg<FM> {
   using Rows = FfnBlockedRows<32 * FM>;
   using Weights = FfnWeightRows;
   using Base::p;
-  __device__ __forceinline__ explicit FfnDx(const FfnArgs& p_) : Base(p_, 2 * p_.H, (p_.D + kFfnCols - 1) / kFfnCols) {}
+  __device__ __forceinline__ explicit FfnDx(const FfnArgs& p_) : Base(p_, 2 * p_.H, (p_.D + kFfnCols - 1) / kFfnCols, p_.slices) {}
   __device__ __forceinline__ int n_org(int wn) const { return wn * 64; }
   __device__ __forceinline__ void setup(int64_t row0, int rows, int tn, Rows& A, Weights& W) const {
     A.init(p.gz, p.ldm, row0, rows, 2 * p.H);
     W.init(p.w, 2 * p.H, tn * kFfnCols, p.D);
   }
-  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int wm, int wn, f32x4 (&acc)[4][FM]) const {
-    Base::store_rows_plain(row0, rows, tn * kFfnCols + wn * 64, acc, wm);
+  __device__ __forceinline__ void epilogue(int64_t row0, int rows, int tn, int slice, int wm, int wn, f32x4 (&acc)[4][FM]) const {
+    Base::store_rows_plain(row0, rows, slice, tn * kFfnCols + wn * 64, acc, wm);
   }
 };
 
-template <class P>
-__global__ __launch_bounds__(kSpanThreads, P::FM == 2 ? 2 : 1) void ffn_tile_kernel(FfnArgs p) {
+template <class P, int STAGES>
+__global__ __launch_bounds__(kSpanThreads, 2) void ffn_tile_kernel(FfnArgs p) {
   if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.ldm : 0;
-  run_ffn_tile(P(p));
+  run_ffn_tile<P, STAGES>(P(p));
+}
+// out = the sum of the slices, in their order; eight are asked for at once (one behind the other: 5.0 us for 16 slices of one token)
+__global__ __launch_bounds__(256) void ffn_sum_slices_kernel(FfnArgs p) {
+  const int64_t n = p.rows * p.D, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  f32x4 sum = {};
+  for (int s = 0; s < p.slices; s += 8) {
+    f32x4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = *(const f32x4*)(p.part + min(s + j, p.slices - 1) * n + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s + j < p.slices) sum += v[j];
+  }
+  *(bf16x4*)(p.out + at) = pack_bf16x4(sum, 1.0f);
 }
 
-template <class P>
+template <class P, int STAGES>
 int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   static LdsLimit lds;
-  const int64_t tiles = cdiv64(a.rows, 32 * P::FM) * col_tiles;
+  const int64_t tiles = cdiv64(a.rows, 32 * P::FM) * col_tiles * a.slices;
   if (tiles >= (1ll << 31) - 8) return MOMOE_ERR_UNSUPPORTED;
-  if (!allow_lds(ffn_tile_kernel<P>, kFfnLds<P>, lds)) return MOMOE_ERR_LAUNCH;
-  ffn_tile_kernel<P><<<(unsigned)(cdiv64(tiles, 8) * 8), kSpanThreads, kFfnLds<P>, st>>>(a);
+  if (!allow_lds(ffn_tile_kernel<P, STAGES>, kFfnLds<P, STAGES>, lds)) return MOMOE_ERR_LAUNCH;
+  ffn_tile_kernel<P, STAGES><<<(unsigned)(cdiv64(tiles, 8) * 8), kSpanThreads, kFfnLds<P, STAGES>, st>>>(a);
+  if (a.slices > 1) ffn_sum_slices_kernel<<<(unsigned)cdiv64(a.rows * a.D, 1024), 256, 0, st>>>(a);
   return launch_status();
 }
-// 128 rows a tile, or 64 where that leaves CUs without one
+// Tiles of 32 rows as long as no CU has more than two of them, else of 64; a contraction is cut, where there is somewhere to leave its
+// sums, until every CU has two, into slices of at least 8 stages and not past 10 MB of sums.  (One CU pulls some 45 GB/s, so a
+// launch of few tiles takes as long as they are few.)  Us, contraction whole | cut in 2 | 4 | 8: 1 token, h W2 of 2048 x 8192 47 | 26 | 16 | 12;
+// 24 tokens, 4096 x 11264 64 | 34 | 22 | 21; 128, 4096 x 4096 25 | 18 | 17 | 21; 300, 2048 x 5632 40 | 26 | 23 | 24; 1000, 1024 x 2816 21 | 17 | 19 | 25;
+// 1000, 2176 x 1152 16 | 23 | 27 | 36.  32 rows | 64: 64 tokens, x W1 of 2048 x 5632 13.9 | 16.1; 128, 4096 x 4096 24.9 | 29.3, gz W1^T 41.7 | 52.0; 24, x W1
+// of 4096 x 11264 32.5 | 30.7.  128 rows a tile, or a deeper ring and one workgroup a CU, were faster nowhere but for 8 % of one launch
+// (1000 tokens, x W1 of 1024 x 2816).
+struct FfnPlan {
+  int fm, slices;
+};
+FfnPlan plan_of(int64_t rows, int64_t col_tiles, int64_t contraction, int64_t cols) {
+  const int64_t room = 2 * persistent_grid();
+  FfnPlan plan{cdiv64(rows, 32) * col_tiles <= room ? 1 : 2, 1};
+  const int64_t tiles = cdiv64(rows, 32 * plan.fm) * col_tiles;
+  if (cols > 0) plan.slices = (int)std::max<int64_t>(1, std::min({room / tiles, cdiv64(contraction, kSpan) / 8, (10 << 20) / (rows * cols * 4), (int64_t)16}));
+  return plan;
+}
 template <template <int> class P>
-int launch_by_rows(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
-  if (cdiv64(a.rows, 128) * col_tiles < persistent_grid()) return launch_tiles<P<2>>(a, col_tiles, st);
-  return launch_tiles<P<4>>(a, col_tiles, st);
+int launch_by_plan(FfnArgs a, const FfnPlan& plan, int64_t col_tiles, hipStream_t st) {
+  a.slices = plan.slices;
+  return plan.fm == 1 ? launch_tiles<P<1>, 4>(a, col_tiles, st) : launch_tiles<P<2>, 3>(a, col_tiles, st);
 }
 template <int FM> using Lin1Fwd = FfnLin1<FM, false>;
 template <int FM> using Lin1Bwd = FfnLin1<FM, true>;
@@ -548,7 +584,14 @@ int launch_dense_span(const FfnArgs& a, int64_t cols, hipStream_t st) {
 // cols, contraction: of the product (of x W1 both halves' columns)
 template <class Span, template <int> class P>
 int launch(const FfnArgs& a, int64_t cols, int64_t contraction, int64_t col_tiles, hipStream_t st) {
-  return takes_span(a.rows, cols, contraction) ? launch_dense_span<Span>(a, cols, st) : launch_by_rows<P>(a, col_tiles, st);
+  if (takes_span(a.rows, cols, contraction)) return launch_dense_span<Span>(a, cols, st);
+  return launch_by_plan<P>(a, plan_of(a.rows, col_tiles, contraction, a.part ? cols : 0), col_tiles, st);
+}
+// fp32 partial sums of a product with D columns that is cut along its contraction
+int64_t slices_bytes(int64_t rows, int64_t D, int64_t contraction) {
+  if (takes_span(rows, D, contraction)) return 0;
+  const FfnPlan plan = plan_of(rows, cdiv64(D, kFfnCols), contraction, D);
+  return plan.slices > 1 ? plan.slices * rows * D * 4 : 0;
 }
 
 int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
@@ -594,13 +637,18 @@ extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H
   return launch<Lin1DenseSpan<false>, Lin1Fwd>(a, 2 * H, D, cdiv64(H, 64), (hipStream_t)stream);
 }
 
+extern "C" int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction) {
+  return rows <= 0 || D <= 0 || contraction <= 0 ? -1 : slices_bytes(rows, D, contraction);
+}
+
 extern "C" int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H,
-                                  void* stream) {
-  if (!h_blocked || !W2_HD || !y) return MOMOE_ERR_BAD_ARG;
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!h_blocked || !W2_HD || !y || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
   const int st = check_ffn(rows, ldm, D, H);
   if (st != MOMOE_OK) return st;
-  if (any_unaligned({h_blocked, W2_HD, y})) return MOMOE_ERR_BAD_ARG;
+  if (any_unaligned({h_blocked, W2_HD, y, workspace}) || workspace_bytes < slices_bytes(rows, D, H)) return MOMOE_ERR_BAD_ARG;
   FfnArgs a{nullptr, 0, (const bf16*)W2_HD, rows, ldm, (int)D, (int)H};
+  a.part = (float*)workspace;
   a.h = (bf16*)h_blocked;
   a.out = (bf16*)y;
   return launch<Lin2DenseSpan, FfnLin2>(a, D, H, cdiv64(D, kFfnCols), (hipStream_t)stream);
@@ -648,13 +696,14 @@ extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void*
 }
 
 extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H,
-                                 void* stream) {
-  if (!gz_blocked || !W1_D2H || !Gx) return MOMOE_ERR_BAD_ARG;
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!gz_blocked || !W1_D2H || !Gx || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
   const int st = check_ffn(rows, rows, D, H);
   if (st != MOMOE_OK) return st;
-  if (any_unaligned({gz_blocked, W1_D2H, Gx})) return MOMOE_ERR_BAD_ARG;
+  if (any_unaligned({gz_blocked, W1_D2H, Gx, workspace}) || workspace_bytes < slices_bytes(rows, D, 2 * H)) return MOMOE_ERR_BAD_ARG;
   FfnArgs a{nullptr, 0, (const bf16*)W1_D2H, rows, rows, (int)D, (int)H};
   a.gz = (bf16*)const_cast<void*>(gz_blocked);
   a.out = (bf16*)Gx;
+  a.part = (float*)workspace;
   return launch<DxDenseSpan, FfnDx>(a, D, 2 * H, cdiv64(D, kFfnCols), (hipStream_t)stream);
 }

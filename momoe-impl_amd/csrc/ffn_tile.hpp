@@ -2,14 +2,14 @@
 //
 // For launches of few tiles, short contractions, few rows; the large ones run in the loop of gemm_span.hpp, whose operands and fragment
 // layout these are (the first input of the MFMA is the weight side: a lane holds, for one tile row (lane % 16), four consecutive
-// columns).  4 waves, 2 x 2; three stages in LDS, two of them on the way; with 72 or 96 KiB a workgroup two of them, or one and the
-// next one's start, share a CU.
+// columns).  4 waves, 2 x 2.  STAGES stages in LDS; the fragments of one half of a stage are read while
+// the other is multiplied (read and then multiplied, one after the other, a stage took 0.36 to 0.75 us whatever was on the way).  A contraction may be cut into `slices`, each a tile of its own that leaves fp32 sums for another kernel.
 #pragma once
 #include "gemm_span.hpp"
 
 namespace momoe {
 
-constexpr int kFfnCols = 128, kFfnStages = 3;
+constexpr int kFfnCols = 128;
 
 // Rows of a matrix at any pitch, k-contiguous, rows past the last one repeat it.  `K`: of 32 k-values the stage's first half is all
 // there is, and stands in the second, too.
@@ -38,6 +38,31 @@ struct FfnBlockedRows : SpanBlockedRows<ROWS> {
   __device__ __forceinline__ void deposit(const bf16* src, uint32_t slot) const {
     constexpr int h = j / Base::PER_HALF, q = j % Base::PER_HALF;
     dma16_at<h * (ROWS * kHalf * 2) + q * kSpanWaves * 1024>(h ? src + far : src, Base::off[q], slot);
+  }
+};
+
+// 32 rows: one deposit of the four waves, two of them a half each
+template <>
+struct FfnBlockedRows<32> {
+  static constexpr int DEP = 1, ELEMS = 32 * kSpan;
+  using Full = SpanBlockedRows<64>;
+  const bf16* base;
+  int64_t kstride;
+  uint32_t off;
+  __device__ __forceinline__ void init(const bf16* mat, int64_t ldm, int64_t row0, int rows, int K) {
+    const int l = fresh_lane(), half = wave_id() >> 1, row = (wave_id() & 1) * 16 + (l >> 2);
+    kstride = ldm * kHalf;
+    base = mat + row0 * kHalf + (half && K != 32 ? kstride : 0);
+    off = (uint32_t)min(row, rows - 1) * (kHalf * 2) + (((l & 3) ^ Full::swz(row)) * 16);
+  }
+  __device__ __forceinline__ const bf16* source(int k) const { return base + (int64_t)(k / kHalf) * kstride; }
+  template <int j>
+  __device__ __forceinline__ void deposit(const bf16* src, uint32_t slot) const {
+    dma16_at<0>(src, off, slot);
+  }
+  using Lane = Full::Lane;
+  static __device__ __forceinline__ bf16x8 frag(const bf16* slot, const Lane& ln, int i, int h) {
+    return *(const bf16x8*)((const char*)slot + ln.o + h * (32 * kHalf * 2) + i * (32 * kHalf));
   }
 };
 
@@ -91,20 +116,33 @@ struct FfnWeightRows : SpanPitchedRows<kFfnCols> {
   }
 };
 
-// A tile program P: P::Rows, P::Weights, FM; K, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column of a wave's
-// fragments in the tile; epilogue(row0, rows, tn, wm, wn, acc).
-template <class P>
+// until of the stages on their way, of `loads` transfers each, at most min(MOST, after) are left
+template <int LOADS, int MOST>
+__device__ __forceinline__ void wait_for_stage(int after) {
+  if constexpr (MOST == 0) {
+    wait_vmcnt<0>();
+  } else {
+    if (after >= MOST) wait_vmcnt<LOADS * MOST>();
+    else wait_for_stage<LOADS, MOST - 1>(after);
+  }
+}
+
+// A tile program P: P::Rows, P::Weights, FM; K, slices, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column of a
+// wave's fragments in the tile; epilogue(row0, rows, tn, slice, wm, wn, acc).
+template <class P, int STAGES>
 __device__ __forceinline__ void run_ffn_tile(const P& prog) {
   using Rows = typename P::Rows;
   using Weights = typename P::Weights;
   constexpr int FM = P::FM, FN = 4, BM = 32 * FM;
   constexpr int LOADS = Rows::DEP + Weights::DEP;
   // An XCD has a contiguous eighth of the tiles, row tiles fastest: those that share weights meet in one L2
-  const int total = prog.row_tiles * prog.col_tiles, chunk = (total + 7) >> 3;
-  const int t = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
+  const int total = prog.row_tiles * prog.col_tiles * prog.slices, chunk = (total + 7) >> 3;
+  int t = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= chunk || t >= total) return;
-  const int tn = t / prog.row_tiles;
-  const int64_t row0 = (int64_t)(t - tn * prog.row_tiles) * BM;
+  const int row_tile = t % prog.row_tiles;
+  t /= prog.row_tiles;
+  const int slice = t % prog.slices, tn = t / prog.slices;
+  const int64_t row0 = (int64_t)row_tile * BM;
   const int rows = (int)min((int64_t)BM, prog.rows - row0);
   Rows A;
   Weights W;
@@ -113,51 +151,70 @@ __device__ __forceinline__ void run_ffn_tile(const P& prog) {
   constexpr int STAGE = Rows::ELEMS + Weights::ELEMS;  // elements
   const uint32_t addr = lds_address(lds) + wave_id() * 1024;
   const int wn = wave_id() & 1, wm = wave_id() >> 1;
-  const SpanStages st(prog.K);
-  const int count = st.count;
-  int k = 0, put = 0, got = 0;
+  // this slice's stages; the last of all may be half a one
+  const SpanStages all(prog.K);
+  const int first = (int)((int64_t)all.count * slice / prog.slices), count = (int)((int64_t)all.count * (slice + 1) / prog.slices) - first;
+  const bool tail = all.tail && slice == prog.slices - 1;
+  int k = first * kSpan, put = 0, got = 0;
+  if (first == all.count - 1) k = max(0, min(k, all.kmax));
   auto request = [&] {
     const bf16 *asrc = A.source(k), *wsrc = W.source(k);
     const uint32_t to = addr + (uint32_t)put * (STAGE * 2);
     unrolled<0, Rows::DEP>([&](auto D) { A.template deposit<decltype(D)::value>(asrc, to); });
     unrolled<0, Weights::DEP>([&](auto D) { W.template deposit<decltype(D)::value>(wsrc, to + Rows::ELEMS * 2); });
-    k = max(0, st.after(k));
-    put = put + 1 == kFfnStages ? 0 : put + 1;
+    k = max(0, all.after(k));
+    put = put + 1 == STAGES ? 0 : put + 1;
   };
-  request();
-  if (count > 1) request();
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (s < count) request();
   f32x4 acc[FN][FM] = {};
   const typename Rows::Lane alane(wm * 16 * FM);
   const typename Weights::Lane wlane(prog.n_org(wn));
-  for (int s = 0; s < count; ++s) {
-    if (s + 1 < count) wait_vmcnt<LOADS>();
-    else wait_vmcnt<0>();
-    wait_lgkm0();
-    __builtin_amdgcn_s_barrier();
-    order_fence();
-    if (s + 2 < count) request();
+  bf16x8 wf[2][FN], af[2][FM];
+  auto read = [&](auto H) {
+    constexpr int h = decltype(H)::value;
     const bf16 *sa = lds + got * STAGE, *sw = sa + Rows::ELEMS;
-    auto half = [&](auto H) {
-      bf16x8 wf[FN], af[FM];
 #pragma unroll
-      for (int j = 0; j < FN; ++j) wf[j] = Weights::frag(sw, wlane, j, decltype(H)::value);
+    for (int j = 0; j < FN; ++j) wf[h][j] = Weights::frag(sw, wlane, j, h);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) af[i] = Rows::frag(sa, alane, i, decltype(H)::value);
+    for (int i = 0; i < FM; ++i) af[h][i] = Rows::frag(sa, alane, i, h);
+  };
+  auto multiply = [&](auto H) {
+    constexpr int h = decltype(H)::value;
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int i = 0; i < FM; ++i) acc[j][i] = mfma16(wf[j], af[i], acc[j][i]);
-    };
+      for (int i = 0; i < FM; ++i) acc[j][i] = mfma16(wf[h][j], af[h][i], acc[j][i]);
+  };
+  wait_for_stage<LOADS, STAGES - 1>(count - 1);
+  __builtin_amdgcn_s_barrier();
+  order_fence();
+  read(IntC<0>{});
+  order_fence();
+  for (int s = 0; s < count; ++s) {
     // a last stage that is not whole starts at K - 64: its first half has been multiplied (of 32 k-values the first is all)
-    const bool part = s + 1 == count && st.tail;
-    if (!part || prog.K == 32) half(IntC<0>{});
-    if (!part) half(IntC<1>{});
-    else if (prog.K != 32) half(IntC<1>{});
-    got = got + 1 == kFfnStages ? 0 : got + 1;
+    const bool part = s + 1 == count && tail;
+    read(IntC<1>{});
+    order_fence();
+    if (!part || prog.K == 32) multiply(IntC<0>{});
+    order_fence();
+    if (s + 1 < count) {  // the next stage has landed, and every wave is done reading this one, whose place the one after takes
+      wait_for_stage<LOADS, STAGES - 2>(count - 2 - s);
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      order_fence();
+      got = got + 1 == STAGES ? 0 : got + 1;
+      read(IntC<0>{});
+      if (s + STAGES < count) request();
+    }
+    order_fence();
+    if (!part || prog.K != 32) multiply(IntC<1>{});
+    order_fence();
   }
-  prog.epilogue(row0, rows, tn, wm, wn, acc);
+  prog.epilogue(row0, rows, tn, slice, wm, wn, acc);
 }
-template <class P>
-constexpr size_t kFfnLds = (size_t)kFfnStages * (P::Rows::ELEMS + P::Weights::ELEMS) * sizeof(bf16);
+template <class P, int STAGES>
+constexpr size_t kFfnLds = (size_t)STAGES * (P::Rows::ELEMS + P::Weights::ELEMS) * sizeof(bf16);
 
 }  // namespace momoe

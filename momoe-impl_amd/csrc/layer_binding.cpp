@@ -579,7 +579,10 @@ FeedForward feed_forward_forward(const Tensor& x, const Tensor& W1, const Tensor
     const Tensor h = empty_bf16({M * H}, dev);
     MOMOE_CALL(momoe_ffn_lin1_fwd, st, f.x.data_ptr(), pitch_of_rows(f.x), f.W1.data_ptr(), h.data_ptr(),
                msave > 0 ? f.ab.data_ptr<float>() : nullptr, (msave + 31) / 32 * 32, M, M, D, H);
-    MOMOE_CALL(momoe_ffn_lin2_fwd, st, h.data_ptr(), f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H);
+    const int64_t bytes = momoe_ffn_workspace_bytes(M, D, H);
+    Tensor ws;
+    if (bytes > 0) ws = empty_f32({bytes / 4}, dev);
+    MOMOE_CALL(momoe_ffn_lin2_fwd, st, h.data_ptr(), f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
   }
   if (x.device() != dev) f.y = f.y.to(x.device());
   return f;
@@ -643,7 +646,10 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
     if (need_w1) weight_gradient(x.data_ptr(), ldx, MOMOE_LAYOUT_ROWS, gz.data_ptr(), M, MOMOE_LAYOUT_KBLOCKED, out[1]);
     if (need_x) {
       const Tensor Gx = empty_bf16({M, D}, dev);
-      MOMOE_CALL(momoe_ffn_dgrad_x, st, gz.data_ptr(), W1.data_ptr(), Gx.data_ptr(), M, D, H);
+      const int64_t bytes = momoe_ffn_workspace_bytes(M, D, 2 * H);
+      Tensor ws;
+      if (bytes > 0) ws = empty_f32({bytes / 4}, dev);
+      MOMOE_CALL(momoe_ffn_dgrad_x, st, gz.data_ptr(), W1.data_ptr(), Gx.data_ptr(), M, D, H, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
       out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
     }
     return out;

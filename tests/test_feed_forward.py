@@ -26,15 +26,20 @@ def test_refusals_of_the_entry_points():
     c = _refuses(lib.momoe_ffn_lin1_fwd, dict(x=P, ldx=64, W=P, h=P, ab=None, ab_rows=0, **sizes), ("x", "W", "h"), ("x", "W", "h"))
     assert c(ldx=56) == c(ldm=39) == c(ab_rows=32) == c(ab=P, ab_rows=-32) == c(ab=P, ab_rows=96) == c(ab=P + 4, ab_rows=32) == 1
     assert c(ldx=68) == c(ab=P, ab_rows=40) == c(ldx=1 << 22) == 2
-    c = _refuses(lib.momoe_ffn_lin2_fwd, dict(h=P, W=P, y=P, **sizes), ("h", "W", "y"), ("h", "W", "y"))
-    assert c(ldm=39) == 1 and c(ldm=1 << 31) == 2
+    room = dict(ws=P, bytes=1 << 40)
+    c = _refuses(lib.momoe_ffn_lin2_fwd, dict(h=P, W=P, y=P, **sizes, **room), ("h", "W", "y", "ws"), ("h", "W", "y", "ws"))
+    assert c(ldm=39) == c(bytes=-1) == 1 and c(ldm=1 << 31) == 2
+    need = lib.momoe_ffn_workspace_bytes(1, 2048, 8192)
+    assert need > 0 and c(rows=1, D=2048, H=8192, bytes=need - 4) == c(rows=1, D=2048, H=8192, ws=None, bytes=0) == 1
+    assert lib.momoe_ffn_workspace_bytes(0, 64, 64) == lib.momoe_ffn_workspace_bytes(1, 0, 64) == lib.momoe_ffn_workspace_bytes(1, 64, 0) == -1
     c = _refuses(lib.momoe_ffn_dgrad_h, dict(Gy=P, ldgy=64, W=P, u=P, rows=40, D=64, H=32), ("Gy", "W", "u"), ("Gy", "W", "u"))
     assert c(ldgy=56) == 1 and c(ldgy=68) == 2
     c = _refuses(lib.momoe_ffn_swiglu_bwd, dict(x=P, ldx=64, W=P, u=P, gz=P, hT=None, counts=None, **sizes), ("x", "W", "u", "gz"), ("x", "W", "u", "gz", "hT"))
     assert c(ldx=56) == c(ldm=39) == 1 and c(ldx=68) == 2
     c = _refuses(lib.momoe_ffn_dgrad_h_saved, dict(Gy=P, ldgy=64, W=P, ab=P, gz=P, hT=None, counts=None, **sizes), ("Gy", "W", "ab", "gz"), ("Gy", "W", "ab", "gz", "hT"))
     assert c(ldgy=56) == c(ldm=39) == 1 and c(ldgy=68) == 2
-    _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, rows=40, D=64, H=32), ("gz", "W", "Gx"), ("gz", "W", "Gx"))
+    c = _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, rows=40, D=64, H=32, **room), ("gz", "W", "Gx", "ws"), ("gz", "W", "Gx", "ws"))
+    assert c(bytes=-1) == c(rows=1, D=2048, H=8192, ws=None, bytes=0) == 1
 
 
 def test_module_refusals():

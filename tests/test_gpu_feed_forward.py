@@ -195,7 +195,8 @@ def test_rows_behind_the_last_stay_as_they_are():
         guard = torch.full((4096,), 7.0, device=DEV, dtype=torch.bfloat16)
         lib, st = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream
         assert lib.momoe_ffn_lin1_fwd(x.data_ptr(), D, W1.data_ptr(), h.data_ptr(), None, 0, M, M, D, H, st) == 0
-        assert lib.momoe_ffn_lin2_fwd(h.data_ptr(), W2.data_ptr(), y.data_ptr(), M, M, D, H, st) == 0
+        ws = torch.empty(max(lib.momoe_ffn_workspace_bytes(M, D, H), 16), dtype=torch.uint8, device=DEV)
+        assert lib.momoe_ffn_lin2_fwd(h.data_ptr(), W2.data_ptr(), y.data_ptr(), M, M, D, H, ws.data_ptr(), ws.numel(), st) == 0
         torch.cuda.synchronize()
         assert torch.equal(y[:M], _block(W1, W2)(x)) and (y[M:] == 7).all() and (guard == 7).all()
 
