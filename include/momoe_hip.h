@@ -566,25 +566,31 @@ int64_t momoe_int4_scale_words(int64_t N, int64_t R, int64_t C, int group);
 int momoe_int4_pack_weights(const void* codes_NRC, const void* scale, int scale_type, const void* zero, int64_t N, int64_t R, int64_t C,
                             int halves, int group, void* packed, void* words, void* stream);
 
-/* The experts.  tile_table: of momoe_index_build for tile_rows = momoe_int4_tile_rows(Msum, N) rows.
- * momoe_int4_lin1_swiglu_fwd: h bf16 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i]; x bf16 with row pitch ldx, a multiple of 8.
- * momoe_int4_lin2_scale_fwd: ys fp32 [Msum][D], ys[r] = (h[r] . Wl2[i]) * s[i, idx[r]].
- * momoe_int4_combine: out_MD bf16 [M][D], out[m] = the sum of its experts' rows, in fp32, rounded once.
+/* The experts.  tile_table: of momoe_index_build for `tile_rows` rows, 32 or 64, whichever momoe_int4_tile_rows says suits the sizes (64
+ * only where the rows of x take less than 4 GiB, M * ldx * 2 < 2^32).  A product of few tiles is cut along its contraction of K into
+ * momoe_int4_slices(Msum, N, cols, K, tile_rows) slices, 1 if it is not.
+ * momoe_int4_lin1_swiglu_fwd (cols 2H, K = D): h bf16 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i]; x bf16 with row pitch ldx, a
+ * multiple of 8; workspace: of more than one slice, slices * Msum * 2H * 4 bytes (else NULL).
+ * momoe_int4_lin2_scale_fwd (cols D, K = H): ys fp32 [slices][Msum][D], the sum over the slices (h[r] . Wl2[i]) * s[i, idx[r]].
+ * momoe_int4_combine: out_MD bf16 [M][D], out[m] = the sum of its experts' rows and their slices, in fp32, rounded once.
  * Pointers to rows, weights and results on 16-byte boundaries. */
-int momoe_int4_tile_rows(int64_t Msum, int64_t N);
+int momoe_int4_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N);
+int momoe_int4_slices(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows);
 int momoe_int4_lin1_swiglu_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, int group,
-                               const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH, int64_t M, int64_t D,
-                               int64_t H, int64_t N, int64_t Msum, void* stream);
+                               const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH, void* workspace,
+                               int64_t workspace_bytes, int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);
 int momoe_int4_lin2_scale_fwd(const void* h_MsumH, const void* Wl2_packed, const void* Wl2_words, int group, const float* s_NM,
                               int64_t s_stride_n, int64_t s_stride_m, const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows,
                               float* ys_MsumD, int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream);
-int momoe_int4_combine(const float* ys_MsumD, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K, int64_t Msum,
+int momoe_int4_combine(const float* ys_MsumD, int slices, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K, int64_t Msum,
                        void* stream);
 
 /* A dense block: y = (a * b * sigmoid(b)) . Wl2, a | b = x . Wl1, weights as of one expert.  x bf16 with row pitch ldx, a multiple of 8;
- * h_MH bf16 [M][H] scratch; y bf16 [M][D].  All on 16-byte boundaries. */
+ * h_MH bf16 [M][H] and workspace (momoe_int4_ffn_workspace_bytes; 0: NULL) scratch; y bf16 [M][D].  All on 16-byte boundaries. */
+int64_t momoe_int4_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H);
 int momoe_int4_ffn_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, const void* Wl2_packed,
-                       const void* Wl2_words, int group, void* h_MH, void* y_MD, int64_t M, int64_t D, int64_t H, void* stream);
+                       const void* Wl2_words, int group, void* h_MH, void* y_MD, void* workspace, int64_t workspace_bytes, int64_t M,
+                       int64_t D, int64_t H, void* stream);
 
 #ifdef __cplusplus
 }

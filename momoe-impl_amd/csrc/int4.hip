@@ -14,8 +14,9 @@
 //           column lane % 16; k-value 2 i in bits 4 i .. +3, 2 i + 1 in bits 16 + 4 i .. +3, so that a shift and a mask give a pair
 //   scales  [expert][16 columns][128 k-values][16][128 / group] words: the scale's fp32 bits (of a 16-bit type: the low 13 are zero) and,
 //           in the low four, the zero
-// zeros past the last k-value.  The columns of the first product are those of its two halves in turn, 16 a and 16 b.
+// Past the last k-value the codes are the zero of their group, or the scales are zero.  The columns of the first product are those of its two halves in turn, 16 a and 16 b.
 #include <algorithm>
+#include <cstdlib>
 
 #include "gemm_span.hpp"
 
@@ -39,6 +40,10 @@ struct Int4Args {
   int64_t sn, sm;
   void* out;                   // h bf16 [.][ldo]; ys fp32 [.][ldo] of experts, y bf16 of a dense block
   int64_t ldo;
+  // tall tiles whose contraction is cut: sums by slices, fp32 [slices][all rows][2 H or D], and what there is of rows
+  int slices;
+  float* part;
+  int64_t all_rows;
 };
 
 // eight codes of a word as 128 + code
@@ -54,34 +59,56 @@ __device__ __forceinline__ float zero_of_word(uint32_t w) { return __uint_as_flo
 // Tiles of experts, by the index build's table, or of a dense block, which has none: all rows are those of one expert
 struct Int4Sched {
   TileSchedT<1> experts;
-  int nb, total, pos, tile_rows, rows;
+  int row_tiles, total, pos, end, tile_rows, rows;
   // (of a dense block `experts` reads the first two words of the codes, and nothing is made of them)
-  __device__ __forceinline__ Int4Sched(const Int4Args& p, int nb_, int tile_rows_)
-      : experts(p.table ? p.table : (const int32_t*)p.w, nb_, tile_rows_), nb(nb_), pos(blockIdx.x), tile_rows(tile_rows_), rows(p.M) {
-    total = (rows + tile_rows - 1) / tile_rows * nb;
+  __device__ __forceinline__ Int4Sched(const Int4Args& p, int nb, int tile_rows_)
+      : experts(p.table ? p.table : (const int32_t*)p.w, nb, tile_rows_), tile_rows(tile_rows_), rows(p.M) {
+    // an XCD has a contiguous eighth, row tiles fastest: those that share weights meet in one L2
+    row_tiles = (rows + tile_rows - 1) / tile_rows;
+    total = row_tiles * nb;
+    const int chunk = (total + 7) >> 3, begin = (int)(blockIdx.x & 7) * chunk;
+    end = min(begin + chunk, total);
+    pos = begin + (int)(blockIdx.x >> 3);
   }
   __device__ __forceinline__ TileCoord next() {
     if (rows == 0) return experts.next();
     TileCoord t = {};
-    t.valid = pos < total;
+    t.valid = pos < end;
     if (!t.valid) return t;
-    t.row0 = pos / nb * tile_rows;
-    t.tn = pos % nb;
+    t.tn = pos / row_tiles;
+    t.row0 = (pos - t.tn * row_tiles) * tile_rows;
     t.rows = min(tile_rows, rows - t.row0);
-    pos += gridDim.x;
+    pos += gridDim.x >> 3;
     return t;
   }
 };
 
-// Tiles of up to 16 FR rows.  A wavefront owns a pair of 16-column groups; KS of them share its contraction, a block of 128 k-values in
+// column `col` of both groups of a pair, of one row: h of a and b, or two columns of the result, of experts times the gate weight
+template <bool FIRST>
+__device__ __forceinline__ void store_pair(const Int4Args& p, int64_t row, int pair, int col, float v0, float v1, float s) {
+  if constexpr (FIRST) {
+    ((bf16*)p.out)[row * p.ldo + 16 * pair + col] = f2bf(v0 * v1 * sigmoidf_fast(v1));
+  } else {
+    const int64_t to = row * p.ldo + 32 * pair + col;
+    if (p.idx) {
+      ((float*)p.out)[to] = v0 * s;
+      ((float*)p.out)[to + 16] = v1 * s;
+    } else {
+      ((bf16*)p.out)[to] = f2bf(v0);
+      ((bf16*)p.out)[to + 16] = f2bf(v1);
+    }
+  }
+}
+
+// Tiles of up to 32 rows.  A wavefront owns a pair of 16-column groups; KS of them share its contraction, a block of 128 k-values in
 // KS each, and their sums meet in LDS.  Codes and scales go straight into registers, AHEAD blocks ahead; the rows come to LDS,
 // kFewBytes of them at a time, for all wavefronts.
-constexpr int kFewThreads = 256, kFewWaves = kFewThreads / 64, kFewBytes = 64 << 10;
+constexpr int kFewThreads = 256, kFewWaves = kFewThreads / 64, kFewBytes = 32 << 10;
 
-template <bool FIRST, int FR, int KS, int SG>
+template <bool FIRST, int KS, int SG>
 __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args p) {
-  constexpr int ROWS = 16 * FR, PW = kFewWaves / KS, CHUNK = kFewBytes / (ROWS * kInt4Block * 2);
-  constexpr int AHEAD = FR * SG >= 16 ? 2 : 4;  // (four of the smallest groups' scales and 64 rows' sums were spilled)
+  constexpr int FR = 2, ROWS = 16 * FR, PW = kFewWaves / KS;
+  constexpr int AHEAD = SG == 4 ? 2 : 4;  // (four of the smallest groups' scales were spilled)
   __shared__ __attribute__((aligned(16))) uint8_t lds[kFewBytes];  // rows [block][row][256], then the sums of KS wavefronts
   static_assert(kFewWaves * 64 * 2 * FR * 16 <= kFewBytes, "sums of all wavefronts");
   typedef uint32_t Words __attribute__((ext_vector_type(SG)));
@@ -96,8 +123,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
     const uint8_t* const w0 = p.w + group * kInt4Frag + l * 16;
     const uint32_t* const s0 = p.scale + (group * 16 + (l & 15)) * SG;
     f32x4 acc[2][FR] = {};
-    for (int k0 = 0; k0 < p.KB; k0 += CHUNK) {
-      const int blocks = min(CHUNK, p.KB - k0), steps = (blocks - kw + KS - 1) / KS;  // (none for a wavefront past the last)
+    const int chunk = kFewBytes / (tc.rows * kInt4Block * 2);  // blocks of the tile's rows that LDS holds, four at least
+    for (int k0 = 0; k0 < p.KB; k0 += chunk) {
+      const int blocks = min(chunk, p.KB - k0), steps = (blocks - kw + KS - 1) / KS;  // (none for a wavefront past the last)
       u32x4 wq[AHEAD][2];
       Words sq[AHEAD][2];
       const auto load = [&](int q, int step) {
@@ -113,7 +141,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
       });
       __syncthreads();  // (the last rows, or sums, are done with)
       // 16 pieces of 8 values a row and block, piece c of row r at c ^ (r % 16): the 16 rows of a fragment read meet different
-      // banks.  (What is left in LDS for rows that the tile does not have goes into rows that nobody stores.)
+      // banks.  Rows that the tile does not have are read as its last one, and nobody stores what becomes of them.
       const int all = blocks * tc.rows * 16;
       for (int q0 = tid; q0 < all; q0 += 2 * kFewThreads) {
         bf16x8 v[2];
@@ -124,7 +152,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
           const int c = (k0 + kb) * kInt4Block + piece * 8, row = tc.row0 + r;
           v[a] = *(const bf16x8*)(p.rows + (int64_t)(FIRST && p.idx ? p.idx[row] : row) * p.ld + min(c, p.K - 8));
           if (c >= p.K) v[a] = bf16x8{};
-          to[a] = (kb * ROWS + r) * 256 + ((piece ^ (r & 15)) << 4);
+          to[a] = (kb * tc.rows + r) * 256 + ((piece ^ (r & 15)) << 4);
         }
 #pragma unroll
         for (int a = 0; a < 2; ++a) *(bf16x8*)(lds + to[a]) = v[a];
@@ -140,10 +168,11 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
         unrolled<0, FR>([&](auto IC) {
           constexpr int i = decltype(IC)::value;
           if (i >= nf) return;  // (the same for all lanes)
-          const uint8_t* const from = lds + (kb * ROWS + 16 * i + (l & 15)) * 256;
+          const int row = min(16 * i + (l & 15), tc.rows - 1);
+          const uint8_t* const from = lds + (kb * tc.rows + row) * 256;
           bf16x8 rf[4];
 #pragma unroll
-          for (int m = 0; m < 4; ++m) rf[m] = *(const bf16x8*)(from + (((4 * m + (l >> 4)) ^ (l & 15)) << 4));
+          for (int m = 0; m < 4; ++m) rf[m] = *(const bf16x8*)(from + (((4 * m + (l >> 4)) ^ (row & 15)) << 4));
 #pragma unroll
           for (int g = 0; g < SG; ++g) {
             f32x4 t[2] = {}, sum = {};
@@ -158,6 +187,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
               const float sc = scale_of_word(sq[q][j][g]), zc = zero_of_word(sq[q][j][g]);
 #pragma unroll
               for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(sc, fmaf(-zc, sum[r], t[j][r]), acc[j][i][r]);
+              asm volatile("" : "+v"(acc[j][i]));  // (the products of all fragments were formed first, and spilled)
             }
           }
         });
@@ -203,27 +233,210 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
         const int at = 16 * i + 4 * (l >> 4) + r;
         if (at >= tc.rows) continue;
         const int64_t row = tc.row0 + at;
-        if constexpr (FIRST) {
-          const float a = acc[0][i][r], b = acc[1][i][r];
-          ((bf16*)p.out)[row * p.ldo + 16 * pair + (l & 15)] = f2bf(a * b * sigmoidf_fast(b));
-        } else {
-          const int64_t to = row * p.ldo + 32 * pair + (l & 15);
-          if (p.idx) {
-            const float s = p.s[(int64_t)tc.expert * p.sn + (int64_t)p.idx[row] * p.sm];
-            ((float*)p.out)[to] = acc[0][i][r] * s;
-            ((float*)p.out)[to + 16] = acc[1][i][r] * s;
-          } else {
-            ((bf16*)p.out)[to] = f2bf(acc[0][i][r]);
-            ((bf16*)p.out)[to + 16] = f2bf(acc[1][i][r]);
-          }
-        }
+        float s = 1.0f;
+        if (!FIRST && p.idx) s = p.s[(int64_t)tc.expert * p.sn + (int64_t)p.idx[row] * p.sm];
+        store_pair<FIRST>(p, row, pair, l & 15, acc[0][i][r], acc[1][i][r], s);
       }
   }
 }
 
-// out[m] = the sum of the rows of its experts, fp32, rounded once.  The row numbers and then the rows with unconditional loads, as in
-// combine_kernel.
-__global__ __launch_bounds__(256) void int4_combine_kernel(const float* __restrict__ rows, const int32_t* __restrict__ inv,
+// Tiles of 64 rows x 256 columns, for more rows than that: a wavefront owns 64 columns of them, two pairs of groups.  The rows come to LDS by
+// direct transfers, 128 k-values a stage, the codes and scales straight into registers; both are requested a stage ahead, and two
+// workgroups share a CU, so that one's products stand beside the other's vector work: for each 64 matrix instructions (and 16 for the
+// sums of the rows) of a wavefront's stage there are 112 instructions that make bf16 of codes and 128 that bring the sums of a group
+// to the others.  Fragments of rows that the tile does not have are left out.  A launch of few tiles has its contraction cut into slices,
+// whose sums int4_h_of_slices_kernel or the last kernel adds up.
+struct Int4Rows {
+  static constexpr int BM = 64, DEP = BM * 256 / (kSpanWaves * 1024), STAGE = BM * 256;  // bytes
+  const char* base;
+  uint32_t off[DEP];
+  __device__ __forceinline__ void init(const Int4Args& p, const TileCoord& tc, bool gather) {
+    const int l = fresh_lane();
+    base = (const char*)p.rows;
+    if (!gather) base += (int64_t)tc.row0 * p.ld * 2;
+#pragma unroll
+    for (int j = 0; j < DEP; ++j) {
+      const int r = min((j * kSpanWaves + wave_id()) * 4 + (l >> 4), tc.rows - 1);
+      off[j] = (uint32_t)(gather ? p.idx[tc.row0 + r] : r) * (uint32_t)(2 * p.ld);
+    }
+  }
+  // 16 rows a deposit; piece c of row r at c ^ (r % 16).  Past the row's end its last piece is repeated: codes that are the zero of their
+  // group, or a scale of zero, make nothing of it.
+  __device__ __forceinline__ void request(int kb, int K, int nf, uint32_t slot) const {
+    const int l = fresh_lane(), piece = (l & 15) ^ ((wave_id() * 4 + (l >> 4)) & 15);
+    const uint32_t at = (uint32_t)min(kb * kInt4Block + piece * 8, K - 8) * 2;
+    unrolled<0, DEP>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      if (j < nf) dma16_at<j * kSpanWaves * 1024>(base, off[j] + at, slot);
+    });
+  }
+};
+
+template <bool FIRST, int SG>
+__global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) {
+  using Rows = Int4Rows;
+  constexpr int PAIRS = 2 * kSpanWaves;
+  typedef uint32_t Words __attribute__((ext_vector_type(SG)));
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Rows::STAGE];
+  const int l = lane_id(), wave = wave_id();
+  const uint32_t addr = lds_address((bf16*)lds) + wave * 1024;
+  const int nb = (p.pairs + PAIRS - 1) / PAIRS;
+  Int4Sched sched(p, nb * p.slices, Rows::BM);
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+  for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
+    const int tn = tc.tn / p.slices, slice = tc.tn - tn * p.slices;
+    const int kb0 = (int)((int64_t)p.KB * slice / p.slices), kb1 = (int)((int64_t)p.KB * (slice + 1) / p.slices);
+    const int nf = (tc.rows + 15) >> 4, pair0 = tn * PAIRS + 2 * wave;
+    const uint8_t* w[4];
+    const uint32_t* sc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t group = (((int64_t)tc.expert * p.pairs + min(pair0 + j / 2, p.pairs - 1)) * 2 + j % 2) * p.KB;
+      w[j] = p.w + group * kInt4Frag;
+      sc[j] = p.scale + group * (16 * SG);
+    }
+    Rows A;
+    A.init(p, tc, FIRST && p.idx);
+    u32x4 wq[4];
+    Words sq[4];
+    const auto load = [&](int kb) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        wq[j] = *(const u32x4*)(w[j] + (int64_t)kb * kInt4Frag + l * 16);
+        sq[j] = *(const Words*)(sc[j] + (int64_t)kb * (16 * SG) + (l & 15) * SG);
+      }
+    };
+    __syncthreads();  // (the last tile's rows have been read)
+    A.request(kb0, p.K, nf, addr);
+    load(kb0);
+    f32x4 acc[4][4] = {};
+    const auto stage = [&](auto Q, int kb) {
+      constexpr int q = decltype(Q)::value;
+      wait_vmcnt<0>();
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      order_fence();
+      if (kb + 1 < kb1) A.request(kb + 1, p.K, nf, addr + (q ^ 1) * Rows::STAGE);
+      order_fence();
+      u32x4 codes[4];
+      Words scales[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) codes[j] = wq[j], scales[j] = sq[j];
+      const uint8_t* const rows = lds + q * Rows::STAGE + (l & 15) * 256;
+      constexpr int STEPS = 4 / SG;
+      bf16x8 wf[4][STEPS], rf[2][STEPS];
+      float s[4], z[4];
+      // fragment i of group g, asked for while the one before is multiplied
+      const auto read = [&](auto NC) {
+        constexpr int n = decltype(NC)::value, g = n / 4, i = n % 4;
+#pragma unroll
+        for (int m = 0; m < STEPS; ++m)
+          rf[n & 1][m] = *(const bf16x8*)(rows + i * (16 * 256) + (((4 * (g * STEPS + m) + (l >> 4)) ^ (l & 15)) << 4));
+      };
+      read(IntC<0>{});
+      unrolled<0, 4 * SG>([&](auto NC) {
+        constexpr int n = decltype(NC)::value, g = n / 4, i = n % 4;
+        if constexpr (i == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[j] = scale_of_word(scales[j][g]), z[j] = zero_of_word(scales[j][g]);
+#pragma unroll
+            for (int m = 0; m < STEPS; ++m) wf[j][m] = bf16_of_codes(codes[j][g * STEPS + m]);
+          }
+          if constexpr (g == SG - 1) load(min(kb + 1, kb1 - 1));
+        }
+        if constexpr (n + 1 < 4 * SG) read(IntC<n + 1>{});
+        if (i >= nf) return;  // (the same for all lanes)
+        f32x4 t[4] = {}, sum = {};
+#pragma unroll
+        for (int m = 0; m < STEPS; ++m) {
+          sum = mfma16(rf[n & 1][m], ones, sum);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[j] = mfma16(rf[n & 1][m], wf[j][m], t[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s[j], fmaf(-z[j], sum[r], t[j][r]), acc[j][i][r]);
+          asm volatile("" : "+v"(acc[j][i]));  // (the products of all fragments were formed first, and spilled)
+        }
+      });
+      order_fence();
+    };
+    for (int kb = kb0; kb < kb1; kb += 2) {
+      stage(IntC<0>{}, kb);
+      if (kb + 1 < kb1) stage(IntC<1>{}, kb + 1);
+    }
+    const int col = l & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= nf) break;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 16 * i + 4 * (l >> 4) + r;
+        if (at >= tc.rows) continue;
+        const int64_t row = tc.row0 + at;
+        float s = 1.0f;
+        if (!FIRST && p.idx) s = p.s[(int64_t)tc.expert * p.sn + (int64_t)p.idx[row] * p.sm];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int pair = pair0 + c;
+          if (pair >= p.pairs) continue;
+          const float v0 = acc[2 * c][i][r], v1 = acc[2 * c + 1][i][r];
+          if (p.slices == 1) {
+            store_pair<FIRST>(p, row, pair, col, v0, v1, s);
+          } else if (FIRST) {
+            float* const to = p.part + (slice * p.all_rows + row) * (2 * p.ldo) + 16 * pair + col;
+            to[0] = v0;
+            to[p.ldo] = v1;
+          } else {
+            float* const to = p.part + (slice * p.all_rows + row) * p.ldo + 32 * pair + col;
+            to[0] = v0 * s;
+            to[16] = v1 * s;
+          }
+        }
+      }
+    }
+  }
+}
+
+// The sum of eight at a time of `slices` values that lie `stride` apart, in their order
+__device__ __forceinline__ f32x4 sum_of_slices(const float* p, int slices, int64_t stride) {
+  f32x4 sum = {};
+  for (int s = 0; s < slices; s += 8) {
+    f32x4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = *(const f32x4*)(p + min(s + j, slices - 1) * stride);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s + j < slices) sum += v[j];
+  }
+  return sum;
+}
+// h from the slices of a | b, fp32 [slices][rows][2H]
+__global__ __launch_bounds__(256) void int4_h_of_slices_kernel(const float* __restrict__ part, bf16* __restrict__ h, int64_t rows, int H,
+                                                               int slices) {
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, row = q / (H / 4);
+  const int col = (int)(q - row * (H / 4)) * 4;
+  if (row >= rows) return;
+  const float* const from = part + row * 2 * H + col;
+  const f32x4 a = sum_of_slices(from, slices, rows * 2 * H), b = sum_of_slices(from + H, slices, rows * 2 * H);
+  bf16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = f2bf(a[e] * b[e] * sigmoidf_fast(b[e]));
+  *(bf16x4*)(h + row * H + col) = v;
+}
+// y of a dense block from its slices, fp32 [slices][n]
+__global__ __launch_bounds__(256) void int4_sum_slices_kernel(const float* __restrict__ part, bf16* __restrict__ y, int64_t n, int slices) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  const f32x4 v = sum_of_slices(part + at, slices, n);
+  *(bf16x4*)(y + at) = pack_bf16x4(v, 1.0f);
+}
+
+// out[m] = the sum of the rows of its experts, slice by slice, fp32, rounded once.  The row numbers and then the rows with unconditional
+// loads, as in combine_kernel.
+__global__ __launch_bounds__(256) void int4_combine_kernel(const float* __restrict__ rows, int slices, const int32_t* __restrict__ inv,
                                                            bf16* __restrict__ out, int D, int K, int64_t msum) {
   const int64_t m = blockIdx.x;
   for (int c = threadIdx.x; c < D / 4; c += blockDim.x) {
@@ -232,17 +445,18 @@ __global__ __launch_bounds__(256) void int4_combine_kernel(const float* __restri
       int32_t r[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] = inv[m * K + min(k0 + j, K - 1)];
-      f32x4 v[8];
+      for (int s = 0; s < slices; ++s) {
+        const float* const from = rows + s * msum * D + c * 4;
+        f32x4 v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool ok = k0 + j < K && (uint32_t)r[j] < (uint64_t)msum;
-        v[j] = *(const f32x4*)(rows + (int64_t)(ok ? r[j] : 0) * D + c * 4);
-        r[j] = ok ? 1 : 0;
+        for (int j = 0; j < 8; ++j) {
+          const bool ok = k0 + j < K && (uint32_t)r[j] < (uint64_t)msum;
+          v[j] = *(const f32x4*)(from + (int64_t)(ok ? r[j] : 0) * D);
+          if (!ok) v[j] = f32x4{};
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += v[j];
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += r[j] ? v[j][e] : 0.0f;
     }
     *(bf16x4*)(out + m * D + c * 4) = pack_bf16x4(sum[0], sum[1], sum[2], sum[3]);
   }
@@ -269,11 +483,13 @@ __global__ __launch_bounds__(256) void int4_pack_codes_kernel(Int4PackArgs p) {
   const int kb = (int)(f % KB), g = (int)(f / KB % groups);
   const int64_t e = f / KB / groups;
   const int k = kb * kInt4Block + 32 * m + 8 * (l >> 4), col = column_of(p, g, l & 15);
+  const int KG = (p.R + p.group - 1) / p.group, kg = k / p.group;
   uint32_t word = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (k + 2 * i >= p.R) break;
-    const uint32_t b = p.w[(e * (p.R / 2) + k / 2 + i) * C + col];
+    uint32_t b = 0;
+    if (k + 2 * i < p.R) b = p.w[(e * (p.R / 2) + k / 2 + i) * C + col];
+    else if (kg < KG) b = (p.zero ? p.zero[(e * KG + kg) * C + col] & 15u : 8u) * 17u;  // the zero of its group
     word |= (b & 15u) << (4 * i) | (b >> 4) << (16 + 4 * i);
   }
   p.codes[q] = word;
@@ -304,31 +520,60 @@ int check_int4(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, int gro
 }
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
-template <bool FIRST, int FR, int SG>
+template <bool FIRST, int SG>
 int launch_few(const Int4Args& a, int64_t tiles, hipStream_t st) {
-  const int64_t wanted = 2 * persistent_grid();
+  const int64_t wanted = 3 * persistent_grid();
   const auto enough = [&](int ks) { return a.KB < 2 * ks || tiles * cdiv64(a.pairs, kFewWaves / ks) >= wanted; };
-  auto kernel = enough(1) ? int4_few_rows_kernel<FIRST, FR, 1, SG> : enough(2) ? int4_few_rows_kernel<FIRST, FR, 2, SG>
-                                                                              : int4_few_rows_kernel<FIRST, FR, 4, SG>;
+  auto kernel = enough(1) ? int4_few_rows_kernel<FIRST, 1, SG> : enough(2) ? int4_few_rows_kernel<FIRST, 2, SG> : int4_few_rows_kernel<FIRST, 4, SG>;
   kernel<<<(unsigned)wanted, kFewThreads, 0, st>>>(a);
+  return launch_status();
+}
+template <bool FIRST, int SG>
+int launch_rows(const Int4Args& a, int64_t tiles, int tile_rows, hipStream_t st) {
+  if (tile_rows == 32) return launch_few<FIRST, SG>(a, tiles, st);
+  int4_tile_kernel<FIRST, SG><<<(unsigned)(2 * persistent_grid()), kSpanThreads, 0, st>>>(a);
   return launch_status();
 }
 // `tiles` of `tile_rows` rows (32 or 64)
 template <bool FIRST>
-int launch_few(const Int4Args& a, int64_t tiles, int tile_rows, int group, hipStream_t st) {
-  if (tile_rows == 32)
-    return group == 128 ? launch_few<FIRST, 2, 1>(a, tiles, st) : group == 64 ? launch_few<FIRST, 2, 2>(a, tiles, st) : launch_few<FIRST, 2, 4>(a, tiles, st);
-  return group == 128 ? launch_few<FIRST, 4, 1>(a, tiles, st) : group == 64 ? launch_few<FIRST, 4, 2>(a, tiles, st) : launch_few<FIRST, 4, 4>(a, tiles, st);
+int launch(const Int4Args& a, int64_t tiles, int tile_rows, int group, hipStream_t st) {
+  return group == 128 ? launch_rows<FIRST, 1>(a, tiles, tile_rows, st)
+         : group == 64 ? launch_rows<FIRST, 2>(a, tiles, tile_rows, st) : launch_rows<FIRST, 4>(a, tiles, tile_rows, st);
 }
-template <bool FIRST>
-int launch_experts(const Int4Args& a, int64_t N, int64_t Msum, int tile_rows, int group, hipStream_t st) {
-  // a tile for each expert that may hold a row; more where the rows fill more than that
-  return launch_few<FIRST>(a, std::max(std::min(N, Msum), Msum / tile_rows), tile_rows, group, st);
+// row tiles that a launch has about: one for each expert that may hold a row; more where the rows fill more than that
+int64_t row_tiles_of(int64_t Msum, int64_t N, int tile_rows) { return std::max(std::min(N, Msum), cdiv64(Msum, tile_rows)); }
+// Which tiles.  Those of 32 rows bring their rows to LDS for few columns at a time, but cut a contraction among the wavefronts of a
+// workgroup: they are the better ones for few rows and small weights, where the taller ones leave sums to another launch.  By what
+// all rows together read of codes, or of one block by its size.  Us, 32 | 64: 8 of 128 experts of 2048 x 768, 1 token 20 | 25, 16 tokens 71 | 63,
+// 131 128 | 85; a dense block of 1024 x 2816, 4 tokens 14 | 19, 16 18 | 19, 32 29 | 23, 200 42 | 41; 512 x 1024, 200 tokens 17 | 27; 2048 x 5632, 4
+// tokens 19 | 21, 16 31 | 24; 4096 x 11264, 1 token 30 | 28; groups of 32, 2176 x 1152, 50 tokens 27 | 37.
+int tile_rows_of(int64_t Msum, int64_t D, int64_t H, int64_t N) {
+  if (const char* e = getenv("INT4_ROWS")) return atoi(e);
+  const int64_t codes = 3 * D * H / 2;
+  return Msum * codes <= (64 << 20) || (N == 1 && Msum <= 256 && codes <= (4 << 20)) ? 32 : 64;
 }
-template <bool FIRST>
-int launch_dense(const Int4Args& a, int group, hipStream_t st) {
-  const int tile_rows = a.M <= 32 ? 32 : 64;
-  return launch_few<FIRST>(a, cdiv64(a.M, tile_rows), tile_rows, group, st);
+// Slices of a contraction of K in 64-row tiles over `cols` columns (of both halves): as many as give every CU two tiles, of two stages at
+// least
+int slices_of(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
+  if (tile_rows != Int4Rows::BM) return 1;
+  const int64_t tiles = row_tiles_of(Msum, N, tile_rows) * cdiv64(cols, 256);
+  int64_t n = std::max<int64_t>(1, std::min(2 * persistent_grid() / tiles, int4_blocks(K) / 2));
+  n = std::max<int64_t>(1, std::min<int64_t>(n, (64 << 20) / (Msum * cols * 4)));
+  if (const char* e = getenv("INT4_SLICES")) n = std::min<int64_t>(atoi(e), int4_blocks(K));
+  return (int)n;
+}
+
+// the first product, of experts or of a dense block, with the sums of its slices in the workspace
+int launch_first(Int4Args a, int64_t N, int64_t Msum, int tile_rows, int group, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  a.slices = slices_of(Msum, N, 2 * a.ldo, a.K, tile_rows);
+  a.part = (float*)workspace;
+  a.all_rows = Msum;
+  if (a.slices > 1 && (!workspace || workspace_bytes < a.slices * Msum * 2 * a.ldo * 4)) return MOMOE_ERR_BAD_ARG;
+  const int status = launch<true>(a, row_tiles_of(Msum, N, tile_rows), tile_rows, group, st);
+  if (status != MOMOE_OK || a.slices == 1) return status;
+  const int64_t quads = Msum * (a.ldo / 4);
+  int4_h_of_slices_kernel<<<(unsigned)cdiv64(quads, 256), 256, 0, st>>>(a.part, (bf16*)a.out, Msum, (int)a.ldo, a.slices);
+  return launch_status();
 }
 
 }  // namespace
@@ -360,23 +605,29 @@ extern "C" int momoe_int4_pack_weights(const void* codes_NRC, const void* scale,
   return launch_status();
 }
 
-extern "C" int momoe_int4_tile_rows(int64_t Msum, int64_t N) {
-  return Msum <= 0 || N <= 0 ? 0 : Msum >= 20 * N ? 64 : 32;
+extern "C" int momoe_int4_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N) {
+  return Msum <= 0 || D <= 0 || H <= 0 || N <= 0 ? 0 : tile_rows_of(Msum, D, H, N);
+}
+extern "C" int momoe_int4_slices(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
+  return Msum <= 0 || N <= 0 || cols <= 0 || K <= 0 ? 0 : slices_of(Msum, N, cols, K, tile_rows);
 }
 
 extern "C" int momoe_int4_lin1_swiglu_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, int group,
-                                          const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH, int64_t M,
-                                          int64_t D, int64_t H, int64_t N, int64_t Msum, void* stream) {
+                                          const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH,
+                                          void* workspace, int64_t workspace_bytes, int64_t M, int64_t D, int64_t H, int64_t N,
+                                          int64_t Msum, void* stream) {
   if (!x_MD || !Wl1_packed || !Wl1_words || !idx_Msum || !tile_table || !h_MsumH || ldx < D) return MOMOE_ERR_BAD_ARG;
   const int st = check_int4(M, D, H, N, Msum, group);
   if (st != MOMOE_OK) return st;
-  if (unaligned16(x_MD) || unaligned16(Wl1_packed) || unaligned16(Wl1_words) || unaligned16(h_MsumH)) return MOMOE_ERR_BAD_ARG;
-  if (ldx % 8 != 0 || (tile_rows != 32 && tile_rows != 64)) return MOMOE_ERR_UNSUPPORTED;
+  if (unaligned16(x_MD) || unaligned16(Wl1_packed) || unaligned16(Wl1_words) || unaligned16(h_MsumH) || unaligned16(workspace))
+    return MOMOE_ERR_BAD_ARG;
+  // (the taller tiles gather their rows at 32-bit offsets)
+  if (ldx % 8 != 0 || (tile_rows != 32 && tile_rows != 64) || (tile_rows == 64 && M * ldx * 2 >= (1ll << 32))) return MOMOE_ERR_UNSUPPORTED;
   Int4Args a{(const bf16*)x_MD, ldx, (const uint8_t*)Wl1_packed, (const uint32_t*)Wl1_words, idx_Msum, tile_table, 0, (int)D,
              (int)int4_blocks(D), (int)(H / 16)};
   a.out = h_MsumH;
   a.ldo = H;
-  return launch_experts<true>(a, N, Msum, tile_rows, group, (hipStream_t)stream);
+  return launch_first(a, N, Msum, tile_rows, group, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int momoe_int4_lin2_scale_fwd(const void* h_MsumH, const void* Wl2_packed, const void* Wl2_words, int group, const float* s_NM,
@@ -395,35 +646,56 @@ extern "C" int momoe_int4_lin2_scale_fwd(const void* h_MsumH, const void* Wl2_pa
   a.sm = s_stride_m;
   a.out = ys_MsumD;
   a.ldo = D;
-  return launch_experts<false>(a, N, Msum, tile_rows, group, (hipStream_t)stream);
+  a.slices = slices_of(Msum, N, D, H, tile_rows);
+  a.part = ys_MsumD;
+  a.all_rows = Msum;
+  return launch<false>(a, row_tiles_of(Msum, N, tile_rows), tile_rows, group, (hipStream_t)stream);
 }
 
-extern "C" int momoe_int4_combine(const float* ys_MsumD, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K, int64_t Msum,
-                                  void* stream) {
-  if (!ys_MsumD || !inv_MK || !out_MD || M <= 0 || D <= 0 || K <= 0 || Msum <= 0) return MOMOE_ERR_BAD_ARG;
+extern "C" int momoe_int4_combine(const float* ys_MsumD, int slices, const int32_t* inv_MK, void* out_MD, int64_t M, int64_t D, int64_t K,
+                                  int64_t Msum, void* stream) {
+  if (!ys_MsumD || !inv_MK || !out_MD || M <= 0 || D <= 0 || K <= 0 || Msum <= 0 || slices <= 0) return MOMOE_ERR_BAD_ARG;
   if (D % 32 != 0 || M >= (1ll << 31) || Msum >= (1ll << 31)) return MOMOE_ERR_UNSUPPORTED;
   if (unaligned16(ys_MsumD) || unaligned16(out_MD)) return MOMOE_ERR_BAD_ARG;
-  int4_combine_kernel<<<(unsigned)M, 256, 0, (hipStream_t)stream>>>(ys_MsumD, inv_MK, (bf16*)out_MD, (int)D, (int)K, Msum);
+  int4_combine_kernel<<<(unsigned)M, 256, 0, (hipStream_t)stream>>>(ys_MsumD, slices, inv_MK, (bf16*)out_MD, (int)D, (int)K, Msum);
   return launch_status();
 }
 
+extern "C" int64_t momoe_int4_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H) {
+  if (M <= 0 || D <= 0 || H <= 0) return -1;
+  const int tile_rows = tile_rows_of(M, D, H, 1);
+  const int64_t n1 = slices_of(M, 1, 2 * H, D, tile_rows), n2 = slices_of(M, 1, D, H, tile_rows);
+  return std::max(n1 > 1 ? n1 * M * 2 * H * 4 : 0, n2 > 1 ? n2 * M * D * 4 : 0);
+}
+
 extern "C" int momoe_int4_ffn_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, const void* Wl2_packed,
-                                  const void* Wl2_words, int group, void* h_MH, void* y_MD, int64_t M, int64_t D, int64_t H, void* stream) {
+                                  const void* Wl2_words, int group, void* h_MH, void* y_MD, void* workspace, int64_t workspace_bytes,
+                                  int64_t M, int64_t D, int64_t H, void* stream) {
   if (!x_MD || !Wl1_packed || !Wl1_words || !Wl2_packed || !Wl2_words || !h_MH || !y_MD || ldx < D) return MOMOE_ERR_BAD_ARG;
   int st = check_int4(M, D, H, 1, M, group);
   if (st != MOMOE_OK) return st;
-  for (const void* q : {x_MD, Wl1_packed, Wl1_words, Wl2_packed, Wl2_words, (const void*)h_MH, (const void*)y_MD})
+  for (const void* q : {x_MD, Wl1_packed, Wl1_words, Wl2_packed, Wl2_words, (const void*)h_MH, (const void*)y_MD, (const void*)workspace})
     if (unaligned16(q)) return MOMOE_ERR_BAD_ARG;
-  if (ldx % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
+  if (ldx % 8 != 0 || ldx >= (1 << 22)) return MOMOE_ERR_UNSUPPORTED;
+  const int64_t need = momoe_int4_ffn_workspace_bytes(M, D, H);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MOMOE_ERR_BAD_ARG;
+  const int tile_rows = tile_rows_of(M, D, H, 1);
   Int4Args a{(const bf16*)x_MD, ldx, (const uint8_t*)Wl1_packed, (const uint32_t*)Wl1_words, nullptr, nullptr, (int)M, (int)D,
              (int)int4_blocks(D), (int)(H / 16)};
   a.out = h_MH;
   a.ldo = H;
-  st = launch_dense<true>(a, group, (hipStream_t)stream);
+  hipStream_t to = (hipStream_t)stream;
+  st = launch_first(a, 1, M, tile_rows, group, workspace, workspace_bytes, to);
   if (st != MOMOE_OK) return st;
   Int4Args b{(const bf16*)h_MH, H, (const uint8_t*)Wl2_packed, (const uint32_t*)Wl2_words, nullptr, nullptr, (int)M, (int)H,
              (int)int4_blocks(H), (int)(D / 32)};
   b.out = y_MD;
   b.ldo = D;
-  return launch_dense<false>(b, group, (hipStream_t)stream);
+  b.slices = slices_of(M, 1, D, H, tile_rows);
+  b.part = (float*)workspace;
+  b.all_rows = M;
+  st = launch<false>(b, cdiv64(M, tile_rows), tile_rows, group, to);
+  if (st != MOMOE_OK || b.slices == 1) return st;
+  int4_sum_slices_kernel<<<(unsigned)cdiv64(M * D, 1024), 256, 0, to>>>(b.part, (bf16*)y_MD, M * D, b.slices);
+  return launch_status();
 }

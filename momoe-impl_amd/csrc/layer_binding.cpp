@@ -712,12 +712,15 @@ std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, c
   if (M == 0) return {x_BSD.device() == dev ? y : y.to(x_BSD.device()), sizes.zero_()};
   const Tensor x = rows_in_bf16(x_BSD, M, D, dev);
 
-  const int tile_rows = momoe_int4_tile_rows(msum, N);
+  // (the taller tiles gather their rows at 32-bit offsets)
+  const int tile_rows = M * pitch_of_rows(x) * 2 >= (1ll << 32) ? 32 : momoe_int4_tile_rows(msum, D, H, N);
+  const int64_t slices1 = momoe_int4_slices(msum, N, 2 * H, D, tile_rows), slices2 = momoe_int4_slices(msum, N, D, H, tile_rows);
+  const int64_t ws1_bytes = slices1 > 1 ? slices1 * msum * 2 * H * 4 : 0, ys_bytes = slices2 * msum * D * 4;
   Index ib(M, N, K, tile_rows, false);
   const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
   const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
-  Transients transients(dev, {index_bytes, scratch_bytes, msum * H * 2, msum * D * 4});
-  Tensor index_own, scratch, h_own, ys_own, counter;
+  Transients transients(dev, {index_bytes, scratch_bytes, msum * H * 2, ws1_bytes, ys_bytes});
+  Tensor index_own, scratch, h_own, ws_own, ys_own, counter;
   ib.base = (int32_t*)transients.take(index_bytes, index_own);
   int32_t* const build = (int32_t*)transients.take(scratch_bytes, scratch);
   int32_t* violations = build;
@@ -729,12 +732,14 @@ std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, c
              ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), tile_rows, (int32_t*)nullptr,
              (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
   void* const h = transients.take(msum * H * 2, h_own);
+  void* const ws1 = ws1_bytes > 0 ? transients.take(ws1_bytes, ws_own) : nullptr;
   MOMOE_CALL(momoe_int4_lin1_swiglu_fwd, st, x.data_ptr(), pitch_of_rows(x), W1.data_ptr(), S1.data_ptr(), (int)group,
-             (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, h, M, D, H, N, msum);
-  float* const ys = (float*)transients.take(msum * D * 4, ys_own);
+             (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, h, ws1, ws1_bytes, M, D, H, N, msum);
+  ws_own.reset();
+  float* const ys = (float*)transients.take(ys_bytes, ys_own);
   MOMOE_CALL(momoe_int4_lin2_scale_fwd, st, h, W2.data_ptr(), S2.data_ptr(), (int)group, (const float*)s.data_ptr<float>(), s.stride(0),
              s.stride(1), (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, ys, M, D, H, N, msum);
-  MOMOE_CALL(momoe_int4_combine, st, (const float*)ys, (const int32_t*)ib.inv(), y.data_ptr(), M, D, K, msum);
+  MOMOE_CALL(momoe_int4_combine, st, (const float*)ys, (int)slices2, (const int32_t*)ib.inv(), y.data_ptr(), M, D, K, msum);
   if (check) {
     const int v = counter.narrow(0, 0, 1).item<int32_t>();
     TORCH_CHECK(v == 0, "mask_NM: ", v, " tokens do not have exactly K = ", K, " experts (or the mask holds more than M*K pairs)");
@@ -760,9 +765,14 @@ Tensor feed_forward_int4(const Tensor& x, const Tensor& W1, const Tensor& S1, co
   const hipStream_t st = stream_of(dev);
   Tensor y = empty_bf16(x.sizes(), dev);
   if (M > 0) {
-    const Tensor rows = rows_in_bf16(x, M, D, dev), h = empty_bf16({M, H}, dev);
+    const Tensor rows = rows_in_bf16(x, M, D, dev);
+    const int64_t ws_bytes = momoe_int4_ffn_workspace_bytes(M, D, H);
+    Transients transients(dev, {M * H * 2, ws_bytes});
+    Tensor h_own, ws_own;
+    void* const h = transients.take(M * H * 2, h_own);
+    void* const ws = ws_bytes > 0 ? transients.take(ws_bytes, ws_own) : nullptr;
     MOMOE_CALL(momoe_int4_ffn_fwd, st, rows.data_ptr(), pitch_of_rows(rows), W1.data_ptr(), S1.data_ptr(), W2.data_ptr(),
-               S2.data_ptr(), (int)group, h.data_ptr(), y.data_ptr(), M, D, H);
+               S2.data_ptr(), (int)group, h, y.data_ptr(), ws, ws_bytes, M, D, H);
   }
   return x.device() == dev ? y : y.to(x.device());
 }

@@ -110,11 +110,13 @@ _SIGNATURES = {
     "momoe_int4_weight_bytes": (_i64, [_i64] * 3),
     "momoe_int4_scale_words": (_i64, [_i64] * 3 + [_int]),
     "momoe_int4_pack_weights": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _int, _int, _p, _p, _p]),
-    "momoe_int4_tile_rows": (_int, [_i64] * 2),
-    "momoe_int4_lin1_swiglu_fwd": (_int, [_p, _i64, _p, _p, _int, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_tile_rows": (_int, [_i64] * 4),
+    "momoe_int4_slices": (_int, [_i64] * 4 + [_int]),
+    "momoe_int4_lin1_swiglu_fwd": (_int, [_p, _i64, _p, _p, _int, _p, _p, _int, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_int4_lin2_scale_fwd": (_int, [_p, _p, _p, _int, _p, _i64, _i64, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p]),
-    "momoe_int4_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
-    "momoe_int4_ffn_fwd": (_int, [_p, _i64, _p, _p, _p, _p, _int, _p, _p, _i64, _i64, _i64, _p]),
+    "momoe_int4_combine": (_int, [_p, _int, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "momoe_int4_ffn_workspace_bytes": (_i64, [_i64] * 3),
+    "momoe_int4_ffn_fwd": (_int, [_p, _i64, _p, _p, _p, _p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_bias_update": (_int, [_p, ctypes.c_float, ctypes.c_float, _i64, _p, _p]),
 }
 
@@ -574,5 +576,5 @@ def int4_pack_weights(codes_NRC, scale, zero, halves, group):
     return packed, words
 
 
-def int4_tile_rows(Msum, N):
-    return _lib.momoe_int4_tile_rows(Msum, N)
+def int4_tile_rows(Msum, D, H, N):
+    return _lib.momoe_int4_tile_rows(Msum, D, H, N)

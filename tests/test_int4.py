@@ -15,8 +15,15 @@ def test_sizes():
     assert lib.momoe_int4_weight_bytes(3, 200, 40) == lib.momoe_int4_weight_bytes(0, 1, 16) == -1
     assert [lib.momoe_int4_scale_words(2, 160, 32, g) for g in (32, 64, 128, 16)] == [2 * 32 * 2 * 4, 2 * 32 * 2 * 2, 2 * 32 * 2, -1]
     assert lib.momoe_int4_scale_words(1, 0, 32, 64) == lib.momoe_int4_scale_words(1, 32, 24, 64) == -1
-    assert lib.momoe_int4_tile_rows(0, 8) == lib.momoe_int4_tile_rows(8, 0) == 0
-    assert lib.momoe_int4_tile_rows(8, 128) == 32 and lib.momoe_int4_tile_rows(8000, 128) == 64
+    rows = lib.momoe_int4_tile_rows
+    assert rows(0, 64, 64, 8) == rows(1, 0, 64, 8) == rows(1, 64, 0, 8) == rows(1, 64, 64, 0) == 0
+    assert rows(8, 2048, 768, 128) == 32 and rows(8000, 2048, 768, 128) == 64 and rows(200, 1024, 1024, 1) == 32 and rows(300, 1024, 1024, 1) == 64
+    slices = lib.momoe_int4_slices
+    assert slices(0, 1, 64, 64, 64) == slices(1, 0, 64, 64, 64) == slices(1, 1, 0, 64, 64) == slices(1, 1, 64, 0, 64) == 0
+    assert slices(16, 1, 4096, 11264, 32) == 1 and slices(16, 1, 4096, 11264, 64) > 1 and slices(8000, 128, 1536, 2048, 64) == 1
+    assert lib.momoe_int4_ffn_workspace_bytes(0, 64, 64) == -1 and lib.momoe_int4_ffn_workspace_bytes(4, 512, 512) == 0
+    n = slices(16, 1, 22528, 4096, 64), slices(16, 1, 4096, 11264, 64)
+    assert lib.momoe_int4_ffn_workspace_bytes(16, 4096, 11264) == max(n[0] * 22528, n[1] * 4096) * 16 * 4
 
 
 def test_refusals_of_the_entry_points():
@@ -24,24 +31,26 @@ def test_refusals_of_the_entry_points():
     assert all(w(**{k: None}) == 1 for k in ("W", "scale", "packed", "words")) and all(w(**{k: 0}) == 1 for k in ("N", "R", "C", "halves"))
     assert w(t=1) == w(t=3) == w(halves=3) == w(packed=P + 8) == w(words=P + 4) == w(scale=P + 1) == 1
     assert w(R=48) == w(C=48) == w(group=16) == w(group=0) == w(R=1 << 22) == 2
-    one = dict(x=P, ld=64, W=P, S=P, group=32, idx=P, table=P, rows=32, h=P, M=16, D=64, H=32, N=8, Msum=32)
+    one = dict(x=P, ld=64, W=P, S=P, group=32, idx=P, table=P, rows=32, h=P, ws=None, bytes=0, M=16, D=64, H=32, N=8, Msum=32)
     lin1 = lambda **c: lib.momoe_int4_lin1_swiglu_fwd(*{**one, **c}.values(), None)
     assert all(lin1(**{k: None}) == 1 for k in ("x", "W", "S", "idx", "table", "h"))
     assert all(lin1(**{k: 0}) == 1 for k in ("M", "D", "H", "N", "Msum")) and all(lin1(**{k: P + 8}) == 1 for k in ("x", "W", "S", "h"))
+    assert lin1(ws=P + 8) == lin1(rows=64, D=1024, ld=1024, N=1, Msum=16) == 1 and lin1(rows=64, M=1 << 21, ld=1024) == 2  # no room for slices; rows past 32 bits
     assert lin1(ld=56) == 1 and lin1(ld=68) == lin1(D=48) == lin1(H=40) == lin1(Msum=1 << 31) == lin1(group=48) == lin1(rows=128) == 2
     two = dict(h=P, W=P, S=P, group=32, s=P, sn=16, sm=1, idx=P, table=P, rows=32, ys=P, M=16, D=64, H=32, N=8, Msum=32)
     lin2 = lambda **c: lib.momoe_int4_lin2_scale_fwd(*{**two, **c}.values(), None)
     assert all(lin2(**{k: None}) == 1 for k in ("h", "W", "S", "s", "idx", "table", "ys"))
     assert all(lin2(**{k: 0}) == 1 for k in ("M", "D", "H", "N", "Msum")) and all(lin2(**{k: P + 8}) == 1 for k in ("h", "W", "S", "ys"))
     assert lin2(D=48) == lin2(H=40) == lin2(group=0) == lin2(rows=0) == 2
-    c = lambda **k: lib.momoe_int4_combine(*{**dict(ys=P, inv=P, out=P, M=4, D=64, K=2, Msum=8), **k}.values(), None)
-    assert all(c(**{k: None}) == 1 for k in ("ys", "inv", "out")) and all(c(**{k: 0}) == 1 for k in ("M", "D", "K", "Msum"))
+    c = lambda **k: lib.momoe_int4_combine(*{**dict(ys=P, slices=1, inv=P, out=P, M=4, D=64, K=2, Msum=8), **k}.values(), None)
+    assert all(c(**{k: None}) == 1 for k in ("ys", "inv", "out")) and all(c(**{k: 0}) == 1 for k in ("slices", "M", "D", "K", "Msum"))
     assert c(ys=P + 8) == c(out=P + 8) == 1 and c(D=48) == c(M=1 << 31) == 2
-    ffn = dict(x=P, ld=64, W1=P, S1=P, W2=P, S2=P, group=32, h=P, y=P, M=16, D=64, H=32)
+    ffn = dict(x=P, ld=64, W1=P, S1=P, W2=P, S2=P, group=32, h=P, y=P, ws=None, bytes=0, M=16, D=64, H=32)
     f = lambda **k: lib.momoe_int4_ffn_fwd(*{**ffn, **k}.values(), None)
     assert all(f(**{k: None}) == 1 for k in ("x", "W1", "S1", "W2", "S2", "h", "y")) and all(f(**{k: 0}) == 1 for k in ("M", "D", "H"))
     assert all(f(**{k: P + 8}) == 1 for k in ("x", "W1", "S1", "W2", "S2", "h", "y"))
-    assert f(ld=56) == 1 and f(ld=68) == f(D=48) == f(H=40) == f(group=100) == f(M=1 << 31) == 2
+    assert f(ws=P + 8) == f(M=16, D=4096, H=11264, ld=4096) == f(M=16, D=4096, H=11264, ld=4096, ws=P, bytes=64) == 1
+    assert f(ld=56) == 1 and f(ld=1 << 22) == f(ld=68) == f(D=48) == f(H=40) == f(group=100) == f(M=1 << 31) == 2
 
 
 def test_constructor_refusals():
