@@ -16,7 +16,6 @@
 //           in the low four, the zero
 // Past the last k-value the codes are the zero of their group, or the scales are zero.  The columns of the first product are those of its two halves in turn, 16 a and 16 b.
 #include <algorithm>
-#include <cstdlib>
 
 #include "gemm_span.hpp"
 
@@ -46,12 +45,16 @@ struct Int4Args {
   int64_t all_rows;
 };
 
-// eight codes of a word as 128 + code
-__device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t w) {
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-  return __builtin_bit_cast(bf16x8, v);
+// Eight codes of a word as 128 + code, two at a time; k128: 0x43004300 in a vector register (of two constants outside them the and and
+// the or are an instruction each)
+__device__ __forceinline__ uint32_t two_codes(uint32_t w, int i, uint32_t k128) { return ((w >> (4 * i)) & 0x000F000Fu) | k128; }
+__device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t w, uint32_t k128) {
+  return __builtin_bit_cast(bf16x8, u32x4{two_codes(w, 0, k128), two_codes(w, 1, k128), two_codes(w, 2, k128), two_codes(w, 3, k128)});
+}
+__device__ __forceinline__ uint32_t two_of_128() {
+  uint32_t v = 0x43004300u;
+  asm volatile("" : "+v"(v));
+  return v;
 }
 __device__ __forceinline__ float scale_of_word(uint32_t w) { return __uint_as_float(w & ~15u); }
 __device__ __forceinline__ float zero_of_word(uint32_t w) { return __uint_as_float(0x43000000u | (w & 15u) << 16); }  // 128 + zero
@@ -114,6 +117,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
   typedef uint32_t Words __attribute__((ext_vector_type(SG)));
   const int tid = threadIdx.x, l = tid & 63, wave = wave_id(), kw = wave % KS, cw = wave / KS;
   Int4Sched sched(p, (p.pairs + PW - 1) / PW, ROWS);
+  const uint32_t k128 = two_of_128();
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
   for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
     const int pair = min(tc.tn * PW + cw, p.pairs - 1);
@@ -164,7 +168,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) wf[j][m] = bf16_of_codes(wq[q][j][m]);
+          for (int m = 0; m < 4; ++m) wf[j][m] = bf16_of_codes(wq[q][j][m], k128);
         unrolled<0, FR>([&](auto IC) {
           constexpr int i = decltype(IC)::value;
           if (i >= nf) return;  // (the same for all lanes)
@@ -275,97 +279,114 @@ struct Int4Rows {
 template <bool FIRST, int SG>
 __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) {
   using Rows = Int4Rows;
-  constexpr int PAIRS = 2 * kSpanWaves;
+  constexpr int PAIRS = 2 * kSpanWaves, STEPS = 4 / SG;
   typedef uint32_t Words __attribute__((ext_vector_type(SG)));
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Rows::STAGE];
   const int l = lane_id(), wave = wave_id();
   const uint32_t addr = lds_address((bf16*)lds) + wave * 1024;
-  const int nb = (p.pairs + PAIRS - 1) / PAIRS;
-  Int4Sched sched(p, nb * p.slices, Rows::BM);
+  Int4Sched sched(p, (p.pairs + PAIRS - 1) / PAIRS * p.slices, Rows::BM);
+  const uint32_t k128 = two_of_128();
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-  for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
-    const int tn = tc.tn / p.slices, slice = tc.tn - tn * p.slices;
-    const int kb0 = (int)((int64_t)p.KB * slice / p.slices), kb1 = (int)((int64_t)p.KB * (slice + 1) / p.slices);
-    const int nf = (tc.rows + 15) >> 4, pair0 = tn * PAIRS + 2 * wave;
-    const uint8_t* w[4];
-    const uint32_t* sc[4];
+  struct Tile {
+    TileCoord tc;
+    int slice, kb0, kb1, nf, pair0;
+    __device__ __forceinline__ void place(const Int4Args& p, const TileCoord& t) {
+      tc = t;
+      const int tn = t.tn / p.slices;
+      slice = t.tn - tn * p.slices;
+      kb0 = (int)((int64_t)p.KB * slice / p.slices), kb1 = (int)((int64_t)p.KB * (slice + 1) / p.slices);
+      nf = (t.rows + 15) >> 4;
+      pair0 = tn * PAIRS + 2 * wave_id();
+    }
+  };
+  Tile cur, next;
+  next.place(p, sched.next());
+  if (!next.tc.valid) return;
+  Rows A;
+  const uint8_t* w[4];
+  const uint32_t* sc[4];
+  u32x4 wq[4];
+  Words sq[4];
+  const auto load = [&](int kb) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t group = (((int64_t)tc.expert * p.pairs + min(pair0 + j / 2, p.pairs - 1)) * 2 + j % 2) * p.KB;
+      wq[j] = *(const u32x4*)(w[j] + (int64_t)kb * kInt4Frag + l * 16);
+      sq[j] = *(const Words*)(sc[j] + (int64_t)kb * (16 * SG) + (l & 15) * SG);
+    }
+  };
+  // the first stage of the next tile, into the half of LDS that nobody reads
+  int q = 0;
+  const auto begin = [&] {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t group = (((int64_t)next.tc.expert * p.pairs + min(next.pair0 + j / 2, p.pairs - 1)) * 2 + j % 2) * p.KB;
       w[j] = p.w + group * kInt4Frag;
       sc[j] = p.scale + group * (16 * SG);
     }
-    Rows A;
-    A.init(p, tc, FIRST && p.idx);
-    u32x4 wq[4];
-    Words sq[4];
-    const auto load = [&](int kb) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        wq[j] = *(const u32x4*)(w[j] + (int64_t)kb * kInt4Frag + l * 16);
-        sq[j] = *(const Words*)(sc[j] + (int64_t)kb * (16 * SG) + (l & 15) * SG);
-      }
-    };
-    __syncthreads();  // (the last tile's rows have been read)
-    A.request(kb0, p.K, nf, addr);
-    load(kb0);
+    A.request(next.kb0, p.K, next.nf, addr + q * Rows::STAGE);
+    load(next.kb0);
+  };
+  A.init(p, next.tc, FIRST && p.idx);
+  begin();
+  while (true) {
+    cur = next;
+    next.place(p, sched.next());
+    Rows B;  // rows of the next tile: their tokens travel meanwhile
+    if (next.tc.valid) B.init(p, next.tc, FIRST && p.idx);
+    const int nf = cur.nf;
     f32x4 acc[4][4] = {};
-    const auto stage = [&](auto Q, int kb) {
-      constexpr int q = decltype(Q)::value;
+    for (int kb = cur.kb0; kb < cur.kb1; ++kb) {
       wait_vmcnt<0>();
       wait_lgkm0();
       __builtin_amdgcn_s_barrier();
       order_fence();
-      if (kb + 1 < kb1) A.request(kb + 1, p.K, nf, addr + (q ^ 1) * Rows::STAGE);
+      if (kb + 1 < cur.kb1) A.request(kb + 1, p.K, nf, addr + (q ^ 1) * Rows::STAGE);
       order_fence();
       u32x4 codes[4];
       Words scales[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) codes[j] = wq[j], scales[j] = sq[j];
+      load(min(kb + 1, cur.kb1 - 1));
+      order_fence();
       const uint8_t* const rows = lds + q * Rows::STAGE + (l & 15) * 256;
-      constexpr int STEPS = 4 / SG;
-      bf16x8 wf[4][STEPS], rf[2][STEPS];
-      float s[4], z[4];
-      // fragment i of group g, asked for while the one before is multiplied
-      const auto read = [&](auto NC) {
-        constexpr int n = decltype(NC)::value, g = n / 4, i = n % 4;
-#pragma unroll
-        for (int m = 0; m < STEPS; ++m)
-          rf[n & 1][m] = *(const bf16x8*)(rows + i * (16 * 256) + (((4 * (g * STEPS + m) + (l >> 4)) ^ (l & 15)) << 4));
-      };
-      read(IntC<0>{});
-      unrolled<0, 4 * SG>([&](auto NC) {
-        constexpr int n = decltype(NC)::value, g = n / 4, i = n % 4;
-        if constexpr (i == 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[j] = scale_of_word(scales[j][g]), z[j] = zero_of_word(scales[j][g]);
-#pragma unroll
-            for (int m = 0; m < STEPS; ++m) wf[j][m] = bf16_of_codes(codes[j][g * STEPS + m]);
-          }
-          if constexpr (g == SG - 1) load(min(kb + 1, kb1 - 1));
-        }
-        if constexpr (n + 1 < 4 * SG) read(IntC<n + 1>{});
-        if (i >= nf) return;  // (the same for all lanes)
-        f32x4 t[4] = {}, sum = {};
-#pragma unroll
-        for (int m = 0; m < STEPS; ++m) {
-          sum = mfma16(rf[n & 1][m], ones, sum);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) t[j] = mfma16(rf[n & 1][m], wf[j][m], t[j]);
-        }
+      unrolled<0, SG>([&](auto GC) {
+        constexpr int g = decltype(GC)::value;
+        bf16x8 wf[4][STEPS];
+        float s[4], z[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          s[j] = scale_of_word(scales[j][g]), z[j] = zero_of_word(scales[j][g]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s[j], fmaf(-z[j], sum[r], t[j][r]), acc[j][i][r]);
-          asm volatile("" : "+v"(acc[j][i]));  // (the products of all fragments were formed first, and spilled)
+          for (int m = 0; m < STEPS; ++m) wf[j][m] = bf16_of_codes(codes[j][g * STEPS + m], k128);
         }
+        unrolled<0, 4>([&](auto IC) {
+          constexpr int i = decltype(IC)::value;
+          if (i >= nf) return;  // (the same for all lanes)
+          bf16x8 rf[STEPS];
+#pragma unroll
+          for (int m = 0; m < STEPS; ++m)
+            rf[m] = *(const bf16x8*)(rows + i * (16 * 256) + (((4 * (g * STEPS + m) + (l >> 4)) ^ (l & 15)) << 4));
+          f32x4 t[4] = {}, sum = {};
+#pragma unroll
+          for (int m = 0; m < STEPS; ++m) {
+            sum = mfma16(rf[m], ones, sum);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = mfma16(rf[m], wf[j][m], t[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s[j], fmaf(-z[j], sum[r], t[j][r]), acc[j][i][r]);
+            asm volatile("" : "+v"(acc[j][i]));  // (the products of all fragments were formed first, and spilled)
+          }
+        });
       });
       order_fence();
-    };
-    for (int kb = kb0; kb < kb1; kb += 2) {
-      stage(IntC<0>{}, kb);
-      if (kb + 1 < kb1) stage(IntC<1>{}, kb + 1);
+      q ^= 1;
+    }
+    if (next.tc.valid) {
+      A = B;
+      begin();
     }
     const int col = l & 15;
 #pragma unroll
@@ -374,29 +395,30 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at = 16 * i + 4 * (l >> 4) + r;
-        if (at >= tc.rows) continue;
-        const int64_t row = tc.row0 + at;
+        if (at >= cur.tc.rows) continue;
+        const int64_t row = cur.tc.row0 + at;
         float s = 1.0f;
-        if (!FIRST && p.idx) s = p.s[(int64_t)tc.expert * p.sn + (int64_t)p.idx[row] * p.sm];
+        if (!FIRST && p.idx) s = p.s[(int64_t)cur.tc.expert * p.sn + (int64_t)p.idx[row] * p.sm];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int pair = pair0 + c;
+          const int pair = cur.pair0 + c;
           if (pair >= p.pairs) continue;
           const float v0 = acc[2 * c][i][r], v1 = acc[2 * c + 1][i][r];
           if (p.slices == 1) {
             store_pair<FIRST>(p, row, pair, col, v0, v1, s);
           } else if (FIRST) {
-            float* const to = p.part + (slice * p.all_rows + row) * (2 * p.ldo) + 16 * pair + col;
+            float* const to = p.part + (cur.slice * p.all_rows + row) * (2 * p.ldo) + 16 * pair + col;
             to[0] = v0;
             to[p.ldo] = v1;
           } else {
-            float* const to = p.part + (slice * p.all_rows + row) * p.ldo + 32 * pair + col;
+            float* const to = p.part + (cur.slice * p.all_rows + row) * p.ldo + 32 * pair + col;
             to[0] = v0 * s;
             to[16] = v1 * s;
           }
         }
       }
     }
+    if (!next.tc.valid) break;
   }
 }
 
@@ -548,18 +570,16 @@ int64_t row_tiles_of(int64_t Msum, int64_t N, int tile_rows) { return std::max(s
 // 131 128 | 85; a dense block of 1024 x 2816, 4 tokens 14 | 19, 16 18 | 19, 32 29 | 23, 200 42 | 41; 512 x 1024, 200 tokens 17 | 27; 2048 x 5632, 4
 // tokens 19 | 21, 16 31 | 24; 4096 x 11264, 1 token 30 | 28; groups of 32, 2176 x 1152, 50 tokens 27 | 37.
 int tile_rows_of(int64_t Msum, int64_t D, int64_t H, int64_t N) {
-  if (const char* e = getenv("INT4_ROWS")) return atoi(e);
   const int64_t codes = 3 * D * H / 2;
   return Msum * codes <= (64 << 20) || (N == 1 && Msum <= 256 && codes <= (4 << 20)) ? 32 : 64;
 }
 // Slices of a contraction of K in 64-row tiles over `cols` columns (of both halves): as many as give every CU two tiles, of two stages at
 // least
 int slices_of(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
-  if (tile_rows != Int4Rows::BM) return 1;
+  if (tile_rows != 64) return 1;
   const int64_t tiles = row_tiles_of(Msum, N, tile_rows) * cdiv64(cols, 256);
   int64_t n = std::max<int64_t>(1, std::min(2 * persistent_grid() / tiles, int4_blocks(K) / 2));
   n = std::max<int64_t>(1, std::min<int64_t>(n, (64 << 20) / (Msum * cols * 4)));
-  if (const char* e = getenv("INT4_SLICES")) n = std::min<int64_t>(atoi(e), int4_blocks(K));
   return (int)n;
 }
 
