@@ -576,13 +576,14 @@ FeedForward feed_forward_forward(const Tensor& x, const Tensor& W1, const Tensor
   f.W2 = packed_bf16(W2);
   if (M > 0) {
     if (msave > 0) f.ab = fragments(msave, 2 * H, dev);
-    const Tensor h = empty_bf16({M * H}, dev);
-    MOMOE_CALL(momoe_ffn_lin1_fwd, st, f.x.data_ptr(), pitch_of_rows(f.x), f.W1.data_ptr(), h.data_ptr(),
-               msave > 0 ? f.ab.data_ptr<float>() : nullptr, (msave + 31) / 32 * 32, M, M, D, H);
-    const int64_t bytes = momoe_ffn_workspace_bytes(M, D, H);
-    Tensor ws;
-    if (bytes > 0) ws = empty_f32({bytes / 4}, dev);
-    MOMOE_CALL(momoe_ffn_lin2_fwd, st, h.data_ptr(), f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
+    const int64_t ws_bytes = momoe_ffn_workspace_bytes(M, D, H);
+    Transients transients(dev, {M * H * 2, ws_bytes});
+    Tensor h_own, ws_own;
+    void* const h = transients.take(M * H * 2, h_own);
+    MOMOE_CALL(momoe_ffn_lin1_fwd, st, f.x.data_ptr(), pitch_of_rows(f.x), f.W1.data_ptr(), h, msave > 0 ? f.ab.data_ptr<float>() : nullptr,
+               (msave + 31) / 32 * 32, M, M, D, H);
+    void* const ws = ws_bytes > 0 ? transients.take(ws_bytes, ws_own) : nullptr;
+    MOMOE_CALL(momoe_ffn_lin2_fwd, st, (const void*)h, f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H, ws, ws_bytes);
   }
   if (x.device() != dev) f.y = f.y.to(x.device());
   return f;
@@ -621,35 +622,41 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
     }
     const Tensor Gy = rows_in_bf16(grads[0], M, D, dev);
     const int64_t ldx = pitch_of_rows(x), ldgy = pitch_of_rows(Gy);
-    Tensor gz = empty_bf16({2 * H * M}, dev), hT, counts = empty_i32(4, dev);
-    if (need_w2) hT = empty_bf16({momoe_padded_rows(M, 1) * H}, dev);
-    // what lies behind row `at`, a multiple of 32
-    const auto rows_at = [](const Tensor& t, int64_t at, int64_t pitch) { return (void*)((char*)t.data_ptr() + at * pitch * 2); };
-    void* const ht = need_w2 ? hT.data_ptr() : nullptr;
+    const int64_t rest = M - msave, gz_bytes = 4 * H * M, ht_bytes = need_w2 ? momoe_padded_rows(M, 1) * H * 2 : 0;
+    const int64_t u_bytes = rest > 0 ? momoe_ffn_fragment_floats(rest, H) * 4 : 0;
+    const int64_t ws1_bytes = need_w1 ? momoe_ffn_wgrad_workspace_bytes(M, D, 2 * H) : 0;
+    const int64_t ws2_bytes = need_w2 ? momoe_ffn_wgrad_workspace_bytes(M, H, D) : 0;
+    const int64_t wsx_bytes = need_x ? momoe_ffn_workspace_bytes(M, D, 2 * H) : 0;
+    Transients transients(dev, {16, gz_bytes, ht_bytes, u_bytes, ws1_bytes, ws2_bytes, wsx_bytes});
+    Tensor counts_own, gz_own, ht_own, u_own, ws1_own, ws2_own, wsx_own;
+    const auto scratch = [&](int64_t bytes, Tensor& own) { return bytes > 0 ? transients.take(bytes, own) : nullptr; };
+    int32_t* const counts = (int32_t*)transients.take(16, counts_own);
+    void* const gz = transients.take(gz_bytes, gz_own);
+    void* const ht = scratch(ht_bytes, ht_own);
+    // what lies behind row msave, a multiple of 32
+    const auto behind = [&](const void* p, int64_t pitch) { return p ? (void*)((char*)p + msave * pitch * 2) : nullptr; };
     if (msave > 0)
-      MOMOE_CALL(momoe_ffn_dgrad_h_saved, st, Gy.data_ptr(), ldgy, W2.data_ptr(), (const float*)saved[3].data_ptr<float>(), gz.data_ptr(), ht,
-                 counts.data_ptr<int32_t>(), msave, M, D, H);
-    if (msave < M) {
-      const Tensor u = fragments(M - msave, H, dev);
-      MOMOE_CALL(momoe_ffn_dgrad_h, st, rows_at(Gy, msave, ldgy), ldgy, W2.data_ptr(), u.data_ptr<float>(), M - msave, D, H);
-      MOMOE_CALL(momoe_ffn_swiglu_bwd, st, rows_at(x, msave, ldx), ldx, W1.data_ptr(), (const float*)u.data_ptr<float>(), rows_at(gz, msave, 32),
-                 need_w2 ? rows_at(hT, msave, H) : nullptr, counts.data_ptr<int32_t>(), M - msave, M, D, H);
+      MOMOE_CALL(momoe_ffn_dgrad_h_saved, st, Gy.data_ptr(), ldgy, W2.data_ptr(), (const float*)saved[3].data_ptr<float>(), gz, ht, counts,
+                 msave, M, D, H);
+    if (rest > 0) {
+      float* const u = (float*)transients.take(u_bytes, u_own);
+      MOMOE_CALL(momoe_ffn_dgrad_h, st, behind(Gy.data_ptr(), ldgy), ldgy, W2.data_ptr(), u, rest, D, H);
+      MOMOE_CALL(momoe_ffn_swiglu_bwd, st, behind(x.data_ptr(), ldx), ldx, W1.data_ptr(), (const float*)u, behind(gz, 32), behind(ht, H), counts,
+                 rest, M, D, H);
+      u_own.reset();
     }
-    const auto weight_gradient = [&](const void* A, int64_t lda, int a_layout, const void* B, int64_t ldb, int b_layout, const Tensor& G) {
-      const int64_t X = G.size(0), Y = G.size(1), bytes = momoe_ffn_wgrad_workspace_bytes(M, X, Y);
-      const Tensor ws = empty_f32({bytes / 4}, dev);
-      MOMOE_CALL(momoe_wgrad, st, A, lda, a_layout, (const int32_t*)nullptr, B, ldb, b_layout, (const int32_t*)nullptr,
-                 (const int32_t*)counts.data_ptr<int32_t>(), G.data_ptr(), M, (int64_t)1, X, Y, M, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
+    const auto weight_gradient = [&](const void* A, int64_t lda, int a_layout, const void* B, int64_t ldb, int b_layout, const Tensor& G,
+                                     int64_t ws_bytes, Tensor& own) {
+      MOMOE_CALL(momoe_wgrad, st, A, lda, a_layout, (const int32_t*)nullptr, B, ldb, b_layout, (const int32_t*)nullptr, (const int32_t*)counts,
+                 G.data_ptr(), M, (int64_t)1, G.size(0), G.size(1), M, scratch(ws_bytes, own), ws_bytes);
+      own.reset();
     };
-    if (need_w2) weight_gradient(ht, H, MOMOE_LAYOUT_TRANSPOSED, Gy.data_ptr(), ldgy, MOMOE_LAYOUT_ROWS, out[2]);
-    hT.reset();
-    if (need_w1) weight_gradient(x.data_ptr(), ldx, MOMOE_LAYOUT_ROWS, gz.data_ptr(), M, MOMOE_LAYOUT_KBLOCKED, out[1]);
+    if (need_w2) weight_gradient(ht, H, MOMOE_LAYOUT_TRANSPOSED, Gy.data_ptr(), ldgy, MOMOE_LAYOUT_ROWS, out[2], ws2_bytes, ws2_own);
+    ht_own.reset();
+    if (need_w1) weight_gradient(x.data_ptr(), ldx, MOMOE_LAYOUT_ROWS, gz, M, MOMOE_LAYOUT_KBLOCKED, out[1], ws1_bytes, ws1_own);
     if (need_x) {
       const Tensor Gx = empty_bf16({M, D}, dev);
-      const int64_t bytes = momoe_ffn_workspace_bytes(M, D, 2 * H);
-      Tensor ws;
-      if (bytes > 0) ws = empty_f32({bytes / 4}, dev);
-      MOMOE_CALL(momoe_ffn_dgrad_x, st, gz.data_ptr(), W1.data_ptr(), Gx.data_ptr(), M, D, H, bytes > 0 ? ws.data_ptr() : nullptr, bytes);
+      MOMOE_CALL(momoe_ffn_dgrad_x, st, (const void*)gz, W1.data_ptr(), Gx.data_ptr(), M, D, H, scratch(wsx_bytes, wsx_own), wsx_bytes);
       out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
     }
     return out;
