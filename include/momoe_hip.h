@@ -514,38 +514,42 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * No counterpart in the reference, whose layers all have a router (of one expert, with a gate weight of 1, its kernels of
  * momoe/momoe.py:69-237 and :356-703 compute the same).  bf16 rows, weights and results, fp32 sums:
  *   a | b = x W1,  h = a b sigmoid(b),  y = h W2;  u = Gy W2^T,  gz = G_a | G_b = u b sigmoid(b) | u a sigmoid(b) (1 + b (1 - sigmoid(b))),
- *   Gx = gz W1^T, and the gradients of the weights as momoe_wgrad of one expert: W2 from hT (MOMOE_LAYOUT_TRANSPOSED) and Gy, W1 from
- *   x and gz (MOMOE_LAYOUT_KBLOCKED, ld = ldm), with counts2 as its cumsums.
- * Layouts: h_blocked [H/32][ldm][32] and gz_blocked [2H/32][ldm][32], element (r, j) at [((j / 32) * ldm + r) * 32 + j % 32];
- * ab and u fp32 as accumulator fragments, momoe_ffn_fragment_floats(rows, 2H or H) values: of rows 16 i .. +15 and columns 16 j .. +15,
- * lane l of 64 has columns 4 (l / 16) .. +3 of row l % 16, at [((i * columns / 16 + j) * 64 + l) * 4]; hT bf16 [(rows + 31) / 32][H][32], zeros
- * past the last row (may be NULL).
- * A launch does `rows` rows; with all pointers moved on by a multiple of 32 rows, several do the rows of one block of ldm rows.
+ *   Gx = gz W1^T,  GW1 = x^T gz,  GW2 = h^T Gy.
+ * Layouts: h_blocked [H/32][ldm][32] and gz_blocked [2H/32][ldm][32], element (r, j) at [((j / 32) * ldm + r) * 32 + j % 32], of gz with zeros
+ * past the last row up to a multiple of 32 (for which ldm has to leave room); ab and u fp32 as accumulator fragments,
+ * momoe_ffn_fragment_floats(rows, 2H or H) values: of rows 16 i .. +15 and columns 16 j .. +15, lane l of 64 has columns 4 (l / 16) .. +3 of row
+ * l % 16, at [((i * columns / 16 + j) * 64 + l) * 4]; hT bf16 [(rows + 31) / 32 + 1][H][32], row r of column j at [r / 32][j][r % 32], zeros past the last row up to
+ * a multiple of 32 (may be NULL; the last group is not written, but may be read).
+ * A launch does `rows` rows; with all pointers moved on by a multiple of 32 rows, several do the rows of one block.
  * D and H multiples of 32, D * H * 4 < 4 GiB; row pitches multiples of 8; pointers to bf16 and fp32 data on 16-byte boundaries.
  * momoe_ffn_lin1_fwd: h; ab, of the first ab_rows rows, a multiple of 32 (0: none).
  * momoe_ffn_lin2_fwd: y [rows][D].
  * momoe_ffn_dgrad_h: u.  momoe_ffn_swiglu_bwd: gz and hT, a | b made again from x.
  * momoe_ffn_dgrad_h_saved: gz and hT from the a | b that were kept, u on the way.
- * Both write {0, ldm} to counts2 (may be NULL).
- * momoe_ffn_dgrad_x: Gx [rows][D].
- * These two take scratch (of at least momoe_ffn_workspace_bytes(rows, D, H, or 2H); 0, NULL: none is needed) for the sums of a contraction
- * that is cut because the launch has few tiles.
- * momoe_ffn_wgrad_workspace_bytes: what to give momoe_wgrad for a gradient [X][Y] of one expert with all rows (any other size will do).
+ * Both write {0, tokens}, the rows of all launches, to counts2 (may be NULL), which the gradients of the weights take.
+ * momoe_ffn_dgrad_x: Gx [rows][D].  momoe_ffn_wgrad_w2, momoe_ffn_wgrad_w1: GW2 [H][D], GW1 [D][2H], over `rows` tokens, all of them; fewer than
+ * 4 GiB of x and Gy each (rows * pitch * 2), ldm below 8388608.
+ * momoe_ffn_lin2_fwd (contraction H) and momoe_ffn_dgrad_x (2H) take scratch of at least momoe_ffn_workspace_bytes(rows, D, contraction), the
+ * gradients of the weights of momoe_ffn_wgrad_workspace_bytes(rows, H, D or D, 2H); 0 (NULL): none is needed.
  */
-int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y);
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
+int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction);
+int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);
-int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction);
 int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* workspace,
                        int64_t workspace_bytes, void* stream);
 int momoe_ffn_dgrad_h(const void* Gy, int64_t ldgy, const void* W2_HD, float* u, int64_t rows, int64_t D, int64_t H, void* stream);
 int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D2H, const float* u, void* gz_blocked, void* hT, int32_t* counts2,
-                         int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
+                         int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
 int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void* W2_HD, const float* ab, void* gz_blocked, void* hT, int32_t* counts2,
-                            int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
-int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H, void* workspace,
-                      int64_t workspace_bytes, void* stream);
+                            int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
+int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, void* workspace, int64_t workspace_bytes, int64_t rows,
+                      int64_t ldm, int64_t D, int64_t H, void* stream);
+int momoe_ffn_wgrad_w2(const void* hT, const void* Gy, int64_t ldgy, const int32_t* counts2, void* GW2_HD, void* workspace,
+                       int64_t workspace_bytes, int64_t rows, int64_t D, int64_t H, void* stream);
+int momoe_ffn_wgrad_w1(const void* x, int64_t ldx, const void* gz_blocked, const int32_t* counts2, void* GW1_D2H, void* workspace,
+                       int64_t workspace_bytes, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
 
 /* ---- SwiGLU blocks with weights in 4 bits, forward only -------------------------------
  * No counterpart in the reference, whose weights are bf16.  A weight is (code - zero) * scale: a 4-bit code, and for each `group`

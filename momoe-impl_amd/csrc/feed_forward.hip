@@ -8,10 +8,11 @@
 // memory in fp32, as whole accumulator fragments ([row / 16][column / 16][64 lanes][4]: 1 KiB a store).  (In bf16 they cost half as much
 // traffic and a rounding each, which doubles the error of the weight gradients.)
 //   h       [H / 32][ldm][32]    k-blocked, as the second product contracts over it
-//   gz      [2H / 32][ldm][32]   G_a | G_b, k-blocked, for G_x and the gradient of W1
+//   gz      [2H / 32][ldm][32]   G_a | G_b, k-blocked, for G_x and the gradient of W1; zeros behind the last row up to a multiple of 32
 //   hT      [rows / 32][H][32]   h once more, feature-major in groups of 32 rows, zeros behind the last row: for the gradient of W2
-// The weights' gradients are momoe_wgrad of one expert.
+// The weights' gradients are momoe_wgrad of one expert where their launches are large, and tiles of 128 x 128 where they are small.
 #include <algorithm>
+#include <type_traits>
 
 #include "ffn_tile.hpp"
 
@@ -33,8 +34,9 @@ struct FfnArgs {
   bf16* ht;
   bf16* out;       // y or G_x, row-major, D columns
   float* part;     // its sums by slices of the contraction, [slices][rows][D], where there are several
+  int64_t total;   // tokens that a gradient of the weights is contracted over
   int slices = 1;
-  int32_t* counts; // {0, ldm}: what momoe_wgrad takes as the rows of its one expert
+  int32_t* counts; // {0, all tokens}: what momoe_wgrad takes as the rows of its one expert
   unsigned long long* clk = clock_trace_buffer();
 };
 
@@ -79,17 +81,16 @@ struct FfnProg {
       }
     }
   }
-  // four columns of G_a, G_b and h of a row; `some`: it is one of the rows, and not of those that pad hT
+  // four columns of G_a, G_b and h of a row; `some`: it is one of the rows, and not of those that pad gz and hT
   __device__ __forceinline__ void store_grads(int64_t row, bool some, int col, const f32x4& a, const f32x4& b, const f32x4& u) const {
     bf16x4 va, vb;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const SwigluGrad g(a[e], b[e], u[e]);
-      va[e] = f2bf(g.a);
-      vb[e] = f2bf(g.b);
-      if (p.ht) p.ht[((row >> 5) * p.H + col + e) * 32 + (row & 31)] = some ? f2bf(g.h) : f2bf(0.0f);
+      va[e] = f2bf(some ? g.a : 0.0f);
+      vb[e] = f2bf(some ? g.b : 0.0f);
+      if (p.ht) p.ht[((row >> 5) * p.H + col + e) * 32 + (row & 31)] = f2bf(some ? g.h : 0.0f);
     }
-    if (!some) return;
     *(bf16x4*)(p.gz + ((int64_t)(col >> 5) * p.ldm + row) * 32 + (col & 31)) = va;
     *(bf16x4*)(p.gz + ((int64_t)((p.H + col) >> 5) * p.ldm + row) * 32 + (col & 31)) = vb;
   }
@@ -214,9 +215,53 @@ struct FfnDx : FfnProg<FM> {
   }
 };
 
+// Gradients of the weights, contracted over the tokens: W2 [H][D] from hT and G_y (the tokens of hT are padded with zeros, those of G_y
+// repeat the last), W1 [D][2H] from x and gz (gz is padded).  p.D is the output's columns, p.out the gradient.
+template <bool SECOND>
+struct FfnWgrad {
+  static constexpr int FM = 4;
+  const FfnArgs& p;
+  int K, slices, row_tiles, col_tiles;
+  int64_t rows;
+  using Rows = std::conditional_t<SECOND, FfnBlockedRows<128>, FfnTokenCols>;
+  using Weights = FfnTokenCols;
+  __device__ __forceinline__ explicit FfnWgrad(const FfnArgs& p_)
+      : p(p_), K((int)((p_.total + 31) & ~31ll)), slices(p_.slices), row_tiles((int)((p_.rows + 127) / 128)),
+        col_tiles((p_.D + kFfnCols - 1) / kFfnCols), rows(p_.rows) {}
+  __device__ __forceinline__ int n_org(int wn) const { return wn * 64; }
+  __device__ __forceinline__ void setup(int64_t row0, int rows_, int tn, Rows& A, Weights& W) const {
+    const int M = (int)p.total, y0 = tn * kFfnCols;
+    if constexpr (SECOND) {
+      A.init(p.ht, p.rows, row0, rows_, K);
+      W.init(p.x + y0, (uint32_t)p.ldx * 2, M, [&](int c) { return (uint32_t)min(c, p.D - 8 - y0) * 2; });
+    } else {
+      A.init(p.x + row0, (uint32_t)p.ldx * 2, M, [&](int c) { return (uint32_t)min(c, rows_ - 8) * 2; });
+      W.init(p.gz + (int64_t)(y0 >> 5) * p.ldm * 32, 64, K, [&](int c) {
+        const int col = min(c, p.D - 8 - y0);
+        return (uint32_t)(col >> 5) * (uint32_t)p.ldm * 64 + (col & 31) * 2;
+      });
+    }
+  }
+  __device__ __forceinline__ void epilogue(int64_t row0, int rows_, int tn, int slice, int wm, int wn, f32x4 (&acc)[4][FM]) const {
+    const int l = lane_id();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = tn * kFfnCols + wn * 64 + 16 * j + 4 * (l >> 4);
+      if (col >= p.D) continue;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = 16 * (wm * FM + i) + (l & 15);
+        if (r >= rows_) continue;
+        if (slices > 1) *(f32x4*)(p.part + (slice * rows + row0 + r) * p.D + col) = acc[j][i];
+        else *(bf16x4*)(p.out + (row0 + r) * p.D + col) = pack_bf16x4(acc[j][i], 1.0f);
+      }
+    }
+  }
+};
+
 template <class P, int STAGES>
 __global__ __launch_bounds__(kSpanThreads, 2) void ffn_tile_kernel(FfnArgs p) {
-  if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.ldm : 0;
+  if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.total : 0;
   run_ffn_tile<P, STAGES>(P(p));
 }
 // out = the sum of the slices, in their order; eight are asked for at once (one behind the other: 5.0 us for 16 slices of one token)
@@ -369,7 +414,7 @@ __device__ __forceinline__ void store_gradients(const FfnArgs& p, const TileCoor
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int q = 0; q < Stager::PASSES; ++q)
-        store16(gza + half * to_b + ((int64_t)q * p.ldm + 16 * i) * 32, off, 16 * i + stager.block_row() < rows && j0 + 32 * q < H, v[i & 1][half][q]);
+        store16(gza + half * to_b + ((int64_t)q * p.ldm + 16 * i) * 32, off, j0 + 32 * q < H, v[i & 1][half][q]);
   };
   bf16* const ht = p.ht + ((r0 >> 5) * H + j0) * 32;  // uniform
   const uint32_t hoff = (l & 15) * 64 + (l >> 4) * 16;
@@ -392,7 +437,7 @@ __device__ __forceinline__ void store_gradients(const FfnArgs& p, const TileCoor
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const SwigluGrad g(a[e], b[e], u[e]);
-        va[e] = g.a, vb[e] = g.b, vh[e] = some ? g.h : 0.0f;
+        va[e] = some ? g.a : 0.0f, vb[e] = some ? g.b : 0.0f, vh[e] = some ? g.h : 0.0f;
       }
       stager.put(0, f, pack_bf16x4(va[0], va[1], va[2], va[3]));
       stager.put(1, f, pack_bf16x4(vb[0], vb[1], vb[2], vb[3]));
@@ -564,7 +609,7 @@ struct DxDenseSpan : DenseSpan {
 template <class P>
 __global__ __launch_bounds__(kSpanThreads, 1) void ffn_span_kernel(FfnArgs p, int nb) {
   const ClockTrace trace(p.clk);
-  if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.ldm : 0;
+  if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.total : 0;
   run_span_tiles_of<P>(p, DenseSpanSched((int)p.rows, nb));
   trace.finish();
 }
@@ -601,6 +646,41 @@ int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
     return MOMOE_ERR_UNSUPPORTED;
   return MOMOE_OK;
 }
+// tokens are addressed at 32-bit offsets
+int check_wgrad(int64_t rows, int64_t ldm, int64_t D, int64_t H, int64_t ld) {
+  const int st = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
+  if (st != MOMOE_OK) return st;
+  return ld % 8 != 0 || rows * ld * 2 >= (1ll << 32) || 8 * ldm * 64 >= (1ll << 32) ? MOMOE_ERR_UNSUPPORTED : MOMOE_OK;
+}
+// Gradients of the weights in tiles of 128 x 128 as long as no CU has more than two of them and none contracts over more than 8192 tokens; where
+// the tiles are fewer, the tokens are cut, into slices of at least 512, and past 10 MB of sums of at least 2048.  Us, W2 and W1, momoe_wgrad |
+// these: 31 tokens, 64 x 96 6.9, 7.1 | 4.1, 4.3; 512, 512 x 512 17.8, 18.5 | 8.7, 9.2; 1000, 1024 x 2816 28.3, 30.8 | 16.6, 23.2; 4096, 512 x 512
+// 87.5, 95.6 | 15.8, 19.1; 8192, 1024 x 2816 79.7, 164 | 69.2, 118; 65536, 1024 x 2816 476, 751 | 952, 933; more tiles than two a CU: 300, 2048 x 5632
+// 17.1, 32.6 | 18.1, 31.4; 2048, 2048 x 8192 56.7, 116 | 84.8, 159.
+int wgrad_slices(int64_t rows, int64_t X, int64_t Y) {
+  const int64_t tiles = cdiv64(X, kFfnCols) * cdiv64(Y, kFfnCols), room = 2 * persistent_grid();
+  return (int)std::max<int64_t>(1, std::min({room / tiles, cdiv64(rows, kSpan) / 8, std::max((10 << 20) / (X * Y * 4), rows / 2048), (int64_t)16}));
+}
+bool wgrad_in_small_tiles(int64_t rows, int64_t X, int64_t Y) {
+  return cdiv64(X, kFfnCols) * cdiv64(Y, kFfnCols) <= 2 * persistent_grid() && rows <= 8192 * (int64_t)wgrad_slices(rows, X, Y);
+}
+// An expert of all rows is cut along them, through the workspace, where its tiles leave CUs idle in their last round; tiles that fill 5 of 6
+// are done whole, which saves the partial sums' way through memory.  Us, 8192 tokens, D = 2048, H = 8192 (256 and 512 tiles of 256 x 256), cut |
+// whole: W2 335 | 256, W1 640 | 470.
+int64_t large_wgrad_bytes(int64_t rows, int64_t X, int64_t Y) {
+  const int64_t bytes = momoe_wgrad_workspace_bytes(1, X, Y, rows);
+  if (bytes <= 0) return bytes;
+  const int64_t tiles = cdiv64(X, 256) * cdiv64(Y, 256), grid = persistent_grid(), rounds = cdiv64(tiles, grid);
+  return 6 * tiles >= 5 * rounds * grid ? 0 : bytes;
+}
+template <bool SECOND>
+int launch_wgrad(FfnArgs a, int64_t tokens, void* out, void* workspace, hipStream_t st) {
+  a.total = tokens;
+  a.out = (bf16*)out;
+  a.part = (float*)workspace;
+  a.slices = wgrad_slices(tokens, a.rows, a.D);
+  return launch_tiles<FfnWgrad<SECOND>, 2>(a, cdiv64(a.D, kFfnCols), st);
+}
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 bool any_unaligned(std::initializer_list<const void*> all) { return std::any_of(all.begin(), all.end(), unaligned16); }
 
@@ -613,14 +693,39 @@ extern "C" int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols) {
   return rows < 0 || cols <= 0 || cols % 16 != 0 ? -1 : (rows + 15) / 16 * 16 * cols;
 }
 
-// An expert of all rows is cut along them, through the workspace, where its tiles leave CUs idle in their last round; tiles that fill 5 of 6
-// are done whole, which saves the partial sums' way through memory.  Us, 8192 tokens, D = 2048, H = 8192 (256 and 512 tiles of 256 x 256), cut |
-// whole: W2 335 | 256, W1 640 | 470.
 extern "C" int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y) {
-  const int64_t bytes = momoe_wgrad_workspace_bytes(1, X, Y, rows);
-  if (bytes <= 0) return bytes;
-  const int64_t tiles = cdiv64(X, 256) * cdiv64(Y, 256), grid = persistent_grid(), rounds = cdiv64(tiles, grid);
-  return 6 * tiles >= 5 * rounds * grid ? 0 : bytes;
+  if (rows <= 0 || X <= 0 || Y <= 0) return -1;
+  if (!wgrad_in_small_tiles(rows, X, Y)) return large_wgrad_bytes(rows, X, Y);
+  const int64_t slices = wgrad_slices(rows, X, Y);
+  return slices > 1 ? slices * X * Y * 4 : 0;
+}
+
+extern "C" int momoe_ffn_wgrad_w2(const void* hT, const void* Gy, int64_t ldgy, const int32_t* counts2, void* GW2_HD, void* workspace,
+                                  int64_t workspace_bytes, int64_t rows, int64_t D, int64_t H, void* stream) {
+  if (!hT || !Gy || !counts2 || !GW2_HD || ldgy < D || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
+  const int st = check_wgrad(rows, (rows + 31) / 32 * 32, D, H, ldgy);
+  if (st != MOMOE_OK) return st;
+  if (any_unaligned({hT, Gy, GW2_HD, workspace}) || workspace_bytes < momoe_ffn_wgrad_workspace_bytes(rows, H, D)) return MOMOE_ERR_BAD_ARG;
+  if (!wgrad_in_small_tiles(rows, H, D))
+    return momoe_wgrad(hT, H, MOMOE_LAYOUT_TRANSPOSED, nullptr, Gy, ldgy, MOMOE_LAYOUT_ROWS, nullptr, counts2, GW2_HD, rows, 1, H, D, rows,
+                       workspace, workspace_bytes, stream);
+  FfnArgs a{(const bf16*)Gy, ldgy, nullptr, H, rows, (int)D, (int)H};
+  a.ht = (bf16*)const_cast<void*>(hT);
+  return launch_wgrad<true>(a, rows, GW2_HD, workspace, (hipStream_t)stream);
+}
+
+extern "C" int momoe_ffn_wgrad_w1(const void* x, int64_t ldx, const void* gz_blocked, const int32_t* counts2, void* GW1_D2H, void* workspace,
+                                  int64_t workspace_bytes, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
+  if (!x || !gz_blocked || !counts2 || !GW1_D2H || ldx < D || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
+  const int st = check_wgrad(rows, ldm, D, H, ldx);
+  if (st != MOMOE_OK) return st;
+  if (any_unaligned({x, gz_blocked, GW1_D2H, workspace}) || workspace_bytes < momoe_ffn_wgrad_workspace_bytes(rows, D, 2 * H)) return MOMOE_ERR_BAD_ARG;
+  if (!wgrad_in_small_tiles(rows, D, 2 * H))
+    return momoe_wgrad(x, ldx, MOMOE_LAYOUT_ROWS, nullptr, gz_blocked, ldm, MOMOE_LAYOUT_KBLOCKED, nullptr, counts2, GW1_D2H, rows, 1, D,
+                       2 * H, rows, workspace, workspace_bytes, stream);
+  FfnArgs a{(const bf16*)x, ldx, nullptr, D, ldm, (int)(2 * H), (int)H};
+  a.gz = (bf16*)const_cast<void*>(gz_blocked);
+  return launch_wgrad<false>(a, rows, GW1_D2H, workspace, (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
@@ -666,9 +771,9 @@ extern "C" int momoe_ffn_dgrad_h(const void* Gy, int64_t ldgy, const void* W2_HD
 }
 
 extern "C" int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D2H, const float* u, void* gz_blocked, void* hT, int32_t* counts2,
-                                    int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
-  if (!x || !W1_D2H || !u || !gz_blocked || ldx < D) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, ldm, D, H);
+                                    int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
+  if (!x || !W1_D2H || !u || !gz_blocked || ldx < D || tokens < rows) return MOMOE_ERR_BAD_ARG;
+  const int st = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
   if (st != MOMOE_OK) return st;
   if (any_unaligned({x, W1_D2H, u, gz_blocked, hT})) return MOMOE_ERR_BAD_ARG;
   if (ldx % 8 != 0 || ldx >= (1 << 22)) return MOMOE_ERR_UNSUPPORTED;
@@ -677,13 +782,14 @@ extern "C" int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D
   a.gz = (bf16*)gz_blocked;
   a.ht = (bf16*)hT;
   a.counts = counts2;
+  a.total = tokens;
   return launch<Lin1DenseSpan<true>, Lin1Bwd>(a, 2 * H, D, cdiv64(H, 64), (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void* W2_HD, const float* ab, void* gz_blocked, void* hT,
-                                       int32_t* counts2, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
-  if (!Gy || !W2_HD || !ab || !gz_blocked || ldgy < D) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, ldm, D, H);
+                                       int32_t* counts2, int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
+  if (!Gy || !W2_HD || !ab || !gz_blocked || ldgy < D || tokens < rows) return MOMOE_ERR_BAD_ARG;
+  const int st = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
   if (st != MOMOE_OK) return st;
   if (any_unaligned({Gy, W2_HD, ab, gz_blocked, hT})) return MOMOE_ERR_BAD_ARG;
   if (ldgy % 8 != 0 || ldgy >= (1 << 22)) return MOMOE_ERR_UNSUPPORTED;
@@ -692,16 +798,17 @@ extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void*
   a.gz = (bf16*)gz_blocked;
   a.ht = (bf16*)hT;
   a.counts = counts2;
+  a.total = tokens;
   return launch<DhDenseSpan<true>, DhSaved>(a, H, D, cdiv64(H, kFfnCols), (hipStream_t)stream);
 }
 
-extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, int64_t rows, int64_t D, int64_t H,
-                                 void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, void* workspace, int64_t workspace_bytes,
+                                 int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
   if (!gz_blocked || !W1_D2H || !Gx || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, rows, D, H);
+  const int st = check_ffn(rows, ldm, D, H);
   if (st != MOMOE_OK) return st;
   if (any_unaligned({gz_blocked, W1_D2H, Gx, workspace}) || workspace_bytes < slices_bytes(rows, D, 2 * H)) return MOMOE_ERR_BAD_ARG;
-  FfnArgs a{nullptr, 0, (const bf16*)W1_D2H, rows, rows, (int)D, (int)H};
+  FfnArgs a{nullptr, 0, (const bf16*)W1_D2H, rows, ldm, (int)D, (int)H};
   a.gz = (bf16*)const_cast<void*>(gz_blocked);
   a.out = (bf16*)Gx;
   a.part = (float*)workspace;

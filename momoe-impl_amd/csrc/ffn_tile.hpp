@@ -104,6 +104,31 @@ struct FfnCols {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
+// Columns of a matrix whose rows are the contraction (tokens), for either side: token t of column c at t * pitch + lane_bytes(c) bytes from
+// base; tokens past the last one repeat it.  LDS and fragments as FfnCols.
+struct FfnTokenCols : FfnCols<false> {
+  using L = FfnCols<false>;
+  uint32_t last;
+  int krow;
+  template <class LaneBytes>
+  __device__ __forceinline__ void init(const void* base_, uint32_t pitch_bytes, int tokens, LaneBytes lane_bytes) {
+    base = (const bf16*)base_;
+    pitch = pitch_bytes;
+    last = tokens - 1;
+    const int l = fresh_lane();
+    krow = wave_id() * RPD + l / PIECES;
+    off = lane_bytes(((l % PIECES) ^ swz(krow)) * 8);
+  }
+  struct Source {
+    const bf16* base;
+    int k;
+  };
+  __device__ __forceinline__ Source source(int k) const { return {base, k}; }
+  template <int j>
+  __device__ __forceinline__ void deposit(const Source& src, uint32_t slot) const {
+    dma16_at<j * kSpanWaves * 1024>(src.base, off + min((uint32_t)(src.k + STEP * j + krow), last) * pitch, slot);
+  }
+};
 // rows at a fixed pitch (k-contiguous weights): a multiple of 32 of them, the last 32 repeated where the tile sticks out
 struct FfnWeightRows : SpanPitchedRows<kFfnCols> {
   using Base = SpanPitchedRows<kFfnCols>;
@@ -158,7 +183,8 @@ __device__ __forceinline__ void run_ffn_tile(const P& prog) {
   int k = first * kSpan, put = 0, got = 0;
   if (first == all.count - 1) k = max(0, min(k, all.kmax));
   auto request = [&] {
-    const bf16 *asrc = A.source(k), *wsrc = W.source(k);
+    const auto asrc = A.source(k);
+    const auto wsrc = W.source(k);
     const uint32_t to = addr + (uint32_t)put * (STAGE * 2);
     unrolled<0, Rows::DEP>([&](auto D) { A.template deposit<decltype(D)::value>(asrc, to); });
     unrolled<0, Weights::DEP>([&](auto D) { W.template deposit<decltype(D)::value>(wsrc, to + Rows::ELEMS * 2); });

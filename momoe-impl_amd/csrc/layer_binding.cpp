@@ -622,12 +622,12 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
     }
     const Tensor Gy = rows_in_bf16(grads[0], M, D, dev);
     const int64_t ldx = pitch_of_rows(x), ldgy = pitch_of_rows(Gy);
-    const int64_t rest = M - msave, gz_bytes = 4 * H * M, ht_bytes = need_w2 ? momoe_padded_rows(M, 1) * H * 2 : 0;
+    const int64_t rest = M - msave, ldm = (M + 31) / 32 * 32, gz_bytes = 4 * H * ldm, ht_bytes = need_w2 ? momoe_padded_rows(M, 1) * H * 2 : 0;
     const int64_t u_bytes = rest > 0 ? momoe_ffn_fragment_floats(rest, H) * 4 : 0;
     const int64_t ws1_bytes = need_w1 ? momoe_ffn_wgrad_workspace_bytes(M, D, 2 * H) : 0;
     const int64_t ws2_bytes = need_w2 ? momoe_ffn_wgrad_workspace_bytes(M, H, D) : 0;
     const int64_t wsx_bytes = need_x ? momoe_ffn_workspace_bytes(M, D, 2 * H) : 0;
-    Transients transients(dev, {16, gz_bytes, ht_bytes, u_bytes, ws1_bytes, ws2_bytes, wsx_bytes});
+    Transients transients(dev, {16, gz_bytes, ht_bytes, u_bytes, ws2_bytes, ws1_bytes, wsx_bytes});
     Tensor counts_own, gz_own, ht_own, u_own, ws1_own, ws2_own, wsx_own;
     const auto scratch = [&](int64_t bytes, Tensor& own) { return bytes > 0 ? transients.take(bytes, own) : nullptr; };
     int32_t* const counts = (int32_t*)transients.take(16, counts_own);
@@ -637,26 +637,26 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
     const auto behind = [&](const void* p, int64_t pitch) { return p ? (void*)((char*)p + msave * pitch * 2) : nullptr; };
     if (msave > 0)
       MOMOE_CALL(momoe_ffn_dgrad_h_saved, st, Gy.data_ptr(), ldgy, W2.data_ptr(), (const float*)saved[3].data_ptr<float>(), gz, ht, counts,
-                 msave, M, D, H);
+                 M, msave, ldm, D, H);
     if (rest > 0) {
       float* const u = (float*)transients.take(u_bytes, u_own);
       MOMOE_CALL(momoe_ffn_dgrad_h, st, behind(Gy.data_ptr(), ldgy), ldgy, W2.data_ptr(), u, rest, D, H);
       MOMOE_CALL(momoe_ffn_swiglu_bwd, st, behind(x.data_ptr(), ldx), ldx, W1.data_ptr(), (const float*)u, behind(gz, 32), behind(ht, H), counts,
-                 rest, M, D, H);
+                 M, rest, ldm, D, H);
       u_own.reset();
     }
-    const auto weight_gradient = [&](const void* A, int64_t lda, int a_layout, const void* B, int64_t ldb, int b_layout, const Tensor& G,
-                                     int64_t ws_bytes, Tensor& own) {
-      MOMOE_CALL(momoe_wgrad, st, A, lda, a_layout, (const int32_t*)nullptr, B, ldb, b_layout, (const int32_t*)nullptr, (const int32_t*)counts,
-                 G.data_ptr(), M, (int64_t)1, G.size(0), G.size(1), M, scratch(ws_bytes, own), ws_bytes);
-      own.reset();
-    };
-    if (need_w2) weight_gradient(ht, H, MOMOE_LAYOUT_TRANSPOSED, Gy.data_ptr(), ldgy, MOMOE_LAYOUT_ROWS, out[2], ws2_bytes, ws2_own);
+    if (need_w2)
+      MOMOE_CALL(momoe_ffn_wgrad_w2, st, (const void*)ht, Gy.data_ptr(), ldgy, (const int32_t*)counts, out[2].data_ptr(),
+                 scratch(ws2_bytes, ws2_own), ws2_bytes, M, D, H);
+    ws2_own.reset();
     ht_own.reset();
-    if (need_w1) weight_gradient(x.data_ptr(), ldx, MOMOE_LAYOUT_ROWS, gz, M, MOMOE_LAYOUT_KBLOCKED, out[1], ws1_bytes, ws1_own);
+    if (need_w1)
+      MOMOE_CALL(momoe_ffn_wgrad_w1, st, x.data_ptr(), ldx, (const void*)gz, (const int32_t*)counts, out[1].data_ptr(),
+                 scratch(ws1_bytes, ws1_own), ws1_bytes, M, ldm, D, H);
+    ws1_own.reset();
     if (need_x) {
       const Tensor Gx = empty_bf16({M, D}, dev);
-      MOMOE_CALL(momoe_ffn_dgrad_x, st, (const void*)gz, W1.data_ptr(), Gx.data_ptr(), M, D, H, scratch(wsx_bytes, wsx_own), wsx_bytes);
+      MOMOE_CALL(momoe_ffn_dgrad_x, st, (const void*)gz, W1.data_ptr(), Gx.data_ptr(), scratch(wsx_bytes, wsx_own), wsx_bytes, M, ldm, D, H);
       out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
     }
     return out;
@@ -679,7 +679,7 @@ Tensor feed_forward(const Tensor& x, const Tensor& W1, const Tensor& W2, double 
   const int64_t M = x.numel() / D;
   if (!wants_autograd({&x, &W1, &W2})) return feed_forward_forward(x, W1, W2, 0).y;
   // the gradients of the weights address tokens at 32-bit offsets (momoe_wgrad): say so now rather than in the backward
-  TORCH_CHECK(!(W1.requires_grad() || W2.requires_grad()) || (M * D * 2 < (1ll << 32) && 8 * M * 64 < (1ll << 32)),
+  TORCH_CHECK(!(W1.requires_grad() || W2.requires_grad()) || ((M + 31) * D * 2 < (1ll << 32) && 8 * (M + 31) * 64 < (1ll << 32)),
               "FeedForward backward supports batches of less than 4 GiB and 8388608 tokens per call, got ", M, " tokens: split the batch");
   const int64_t part = (int64_t)((double)M * save_percent / 100.0), msave = part == M ? M : part / 32 * 32;
   return FeedForwardFn::apply(x, W1, W2, msave)[0];

@@ -22,7 +22,7 @@ def _refuses(fn, good, pointers, aligned, optional=()):
 
 
 def test_refusals_of_the_entry_points():
-    sizes = dict(rows=40, ldm=40, D=64, H=32)
+    sizes, padded = dict(rows=40, ldm=40, D=64, H=32), dict(rows=40, ldm=64, D=64, H=32)
     c = _refuses(lib.momoe_ffn_lin1_fwd, dict(x=P, ldx=64, W=P, h=P, ab=None, ab_rows=0, **sizes), ("x", "W", "h"), ("x", "W", "h"))
     assert c(ldx=56) == c(ldm=39) == c(ab_rows=32) == c(ab=P, ab_rows=-32) == c(ab=P, ab_rows=96) == c(ab=P + 4, ab_rows=32) == 1
     assert c(ldx=68) == c(ab=P, ab_rows=40) == c(ldx=1 << 22) == 2
@@ -34,12 +34,21 @@ def test_refusals_of_the_entry_points():
     assert lib.momoe_ffn_workspace_bytes(0, 64, 64) == lib.momoe_ffn_workspace_bytes(1, 0, 64) == lib.momoe_ffn_workspace_bytes(1, 64, 0) == -1
     c = _refuses(lib.momoe_ffn_dgrad_h, dict(Gy=P, ldgy=64, W=P, u=P, rows=40, D=64, H=32), ("Gy", "W", "u"), ("Gy", "W", "u"))
     assert c(ldgy=56) == 1 and c(ldgy=68) == 2
-    c = _refuses(lib.momoe_ffn_swiglu_bwd, dict(x=P, ldx=64, W=P, u=P, gz=P, hT=None, counts=None, **sizes), ("x", "W", "u", "gz"), ("x", "W", "u", "gz", "hT"))
-    assert c(ldx=56) == c(ldm=39) == 1 and c(ldx=68) == 2
-    c = _refuses(lib.momoe_ffn_dgrad_h_saved, dict(Gy=P, ldgy=64, W=P, ab=P, gz=P, hT=None, counts=None, **sizes), ("Gy", "W", "ab", "gz"), ("Gy", "W", "ab", "gz", "hT"))
-    assert c(ldgy=56) == c(ldm=39) == 1 and c(ldgy=68) == 2
-    c = _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, rows=40, D=64, H=32, **room), ("gz", "W", "Gx", "ws"), ("gz", "W", "Gx", "ws"))
-    assert c(bytes=-1) == c(rows=1, D=2048, H=8192, ws=None, bytes=0) == 1
+    c = _refuses(lib.momoe_ffn_swiglu_bwd, dict(x=P, ldx=64, W=P, u=P, gz=P, hT=None, counts=None, tokens=40, **padded), ("x", "W", "u", "gz"), ("x", "W", "u", "gz", "hT"))
+    assert c(ldx=56) == c(ldm=63) == c(tokens=39) == 1 and c(ldx=68) == 2
+    c = _refuses(lib.momoe_ffn_dgrad_h_saved, dict(Gy=P, ldgy=64, W=P, ab=P, gz=P, hT=None, counts=None, tokens=40, **padded), ("Gy", "W", "ab", "gz"), ("Gy", "W", "ab", "gz", "hT"))
+    assert c(ldgy=56) == c(ldm=63) == c(tokens=39) == 1 and c(ldgy=68) == 2
+    c = _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, **room, **sizes), ("gz", "W", "Gx", "ws"), ("gz", "W", "Gx", "ws"))
+    assert c(ldm=39) == c(bytes=-1) == c(rows=1, D=2048, H=8192, ws=None, bytes=0) == 1
+    wgrad = dict(rows=40, D=64, H=32)
+    assert all(lib.momoe_ffn_wgrad_workspace_bytes(*n) == -1 for n in ((0, 64, 64), (64, 0, 64), (64, 64, 0)))
+    need = lib.momoe_ffn_wgrad_workspace_bytes(1024, 512, 1024)
+    c = _refuses(lib.momoe_ffn_wgrad_w2, dict(hT=P, Gy=P, ldgy=64, counts=P, G=P, **room, **wgrad), ("hT", "Gy", "counts", "G", "ws"), ("hT", "Gy", "G", "ws"))
+    assert need > 0 and c(ldgy=56) == c(bytes=-1) == c(rows=1024, D=1024, H=512, ldgy=1024, bytes=need - 4) == 1
+    assert c(ldgy=68) == c(rows=1 << 20, ldgy=2048) == c(rows=1 << 23) == 2
+    c = _refuses(lib.momoe_ffn_wgrad_w1, dict(x=P, ldx=64, gz=P, counts=P, G=P, **room, rows=40, ldm=64, D=64, H=32), ("x", "gz", "counts", "G", "ws"), ("x", "gz", "G", "ws"))
+    assert c(ldx=56) == c(ldm=63) == c(bytes=-1) == c(rows=1024, ldm=1024, D=512, H=512, ldx=512, bytes=need - 4) == 1
+    assert c(ldx=68) == c(rows=1 << 20, ldm=1 << 20, ldx=2048) == c(ldm=1 << 23) == 2
 
 
 def test_module_refusals():

@@ -71,6 +71,8 @@ SIZES = [
     (130, 224, 160), (257, 416, 352), (300, 640, 96), (513, 128, 1056), (700, 1056, 128), (1025, 320, 576), (2000, 96, 32), (5000, 64, 160),
     # large launches: of x W1 and G_y W2^T, of h W2 and gz W1^T; contractions of an odd number of 32
     (8200, 160, 1056), (8200, 1056, 160), (17000, 128, 544),
+    # gradients of W1 or of both weights that are large launches
+    (40, 1056, 4256), (35, 2080, 4224),
 ]
 
 
