@@ -73,6 +73,9 @@ DENSE = [
     (1, 32, 32, 32, True), (1, 32, 32, 128, False), (1, 2080, 64, 128, True), (2, 64, 2080, 64, True), (7, 96, 160, 64, True), (16, 128, 128, 128, False),
     (17, 288, 96, 32, True), (32, 160, 416, 128, True), (33, 288, 1056, 64, False), (64, 1056, 288, 32, True), (65, 128, 64, 128, True),
     (131, 96, 2208, 32, False), (200, 640, 352, 64, True), (300, 2080, 96, 128, True), (517, 64, 640, 128, False), (1000, 160, 160, 32, True),
+    # tiles of 64 rows, contractions cut into slices and whole: their ends in rows and columns, half a block of 128 left over
+    (300, 1056, 160, 32, True), (270, 416, 416, 128, False), (33, 2080, 1408, 64, True), (70, 1408, 2080, 32, False), (129, 2208, 1312, 128, True),
+    (400, 352, 352, 64, True), (1000, 288, 160, 128, True), (2100, 160, 160, 32, False), (5000, 96, 96, 64, True), (12000, 64, 64, 128, True),
 ]
 
 
@@ -92,6 +95,8 @@ EXPERTS = [
     (1, 32, 32, 2, 1, 0, 0, 32), (1, 256, 128, 8, 8, 0, 0, 128), (7, 96, 160, 4, 2, 0, 0, 64), (50, 288, 416, 5, 2, 1, 0, 128),
     (33, 2208, 64, 3, 1, 0, 0, 64), (64, 64, 2208, 2, 2, 1, 0, 32), (200, 128, 128, 16, 2, 0, 1.5, 128), (300, 96, 64, 4, 2, 0, 0, 32),
     (517, 288, 160, 5, 2, 1, 0, 64), (700, 128, 416, 4, 3, 1, 2.0, 128), (90, 1056, 352, 40, 4, 0, 0, 128), (300, 128, 96, 40, 2, 0, 2.0, 64),
+    # tiles of 64 rows, few of them in an expert and many
+    (300, 288, 416, 5, 2, 1, 2.0, 64), (100, 1056, 352, 8, 2, 0, 0, 32), (330, 2080, 96, 3, 1, 0, 1.0, 128), (3000, 160, 96, 3, 1, 0, 0, 32),
 ]
 
 
@@ -126,7 +131,7 @@ def test_weights_come_back(D, H, group):
             assert a.dtype == b.dtype and torch.equal(a.cpu(), b) and torch.equal(c.cpu(), b[1])
 
 
-@pytest.mark.parametrize("M", [1, 40, 200])
+@pytest.mark.parametrize("M", [1, 40, 200, 8000])
 def test_strides_types_and_places_of_x(M):
     D, H, group = 96, 64, 32
     w = _weights((), D, H, group)
@@ -162,7 +167,7 @@ def test_tokens_of_nan_and_infinity_stay_with_themselves(M):
         assert y[0, [3, 17, M - 1]].isnan().all() and (y[0, 20] == 0).all() and torch.equal(y[0, keep], ref[0, keep])
 
 
-@pytest.mark.parametrize("M", [40, 600])
+@pytest.mark.parametrize("M", [40, 600, 8000])
 def test_routing_that_is_not_k_of_n(M, monkeypatch):
     """Too few experts: what is missing is absent.  Too many: zeros.  CHECK_ROUTING raises for both."""
     D, H, N, K, group = 96, 64, 4, 2, 32
@@ -183,7 +188,7 @@ def test_routing_that_is_not_k_of_n(M, monkeypatch):
             layer(x, m.to(DEV), s.to(DEV))
 
 
-@pytest.mark.parametrize("M", [3, 150])
+@pytest.mark.parametrize("M", [3, 150, 500])
 def test_streams_and_replayed_graphs(M):
     """Two calls at once on streams of their own, and a graph of both replayed on other inputs between eager calls."""
     D, H, N, K, group = 288, 416, 8, 2, 64
