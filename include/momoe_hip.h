@@ -527,14 +527,15 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * momoe_ffn_dgrad_h: u.  momoe_ffn_swiglu_bwd: gz and hT, a | b made again from x.
  * momoe_ffn_dgrad_h_saved: gz and hT from the a | b that were kept, u on the way.
  * Both write {0, tokens}, the rows of all launches, to counts2 (may be NULL), which the gradients of the weights take.
- * momoe_ffn_dgrad_x: Gx [rows][D].  momoe_ffn_wgrad_w2, momoe_ffn_wgrad_w1: GW2 [H][D], GW1 [D][2H], over `rows` tokens, all of them; fewer than
- * 4 GiB of x and Gy each (rows * pitch * 2), ldm below 8388608.
- * momoe_ffn_lin2_fwd (contraction H) and momoe_ffn_dgrad_x (2H) take scratch of at least momoe_ffn_workspace_bytes(rows, D, contraction), the
- * gradients of the weights of momoe_ffn_wgrad_workspace_bytes(rows, H, D or D, 2H); 0 (NULL): none is needed.
+ * momoe_ffn_gradients: Gx [rows][D], GW1 [D][2H] and GW2 [H][D], over `rows` tokens, all of them; NULL: is not wanted, and what only it needs
+ * (W1 for Gx; x for GW1; hT and Gy for GW2; counts2 for either) is not read and may be NULL.  For gradients of the weights fewer than 4 GiB of x
+ * and Gy each (rows * pitch * 2) and ldm below 8388608.
+ * momoe_ffn_lin2_fwd takes scratch of at least momoe_ffn_workspace_bytes(rows, D, H), momoe_ffn_gradients of
+ * momoe_ffn_gradients_workspace_bytes(rows, D, H, which are wanted); 0 (NULL): none is needed.
  */
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
 int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction);
-int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y);
+int64_t momoe_ffn_gradients_workspace_bytes(int64_t rows, int64_t D, int64_t H, int wants_x, int wants_W1, int wants_W2);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);
 int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* workspace,
@@ -544,12 +545,9 @@ int momoe_ffn_swiglu_bwd(const void* x, int64_t ldx, const void* W1_D2H, const f
                          int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
 int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void* W2_HD, const float* ab, void* gz_blocked, void* hT, int32_t* counts2,
                             int64_t tokens, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
-int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, void* workspace, int64_t workspace_bytes, int64_t rows,
-                      int64_t ldm, int64_t D, int64_t H, void* stream);
-int momoe_ffn_wgrad_w2(const void* hT, const void* Gy, int64_t ldgy, const int32_t* counts2, void* GW2_HD, void* workspace,
-                       int64_t workspace_bytes, int64_t rows, int64_t D, int64_t H, void* stream);
-int momoe_ffn_wgrad_w1(const void* x, int64_t ldx, const void* gz_blocked, const int32_t* counts2, void* GW1_D2H, void* workspace,
-                       int64_t workspace_bytes, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream);
+int momoe_ffn_gradients(const void* x, int64_t ldx, const void* Gy, int64_t ldgy, const void* gz_blocked, const void* hT, const void* W1_D2H,
+                        const int32_t* counts2, void* Gx, void* GW1_D2H, void* GW2_HD, void* workspace, int64_t workspace_bytes, int64_t rows,
+                        int64_t ldm, int64_t D, int64_t H, void* stream);
 
 /* ---- SwiGLU blocks with weights in 4 bits, forward only -------------------------------
  * No counterpart in the reference, whose weights are bf16.  A weight is (code - zero) * scale: a 4-bit code, and for each `group`

@@ -262,24 +262,48 @@ struct FfnWgrad {
 template <class P, int STAGES>
 __global__ __launch_bounds__(kSpanThreads, 2) void ffn_tile_kernel(FfnArgs p) {
   if (p.counts && blockIdx.x == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = threadIdx.x ? (int)p.total : 0;
-  run_ffn_tile<P, STAGES>(P(p));
+  run_ffn_tile<P, STAGES>(P(p), blockIdx.x);
 }
-// out = the sum of the slices, in their order; eight are asked for at once (one behind the other: 5.0 us for 16 slices of one token)
-__global__ __launch_bounds__(256) void ffn_sum_slices_kernel(FfnArgs p) {
-  const int64_t n = p.rows * p.D, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// Sums of slices, in their order, of the products of a launch; eight are asked for at once (one behind the other: 5.0 us for 16 slices of
+// one token)
+struct FfnSums {
+  const float* part[3];
+  bf16* out[3];
+  int64_t n[3];
+  int slices[3], count = 0;
+  void add(const FfnArgs& a) {
+    if (a.slices == 1) return;
+    part[count] = a.part, out[count] = a.out, n[count] = a.rows * a.D, slices[count++] = a.slices;
+  }
+};
+__global__ __launch_bounds__(256) void ffn_sum_slices_kernel(FfnSums p) {
+  const int64_t n = p.n[blockIdx.y], at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= n) return;
+  const float* const part = p.part[blockIdx.y];
+  const int slices = p.slices[blockIdx.y];
   f32x4 sum = {};
-  for (int s = 0; s < p.slices; s += 8) {
+  for (int s = 0; s < slices; s += 8) {
     f32x4 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *(const f32x4*)(p.part + min(s + j, p.slices - 1) * n + at);
+    for (int j = 0; j < 8; ++j) v[j] = *(const f32x4*)(part + min(s + j, slices - 1) * n + at);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (s + j < p.slices) sum += v[j];
+      if (s + j < slices) sum += v[j];
   }
-  *(bf16x4*)(p.out + at) = pack_bf16x4(sum, 1.0f);
+  *(bf16x4*)(p.out[blockIdx.y] + at) = pack_bf16x4(sum, 1.0f);
+}
+int sum_slices(const FfnSums& sums, hipStream_t st) {
+  if (sums.count > 0) {
+    const int64_t most = *std::max_element(sums.n, sums.n + sums.count);
+    ffn_sum_slices_kernel<<<dim3((unsigned)cdiv64(most, 1024), (unsigned)sums.count), 256, 0, st>>>(sums);
+  }
+  return launch_status();
 }
 
+template <class P>
+int64_t blocks_of(const FfnArgs& a) {
+  return cdiv64(cdiv64(a.rows, 32 * P::FM) * cdiv64(a.D, kFfnCols) * a.slices, 8) * 8;
+}
 template <class P, int STAGES>
 int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   static LdsLimit lds;
@@ -287,8 +311,32 @@ int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   if (tiles >= (1ll << 31) - 8) return MOMOE_ERR_UNSUPPORTED;
   if (!allow_lds(ffn_tile_kernel<P, STAGES>, kFfnLds<P, STAGES>, lds)) return MOMOE_ERR_LAUNCH;
   ffn_tile_kernel<P, STAGES><<<(unsigned)(cdiv64(tiles, 8) * 8), kSpanThreads, kFfnLds<P, STAGES>, st>>>(a);
-  if (a.slices > 1) ffn_sum_slices_kernel<<<(unsigned)cdiv64(a.rows * a.D, 1024), 256, 0, st>>>(a);
-  return launch_status();
+  FfnSums sums;
+  sums.add(a);
+  return sum_slices(sums, st);
+}
+// The three products that need gz or hT and no more, in one launch; x, w1, w2: null, or what is wanted
+template <class Dx, int STAGES>
+__global__ __launch_bounds__(kSpanThreads, 2) void ffn_gradients_kernel(FfnArgs x, FfnArgs w1, FfnArgs w2, int x_blocks, int w1_blocks) {
+  const int block = blockIdx.x;
+  if (block < x_blocks) run_ffn_tile<Dx, STAGES>(Dx(x), block);
+  else if (block < x_blocks + w1_blocks) run_ffn_tile<FfnWgrad<false>, 2>(FfnWgrad<false>(w1), block - x_blocks);
+  else run_ffn_tile<FfnWgrad<true>, 2>(FfnWgrad<true>(w2), block - x_blocks - w1_blocks);
+}
+template <class Dx, int STAGES>
+int launch_gradients(const FfnArgs* x, const FfnArgs* w1, const FfnArgs* w2, hipStream_t st) {
+  static LdsLimit lds;
+  constexpr size_t bytes = std::max(kFfnLds<Dx, STAGES>, std::max(kFfnLds<FfnWgrad<false>, 2>, kFfnLds<FfnWgrad<true>, 2>));
+  const int64_t bx = x ? blocks_of<Dx>(*x) : 0, b1 = w1 ? blocks_of<FfnWgrad<false>>(*w1) : 0, b2 = w2 ? blocks_of<FfnWgrad<true>>(*w2) : 0;
+  if (bx + b1 + b2 == 0) return MOMOE_OK;
+  if (bx + b1 + b2 >= (1ll << 31)) return MOMOE_ERR_UNSUPPORTED;
+  if (!allow_lds(ffn_gradients_kernel<Dx, STAGES>, bytes, lds)) return MOMOE_ERR_LAUNCH;
+  const FfnArgs none{};
+  ffn_gradients_kernel<Dx, STAGES><<<(unsigned)(bx + b1 + b2), kSpanThreads, bytes, st>>>(x ? *x : none, w1 ? *w1 : none, w2 ? *w2 : none, (int)bx, (int)b1);
+  FfnSums sums;
+  for (const FfnArgs* a : {x, w1, w2})
+    if (a) sums.add(*a);
+  return sum_slices(sums, st);
 }
 // Tiles of 32 rows as long as no CU has more than two of them, else of 64; a contraction is cut, where there is somewhere to leave its
 // sums, until every CU has two, into slices of at least 8 stages and not past 10 MB of sums.  (One CU pulls some 45 GB/s, so a
@@ -646,12 +694,6 @@ int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
     return MOMOE_ERR_UNSUPPORTED;
   return MOMOE_OK;
 }
-// tokens are addressed at 32-bit offsets
-int check_wgrad(int64_t rows, int64_t ldm, int64_t D, int64_t H, int64_t ld) {
-  const int st = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
-  if (st != MOMOE_OK) return st;
-  return ld % 8 != 0 || rows * ld * 2 >= (1ll << 32) || 8 * ldm * 64 >= (1ll << 32) ? MOMOE_ERR_UNSUPPORTED : MOMOE_OK;
-}
 // Gradients of the weights in tiles of 128 x 128 as long as no CU has more than two of them and none contracts over more than 8192 tokens; where
 // the tiles are fewer, the tokens are cut, into slices of at least 512, and past 10 MB of sums of at least 2048.  Us, W2 and W1, momoe_wgrad |
 // these: 31 tokens, 64 x 96 6.9, 7.1 | 4.1, 4.3; 512, 512 x 512 17.8, 18.5 | 8.7, 9.2; 1000, 1024 x 2816 28.3, 30.8 | 16.6, 23.2; 4096, 512 x 512
@@ -673,14 +715,20 @@ int64_t large_wgrad_bytes(int64_t rows, int64_t X, int64_t Y) {
   const int64_t tiles = cdiv64(X, 256) * cdiv64(Y, 256), grid = persistent_grid(), rounds = cdiv64(tiles, grid);
   return 6 * tiles >= 5 * rounds * grid ? 0 : bytes;
 }
-template <bool SECOND>
-int launch_wgrad(FfnArgs a, int64_t tokens, void* out, void* workspace, hipStream_t st) {
-  a.total = tokens;
-  a.out = (bf16*)out;
-  a.part = (float*)workspace;
-  a.slices = wgrad_slices(tokens, a.rows, a.D);
-  return launch_tiles<FfnWgrad<SECOND>, 2>(a, cdiv64(a.D, kFfnCols), st);
+// scratch of one gradient
+int64_t wgrad_bytes(int64_t rows, int64_t X, int64_t Y) {
+  if (!wgrad_in_small_tiles(rows, X, Y)) return std::max<int64_t>(0, large_wgrad_bytes(rows, X, Y));
+  const int64_t slices = wgrad_slices(rows, X, Y);
+  return slices > 1 ? slices * X * Y * 4 : 0;
 }
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+struct FfnScratch {
+  int64_t x, w1, w2;
+  FfnScratch(int64_t rows, int64_t D, int64_t H, bool x_, bool w1_, bool w2_)
+      : x(x_ ? aligned(slices_bytes(rows, D, 2 * H)) : 0), w1(w1_ ? aligned(wgrad_bytes(rows, D, 2 * H)) : 0),
+        w2(w2_ ? aligned(wgrad_bytes(rows, H, D)) : 0) {}
+  int64_t bytes() const { return x + w1 + w2; }
+};
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 bool any_unaligned(std::initializer_list<const void*> all) { return std::any_of(all.begin(), all.end(), unaligned16); }
 
@@ -691,41 +739,6 @@ using namespace momoe;
 
 extern "C" int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols) {
   return rows < 0 || cols <= 0 || cols % 16 != 0 ? -1 : (rows + 15) / 16 * 16 * cols;
-}
-
-extern "C" int64_t momoe_ffn_wgrad_workspace_bytes(int64_t rows, int64_t X, int64_t Y) {
-  if (rows <= 0 || X <= 0 || Y <= 0) return -1;
-  if (!wgrad_in_small_tiles(rows, X, Y)) return large_wgrad_bytes(rows, X, Y);
-  const int64_t slices = wgrad_slices(rows, X, Y);
-  return slices > 1 ? slices * X * Y * 4 : 0;
-}
-
-extern "C" int momoe_ffn_wgrad_w2(const void* hT, const void* Gy, int64_t ldgy, const int32_t* counts2, void* GW2_HD, void* workspace,
-                                  int64_t workspace_bytes, int64_t rows, int64_t D, int64_t H, void* stream) {
-  if (!hT || !Gy || !counts2 || !GW2_HD || ldgy < D || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
-  const int st = check_wgrad(rows, (rows + 31) / 32 * 32, D, H, ldgy);
-  if (st != MOMOE_OK) return st;
-  if (any_unaligned({hT, Gy, GW2_HD, workspace}) || workspace_bytes < momoe_ffn_wgrad_workspace_bytes(rows, H, D)) return MOMOE_ERR_BAD_ARG;
-  if (!wgrad_in_small_tiles(rows, H, D))
-    return momoe_wgrad(hT, H, MOMOE_LAYOUT_TRANSPOSED, nullptr, Gy, ldgy, MOMOE_LAYOUT_ROWS, nullptr, counts2, GW2_HD, rows, 1, H, D, rows,
-                       workspace, workspace_bytes, stream);
-  FfnArgs a{(const bf16*)Gy, ldgy, nullptr, H, rows, (int)D, (int)H};
-  a.ht = (bf16*)const_cast<void*>(hT);
-  return launch_wgrad<true>(a, rows, GW2_HD, workspace, (hipStream_t)stream);
-}
-
-extern "C" int momoe_ffn_wgrad_w1(const void* x, int64_t ldx, const void* gz_blocked, const int32_t* counts2, void* GW1_D2H, void* workspace,
-                                  int64_t workspace_bytes, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
-  if (!x || !gz_blocked || !counts2 || !GW1_D2H || ldx < D || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
-  const int st = check_wgrad(rows, ldm, D, H, ldx);
-  if (st != MOMOE_OK) return st;
-  if (any_unaligned({x, gz_blocked, GW1_D2H, workspace}) || workspace_bytes < momoe_ffn_wgrad_workspace_bytes(rows, D, 2 * H)) return MOMOE_ERR_BAD_ARG;
-  if (!wgrad_in_small_tiles(rows, D, 2 * H))
-    return momoe_wgrad(x, ldx, MOMOE_LAYOUT_ROWS, nullptr, gz_blocked, ldm, MOMOE_LAYOUT_KBLOCKED, nullptr, counts2, GW1_D2H, rows, 1, D,
-                       2 * H, rows, workspace, workspace_bytes, stream);
-  FfnArgs a{(const bf16*)x, ldx, nullptr, D, ldm, (int)(2 * H), (int)H};
-  a.gz = (bf16*)const_cast<void*>(gz_blocked);
-  return launch_wgrad<false>(a, rows, GW1_D2H, workspace, (hipStream_t)stream);
 }
 
 extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
@@ -802,15 +815,57 @@ extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void*
   return launch<DhDenseSpan<true>, DhSaved>(a, H, D, cdiv64(H, kFfnCols), (hipStream_t)stream);
 }
 
-extern "C" int momoe_ffn_dgrad_x(const void* gz_blocked, const void* W1_D2H, void* Gx, void* workspace, int64_t workspace_bytes,
-                                 int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
-  if (!gz_blocked || !W1_D2H || !Gx || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, ldm, D, H);
-  if (st != MOMOE_OK) return st;
-  if (any_unaligned({gz_blocked, W1_D2H, Gx, workspace}) || workspace_bytes < slices_bytes(rows, D, 2 * H)) return MOMOE_ERR_BAD_ARG;
-  FfnArgs a{nullptr, 0, (const bf16*)W1_D2H, rows, ldm, (int)D, (int)H};
-  a.gz = (bf16*)const_cast<void*>(gz_blocked);
-  a.out = (bf16*)Gx;
-  a.part = (float*)workspace;
-  return launch<DxDenseSpan, FfnDx>(a, D, 2 * H, cdiv64(D, kFfnCols), (hipStream_t)stream);
+extern "C" int64_t momoe_ffn_gradients_workspace_bytes(int64_t rows, int64_t D, int64_t H, int wants_x, int wants_W1, int wants_W2) {
+  return rows <= 0 || D <= 0 || H <= 0 ? -1 : FfnScratch(rows, D, H, wants_x, wants_W1, wants_W2).bytes();
+}
+
+extern "C" int momoe_ffn_gradients(const void* x, int64_t ldx, const void* Gy, int64_t ldgy, const void* gz_blocked, const void* hT,
+                                   const void* W1_D2H, const int32_t* counts2, void* Gx, void* GW1_D2H, void* GW2_HD, void* workspace,
+                                   int64_t workspace_bytes, int64_t rows, int64_t ldm, int64_t D, int64_t H, void* stream) {
+  if ((Gx && (!gz_blocked || !W1_D2H)) || (GW1_D2H && (!x || !gz_blocked || !counts2 || ldx < D)) || (GW2_HD && (!hT || !Gy || !counts2 || ldgy < D)))
+    return MOMOE_ERR_BAD_ARG;
+  if (rows <= 0 || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
+  const int status = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
+  if (status != MOMOE_OK) return status;
+  // tokens are addressed at 32-bit offsets
+  if ((GW1_D2H && (ldx % 8 != 0 || rows * ldx * 2 >= (1ll << 32) || 8 * ldm * 64 >= (1ll << 32))) ||
+      (GW2_HD && (ldgy % 8 != 0 || rows * ldgy * 2 >= (1ll << 32))))
+    return MOMOE_ERR_UNSUPPORTED;
+  const FfnScratch scratch(rows, D, H, Gx, GW1_D2H, GW2_HD);
+  if (any_unaligned({x, Gy, gz_blocked, hT, W1_D2H, Gx, GW1_D2H, GW2_HD, workspace}) || workspace_bytes < scratch.bytes()) return MOMOE_ERR_BAD_ARG;
+  const hipStream_t st = (hipStream_t)stream;
+  char* const ws = (char*)workspace;
+  const auto args = [&](const void* tokens, int64_t ld, const void* w, int64_t out_rows, int64_t out_cols, void* out, char* part) {
+    FfnArgs a{(const bf16*)tokens, ld, (const bf16*)w, out_rows, ldm, (int)out_cols, (int)H};
+    a.gz = (bf16*)const_cast<void*>(gz_blocked);
+    a.ht = (bf16*)const_cast<void*>(hT);
+    a.out = (bf16*)out;
+    a.part = (float*)part;
+    a.total = rows;
+    return a;
+  };
+  FfnArgs ax = args(nullptr, 0, W1_D2H, rows, D, Gx, ws), a1 = args(x, ldx, nullptr, D, 2 * H, GW1_D2H, ws + scratch.x),
+          a2 = args(Gy, ldgy, nullptr, H, D, GW2_HD, ws + scratch.x + scratch.w1);
+  const FfnPlan plan = plan_of(rows, cdiv64(D, kFfnCols), 2 * H, D);
+  ax.slices = plan.slices;
+  a1.slices = wgrad_slices(rows, D, 2 * H);
+  a2.slices = wgrad_slices(rows, H, D);
+  const bool x_span = takes_span(rows, D, 2 * H), small1 = wgrad_in_small_tiles(rows, D, 2 * H), small2 = wgrad_in_small_tiles(rows, H, D);
+  if (GW2_HD && !small2) {
+    const int s = momoe_wgrad(hT, H, MOMOE_LAYOUT_TRANSPOSED, nullptr, Gy, ldgy, MOMOE_LAYOUT_ROWS, nullptr, counts2, GW2_HD, rows, 1, H, D, rows,
+                              scratch.w2 ? a2.part : nullptr, scratch.w2, stream);
+    if (s != MOMOE_OK) return s;
+  }
+  if (GW1_D2H && !small1) {
+    const int s = momoe_wgrad(x, ldx, MOMOE_LAYOUT_ROWS, nullptr, gz_blocked, ldm, MOMOE_LAYOUT_KBLOCKED, nullptr, counts2, GW1_D2H, rows, 1, D,
+                              2 * H, rows, scratch.w1 ? a1.part : nullptr, scratch.w1, stream);
+    if (s != MOMOE_OK) return s;
+  }
+  if (Gx && x_span) {
+    ax.slices = 1;
+    const int s = launch_dense_span<DxDenseSpan>(ax, D, st);
+    if (s != MOMOE_OK) return s;
+  }
+  const FfnArgs *px = Gx && !x_span ? &ax : nullptr, *p1 = GW1_D2H && small1 ? &a1 : nullptr, *p2 = GW2_HD && small2 ? &a2 : nullptr;
+  return plan.fm == 1 ? launch_gradients<FfnDx<1>, 4>(px, p1, p2, st) : launch_gradients<FfnDx<2>, 3>(px, p1, p2, st);
 }

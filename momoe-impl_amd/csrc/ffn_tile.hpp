@@ -153,17 +153,17 @@ __device__ __forceinline__ void wait_for_stage(int after) {
 }
 
 // A tile program P: P::Rows, P::Weights, FM; K, slices, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column of a
-// wave's fragments in the tile; epilogue(row0, rows, tn, slice, wm, wn, acc).
+// wave's fragments in the tile; epilogue(row0, rows, tn, slice, wm, wn, acc).  block: of this program's, from a multiple of 8 on.
 template <class P, int STAGES>
-__device__ __forceinline__ void run_ffn_tile(const P& prog) {
+__device__ __forceinline__ void run_ffn_tile(const P& prog, int block) {
   using Rows = typename P::Rows;
   using Weights = typename P::Weights;
   constexpr int FM = P::FM, FN = 4, BM = 32 * FM;
   constexpr int LOADS = Rows::DEP + Weights::DEP;
   // An XCD has a contiguous eighth of the tiles, row tiles fastest: those that share weights meet in one L2
   const int total = prog.row_tiles * prog.col_tiles * prog.slices, chunk = (total + 7) >> 3;
-  int t = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= chunk || t >= total) return;
+  int t = (block & 7) * chunk + (block >> 3);
+  if ((block >> 3) >= chunk || t >= total) return;
   const int row_tile = t % prog.row_tiles;
   t /= prog.row_tiles;
   const int slice = t % prog.slices, tn = t / prog.slices;

@@ -624,11 +624,9 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
     const int64_t ldx = pitch_of_rows(x), ldgy = pitch_of_rows(Gy);
     const int64_t rest = M - msave, ldm = (M + 31) / 32 * 32, gz_bytes = 4 * H * ldm, ht_bytes = need_w2 ? momoe_padded_rows(M, 1) * H * 2 : 0;
     const int64_t u_bytes = rest > 0 ? momoe_ffn_fragment_floats(rest, H) * 4 : 0;
-    const int64_t ws1_bytes = need_w1 ? momoe_ffn_wgrad_workspace_bytes(M, D, 2 * H) : 0;
-    const int64_t ws2_bytes = need_w2 ? momoe_ffn_wgrad_workspace_bytes(M, H, D) : 0;
-    const int64_t wsx_bytes = need_x ? momoe_ffn_workspace_bytes(M, D, 2 * H) : 0;
-    Transients transients(dev, {16, gz_bytes, ht_bytes, u_bytes, ws2_bytes, ws1_bytes, wsx_bytes});
-    Tensor counts_own, gz_own, ht_own, u_own, ws1_own, ws2_own, wsx_own;
+    const int64_t ws_bytes = momoe_ffn_gradients_workspace_bytes(M, D, H, need_x, need_w1, need_w2);
+    Transients transients(dev, {16, gz_bytes, ht_bytes, u_bytes, ws_bytes});
+    Tensor counts_own, gz_own, ht_own, u_own, ws_own;
     const auto scratch = [&](int64_t bytes, Tensor& own) { return bytes > 0 ? transients.take(bytes, own) : nullptr; };
     int32_t* const counts = (int32_t*)transients.take(16, counts_own);
     void* const gz = transients.take(gz_bytes, gz_own);
@@ -645,20 +643,12 @@ struct FeedForwardFn : torch::autograd::Function<FeedForwardFn> {
                  M, rest, ldm, D, H);
       u_own.reset();
     }
-    if (need_w2)
-      MOMOE_CALL(momoe_ffn_wgrad_w2, st, (const void*)ht, Gy.data_ptr(), ldgy, (const int32_t*)counts, out[2].data_ptr(),
-                 scratch(ws2_bytes, ws2_own), ws2_bytes, M, D, H);
-    ws2_own.reset();
-    ht_own.reset();
-    if (need_w1)
-      MOMOE_CALL(momoe_ffn_wgrad_w1, st, x.data_ptr(), ldx, (const void*)gz, (const int32_t*)counts, out[1].data_ptr(),
-                 scratch(ws1_bytes, ws1_own), ws1_bytes, M, ldm, D, H);
-    ws1_own.reset();
-    if (need_x) {
-      const Tensor Gx = empty_bf16({M, D}, dev);
-      MOMOE_CALL(momoe_ffn_dgrad_x, st, (const void*)gz, W1.data_ptr(), Gx.data_ptr(), scratch(wsx_bytes, wsx_own), wsx_bytes, M, ldm, D, H);
-      out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
-    }
+    Tensor Gx;
+    if (need_x) Gx = empty_bf16({M, D}, dev);
+    const auto result = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    MOMOE_CALL(momoe_ffn_gradients, st, x.data_ptr(), ldx, Gy.data_ptr(), ldgy, (const void*)gz, (const void*)ht, W1.data_ptr(), (const int32_t*)counts,
+               result(Gx), result(out[1]), result(out[2]), scratch(ws_bytes, ws_own), ws_bytes, M, ldm, D, H);
+    if (need_x) out[0] = Gx.view(grads[0].sizes()).to(grads[0].device());
     return out;
   }
 };

@@ -99,16 +99,14 @@ _SIGNATURES = {
     "momoe_fp8_few_lin2_scale_fwd": (_int, [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_fragment_floats": (_i64, [_i64] * 2),
-    "momoe_ffn_wgrad_workspace_bytes": (_i64, [_i64] * 3),
+    "momoe_ffn_gradients_workspace_bytes": (_i64, [_i64] * 3 + [_int] * 3),
     "momoe_ffn_lin1_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_workspace_bytes": (_i64, [_i64] * 3),
     "momoe_ffn_lin2_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "momoe_ffn_dgrad_h": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _p]),
     "momoe_ffn_swiglu_bwd": (_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_dgrad_h_saved": (_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
-    "momoe_ffn_dgrad_x": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
-    "momoe_ffn_wgrad_w2": (_int, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
-    "momoe_ffn_wgrad_w1": (_int, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_ffn_gradients": (_int, [_p, _i64, _p, _i64] + [_p] * 8 + [_i64] * 5 + [_p]),
     "momoe_int4_weight_bytes": (_i64, [_i64] * 3),
     "momoe_int4_scale_words": (_i64, [_i64] * 3 + [_int]),
     "momoe_int4_pack_weights": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _int, _int, _p, _p, _p]),

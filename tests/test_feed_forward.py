@@ -38,17 +38,18 @@ def test_refusals_of_the_entry_points():
     assert c(ldx=56) == c(ldm=63) == c(tokens=39) == 1 and c(ldx=68) == 2
     c = _refuses(lib.momoe_ffn_dgrad_h_saved, dict(Gy=P, ldgy=64, W=P, ab=P, gz=P, hT=None, counts=None, tokens=40, **padded), ("Gy", "W", "ab", "gz"), ("Gy", "W", "ab", "gz", "hT"))
     assert c(ldgy=56) == c(ldm=63) == c(tokens=39) == 1 and c(ldgy=68) == 2
-    c = _refuses(lib.momoe_ffn_dgrad_x, dict(gz=P, W=P, Gx=P, **room, **sizes), ("gz", "W", "Gx", "ws"), ("gz", "W", "Gx", "ws"))
-    assert c(ldm=39) == c(bytes=-1) == c(rows=1, D=2048, H=8192, ws=None, bytes=0) == 1
-    wgrad = dict(rows=40, D=64, H=32)
-    assert all(lib.momoe_ffn_wgrad_workspace_bytes(*n) == -1 for n in ((0, 64, 64), (64, 0, 64), (64, 64, 0)))
-    need = lib.momoe_ffn_wgrad_workspace_bytes(1024, 512, 1024)
-    c = _refuses(lib.momoe_ffn_wgrad_w2, dict(hT=P, Gy=P, ldgy=64, counts=P, G=P, **room, **wgrad), ("hT", "Gy", "counts", "G", "ws"), ("hT", "Gy", "G", "ws"))
-    assert need > 0 and c(ldgy=56) == c(bytes=-1) == c(rows=1024, D=1024, H=512, ldgy=1024, bytes=need - 4) == 1
-    assert c(ldgy=68) == c(rows=1 << 20, ldgy=2048) == c(rows=1 << 23) == 2
-    c = _refuses(lib.momoe_ffn_wgrad_w1, dict(x=P, ldx=64, gz=P, counts=P, G=P, **room, rows=40, ldm=64, D=64, H=32), ("x", "gz", "counts", "G", "ws"), ("x", "gz", "G", "ws"))
-    assert c(ldx=56) == c(ldm=63) == c(bytes=-1) == c(rows=1024, ldm=1024, D=512, H=512, ldx=512, bytes=need - 4) == 1
-    assert c(ldx=68) == c(rows=1 << 20, ldm=1 << 20, ldx=2048) == c(ldm=1 << 23) == 2
+    need = lib.momoe_ffn_gradients_workspace_bytes
+    assert all(need(*n, 1, 1, 1) == -1 for n in ((0, 64, 64), (64, 0, 64), (64, 64, 0))) and need(40, 64, 32, 0, 0, 0) == 0
+    each = [need(1024, 512, 1024, *w) for w in ((1, 0, 0), (0, 1, 0), (0, 0, 1))]
+    assert all(n > 0 for n in each) and need(1024, 512, 1024, 1, 1, 1) == sum(each)
+    good = dict(x=P, ldx=64, Gy=P, ldgy=64, gz=P, hT=P, W=P, counts=P, Gx=P, GW1=P, GW2=P, **room, rows=40, ldm=64, D=64, H=32)
+    c = _refuses(lib.momoe_ffn_gradients, good, ("x", "Gy", "gz", "hT", "W", "counts", "ws"), ("x", "Gy", "gz", "hT", "W", "Gx", "GW1", "GW2", "ws"))
+    assert c(ldx=56) == c(ldgy=56) == c(ldm=63) == c(bytes=-1) == c(rows=-40) == 1
+    assert c(rows=1024, ldm=1024, D=512, H=1024, ldx=512, ldgy=512, bytes=sum(each) - 4) == 1
+    assert c(ldx=68) == c(ldgy=68) == c(rows=1 << 20, ldm=1 << 20, ldx=2048) == c(rows=1 << 20, ldm=1 << 20, ldgy=2048) == c(ldm=1 << 23) == 2
+    for wants, needs in ((("Gx",), ("gz", "W")), (("GW1",), ("x", "gz", "counts")), (("GW2",), ("Gy", "hT", "counts"))):
+        one = {**{k: None for k in ("x", "Gy", "gz", "hT", "W", "counts", "Gx", "GW1", "GW2")}, **{k: P for k in wants + needs}}
+        assert all(c(**{**one, k: None}) == 1 for k in needs)
 
 
 def test_module_refusals():
