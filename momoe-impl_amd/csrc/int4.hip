@@ -4,7 +4,7 @@
 // k-values of a column.  A product over a group is
 //   sum_k x_k (code_k - zero) scale = scale * (sum_k x_k (128 + code_k) - (128 + zero) * sum_k x_k)
 // 128 + code is a bf16 whose low bits are the code: bits 0x4300 | code, one instruction for two of them and no conversion.  The sum of
-// x_k is a product with ones by the same matrix instruction, whose rate such a call does not use up; it comes in the same lanes.  All
+// x_k is a product with ones by the same matrix instruction, whose rate a call of few rows does not use up; it comes in the same lanes.  All
 // of it in fp32: what is subtracted is up to 143 / 8 times as large as what is left, so that four bits of 24 go.  The scale, fp32 again,
 // meets the sum: a weight itself is never rounded.
 //
@@ -105,7 +105,8 @@ __device__ __forceinline__ void store_pair(const Int4Args& p, int64_t row, int p
 
 // Tiles of up to 32 rows.  A wavefront owns a pair of 16-column groups; KS of them share its contraction, a block of 128 k-values in
 // KS each, and their sums meet in LDS.  Codes and scales go straight into registers, AHEAD blocks ahead; the rows come to LDS,
-// kFewBytes of them at a time, for all wavefronts.
+// kFewBytes of them at a time, for all wavefronts.  Bound by the codes' way from memory where they are many, 1 token through 4096 x 11264 in
+// 27 us (71 MB, 2.6 TB/s over both launches), else by the first answer of memory: 8 of 128 experts of 2048 x 768, 7.7 and 6.0 us.
 constexpr int kFewThreads = 256, kFewWaves = kFewThreads / 64, kFewBytes = 32 << 10;
 
 template <bool FIRST, int KS, int SG>
@@ -246,9 +247,15 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
 
 // Tiles of 64 rows x 256 columns, for more rows than that: a wavefront owns 64 columns of them, two pairs of groups.  The rows come to LDS by
 // direct transfers, 128 k-values a stage, the codes and scales straight into registers; both are requested a stage ahead, and two
-// workgroups share a CU, so that one's products stand beside the other's vector work: for each 64 matrix instructions (and 16 for the
-// sums of the rows) of a wavefront's stage there are 112 instructions that make bf16 of codes and 128 that bring the sums of a group
-// to the others.  Fragments of rows that the tile does not have are left out.  A launch of few tiles has its contraction cut into slices,
+// workgroups share a CU, so that one's products stand beside the other's vector work: for each 64 matrix instructions of a wavefront's stage
+// there are 112 instructions that make bf16 of codes and 64 that bring the sums of a group to the others (groups of 32: 256).
+// acc += scale * sum_k x_k (128 + code_k) as each group ends; what that is too much by, (128 + zero) scale * sum_k x_k, is a product of fp32
+// itself, contracted over the groups, and taken away four of them at a time by v_mfma_f32_16x16x4_f32.  (All at the end would let sums of
+// thousands of 128 x_k meet.)  Each of the first wavefronts sums one fragment of rows, for all of them, in LDS; two sets in turn, as a barrier a stage
+// lies between the writing of one and its use.  4096 tokens, 4096 x 11264: 1333 us with sums and differences of their own in each
+// wavefront, 1243 this way, 0.91 PFLOP/s.  It is bound by issue, the matrix instructions being busy half of the time and the vector ones two thirds.
+// Not faster: 128 rows a tile; eight wavefronts of 32 columns (1672); all fragments without a branch between them, which spills (1566).
+// Fragments of rows that the tile does not have are left out.  A launch of few tiles has its contraction cut into slices,
 // whose sums int4_h_of_slices_kernel or the last kernel adds up.
 struct Int4Rows {
   static constexpr int BM = 64, DEP = BM * 256 / (kSpanWaves * 1024), STAGE = BM * 256;  // bytes
@@ -282,6 +289,7 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
   constexpr int PAIRS = 2 * kSpanWaves, STEPS = 4 / SG;
   typedef uint32_t Words __attribute__((ext_vector_type(SG)));
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Rows::STAGE];
+  __shared__ float sums[2][4][Rows::BM];  // of x_k over each of four groups, of a row
   const int l = lane_id(), wave = wave_id();
   const uint32_t addr = lds_address((bf16*)lds) + wave * 1024;
   Int4Sched sched(p, (p.pairs + PAIRS - 1) / PAIRS * p.slices, Rows::BM);
@@ -315,7 +323,7 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
     }
   };
   // the first stage of the next tile, into the half of LDS that nobody reads
-  int q = 0;
+  int q = 0, parity = 0;
   const auto begin = [&] {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -335,11 +343,28 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
     if (next.tc.valid) B.init(p, next.tc, FIRST && p.idx);
     const int nf = cur.nf;
     f32x4 acc[4][4] = {};
+    // -(128 + zero) scale of up to four groups, lane l that of group l / 16 and column l % 16, for what these take away of acc
+    float away[4] = {};
+    int held = 0;
+    const auto take_away = [&] {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= nf) break;
+        const float sum = l >> 4 < held ? sums[parity][l >> 4][16 * i + (l & 15)] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum, away[j], acc[j][i], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) away[j] = 0.0f;
+      held = 0;
+      parity ^= 1;
+    };
     for (int kb = cur.kb0; kb < cur.kb1; ++kb) {
       wait_vmcnt<0>();
       wait_lgkm0();
       __builtin_amdgcn_s_barrier();
       order_fence();
+      if (held == 4) take_away();
       if (kb + 1 < cur.kb1) A.request(kb + 1, p.K, nf, addr + (q ^ 1) * Rows::STAGE);
       order_fence();
       u32x4 codes[4];
@@ -352,10 +377,11 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
       unrolled<0, SG>([&](auto GC) {
         constexpr int g = decltype(GC)::value;
         bf16x8 wf[4][STEPS];
-        float s[4], z[4];
+        float s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[j] = scale_of_word(scales[j][g]), z[j] = zero_of_word(scales[j][g]);
+          s[j] = scale_of_word(scales[j][g]);
+          if (l >> 4 == held + g) away[j] = -s[j] * zero_of_word(scales[j][g]);
 #pragma unroll
           for (int m = 0; m < STEPS; ++m) wf[j][m] = bf16_of_codes(codes[j][g * STEPS + m], k128);
         }
@@ -366,24 +392,33 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
 #pragma unroll
           for (int m = 0; m < STEPS; ++m)
             rf[m] = *(const bf16x8*)(rows + i * (16 * 256) + (((4 * (g * STEPS + m) + (l >> 4)) ^ (l & 15)) << 4));
-          f32x4 t[4] = {}, sum = {};
+          f32x4 t[4] = {};
 #pragma unroll
-          for (int m = 0; m < STEPS; ++m) {
-            sum = mfma16(rf[m], ones, sum);
+          for (int m = 0; m < STEPS; ++m)
 #pragma unroll
             for (int j = 0; j < 4; ++j) t[j] = mfma16(rf[m], wf[j][m], t[j]);
+          if (i == wave) {
+            f32x4 sum = {};
+#pragma unroll
+            for (int m = 0; m < STEPS; ++m) sum = mfma16(ones, rf[m], sum);
+            if (l < 16) sums[parity][held + g][16 * i + l] = sum[0];
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s[j], fmaf(-z[j], sum[r], t[j][r]), acc[j][i][r]);
+            for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s[j], t[j][r], acc[j][i][r]);
             asm volatile("" : "+v"(acc[j][i]));  // (the products of all fragments were formed first, and spilled)
           }
         });
       });
+      held += SG;
       order_fence();
       q ^= 1;
     }
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    order_fence();
+    take_away();
     if (next.tc.valid) {
       A = B;
       begin();

@@ -41,11 +41,11 @@ def _on(w):
 
 def _sum_bound(x, scale, group):
     """How far a sum over the contraction may be off: what is added up in a group is at most 143 |x| and what is subtracted 143 times the
-    sum of x, each of at most group + 2 roundings, then a product, a difference and the sum over the groups (of which the values are
-    at most 15 |x| scale)."""
+    sum of x, each of at most group + 2 roundings, then, scaled, 143 of up to four groups stand in the sum until they are taken away again:
+    two roundings a group, of the values of up to four; then the sum over the groups (of which the values are at most 15 |x| scale)."""
     k = x.shape[1]
     s = scale.double().abs().repeat_interleave(group, -2)[:k]
-    return (x.abs() @ s) * E * (2 * 143 * (group + 4) + 15 * (scale.shape[-2] + 8))
+    return (x.abs() @ s) * E * (2 * 143 * (group + 4 + 4) + 15 * (scale.shape[-2] + 8))
 
 
 def _block(x, w, group):
