@@ -254,8 +254,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
 // thousands of 128 x_k meet.)  Each of the first wavefronts sums one fragment of rows, for all of them, in LDS; two sets in turn, as a barrier a stage
 // lies between the writing of one and its use.  4096 tokens, 4096 x 11264: 1333 us with sums and differences of their own in each
 // wavefront, 1243 this way, 0.91 PFLOP/s.  It is bound by issue, the matrix instructions being busy half of the time and the vector ones two thirds.
-// Not faster: 128 rows a tile; wavefronts of 32 columns, eight a workgroup (1672) or four, three workgroups a CU (1391; 1000 tokens to 8 of 128
-// experts, groups of 64, 224 | 227); all fragments without a branch between them, which spills (1566).
+// Not faster: 128 rows a tile; wavefronts of 32 columns, eight a workgroup (1672) or four, of 64 rows and three workgroups a CU (1391; 1000 tokens to
+// 8 of 128 experts, groups of 64, 224 | 227) or of 96 and two (1439; 232); all fragments without a branch between them, which spills (1566).
 // Fragments of rows that the tile does not have are left out.  A launch of few tiles has its contraction cut into slices,
 // whose sums int4_h_of_slices_kernel or the last kernel adds up.
 struct Int4Rows {

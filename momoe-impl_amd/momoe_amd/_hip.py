@@ -574,7 +574,3 @@ def int4_pack_weights(codes_NRC, scale, zero, halves, group):
         _call("momoe_int4_pack_weights", _ptr(codes_NRC), _ptr(scale), _TYPES[scale.dtype], _ptr(zero), N, R, C, halves, group, _ptr(packed),
               _ptr(words), _stream())
     return packed, words
-
-
-def int4_tile_rows(Msum, D, H, N):
-    return _lib.momoe_int4_tile_rows(Msum, D, H, N)

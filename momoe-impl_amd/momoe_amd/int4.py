@@ -91,7 +91,8 @@ class MoMoEInt4(_Int4Block):
         Wl1_zero, Wl2_zero: uint8 0..15 (of greater ones the low four bits) of the same sizes; None: 8 throughout.
         group_size: k-values that share a scale and a zero, 32, 64 or 128.
     A weight is (code - zero) * scale, and is multiplied as that, unrounded, with sums in fp32; x and h are bf16 (x of any other type is
-    rounded to bf16).  D and H must be multiples of 32.  A NaN or an infinity in a token makes NaN of it; so may a value above 2^113.
+    rounded to bf16).  D and H must be multiples of 32.  A NaN or an infinity in a token makes NaN of it; so may a value above
+    2^113, or one above 2^111 when it is multiplied by a scale.
 
     The weights are laid out once, in the order that the kernels read them in; `weights()` gives them back.
     `from_momoe` quantizes the weights of a `MoMoE`.
