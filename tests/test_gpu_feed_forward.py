@@ -187,6 +187,40 @@ def test_rows_of_nan_and_infinity_stay_with_themselves(M, save):
     assert torch.equal(ok[:, cols], ref[3][:, cols]) and not ok[:, 5].isfinite().any() and not ok[:, 0].isfinite().any()
 
 
+@pytest.mark.parametrize("M,D,H", [(3, 96, 64), (70, 160, 288), (1100, 96, 64), (40, 1056, 4256)])
+def test_gradients_leave_what_lies_behind(M, D, H):
+    """The entry points of the backward on buffers with room behind them: the last rows' padding is zeros, and the rest keeps its bits."""
+    lib, st, P = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream, (M + 31) // 32 * 32
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(M, D, H)]
+    flat = lambda n: torch.full((n + 4096,), 7.0, device=DEV, dtype=torch.bfloat16)
+    u = torch.full((lib.momoe_ffn_fragment_floats(M, H) + 1024,), 7.0, device=DEV)
+    gz, hT, Gx, G1, G2 = flat(2 * H * P), flat(P * H + 32 * H), flat(M * D), flat(2 * D * H), flat(D * H)
+    counts = torch.full((6,), 7, device=DEV, dtype=torch.int32)
+    need = lib.momoe_ffn_gradients_workspace_bytes(M, D, H, 1, 1, 1)
+    ws = torch.full((need + 64,), 7, device=DEV, dtype=torch.uint8)
+    assert lib.momoe_ffn_dgrad_h(Gy.data_ptr(), D, W2.data_ptr(), u.data_ptr(), M, D, H, st) == 0
+    assert lib.momoe_ffn_swiglu_bwd(x.data_ptr(), D, W1.data_ptr(), u.data_ptr(), gz.data_ptr(), hT.data_ptr(), counts.data_ptr(), M, M, P, D, H, st) == 0
+    assert lib.momoe_ffn_gradients(x.data_ptr(), D, Gy.data_ptr(), D, gz.data_ptr(), hT.data_ptr(), W1.data_ptr(), counts.data_ptr(), Gx.data_ptr(),
+                                   G1.data_ptr(), G2.data_ptr(), ws.data_ptr(), need, M, P, D, H, st) == 0
+    torch.cuda.synchronize()
+    assert counts.tolist() == [0, M, 7, 7, 7, 7] and (ws[need:] == 7).all() and (u[lib.momoe_ffn_fragment_floats(M, H):] == 7).all()
+    for t, n in ((gz, 2 * H * P), (hT, P * H), (Gx, M * D), (G1, 2 * D * H), (G2, D * H)):
+        assert (t[n:] == 7).all()
+    assert (gz[:2 * H * P].view(-1, P, 32)[:, M:] == 0).all() and (hT[:P * H].view(-1, H, 32).transpose(1, 2).reshape(P, H)[M:] == 0).all()
+    want = _step(_block(W1, W2), x, Gy)
+    got = Gx[:M * D].view(M, D), G1[:2 * D * H].view(D, 2 * H), G2[:D * H].view(H, D)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))
+
+
+def test_gradients_of_rows_that_share_memory():
+    """A gradient or an input that one row, or one value, stands for."""
+    x, W1, W2, Gy = [t.to(DEV) for t in _inputs(70, 96, 64)]
+    block = _block(W1, W2, 50)
+    for a, b in ((x, Gy[:1].expand(70, 96)), (x, Gy[:1, :1].expand(70, 96)), (x[:1].expand(70, 96), Gy)):
+        got, want = _step(block, a, b), _step(block, a.contiguous(), b.contiguous())
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
 def test_rows_behind_the_last_stay_as_they_are():
     """Results lie in a larger buffer of the allocator's: what is behind them keeps its bits."""
     D, H = 96, 64

@@ -90,6 +90,16 @@ def test_dense_block(M, D, H, group, zeros, scale_type):
     _check(y, *_block(x.double(), w, group))
 
 
+@pytest.mark.parametrize("M,D,H,group,zeros", [(20, 1056, 96, 128, True), (700, 1056, 160, 32, True), (700, 1120, 160, 64, False), (700, 1184, 160, 128, True)])
+def test_rows_of_one_sign(M, D, H, group, zeros):
+    """The most that codes' offsets add up to, and is to be taken away again; the last groups of four not all there."""
+    w = _weights((), D, H, group, zeros)
+    x = (3 + 0.1 * _x(M, D).float().sign()).to(torch.bfloat16)
+    x[1::2] = -x[1::2]
+    block = momoe_amd.FeedForwardInt4(D, H, *_on(w), group_size=group)
+    _check(block(x.to(DEV)), *_block(x.double(), w, group))
+
+
 # M, D, H, N, K, Ks, skew, group: experts without a token and with nearly all
 EXPERTS = [
     (1, 32, 32, 2, 1, 0, 0, 32), (1, 256, 128, 8, 8, 0, 0, 128), (7, 96, 160, 4, 2, 0, 0, 64), (50, 288, 416, 5, 2, 1, 0, 128),
