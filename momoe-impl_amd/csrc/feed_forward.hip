@@ -315,7 +315,8 @@ int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   sums.add(a);
   return sum_slices(sums, st);
 }
-// The three products that need gz or hT and no more, in one launch; x, w1, w2: null, or what is wanted
+// The three products that need gz or hT and no more, in one launch, as none of them fills the CUs; x, w1, w2: null, or what is wanted.  1000 tokens,
+// 2176 x 1152: 15.5 + 23.6 + 25.3 us apart, 40 so (0.75 PFLOP/s); 128, 96 x 64: 4.5 + 4.9 + 3.5 and 5.
 template <class Dx, int STAGES>
 __global__ __launch_bounds__(kSpanThreads, 2) void ffn_gradients_kernel(FfnArgs x, FfnArgs w1, FfnArgs w2, int x_blocks, int w1_blocks) {
   const int block = blockIdx.x;
@@ -663,9 +664,13 @@ __global__ __launch_bounds__(kSpanThreads, 1) void ffn_span_kernel(FfnArgs p, in
 }
 
 // ---- which of the two -----------------------------------------------------------------------------------------------------------
-// 256 x 256 tiles where they are half a round of one a CU at least (and there are two stages of k-values)
+// 256 x 256 tiles where the results are three tenths of a round of one a CU at least (and there are two stages of k-values).  Us, small tiles | these,
+// by the number of these: x W1 of 2048 x 2816 for 700 tokens, 66 of them, 25.4 | 27.5; 1250, 2048 x 2048, 80, 35.4 | 27.0; 1200, 1024 x 2176, 85,
+// 19.9 | 16.9; 2000, 2048 x 2048, 128, 44.5 | 31.8; 4000, 256, 93.0 | 51.6; h W2, 2000, 2048 x 2048, 64, 26.3 | 26.5; 1250, 1024 x 4096, 80, 22.0 | 17.3;
+// 1000, 4096 x 2048, 32, 34.4 | 48.5; 24 tokens, x W1 of 4096 x 11264, 88, hardly filled, 36.5 | 58.  8192 tokens through 2048 x 8192: 414 (1.33 PFLOP/s) and 199 (1.38), 16384 through 4096 x 11264: 2329 (1.30)
+// and 1064 (1.42): what a large library product of these sizes reaches; bound by the matrix instructions at the clock that the card holds.
 inline bool takes_span(int64_t rows, int64_t cols, int64_t contraction) {
-  return contraction >= WideSpan::AHEAD * kSpan && 2 * cdiv64(rows, WideSpan::MAX_ROWS) * cdiv64(cols, WideSpan::COLS) >= persistent_grid();
+  return contraction >= WideSpan::AHEAD * kSpan && 10 * rows * cols >= 3 * persistent_grid() * (int64_t)(WideSpan::MAX_ROWS * WideSpan::COLS);
 }
 template <class P>
 int launch_dense_span(const FfnArgs& a, int64_t cols, hipStream_t st) {

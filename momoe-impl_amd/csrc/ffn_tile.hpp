@@ -3,7 +3,10 @@
 // For launches of few tiles, short contractions, few rows; the large ones run in the loop of gemm_span.hpp, whose operands and fragment
 // layout these are (the first input of the MFMA is the weight side: a lane holds, for one tile row (lane % 16), four consecutive
 // columns).  4 waves, 2 x 2.  STAGES stages in LDS; the fragments of one half of a stage are read while
-// the other is multiplied (read and then multiplied, one after the other, a stage took 0.36 to 0.75 us whatever was on the way).  A contraction may be cut into `slices`, each a tile of its own that leaves fp32 sums for another kernel.
+// the other is multiplied (read and then multiplied, one after the other, a stage took 0.36 to 0.75 us whatever was on the way).  A
+// contraction may be cut into `slices`, each a tile of its own that leaves fp32 sums for another kernel.
+// Bound by what a CU pulls, some 30 GB/s by one workgroup and 45 by two: 24 tokens through 4096 x 11264, x W1 36.5 us (5.1 TB/s, 176 workgroups),
+// h W2 17.6 (5.2 TB/s, 512); 1000 through 2176 x 1152, 26 and 16 (0.38 and 0.31 PFLOP/s).
 #pragma once
 #include "gemm_span.hpp"
 
@@ -104,6 +107,7 @@ struct FfnCols {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
+
 // Columns of a matrix whose rows are the contraction (tokens), for either side: token t of column c at t * pitch + lane_bytes(c) bytes from
 // base; tokens past the last one repeat it.  LDS and fragments as FfnCols.
 struct FfnTokenCols : FfnCols<false> {
@@ -129,6 +133,7 @@ struct FfnTokenCols : FfnCols<false> {
     dma16_at<j * kSpanWaves * 1024>(src.base, off + min((uint32_t)(src.k + STEP * j + krow), last) * pitch, slot);
   }
 };
+
 // rows at a fixed pitch (k-contiguous weights): a multiple of 32 of them, the last 32 repeated where the tile sticks out
 struct FfnWeightRows : SpanPitchedRows<kFfnCols> {
   using Base = SpanPitchedRows<kFfnCols>;
