@@ -522,6 +522,8 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * a multiple of 32 (may be NULL; the last group is not written, but may be read).
  * A launch does `rows` rows; with all pointers moved on by a multiple of 32 rows, several do the rows of one block.
  * D and H multiples of 32, D * H * 4 < 4 GiB; row pitches multiples of 8; pointers to bf16 and fp32 data on 16-byte boundaries.
+ * h of up to 16 rows takes two rows each, bf16 of it and, `rows` further on, of what that leaves: momoe_ffn_h_rows(rows) says how many, and ldm is
+ * that many at least for the two products of the forward.
  * momoe_ffn_lin1_fwd: h; ab, of the first ab_rows rows, a multiple of 32 (0: none).
  * momoe_ffn_lin2_fwd: y [rows][D].
  * momoe_ffn_dgrad_h: u.  momoe_ffn_swiglu_bwd: gz and hT, a | b made again from x.
@@ -534,7 +536,8 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * momoe_ffn_gradients_workspace_bytes(rows, D, H, which are wanted); 0 (NULL): none is needed.
  */
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
-int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction);
+int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t H);
+int64_t momoe_ffn_h_rows(int64_t rows);
 int64_t momoe_ffn_gradients_workspace_bytes(int64_t rows, int64_t D, int64_t H, int wants_x, int wants_W1, int wants_W2);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);
@@ -571,12 +574,14 @@ int momoe_int4_pack_weights(const void* codes_NRC, const void* scale, int scale_
 /* The experts.  tile_table: of momoe_index_build for `tile_rows` rows, 32 or 64, whichever momoe_int4_tile_rows says suits the sizes (64
  * only where the rows of x take less than 4 GiB, M * ldx * 2 < 2^32).  A product of few tiles is cut along its contraction of K into
  * momoe_int4_slices(Msum, N, cols, K, tile_rows) slices, 1 if it is not.
+ * h has momoe_int4_h_rows(Msum, N) rows: behind Msum of them, of up to 16 an expert on average, what bf16 leaves of each (of a dense block N = 1).
  * momoe_int4_lin1_swiglu_fwd (cols 2H, K = D): h bf16 [Msum][H] = a * b * sigmoid(b), a | b = x[idx[r]] . Wl1[i]; x bf16 with row pitch ldx, a
  * multiple of 8; workspace: of more than one slice, slices * Msum * 2H * 4 bytes (else NULL).
  * momoe_int4_lin2_scale_fwd (cols D, K = H): ys fp32 [slices][Msum][D], the sum over the slices (h[r] . Wl2[i]) * s[i, idx[r]].
  * momoe_int4_combine: out_MD bf16 [M][D], out[m] = the sum of its experts' rows and their slices, in fp32, rounded once.
  * Pointers to rows, weights and results on 16-byte boundaries. */
 int momoe_int4_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N);
+int64_t momoe_int4_h_rows(int64_t Msum, int64_t N);
 int momoe_int4_slices(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows);
 int momoe_int4_lin1_swiglu_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, int group,
                                const int32_t* idx_Msum, const int32_t* tile_table, int tile_rows, void* h_MsumH, void* workspace,
@@ -588,7 +593,7 @@ int momoe_int4_combine(const float* ys_MsumD, int slices, const int32_t* inv_MK,
                        void* stream);
 
 /* A dense block: y = (a * b * sigmoid(b)) . Wl2, a | b = x . Wl1, weights as of one expert.  x bf16 with row pitch ldx, a multiple of 8;
- * h_MH bf16 [M][H] and workspace (momoe_int4_ffn_workspace_bytes; 0: NULL) scratch; y bf16 [M][D].  All on 16-byte boundaries. */
+ * h_MH bf16 [momoe_int4_h_rows(M, 1)][H] and workspace (momoe_int4_ffn_workspace_bytes; 0: NULL) scratch; y bf16 [M][D].  All on 16-byte boundaries. */
 int64_t momoe_int4_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H);
 int momoe_int4_ffn_fwd(const void* x_MD, int64_t ldx, const void* Wl1_packed, const void* Wl1_words, const void* Wl2_packed,
                        const void* Wl2_words, int group, void* h_MH, void* y_MD, void* workspace, int64_t workspace_bytes, int64_t M,

@@ -171,6 +171,11 @@ using TileSched = TileSchedT<>;
 
 __device__ __forceinline__ float bf2f(bf16 v) { return (float)v; }
 __device__ __forceinline__ bf16 f2bf(float v) { return (bf16)v; }
+// what is left of v where `first` is v rounded to bf16: of an infinity nothing, so that it stays one
+__device__ __forceinline__ float rest_of(float v, bf16 first) {
+  const float d = v - bf2f(first);
+  return fabsf(d) <= fabsf(v) ? d : 0.0f;
+}
 
 // 1 / (1 + e^-v) with the hardware reciprocal (1 ulp): a plain `1.0f / x` compiles to the
 // correctly rounded division, ten instructions where the results are rounded to bf16 anyway

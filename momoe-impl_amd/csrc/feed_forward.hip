@@ -7,7 +7,9 @@
 // what meets in an epilogue is not rounded before: a | b that are kept for the backward, and u where a | b are made again, go through
 // memory in fp32, as whole accumulator fragments ([row / 16][column / 16][64 lanes][4]: 1 KiB a store).  (In bf16 they cost half as much
 // traffic and a rounding each, which doubles the error of the weight gradients.)
-//   h       [H / 32][ldm][32]    k-blocked, as the second product contracts over it
+//   h       [H / 32][ldm][32]    k-blocked, as the second product contracts over it; of up to kTwiceRows rows each of them is two, bf16 of
+//                                it and of what that leaves, as a tile has room for both: rounded, the h of one token, few of which are large,
+//                                can be more of y's error than y's own rounding (0.0023 to 0.0024 of the norm against 64 bits, then 0.0017)
 //   gz      [2H / 32][ldm][32]   G_a | G_b, k-blocked, for G_x and the gradient of W1; zeros behind the last row up to a multiple of 32
 //   hT      [rows / 32][H][32]   h once more, feature-major in groups of 32 rows, zeros behind the last row: for the gradient of W2
 // The weights' gradients are momoe_wgrad of one expert where their launches are large, and tiles of 128 x 128 where they are small.
@@ -18,6 +20,9 @@
 
 namespace momoe {
 namespace {
+
+constexpr int64_t kTwiceRows = 16;
+int64_t rows_of_h(int64_t rows) { return rows <= kTwiceRows ? 2 * rows : rows; }
 
 struct FfnArgs {
   const bf16* x;   // x, or G_y of the products with W2^T
@@ -36,6 +41,7 @@ struct FfnArgs {
   float* part;     // its sums by slices of the contraction, [slices][rows][D], where there are several
   int64_t total;   // tokens that a gradient of the weights is contracted over
   int slices = 1;
+  bool twice = false;  // h W2 of rows that are two each: sums of both go to `part`
   int32_t* counts; // {0, all tokens}: what momoe_wgrad takes as the rows of its one expert
   unsigned long long* clk = clock_trace_buffer();
 };
@@ -76,7 +82,7 @@ struct FfnProg {
       for (int i = 0; i < FM; ++i) {
         const int r = 16 * (wm * FM + i) + (l & 15);
         if (r >= rows_) continue;
-        if (slices > 1) *(f32x4*)(p.part + (slice * rows + row0 + r) * p.D + col) = acc[j][i];
+        if (slices > 1 || p.twice) *(f32x4*)(p.part + (slice * rows + row0 + r) * p.D + col) = acc[j][i];
         else *(bf16x4*)(p.out + (row0 + r) * p.D + col) = pack_bf16x4(acc[j][i], 1.0f);
       }
     }
@@ -127,9 +133,18 @@ struct FfnLin1 : FfnProg<FM> {
           if (r0 < rows) u = *(const f32x4*)(p.u + fragment_at((row0 + r0) >> 4, (j0 >> 4) + f, p.H, l));
           Base::store_grads(row, r < rows, col, a, b, u);
         } else {
-          if (p.h && r < rows)
-            *(bf16x4*)(p.h + ((int64_t)(col >> 5) * p.ldm + row) * 32 + (col & 31)) =
-                pack_bf16x4(f32x4{swiglu(a[0], b[0]), swiglu(a[1], b[1]), swiglu(a[2], b[2]), swiglu(a[3], b[3])}, 1.0f);
+          if (r < rows) {
+            const f32x4 h{swiglu(a[0], b[0]), swiglu(a[1], b[1]), swiglu(a[2], b[2]), swiglu(a[3], b[3])};
+            bf16* const to = p.h + ((int64_t)(col >> 5) * p.ldm + row) * 32 + (col & 31);
+            const bf16x4 first = pack_bf16x4(h, 1.0f);
+            *(bf16x4*)to = first;
+            if (p.rows <= kTwiceRows) {
+              bf16x4 rest;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) rest[e] = f2bf(rest_of(h[e], first[e]));
+              *(bf16x4*)(to + p.rows * 32) = rest;
+            }
+          }
           if (row0 + r0 < p.ab_rows) {
             *(f32x4*)(p.ab + fragment_at((row0 + r0) >> 4, (j0 >> 4) + f, 2 * p.H, l)) = a;
             *(f32x4*)(p.ab + fragment_at((row0 + r0) >> 4, ((p.H + j0) >> 4) + f, 2 * p.H, l)) = b;
@@ -272,8 +287,9 @@ struct FfnSums {
   int64_t n[3];
   int slices[3], count = 0;
   void add(const FfnArgs& a) {
-    if (a.slices == 1) return;
-    part[count] = a.part, out[count] = a.out, n[count] = a.rows * a.D, slices[count++] = a.slices;
+    if (a.slices == 1 && !a.twice) return;
+    // (the second half of a slice's rows as a slice of its own)
+    part[count] = a.part, out[count] = a.out, n[count] = a.rows * a.D / (a.twice ? 2 : 1), slices[count++] = a.slices * (a.twice ? 2 : 1);
   }
 };
 __global__ __launch_bounds__(256) void ffn_sum_slices_kernel(FfnSums p) {
@@ -670,7 +686,7 @@ __global__ __launch_bounds__(kSpanThreads, 1) void ffn_span_kernel(FfnArgs p, in
 // 1000, 4096 x 2048, 32, 34.4 | 48.5; 24 tokens, x W1 of 4096 x 11264, 88, hardly filled, 36.5 | 58.  8192 tokens through 2048 x 8192: 414 (1.33 PFLOP/s) and 199 (1.38), 16384 through 4096 x 11264: 2329 (1.30)
 // and 1064 (1.42): what a large library product of these sizes reaches; bound by the matrix instructions at the clock that the card holds.
 inline bool takes_span(int64_t rows, int64_t cols, int64_t contraction) {
-  return contraction >= WideSpan::AHEAD * kSpan && 10 * rows * cols >= 3 * persistent_grid() * (int64_t)(WideSpan::MAX_ROWS * WideSpan::COLS);
+  return rows > 2 * kTwiceRows && contraction >= WideSpan::AHEAD * kSpan && 10 * rows * cols >= 3 * persistent_grid() * (int64_t)(WideSpan::MAX_ROWS * WideSpan::COLS);
 }
 template <class P>
 int launch_dense_span(const FfnArgs& a, int64_t cols, hipStream_t st) {
@@ -690,6 +706,12 @@ int64_t slices_bytes(int64_t rows, int64_t D, int64_t contraction) {
   if (takes_span(rows, D, contraction)) return 0;
   const FfnPlan plan = plan_of(rows, cdiv64(D, kFfnCols), contraction, D);
   return plan.slices > 1 ? plan.slices * rows * D * 4 : 0;
+}
+
+// of h W2, whose rows may be two each
+int64_t lin2_bytes(int64_t rows, int64_t D, int64_t H) {
+  if (rows > kTwiceRows) return slices_bytes(rows, D, H);
+  return plan_of(2 * rows, cdiv64(D, kFfnCols), H, D).slices * 2 * rows * D * 4;
 }
 
 int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
@@ -749,7 +771,7 @@ extern "C" int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols) {
 extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                                   int64_t ldm, int64_t D, int64_t H, void* stream) {
   if (!x || !W1_D2H || !h_blocked || (ab_rows > 0 && !ab) || ab_rows < 0 || ab_rows > (rows + 31) / 32 * 32 || ldx < D) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, ldm, D, H);
+  const int st = check_ffn(rows_of_h(rows), ldm, D, H);
   if (st != MOMOE_OK) return st;
   if (any_unaligned({x, W1_D2H, h_blocked, ab})) return MOMOE_ERR_BAD_ARG;
   if (ldx % 8 != 0 || ldx >= (1 << 22) || ab_rows % 32 != 0) return MOMOE_ERR_UNSUPPORTED;
@@ -760,17 +782,19 @@ extern "C" int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H
   return launch<Lin1DenseSpan<false>, Lin1Fwd>(a, 2 * H, D, cdiv64(H, 64), (hipStream_t)stream);
 }
 
-extern "C" int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t contraction) {
-  return rows <= 0 || D <= 0 || contraction <= 0 ? -1 : slices_bytes(rows, D, contraction);
+extern "C" int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t H) {
+  return rows <= 0 || D <= 0 || H <= 0 ? -1 : lin2_bytes(rows, D, H);
 }
+extern "C" int64_t momoe_ffn_h_rows(int64_t rows) { return rows < 0 ? -1 : rows_of_h(rows); }
 
 extern "C" int momoe_ffn_lin2_fwd(const void* h_blocked, const void* W2_HD, void* y, int64_t rows, int64_t ldm, int64_t D, int64_t H,
                                   void* workspace, int64_t workspace_bytes, void* stream) {
   if (!h_blocked || !W2_HD || !y || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
-  const int st = check_ffn(rows, ldm, D, H);
+  const int st = check_ffn(rows_of_h(rows), ldm, D, H);
   if (st != MOMOE_OK) return st;
-  if (any_unaligned({h_blocked, W2_HD, y, workspace}) || workspace_bytes < slices_bytes(rows, D, H)) return MOMOE_ERR_BAD_ARG;
-  FfnArgs a{nullptr, 0, (const bf16*)W2_HD, rows, ldm, (int)D, (int)H};
+  if (any_unaligned({h_blocked, W2_HD, y, workspace}) || workspace_bytes < lin2_bytes(rows, D, H)) return MOMOE_ERR_BAD_ARG;
+  FfnArgs a{nullptr, 0, (const bf16*)W2_HD, rows_of_h(rows), ldm, (int)D, (int)H};
+  a.twice = rows <= kTwiceRows;
   a.part = (float*)workspace;
   a.h = (bf16*)h_blocked;
   a.out = (bf16*)y;

@@ -43,6 +43,8 @@ struct Int4Args {
   int slices;
   float* part;
   int64_t all_rows;
+  // elements from h to what its rounding to bf16 leaves, of tiles of up to 16 rows; 0: not kept
+  int64_t rest;
 };
 
 // Eight codes of a word as 128 + code, two at a time; k128: 0x43004300 in a vector register (of two constants outside them the and and
@@ -90,7 +92,11 @@ struct Int4Sched {
 template <bool FIRST>
 __device__ __forceinline__ void store_pair(const Int4Args& p, int64_t row, int pair, int col, float v0, float v1, float s) {
   if constexpr (FIRST) {
-    ((bf16*)p.out)[row * p.ldo + 16 * pair + col] = f2bf(v0 * v1 * sigmoidf_fast(v1));
+    const float h = v0 * v1 * sigmoidf_fast(v1);
+    bf16* const to = (bf16*)p.out + row * p.ldo + 16 * pair + col;
+    const bf16 first = f2bf(h);
+    to[0] = first;
+    if (p.rest) to[p.rest] = f2bf(rest_of(h, first));
   } else {
     const int64_t to = row * p.ldo + 32 * pair + col;
     if (p.idx) {
@@ -105,11 +111,12 @@ __device__ __forceinline__ void store_pair(const Int4Args& p, int64_t row, int p
 
 // Tiles of up to 32 rows.  A wavefront owns a pair of 16-column groups; KS of them share its contraction, a block of 128 k-values in
 // KS each, and their sums meet in LDS.  Codes and scales go straight into registers, AHEAD blocks ahead; the rows come to LDS,
-// kFewBytes of them at a time, for all wavefronts.  Bound by the codes' way from memory where they are many, 1 token through 4096 x 11264 in
-// 27 us (71 MB, 2.6 TB/s over both launches), else by the first answer of memory: 8 of 128 experts of 2048 x 768, 7.7 and 6.0 us.
+// kFewBytes of them at a time, for all wavefronts.  Bound by the rows' way to LDS where they are many, 50 tokens through 2176 x 1152
+// in groups of 32 in 14.6 and 11.1 us, else by the first answer of memory: 8 of 128 experts of 2048 x 768, 7.7 and 6.0 us.
 constexpr int kFewThreads = 256, kFewWaves = kFewThreads / 64, kFewBytes = 32 << 10;
 
-template <bool FIRST, int KS, int SG>
+// REST: of the second product, with what bf16 left of h (for all of them: 50 tokens, 2176 x 1152, groups of 32, 28 us instead of 25).
+template <bool FIRST, bool REST, int KS, int SG>
 __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args p) {
   constexpr int FR = 2, ROWS = 16 * FR, PW = kFewWaves / KS;
   constexpr int AHEAD = SG == 4 ? 2 : 4;  // (four of the smallest groups' scales were spilled)
@@ -123,12 +130,17 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
   for (TileCoord tc = sched.next(); tc.valid; tc = sched.next()) {
     const int pair = min(tc.tn * PW + cw, p.pairs - 1);
     const bool real = tc.tn * PW + cw < p.pairs;
-    const int nf = (tc.rows + 15) >> 4;
+    // of up to 16 rows of h a second fragment holds what the first one's rounding left
+    const bool twice = REST && tc.rows <= 16;
+    const int nf = twice ? 2 : (tc.rows + 15) >> 4, held = twice ? 2 * tc.rows : tc.rows;
+    int at_row[FR];
+#pragma unroll
+    for (int i = 0; i < FR; ++i) at_row[i] = min((twice ? 0 : 16 * i) + (l & 15), tc.rows - 1) + (twice ? i * tc.rows : 0);
     const int64_t group = ((int64_t)tc.expert * p.pairs + pair) * 2 * p.KB;
     const uint8_t* const w0 = p.w + group * kInt4Frag + l * 16;
     const uint32_t* const s0 = p.scale + (group * 16 + (l & 15)) * SG;
     f32x4 acc[2][FR] = {};
-    const int chunk = kFewBytes / (tc.rows * kInt4Block * 2);  // blocks of the tile's rows that LDS holds, four at least
+    const int chunk = kFewBytes / (held * kInt4Block * 2);  // blocks of the tile's rows that LDS holds, four at least
     for (int k0 = 0; k0 < p.KB; k0 += chunk) {
       const int blocks = min(chunk, p.KB - k0), steps = (blocks - kw + KS - 1) / KS;  // (none for a wavefront past the last)
       u32x4 wq[AHEAD][2];
@@ -147,17 +159,18 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
       __syncthreads();  // (the last rows, or sums, are done with)
       // 16 pieces of 8 values a row and block, piece c of row r at c ^ (r % 16): the 16 rows of a fragment read meet different
       // banks.  Rows that the tile does not have are read as its last one, and nobody stores what becomes of them.
-      const int all = blocks * tc.rows * 16;
+      const int all = blocks * held * 16;
       for (int q0 = tid; q0 < all; q0 += 2 * kFewThreads) {
         bf16x8 v[2];
         int to[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          const int q = min(q0 + a * kFewThreads, all - 1), piece = q & 15, kb = (q >> 4) / tc.rows, r = (q >> 4) - kb * tc.rows;
-          const int c = (k0 + kb) * kInt4Block + piece * 8, row = tc.row0 + r;
-          v[a] = *(const bf16x8*)(p.rows + (int64_t)(FIRST && p.idx ? p.idx[row] : row) * p.ld + min(c, p.K - 8));
+          const int q = min(q0 + a * kFewThreads, all - 1), piece = q & 15, kb = (q >> 4) / held, r = (q >> 4) - kb * held;
+          const bool rest = REST && r >= tc.rows;
+          const int c = (k0 + kb) * kInt4Block + piece * 8, row = tc.row0 + (rest ? r - tc.rows : r);
+          v[a] = *(const bf16x8*)(p.rows + (rest ? p.rest : 0) + (int64_t)(FIRST && p.idx ? p.idx[row] : row) * p.ld + min(c, p.K - 8));
           if (c >= p.K) v[a] = bf16x8{};
-          to[a] = (kb * tc.rows + r) * 256 + ((piece ^ (r & 15)) << 4);
+          to[a] = (kb * held + r) * 256 + ((piece ^ (r & 15)) << 4);
         }
 #pragma unroll
         for (int a = 0; a < 2; ++a) *(bf16x8*)(lds + to[a]) = v[a];
@@ -173,8 +186,8 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
         unrolled<0, FR>([&](auto IC) {
           constexpr int i = decltype(IC)::value;
           if (i >= nf) return;  // (the same for all lanes)
-          const int row = min(16 * i + (l & 15), tc.rows - 1);
-          const uint8_t* const from = lds + (kb * tc.rows + row) * 256;
+          const int row = at_row[i];
+          const uint8_t* const from = lds + (kb * held + row) * 256;
           bf16x8 rf[4];
 #pragma unroll
           for (int m = 0; m < 4; ++m) rf[m] = *(const bf16x8*)(from + (((4 * m + (l >> 4)) ^ (row & 15)) << 4));
@@ -215,6 +228,10 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
         constexpr int q = decltype(QC)::value;
         if (step + q + AHEAD < steps) multiply(q, step + q + AHEAD);
       });
+    }
+    if (twice) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[j][0] += acc[j][1];
     }
     if constexpr (KS > 1) {
       __syncthreads();
@@ -260,15 +277,16 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
 // whose sums int4_h_of_slices_kernel or the last kernel adds up.
 struct Int4Rows {
   static constexpr int BM = 64, DEP = BM * 256 / (kSpanWaves * 1024), STAGE = BM * 256;  // bytes
-  const char* base;
+  const char *base, *second;  // of the second deposit, which may be what the first one's rounding left
   uint32_t off[DEP];
-  __device__ __forceinline__ void init(const Int4Args& p, const TileCoord& tc, bool gather) {
+  __device__ __forceinline__ void init(const Int4Args& p, const TileCoord& tc, bool gather, bool twice) {
     const int l = fresh_lane();
     base = (const char*)p.rows;
     if (!gather) base += (int64_t)tc.row0 * p.ld * 2;
+    second = twice ? base + p.rest * 2 : base;
 #pragma unroll
     for (int j = 0; j < DEP; ++j) {
-      const int r = min((j * kSpanWaves + wave_id()) * 4 + (l >> 4), tc.rows - 1);
+      const int r = min(((twice ? 0 : j) * kSpanWaves + wave_id()) * 4 + (l >> 4), tc.rows - 1);
       off[j] = (uint32_t)(gather ? p.idx[tc.row0 + r] : r) * (uint32_t)(2 * p.ld);
     }
   }
@@ -279,7 +297,7 @@ struct Int4Rows {
     const uint32_t at = (uint32_t)min(kb * kInt4Block + piece * 8, K - 8) * 2;
     unrolled<0, DEP>([&](auto J) {
       constexpr int j = decltype(J)::value;
-      if (j < nf) dma16_at<j * kSpanWaves * 1024>(base, off[j] + at, slot);
+      if (j < nf) dma16_at<j * kSpanWaves * 1024>(j == 1 ? second : base, off[j] + at, slot);
     });
   }
 };
@@ -299,12 +317,14 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
   struct Tile {
     TileCoord tc;
     int slice, kb0, kb1, nf, pair0;
+    bool twice;  // of up to 16 rows of h a second fragment holds what the first one's rounding left
     __device__ __forceinline__ void place(const Int4Args& p, const TileCoord& t) {
       tc = t;
       const int tn = t.tn / p.slices;
       slice = t.tn - tn * p.slices;
       kb0 = (int)((int64_t)p.KB * slice / p.slices), kb1 = (int)((int64_t)p.KB * (slice + 1) / p.slices);
-      nf = (t.rows + 15) >> 4;
+      twice = !FIRST && p.rest && t.rows <= 16;
+      nf = twice ? 2 : (t.rows + 15) >> 4;
       pair0 = tn * PAIRS + 2 * wave_id();
     }
   };
@@ -335,13 +355,13 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
     A.request(next.kb0, p.K, next.nf, addr + q * Rows::STAGE);
     load(next.kb0);
   };
-  A.init(p, next.tc, FIRST && p.idx);
+  A.init(p, next.tc, FIRST && p.idx, next.twice);
   begin();
   while (true) {
     cur = next;
     next.place(p, sched.next());
     Rows B;  // rows of the next tile: their tokens travel meanwhile
-    if (next.tc.valid) B.init(p, next.tc, FIRST && p.idx);
+    if (next.tc.valid) B.init(p, next.tc, FIRST && p.idx, next.twice);
     const int nf = cur.nf;
     f32x4 acc[4][4] = {};
     // -(128 + zero) scale of up to four groups, lane l that of group l / 16 and column l % 16, for what these take away of acc
@@ -420,6 +440,10 @@ __global__ __launch_bounds__(kSpanThreads, 2) void int4_tile_kernel(Int4Args p) 
     __builtin_amdgcn_s_barrier();
     order_fence();
     take_away();
+    if (cur.twice) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j][0] += acc[j][1];
+    }
     if (next.tc.valid) {
       A = B;
       begin();
@@ -473,16 +497,21 @@ __device__ __forceinline__ f32x4 sum_of_slices(const float* p, int slices, int64
 }
 // h from the slices of a | b, fp32 [slices][rows][2H]
 __global__ __launch_bounds__(256) void int4_h_of_slices_kernel(const float* __restrict__ part, bf16* __restrict__ h, int64_t rows, int H,
-                                                               int slices) {
+                                                               int slices, int64_t rest) {
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, row = q / (H / 4);
   const int col = (int)(q - row * (H / 4)) * 4;
   if (row >= rows) return;
   const float* const from = part + row * 2 * H + col;
   const f32x4 a = sum_of_slices(from, slices, rows * 2 * H), b = sum_of_slices(from + H, slices, rows * 2 * H);
-  bf16x4 v;
+  bf16x4 v, left;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = f2bf(a[e] * b[e] * sigmoidf_fast(b[e]));
+  for (int e = 0; e < 4; ++e) {
+    const float x = a[e] * b[e] * sigmoidf_fast(b[e]);
+    v[e] = f2bf(x);
+    left[e] = f2bf(rest_of(x, v[e]));
+  }
   *(bf16x4*)(h + row * H + col) = v;
+  if (rest) *(bf16x4*)(h + rest + row * H + col) = left;
 }
 // y of a dense block from its slices, fp32 [slices][n]
 __global__ __launch_bounds__(256) void int4_sum_slices_kernel(const float* __restrict__ part, bf16* __restrict__ y, int64_t n, int slices) {
@@ -578,17 +607,21 @@ int check_int4(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, int gro
 }
 bool unaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
-template <bool FIRST, int SG>
+template <bool FIRST, bool REST, int SG>
 int launch_few(const Int4Args& a, int64_t tiles, hipStream_t st) {
   const int64_t wanted = 3 * persistent_grid();
   const auto enough = [&](int ks) { return a.KB < 2 * ks || tiles * cdiv64(a.pairs, kFewWaves / ks) >= wanted; };
-  auto kernel = enough(1) ? int4_few_rows_kernel<FIRST, 1, SG> : enough(2) ? int4_few_rows_kernel<FIRST, 2, SG> : int4_few_rows_kernel<FIRST, 4, SG>;
+  auto kernel = enough(1)   ? int4_few_rows_kernel<FIRST, REST, 1, SG>
+                : enough(2) ? int4_few_rows_kernel<FIRST, REST, 2, SG>
+                            : int4_few_rows_kernel<FIRST, REST, 4, SG>;
   kernel<<<(unsigned)wanted, kFewThreads, 0, st>>>(a);
   return launch_status();
 }
 template <bool FIRST, int SG>
 int launch_rows(const Int4Args& a, int64_t tiles, int tile_rows, hipStream_t st) {
-  if (tile_rows == 32) return launch_few<FIRST, SG>(a, tiles, st);
+  if constexpr (!FIRST)
+    if (tile_rows == 32 && a.rest) return launch_few<false, true, SG>(a, tiles, st);
+  if (tile_rows == 32) return launch_few<FIRST, false, SG>(a, tiles, st);
   int4_tile_kernel<FIRST, SG><<<(unsigned)(2 * persistent_grid()), kSpanThreads, 0, st>>>(a);
   return launch_status();
 }
@@ -620,16 +653,21 @@ int slices_of(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
   return (int)n;
 }
 
+// What bf16 leaves of h is kept, too, of up to 16 rows an expert on average, and meets the weights as rows of their tiles' second fragments: of
+// so few results the error depends on the few large values of h (one token against 64 bits 0.0017 to 0.0024 of the norm, 0.0017 this way).
+bool keeps_rest(int64_t Msum, int64_t N) { return Msum <= 16 * N; }
+
 // the first product, of experts or of a dense block, with the sums of its slices in the workspace
 int launch_first(Int4Args a, int64_t N, int64_t Msum, int tile_rows, int group, void* workspace, int64_t workspace_bytes, hipStream_t st) {
   a.slices = slices_of(Msum, N, 2 * a.ldo, a.K, tile_rows);
   a.part = (float*)workspace;
   a.all_rows = Msum;
+  a.rest = keeps_rest(Msum, N) ? Msum * a.ldo : 0;
   if (a.slices > 1 && (!workspace || workspace_bytes < a.slices * Msum * 2 * a.ldo * 4)) return MOMOE_ERR_BAD_ARG;
   const int status = launch<true>(a, row_tiles_of(Msum, N, tile_rows), tile_rows, group, st);
   if (status != MOMOE_OK || a.slices == 1) return status;
   const int64_t quads = Msum * (a.ldo / 4);
-  int4_h_of_slices_kernel<<<(unsigned)cdiv64(quads, 256), 256, 0, st>>>(a.part, (bf16*)a.out, Msum, (int)a.ldo, a.slices);
+  int4_h_of_slices_kernel<<<(unsigned)cdiv64(quads, 256), 256, 0, st>>>(a.part, (bf16*)a.out, Msum, (int)a.ldo, a.slices, a.rest);
   return launch_status();
 }
 
@@ -665,6 +703,7 @@ extern "C" int momoe_int4_pack_weights(const void* codes_NRC, const void* scale,
 extern "C" int momoe_int4_tile_rows(int64_t Msum, int64_t D, int64_t H, int64_t N) {
   return Msum <= 0 || D <= 0 || H <= 0 || N <= 0 ? 0 : tile_rows_of(Msum, D, H, N);
 }
+extern "C" int64_t momoe_int4_h_rows(int64_t Msum, int64_t N) { return Msum < 0 || N <= 0 ? -1 : keeps_rest(Msum, N) ? 2 * Msum : Msum; }
 extern "C" int momoe_int4_slices(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
   return Msum <= 0 || N <= 0 || cols <= 0 || K <= 0 ? 0 : slices_of(Msum, N, cols, K, tile_rows);
 }
@@ -706,6 +745,7 @@ extern "C" int momoe_int4_lin2_scale_fwd(const void* h_MsumH, const void* Wl2_pa
   a.slices = slices_of(Msum, N, D, H, tile_rows);
   a.part = ys_MsumD;
   a.all_rows = Msum;
+  a.rest = keeps_rest(Msum, N) ? Msum * H : 0;
   return launch<false>(a, row_tiles_of(Msum, N, tile_rows), tile_rows, group, (hipStream_t)stream);
 }
 
@@ -751,6 +791,7 @@ extern "C" int momoe_int4_ffn_fwd(const void* x_MD, int64_t ldx, const void* Wl1
   b.slices = slices_of(M, 1, D, H, tile_rows);
   b.part = (float*)workspace;
   b.all_rows = M;
+  b.rest = keeps_rest(M, 1) ? M * H : 0;
   st = launch<false>(b, cdiv64(M, tile_rows), tile_rows, group, to);
   if (st != MOMOE_OK || b.slices == 1) return st;
   int4_sum_slices_kernel<<<(unsigned)cdiv64(M * D, 1024), 256, 0, to>>>(b.part, (bf16*)y_MD, M * D, b.slices);

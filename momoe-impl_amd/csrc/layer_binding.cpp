@@ -577,13 +577,14 @@ FeedForward feed_forward_forward(const Tensor& x, const Tensor& W1, const Tensor
   if (M > 0) {
     if (msave > 0) f.ab = fragments(msave, 2 * H, dev);
     const int64_t ws_bytes = momoe_ffn_workspace_bytes(M, D, H);
-    Transients transients(dev, {M * H * 2, ws_bytes});
+    const int64_t ldm = momoe_ffn_h_rows(M), h_bytes = ldm * H * 2;
+    Transients transients(dev, {h_bytes, ws_bytes});
     Tensor h_own, ws_own;
-    void* const h = transients.take(M * H * 2, h_own);
+    void* const h = transients.take(h_bytes, h_own);
     MOMOE_CALL(momoe_ffn_lin1_fwd, st, f.x.data_ptr(), pitch_of_rows(f.x), f.W1.data_ptr(), h, msave > 0 ? f.ab.data_ptr<float>() : nullptr,
-               (msave + 31) / 32 * 32, M, M, D, H);
+               (msave + 31) / 32 * 32, M, ldm, D, H);
     void* const ws = ws_bytes > 0 ? transients.take(ws_bytes, ws_own) : nullptr;
-    MOMOE_CALL(momoe_ffn_lin2_fwd, st, (const void*)h, f.W2.data_ptr(), f.y.data_ptr(), M, M, D, H, ws, ws_bytes);
+    MOMOE_CALL(momoe_ffn_lin2_fwd, st, (const void*)h, f.W2.data_ptr(), f.y.data_ptr(), M, ldm, D, H, ws, ws_bytes);
   }
   if (x.device() != dev) f.y = f.y.to(x.device());
   return f;
@@ -716,7 +717,8 @@ std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, c
   Index ib(M, N, K, tile_rows, false);
   const int64_t ws_bytes = momoe_index_workspace_bytes(M, N), index_bytes = ib.ints * 4;
   const int64_t scratch_bytes = (4 + ((msum + 3) & ~(int64_t)3) + (ws_bytes + 3) / 4) * 4;
-  Transients transients(dev, {index_bytes, scratch_bytes, msum * H * 2, ws1_bytes, ys_bytes});
+  const int64_t h_bytes = momoe_int4_h_rows(msum, N) * H * 2;
+  Transients transients(dev, {index_bytes, scratch_bytes, h_bytes, ws1_bytes, ys_bytes});
   Tensor index_own, scratch, h_own, ws_own, ys_own, counter;
   ib.base = (int32_t*)transients.take(index_bytes, index_own);
   int32_t* const build = (int32_t*)transients.take(scratch_bytes, scratch);
@@ -728,7 +730,7 @@ std::tuple<Tensor, Tensor> experts_int4(const Tensor& x_BSD, const Tensor& W1, c
   MOMOE_CALL(momoe_index_build, st, mask.data_ptr<int32_t>(), mask.stride(0), mask.stride(1), M, N, K, sizes.data_ptr<int64_t>(),
              ib.cumsums(), ib.idx(), build + 4, ib.inv(), ib.table(), tile_rows, (int32_t*)nullptr,
              (void*)(build + 4 + ((msum + 3) & ~(int64_t)3)), ws_bytes, violations);
-  void* const h = transients.take(msum * H * 2, h_own);
+  void* const h = transients.take(h_bytes, h_own);
   void* const ws1 = ws1_bytes > 0 ? transients.take(ws1_bytes, ws_own) : nullptr;
   MOMOE_CALL(momoe_int4_lin1_swiglu_fwd, st, x.data_ptr(), pitch_of_rows(x), W1.data_ptr(), S1.data_ptr(), (int)group,
              (const int32_t*)ib.idx(), (const int32_t*)ib.table(), tile_rows, h, ws1, ws1_bytes, M, D, H, N, msum);
@@ -764,9 +766,10 @@ Tensor feed_forward_int4(const Tensor& x, const Tensor& W1, const Tensor& S1, co
   if (M > 0) {
     const Tensor rows = rows_in_bf16(x, M, D, dev);
     const int64_t ws_bytes = momoe_int4_ffn_workspace_bytes(M, D, H);
-    Transients transients(dev, {M * H * 2, ws_bytes});
+    const int64_t h_bytes = momoe_int4_h_rows(M, 1) * H * 2;
+    Transients transients(dev, {h_bytes, ws_bytes});
     Tensor h_own, ws_own;
-    void* const h = transients.take(M * H * 2, h_own);
+    void* const h = transients.take(h_bytes, h_own);
     void* const ws = ws_bytes > 0 ? transients.take(ws_bytes, ws_own) : nullptr;
     MOMOE_CALL(momoe_int4_ffn_fwd, st, rows.data_ptr(), pitch_of_rows(rows), W1.data_ptr(), S1.data_ptr(), W2.data_ptr(),
                S2.data_ptr(), (int)group, h, y.data_ptr(), ws, ws_bytes, M, D, H);

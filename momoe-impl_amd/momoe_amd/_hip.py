@@ -101,6 +101,7 @@ _SIGNATURES = {
     "momoe_ffn_fragment_floats": (_i64, [_i64] * 2),
     "momoe_ffn_gradients_workspace_bytes": (_i64, [_i64] * 3 + [_int] * 3),
     "momoe_ffn_lin1_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "momoe_ffn_h_rows": (_i64, [_i64]),
     "momoe_ffn_workspace_bytes": (_i64, [_i64] * 3),
     "momoe_ffn_lin2_fwd": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "momoe_ffn_dgrad_h": (_int, [_p, _i64, _p, _p, _i64, _i64, _i64, _p]),
@@ -111,6 +112,7 @@ _SIGNATURES = {
     "momoe_int4_scale_words": (_i64, [_i64] * 3 + [_int]),
     "momoe_int4_pack_weights": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _int, _int, _p, _p, _p]),
     "momoe_int4_tile_rows": (_int, [_i64] * 4),
+    "momoe_int4_h_rows": (_i64, [_i64] * 2),
     "momoe_int4_slices": (_int, [_i64] * 4 + [_int]),
     "momoe_int4_lin1_swiglu_fwd": (_int, [_p, _i64, _p, _p, _int, _p, _p, _int, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_int4_lin2_scale_fwd": (_int, [_p, _p, _p, _int, _p, _i64, _i64, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p]),

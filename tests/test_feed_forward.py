@@ -13,6 +13,11 @@ def test_sizes():
     assert lib.momoe_ffn_fragment_floats(-1, 64) == lib.momoe_ffn_fragment_floats(1, 24) == lib.momoe_ffn_fragment_floats(1, 0) == -1
 
 
+def test_rows_of_h():
+    assert [lib.momoe_ffn_h_rows(n) for n in (-1, 0, 1, 16, 17, 100)] == [-1, 0, 2, 32, 17, 100]
+    assert lib.momoe_ffn_workspace_bytes(5, 64, 64) == 2 * 5 * 64 * 4 and lib.momoe_ffn_lin1_fwd(P, 64, P, P, None, 0, 16, 31, 64, 32, None) == 1
+
+
 def _refuses(fn, good, pointers, aligned, optional=()):
     call = lambda **c: fn(*{**good, **c}.values(), None)
     assert all(call(**{k: None}) == 1 for k in pointers) and all(call(**{k: P + 8}) == 1 for k in aligned)

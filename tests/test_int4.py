@@ -18,6 +18,7 @@ def test_sizes():
     rows = lib.momoe_int4_tile_rows
     assert rows(0, 64, 64, 8) == rows(1, 0, 64, 8) == rows(1, 64, 0, 8) == rows(1, 64, 64, 0) == 0
     assert rows(8, 2048, 768, 128) == 32 and rows(8000, 2048, 768, 128) == 64 and rows(200, 1024, 1024, 1) == 32 and rows(300, 1024, 1024, 1) == 64
+    assert [lib.momoe_int4_h_rows(*n) for n in ((-1, 1), (1, 0), (0, 1), (16, 1), (17, 1), (2048, 128), (2049, 128))] == [-1, -1, 0, 32, 17, 4096, 2049]
     slices = lib.momoe_int4_slices
     assert slices(0, 1, 64, 64, 64) == slices(1, 0, 64, 64, 64) == slices(1, 1, 0, 64, 64) == slices(1, 1, 64, 0, 64) == 0
     assert slices(16, 1, 4096, 11264, 32) == 1 and slices(16, 1, 4096, 11264, 64) > 1 and slices(8000, 128, 1536, 2048, 64) == 1
