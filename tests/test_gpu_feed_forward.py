@@ -190,6 +190,23 @@ def test_rows_of_nan_and_infinity_stay_with_themselves(M, save):
     assert torch.equal(ok[:, cols], ref[3][:, cols]) and not ok[:, 5].isfinite().any() and not ok[:, 0].isfinite().any()
 
 
+def test_few_rows_of_nan_and_infinity():
+    """Rows that are two each; an infinite h stays one, and y with it."""
+    x, W1, W2, _ = [t.to(DEV) for t in _inputs(9, 96, 64)]
+    W2 = W2.abs() + 1
+    bad = x.clone()
+    bad[2, 5], bad[4] = float("nan"), 3e38
+    W1[:, 0], W1[:, 64] = 1, 1  # a and b of column 0 overflow together: h = inf
+    y, ref = _block(W1, W2)(bad), _block(W1, W2)(x)
+    keep = [0, 1, 3, 5, 6, 7, 8]
+    assert torch.equal(y[keep], ref[keep]) and y[2].isnan().all() and not y[4].isfinite().any()
+    big = torch.zeros(1, 96, device=DEV, dtype=torch.bfloat16)
+    big[0, 0] = 2.0 ** 70
+    V1, V2 = torch.zeros(96, 128, device=DEV), torch.ones(64, 96, device=DEV)
+    V1[0, 0], V1[0, 64] = 1, 1
+    assert (_block(V1, V2)(big) == float("inf")).all()
+
+
 @pytest.mark.parametrize("M,D,H", [(3, 96, 64), (70, 160, 288), (1100, 96, 64), (40, 1056, 4256)])
 def test_gradients_leave_what_lies_behind(M, D, H):
     """The entry points of the backward on buffers with room behind them: the last rows' padding is zeros, and the rest keeps its bits."""
