@@ -18,7 +18,8 @@ def _groups(n, group):
 
 def quantize(W, group_size=128):
     """Weights [.., R, C] -> (codes uint8 [.., R / 2, C], scale bf16 and zero uint8 [.., ceil(R / group_size), C]): the 16 values of a group
-    of a column reach from the lesser of its least weight and 0 to the greater of its greatest and 0, with 0 among them."""
+    of a column reach from the lesser of its least weight and 0 to the greater of its greatest and 0, with 0 among them.  A NaN or an infinity
+    leaves no number in its group: the scale is NaN or infinite, too."""
     if W.dim() > 2:
         parts = [quantize(w, group_size) for w in W]
         return tuple(torch.stack(t) for t in zip(*parts))
@@ -27,9 +28,10 @@ def quantize(W, group_size=128):
     w = torch.nn.functional.pad(W.detach().float(), (0, 0, 0, G * group_size - R)).view(G, group_size, C)
     lo, hi = w.amin(1).clamp_max(0), w.amax(1).clamp_min(0)
     scale = ((hi - lo) / 15).to(torch.bfloat16)
-    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
-    zero = torch.round(-lo / scale.float()).clamp(0, 15)
-    q = (torch.round(w / scale.float()[:, None]) + zero[:, None]).clamp(0, 15).to(torch.uint8).view(G * group_size, C)[:R]
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    # (what such a scale divides may be NaN, of which no whole number can be made)
+    zero = torch.round(-lo / scale.float()).nan_to_num(0).clamp(0, 15)
+    q = (torch.round(w / scale.float()[:, None]).nan_to_num(0) + zero[:, None]).clamp(0, 15).to(torch.uint8).view(G * group_size, C)[:R]
     return q[0::2] | (q[1::2] << 4), scale, zero.to(torch.uint8)
 
 

@@ -321,3 +321,24 @@ def test_refusals():
     for h, g in ((32, group), (H, 64), (H, 16), (0, group)):
         with pytest.raises(AssertionError):
             torch.ops.momoe.feed_forward_int4(x, *held, h, g)
+
+
+@pytest.mark.parametrize("M", [3, 40, 1100])
+def test_weights_of_nan_and_infinity_reach_the_results(M):
+    """A weight of the first matrix reaches every result, one of the second its column."""
+    D, H, N = 288, 160, 2
+    g = torch.Generator().manual_seed(4)
+    W1, W2 = torch.randn(N, D, 2 * H, generator=g) / D ** 0.5, torch.randn(N, H, D, generator=g) / H ** 0.5
+    x = _x(M, D).view(1, M, D).to(DEV)
+    mask, s = torch.ones(N, M, dtype=torch.int32, device=DEV), torch.ones(N, M, device=DEV)
+    for value in ("nan", "inf", "-inf"):
+        for first in (True, False):
+            V1, V2 = W1.clone(), W2.clone()
+            (V1 if first else V2)[0, 70, 33] = float(value)
+            moe = momoe_amd.MoMoE(D, H, N, N, 0, Wl1_ND2H=V1.to(DEV), Wl2_NHD=V2.to(DEV))
+            ffn = momoe_amd.FeedForward(D, H, 0, V1[0].to(DEV), V2[0].to(DEV))
+            for y in (momoe_amd.MoMoEInt4.from_momoe(moe, 64)(x, mask, s)[0], ffn.to_int4(64)(x)):
+                hit = torch.zeros(D, dtype=torch.bool, device=DEV)
+                hit[:] = first
+                hit[33] = True
+                assert not y[..., hit].isfinite().any() and y[..., ~hit].isfinite().all()

@@ -91,3 +91,21 @@ def test_quantize(group):
     # the nearest, but for a value half way between two, by fp32's rounding of the quotient
     assert ((v - W.double()).abs() <= (grid - W.double()).abs().amin(0) + each(scale) * 2.0 ** -18).all()
     assert (v[0, :, 3] == 0).all() and (zero[0, :, 4] == 0).all() and (zero[1, :, 5] == 15).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_of_nan_and_infinity(group):
+    """A weight that is no number leaves none in its group and column; every other group is as without it."""
+    W = torch.randn(2, 160, 24, generator=torch.Generator().manual_seed(1)) * 0.02
+    clean = quantize(W, group)
+    bad = W.clone()
+    where = ((0, 3, 5, "nan"), (0, 159, 7, "inf"), (1, 40, 0, "-inf"), (1, 0, 23, "nan"))
+    for n, r, c, v in where:
+        bad[n, r, c] = float(v)
+    bad[1, 41, 0] = float("inf")
+    q, scale, zero = quantize(bad, group)
+    assert zero.max() <= 15
+    v, hit = oracle.int4_weights(q, scale, zero, group), torch.zeros(2, 160, 24, dtype=torch.bool)
+    for n, r, c, _ in where:
+        hit[n, r // group * group:(r // group + 1) * group, c] = True
+    assert not v[hit].isfinite().any() and torch.equal(v[~hit], oracle.int4_weights(*clean, group)[~hit])
