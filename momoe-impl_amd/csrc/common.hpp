@@ -182,6 +182,9 @@ __device__ __forceinline__ float rest_of(float v, bf16 first) {
 __device__ __forceinline__ float sigmoidf_fast(float v) {
   return __builtin_amdgcn_rcpf(1.0f + __expf(-v));
 }
+// d (b sg) / d b where sg is b's sigmoid.  (sg + t - t sg of t = b sg is one instruction less, but loses the sum's ones to b from 2^24 on:
+// the slope came out as 0 there.)
+__device__ __forceinline__ float silu_slope(float b, float sg) { return sg * __builtin_fmaf(b, 1.0f - sg, 1.0f); }
 
 // Measurement aid (momoe_set_clock_trace): while a trace buffer is set, one wavefront of every
 // grouped-GEMM launch adds the shader-clock ticks it ran for to buf[0] and the ticks of the

@@ -58,7 +58,7 @@ struct SwigluGrad {
     const float sg = sigmoidf_fast(bv), t = bv * sg;  // silu(b)
     h = av * t;
     a = u * t;
-    b = (u * av) * __builtin_fmaf(-t, sg, sg + t);  // d silu / d b = sg (1 + b (1 - sg))
+    b = (u * av) * silu_slope(bv, sg);
   }
 };
 
