@@ -230,8 +230,7 @@ struct Lin1BwdSpan {
           part += u * hval;
           const float gh = sv * u;
           va[e] = gh * t;
-          // d silu / d b = sg (1 + b (1 - sg)) = sg + t - t sg
-          vb[e] = (gh * a) * __builtin_fmaf(-t, sg, sg + t);
+          vb[e] = (gh * a) * silu_slope(b, sg);
           hs[e] = some ? sv * hval : 0.0f;
         }
         if (j0 + 16 * f < H) gsum += part;
@@ -453,8 +452,7 @@ struct Lin1Prog {
           gsum += u * hval;
           const float gh = sv * u;
           va[e] = gh * t;
-          // d silu / d b = sg (1 + b (1 - sg)) = sg + t - t sg
-          vb[e] = (gh * a) * __builtin_fmaf(-t, sg, sg + t);
+          vb[e] = (gh * a) * silu_slope(b, sg);
           acc[0][i][4 * q + e] = sv * hval;  // a is not needed any more: keep hs in its place
         }
         stager.put(0, q, pack_bf16x4(va[0], va[1], va[2], va[3]));

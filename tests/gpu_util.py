@@ -170,3 +170,38 @@ def sampled_parity_on_device_inputs(M, D, H, N, K, Ks, skew, sp, B, experts, n_t
         assert_close(layer.Wl1_ND2H.grad[i], gW1[0], f"G_W1[{i}]")
         assert_close(layer.Wl2_NHD.grad[i], gW2[0], f"G_W2[{i}]")
         assert_close(sd.grad[i, sel.to(dev)], gs[0], f"G_s[{i}]")
+
+
+def large_gate_inputs(M, D, H):
+    """bf16 (x, W1, W2, G_y) of a SwiGLU block with gates of up to 2^30 either way, and ordinary ones, as W1 has them: rows of x that pick
+    its rows 0 (b) and 1 (a), rows of G_y that pick a column of W2 (u), so that a, b and u are exact."""
+    g = torch.Generator().manual_seed(M)
+    gates = torch.tensor([s * 2.0 ** k for k in range(10, 31) for s in (1, -1)] + [0, 1, -1, 3.5, -3.5, 8, -8, 12, -12, 20, 33])
+    W1, W2 = torch.zeros(D, 2 * H), 1 + torch.rand(H, D, generator=g)
+    W1[0, H:] = gates[torch.arange(H) % len(gates)]
+    W1[1, :H] = 1 + torch.rand(H, generator=g)
+    x, Gy, at = torch.zeros(M, D), torch.zeros(M, D), torch.arange(M)
+    x[:, :2], x[at, 2 + at % (D - 2)], Gy[at, at % D] = 1, 1, 1
+    return [t.to(torch.bfloat16) for t in (x, W1, W2, Gy)]
+
+
+def gate_errors(b):
+    """(sg, how far it may be off in fp32, how far the slope sg (1 + b (1 - sg)) of silu may be) of gates b in 64 bits.  e^-b is off by
+    (16 + |b|) 2 e of itself, e = 2^-24, which reaches sg times 1 - sg, the reciprocal by 2 e; the slope by that of sg in both its places,
+    and the roundings of its own products and sums.  Where 1 + e^-b is 1 there is nothing of the first, sg is 1, and 1 - sg is 0; where e^-b
+    is infinite, sg is 0."""
+    e, sig = 2.0 ** -24, torch.sigmoid(b)
+    dsig = ((1 - sig) * (16 + b.abs()) * 2 + 2) * e
+    dslope = dsig * (1 + 2 * b.abs()) + b.abs() * e + 5 * e
+    one, none = b >= 18, b <= -104
+    zero = torch.zeros_like(b)
+    return sig, torch.where(one | none, zero, dsig), torch.where(one, zero + 8 * e, torch.where(none, zero, dslope))
+
+
+def gz_and_error(a, b, u):
+    """G_a | G_b in 64 bits from exact a, b and u, and how far they may be off in bf16."""
+    sig, dsig, dslope = gate_errors(b)
+    slope = sig * (1 + b * (1 - sig))
+    gz = torch.cat([u * b * sig, u * a * slope], 1)
+    d = torch.cat([(u * b).abs() * dsig, (u * a).abs() * dslope], 1) + gz.abs() * 8 * 2.0 ** -24
+    return gz, d + (gz.abs() + d) * 2.0 ** -8 + 1e-37

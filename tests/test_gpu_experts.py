@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oracle
-from gpu_util import (assert_close, device_layer_inputs, oracle_forward_for_tokens, rel_err,
+from gpu_util import (assert_close, device_layer_inputs, gz_and_error, large_gate_inputs, oracle_forward_for_tokens, rel_err,
                       run_device_layer, run_oracle_layer,
                       sampled_parity_on_device_inputs as _sampled_parity_on_device_inputs)
 from helpers import make_layer_inputs, make_routing
@@ -1080,3 +1080,30 @@ def test_both_row_tile_geometries_give_the_same_layer(sp):
     for rows, got in outs.items():
         for k in base:
             assert torch.equal(got[k], base[k]), (rows, k)
+
+
+@pytest.mark.parametrize("sp", [0, 100])
+@pytest.mark.parametrize("M,D,H,N,stage", [(70, 96, 64, 2, 32), (6000, 224, 1024, 2, 32), (2200, 1152, 64, 8, 64)])
+def test_gradients_of_large_gates(M, D, H, N, stage, sp):
+    """G_x and G_W1, of which the slope at the gate is a factor, where it is 1 or 0 and where it is not; one expert a token, gate weights of 1."""
+    import momoe_amd
+    dev, E, B = "cuda:0", 2.0 ** -24, 2.0 ** -8
+    assert momoe_amd._hip._lib.momoe_recompute_stage_k(M, N, D, H) == stage
+    x, W1, W2, Gy = large_gate_inputs(M, D, H)
+    mask = (torch.arange(M) % N == torch.arange(N)[:, None]).to(torch.int32)
+    layer = momoe_amd.MoMoE(D, H, N, 1, save_percent=sp, Wl1_ND2H=W1.expand(N, -1, -1).to(dev), Wl2_NHD=W2.expand(N, -1, -1).to(dev))
+    leaf = x.to(dev).view(1, M, D).requires_grad_()
+    layer(leaf, mask.to(dev), torch.ones(N, M, device=dev))[0].backward(Gy.to(dev).view(1, M, D))
+    G1 = layer.Wl1_ND2H.grad.cpu().double()
+
+    def check(got, want, off, what):
+        off = off + (want.abs() + off) * B + 1e-37
+        assert bool(((got - want).abs() <= off).all()), (what, ((got - want).abs() / off).max())
+
+    dx, d1, d2, dy = [t.double() for t in (x, W1, W2, Gy)]
+    z = dx @ d1
+    gz, dgz = gz_and_error(z[:, :H], z[:, H:], dy @ d2.T)
+    check(leaf.grad.cpu().double().view(M, D), gz @ d1.T, dgz @ d1.abs().T + (gz.abs() + dgz) @ d1.abs().T * 2 * (2 * H + 8) * E, "G_x")
+    for i in range(N):
+        rows = mask[i].nonzero()[:, 0]
+        check(G1[i], dx[rows].T @ gz[rows], dx[rows].T @ dgz[rows] + dx[rows].T @ (gz.abs() + dgz)[rows] * 2 * (len(rows) + 8) * E, f"G_W1 {i}")

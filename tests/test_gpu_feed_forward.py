@@ -6,6 +6,7 @@ import torch
 
 import momoe_amd
 import oracle
+from gpu_util import gz_and_error, large_gate_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -372,40 +373,16 @@ def test_refusals():
             y.backward(Gy.view(shape))
 
 
-def _gate_errors(b):
-    """How far sg = 1 / (1 + e^-b) and the slope sg (1 + b (1 - sg)) of silu may be off in fp32.  e^-b is off by (16 + |b|) 2 E of itself,
-    which reaches sg times 1 - sg, the reciprocal by 2 E; the slope by that of sg in both its places, and the roundings of its own
-    products and sums.  Where 1 + e^-b is 1 there is nothing of the first, sg is 1, and 1 - sg is 0; where e^-b is infinite, sg is 0."""
-    sig = torch.sigmoid(b)
-    dsig = ((1 - sig) * (16 + b.abs()) * 2 + 2) * E
-    dslope = dsig * (1 + 2 * b.abs()) + b.abs() * E + 5 * E
-    one, none = b >= 18, b <= -104
-    zero = torch.zeros_like(b)
-    return sig, torch.where(one | none, zero, dsig), torch.where(one, zero + 8 * E, torch.where(none, zero, dslope))
-
-
 @pytest.mark.parametrize("save", [0, 50, 100])
 @pytest.mark.parametrize("M,D,H", [(5, 96, 64), (70, 96, 64), (5100, 224, 1024)])
 def test_gradients_of_large_gates(M, D, H, save):
-    """Gates of up to 2^30 either way, and ordinary ones, as W1 has them: rows of x that pick its rows 0 (b) and 1 (a), rows of G_y that pick
-    a column of W2 (u), so that a, b and u are exact."""
-    g = torch.Generator().manual_seed(M)
-    gates = torch.tensor([s * 2.0 ** k for k in range(10, 31) for s in (1, -1)] + [0, 1, -1, 3.5, -3.5, 8, -8, 12, -12, 20, 33])
-    W1, W2 = torch.zeros(D, 2 * H), 1 + torch.rand(H, D, generator=g)
-    W1[0, H:] = gates[torch.arange(H) % len(gates)]
-    W1[1, :H] = 1 + torch.rand(H, generator=g)
-    x, Gy, at = torch.zeros(M, D), torch.zeros(M, D), torch.arange(M)
-    x[:, :2], x[at, 2 + at % (D - 2)], Gy[at, at % D] = 1, 1, 1
-    x, W1, W2, Gy = [t.to(torch.bfloat16) for t in (x, W1, W2, Gy)]
+    """G_x and G_W1, of which the slope at the gate is a factor, where it is 1 or 0 and where it is not."""
+    x, W1, W2, Gy = large_gate_inputs(M, D, H)
     got = _step(_block(W1, W2, save), x.to(DEV), Gy.to(DEV))
     dx, d1, d2, dy = [t.double() for t in (x, W1, W2, Gy)]
     a, b, _, _ = oracle.swiglu_block(dx, d1, d2)
     u = dy @ d2.T
-    sig, dsig, dslope = _gate_errors(b)
-    slope = sig * (1 + b * (1 - sig))
-    gz = torch.cat([u * b * sig, u * a * slope], 1)
-    dgz = torch.cat([(u * b).abs() * dsig, (u * a).abs() * dslope], 1) + gz.abs() * 8 * E
-    dgz = dgz + (gz.abs() + dgz) * B + 1e-37
+    gz, dgz = gz_and_error(a, b, u)
     want = oracle.swiglu_block_gradients(dx, d1, d2, dy)
     off = dgz @ d1.abs().T + (gz.abs() + dgz) @ d1.abs().T * 2 * (2 * H + 8) * E, dx.abs().T @ dgz + dx.abs().T @ (gz.abs() + dgz) * 2 * (M + 8) * E
     for name, t, v, o in zip(("Gx", "GW1"), got[1:3], want, off):
