@@ -521,7 +521,7 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * l % 16, at [((i * columns / 16 + j) * 64 + l) * 4]; hT bf16 [(rows + 31) / 32 + 1][H][32], row r of column j at [r / 32][j][r % 32], zeros past the last row up to
  * a multiple of 32 (may be NULL; the last group is not written, but may be read).
  * A launch does `rows` rows; with all pointers moved on by a multiple of 32 rows, several do the rows of one block.
- * D and H multiples of 32, D * H * 4 < 4 GiB; row pitches multiples of 8; pointers to bf16 and fp32 data on 16-byte boundaries.
+ * D and H multiples of 32 and below 2^22, D * H * 4 < 4 GiB; row pitches multiples of 8; pointers to bf16 and fp32 data on 16-byte boundaries.
  * h of up to 16 rows takes two rows each, bf16 of it and, `rows` further on, of what that leaves: momoe_ffn_h_rows(rows) says how many, and ldm is
  * that many at least for the two products of the forward.
  * momoe_ffn_lin1_fwd: h; ab, of the first ab_rows rows, a multiple of 32 (0: none).
@@ -531,13 +531,15 @@ int momoe_fp8_combine(const void* ys_packets, const int32_t* inv_MK, void* out_M
  * Both write {0, tokens}, the rows of all launches, to counts2 (may be NULL), which the gradients of the weights take.
  * momoe_ffn_gradients: Gx [rows][D], GW1 [D][2H] and GW2 [H][D], over `rows` tokens, all of them; NULL: is not wanted, and what only it needs
  * (W1 for Gx; x for GW1; hT and Gy for GW2; counts2 for either) is not read and may be NULL.  For gradients of the weights fewer than 4 GiB of x
- * and Gy each (rows * pitch * 2) and ldm below 8388608.
+ * and Gy each (rows * pitch * 2), ldm below 8388608, and D, and 2H of W1 or H of W2, up to 2^20: momoe_ffn_gradients_take says whether
+ * those sizes will do, 1 or 0.
  * momoe_ffn_lin2_fwd takes scratch of at least momoe_ffn_workspace_bytes(rows, D, H), momoe_ffn_gradients of
  * momoe_ffn_gradients_workspace_bytes(rows, D, H, which are wanted); 0 (NULL): none is needed.
  */
 int64_t momoe_ffn_fragment_floats(int64_t rows, int64_t cols);
 int64_t momoe_ffn_workspace_bytes(int64_t rows, int64_t D, int64_t H);
 int64_t momoe_ffn_h_rows(int64_t rows);
+int momoe_ffn_gradients_take(int64_t D, int64_t H, int wants_W1, int wants_W2);
 int64_t momoe_ffn_gradients_workspace_bytes(int64_t rows, int64_t D, int64_t H, int wants_x, int wants_W1, int wants_W2);
 int momoe_ffn_lin1_fwd(const void* x, int64_t ldx, const void* W1_D2H, void* h_blocked, float* ab, int64_t ab_rows, int64_t rows,
                        int64_t ldm, int64_t D, int64_t H, void* stream);

@@ -844,6 +844,12 @@ extern "C" int momoe_ffn_dgrad_h_saved(const void* Gy, int64_t ldgy, const void*
   return launch<DhDenseSpan<true>, DhSaved>(a, H, D, cdiv64(H, kFfnCols), (hipStream_t)stream);
 }
 
+// (no size that momoe_wgrad refuses has few enough tiles for the small ones)
+extern "C" int momoe_ffn_gradients_take(int64_t D, int64_t H, int wants_W1, int wants_W2) {
+  constexpr int64_t most = 1 << 20;
+  return D > 0 && H > 0 && (!(wants_W1 || wants_W2) || D <= most) && (!wants_W1 || 2 * H <= most) && (!wants_W2 || H <= most);
+}
+
 extern "C" int64_t momoe_ffn_gradients_workspace_bytes(int64_t rows, int64_t D, int64_t H, int wants_x, int wants_W1, int wants_W2) {
   return rows <= 0 || D <= 0 || H <= 0 ? -1 : FfnScratch(rows, D, H, wants_x, wants_W1, wants_W2).bytes();
 }
@@ -856,6 +862,7 @@ extern "C" int momoe_ffn_gradients(const void* x, int64_t ldx, const void* Gy, i
   if (rows <= 0 || workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return MOMOE_ERR_BAD_ARG;
   const int status = check_ffn((rows + 31) / 32 * 32, ldm, D, H);
   if (status != MOMOE_OK) return status;
+  if (!momoe_ffn_gradients_take(D, H, GW1_D2H != nullptr, GW2_HD != nullptr)) return MOMOE_ERR_UNSUPPORTED;
   // tokens are addressed at 32-bit offsets
   if ((GW1_D2H && (ldx % 8 != 0 || rows * ldx * 2 >= (1ll << 32) || 8 * ldm * 64 >= (1ll << 32))) ||
       (GW2_HD && (ldgy % 8 != 0 || rows * ldgy * 2 >= (1ll << 32))))

@@ -664,12 +664,15 @@ Tensor feed_forward(const Tensor& x, const Tensor& W1, const Tensor& W2, double 
   if (x.dim() < 1 || W1.dim() != 2 || W2.dim() != 2 || W1.size(0) != x.size(-1) || W2.size(1) != x.size(-1) || W1.size(1) != 2 * W2.size(0))
     throw_python(PyExc_AssertionError, "x [.., D], Wl1_D2H [D,2H] and Wl2_HD [H,D] do not fit together");
   const int64_t D = W1.size(0), H = W2.size(0);
-  TORCH_CHECK(D > 0 && H > 0 && D % 32 == 0 && H % 32 == 0 && D * H * 4 < (1ll << 32),
-              "FeedForward takes D and H that are multiples of 32 with weights below 4 GiB, got ", D, " and ", H);
+  TORCH_CHECK(D > 0 && H > 0 && D % 32 == 0 && H % 32 == 0 && D < (1 << 22) && H < (1 << 22) && D * H * 4 < (1ll << 32),
+              "FeedForward takes D and H that are multiples of 32 and below 4194304 with weights below 4 GiB, got ", D, " and ", H);
   TORCH_CHECK(save_percent >= 0 && save_percent <= 100, "save_percent must be between 0 and 100, got ", save_percent);
   const int64_t M = x.numel() / D;
   if (!wants_autograd({&x, &W1, &W2})) return feed_forward_forward(x, W1, W2, 0).y;
-  // the gradients of the weights address tokens at 32-bit offsets (momoe_wgrad): say so now rather than in the backward
+  // what the gradients of the weights do not take (momoe_wgrad): say so now rather than in the backward.  Their rows and columns,
+  // and tokens at 32-bit offsets
+  TORCH_CHECK(momoe_ffn_gradients_take(D, H, W1.requires_grad(), W2.requires_grad()),
+              "FeedForward backward supports weights with gradients of up to 1048576 rows and columns, got D = ", D, " and H = ", H);
   TORCH_CHECK(!(W1.requires_grad() || W2.requires_grad()) || ((M + 31) * D * 2 < (1ll << 32) && 8 * (M + 31) * 64 < (1ll << 32)),
               "FeedForward backward supports batches of less than 4 GiB and 8388608 tokens per call, got ", M, " tokens: split the batch");
   const int64_t part = (int64_t)((double)M * save_percent / 100.0), msave = part == M ? M : part / 32 * 32;

@@ -100,6 +100,7 @@ _SIGNATURES = {
     "momoe_fp8_combine": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_fragment_floats": (_i64, [_i64] * 2),
     "momoe_ffn_gradients_workspace_bytes": (_i64, [_i64] * 3 + [_int] * 3),
+    "momoe_ffn_gradients_take": (_int, [_i64] * 2 + [_int] * 2),
     "momoe_ffn_lin1_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "momoe_ffn_h_rows": (_i64, [_i64]),
     "momoe_ffn_workspace_bytes": (_i64, [_i64] * 3),

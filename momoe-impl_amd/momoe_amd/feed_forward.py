@@ -25,7 +25,7 @@ class FeedForward(nn.Module):
     """y = (a * b * sigmoid(b)) Wl2 with a | b = x Wl1.
 
     Args:
-        embedding_dim: D.  intermediate_dim: H.  Both multiples of 32.
+        embedding_dim: D.  intermediate_dim: H.  Both multiples of 32, and where weights are trained D up to 2^20, H up to 2^19.
         save_percent: share of the rows whose pre-activations are kept for the backward, 0..100: 8 * H bytes a row, for a sixth less to
         compute in a step.
         Wl1_D2H / Wl2_HD: optional initial weights, [D, 2H] and [H, D]; the first H columns of Wl1 are the linear half, the last H go

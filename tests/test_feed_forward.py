@@ -64,3 +64,16 @@ def test_module_refusals():
             momoe_amd.FeedForward(32, 32, save, W1, W2)
     with pytest.raises(RuntimeError, match="no CPU compute path"):
         momoe_amd.FeedForward(32, 32, 0, W1, W2)(torch.zeros(4, 32))
+
+
+def test_gradients_of_weights_that_are_too_wide_are_refused_before_any_is_computed():
+    """A gradient of more than 2^20 rows or columns, beside one that could be had."""
+    good = dict(x=P, ldx=64, Gy=P, ldgy=64, gz=P, hT=P, W=P, counts=P, Gx=None, GW1=None, GW2=None, ws=P, bytes=1 << 40, rows=40, ldm=64, D=32, H=32)
+    c = lambda **k: lib.momoe_ffn_gradients(*{**good, **k}.values(), None)
+    for wants, sizes in ((("GW1", "GW2"), dict(H=(1 << 19) + 32)), (("GW1",), dict(H=(1 << 19) + 32)), (("GW2",), dict(H=(1 << 20) + 32)),
+                         (("GW1", "GW2"), dict(D=(1 << 20) + 32)), (("Gx", "GW2"), dict(D=(1 << 20) + 32))):
+        ld = sizes.get("D", 64)
+        assert c(**sizes, **{k: P for k in wants}, ldx=ld, ldgy=ld) == 2, (wants, sizes)
+    take, most = lib.momoe_ffn_gradients_take, 1 << 20
+    assert take(most, most // 2, 1, 1) == take(most, most, 0, 1) == take(2 * most, 2 * most, 0, 0) == 1
+    assert take(most + 32, 32, 1, 0) == take(most + 32, 32, 0, 1) == take(32, most // 2 + 32, 1, 0) == take(32, most + 32, 0, 1) == take(0, 32, 0, 0) == 0

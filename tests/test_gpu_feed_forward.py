@@ -389,3 +389,29 @@ def test_gradients_of_large_gates(M, D, H, save):
         o = o + (v.abs() + o) * B + 1e-37
         t = t.detach().cpu().double()
         assert ((t - v).abs() <= o).all(), (name, ((t - v).abs() / o).max())
+
+
+@pytest.mark.parametrize("D,H,which", [(32, (1 << 19) + 32, 1), (32, (1 << 20) + 32, 2), ((1 << 20) + 32, 32, 1), ((1 << 20) + 32, 32, 2)])
+def test_weights_too_wide_for_their_gradients(D, H, which):
+    """Refused before the forward computes; without that gradient, such a block does what any other does."""
+    x, W1, W2, Gy = _inputs(3, D, H)
+    block, leaf = _block(W1, W2), x.to(DEV).requires_grad_()
+    leaves = [leaf, block.Wl1_D2H, block.Wl2_HD]
+    block.requires_grad_(False)
+    leaves[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="1048576"):
+        block(leaf)
+    with torch.no_grad():
+        y = block(leaf)
+    leaves[which].requires_grad_(False)
+    z = block(leaf)
+    z.backward(Gy.to(DEV))
+    assert torch.equal(y, z)
+    _check((y, leaf.grad), _bounds(x, W1, W2, Gy)[:2])
+
+
+def test_weights_too_wide():
+    W = torch.empty(1, 1, device=DEV, dtype=torch.bfloat16)
+    x = W.expand(2, 1 << 22)
+    with pytest.raises(RuntimeError, match="4194304"):
+        momoe_amd.FeedForwardFunction.apply(x, W.expand(1 << 22, 64), W.expand(32, 1 << 22))
