@@ -415,3 +415,52 @@ def test_weights_too_wide():
     x = W.expand(2, 1 << 22)
     with pytest.raises(RuntimeError, match="4194304"):
         momoe_amd.FeedForwardFunction.apply(x, W.expand(1 << 22, 64), W.expand(32, 1 << 22))
+
+
+def _check_on_gpu(got, ins):
+    """As _check, the 64-bit side on the GPU."""
+    for name, t, (v, off) in zip(("y", "Gx", "GW1", "GW2"), got, _bounds(*[t.to(DEV) for t in ins])):
+        t = t.detach().double()
+        assert torch.isfinite(t).all() and ((t - v).abs() <= off).all(), (name, ((t - v).abs() / off).max())
+
+
+# M, D, H, of the gradients of W1 and of W2: "small" tiles of 128 x 128; "large" launches of 256 x 256 that are whole because they fill the
+# CUs ("whole"), or with scratch for pieces of the tokens, which 300 of them are not cut into ("kept"), or which they are ("cut")
+LARGE = [(300, 2048, 5632, "kept", "kept"), (4133, 1056, 4256, "cut", "small"), (4133, 2080, 4224, "cut", "cut"), (4133, 2048, 8192, "whole", "whole"),
+         (6049, 1056, 4256, "cut", "small")]
+
+
+@pytest.mark.parametrize("M,D,H,first,second", LARGE)
+def test_large_gradients_of_the_weights(M, D, H, first, second):
+    """Many stages, an odd number of groups of 32 rows, a ragged end."""
+    lib = momoe_amd._hip._lib
+    for kind, X, Y, which, layout in ((first, D, 2 * H, (0, 1, 0), 2), (second, H, D, (0, 0, 1), 0)):
+        tiles, need = -(-X // 128) * -(-Y // 128), lib.momoe_ffn_gradients_workspace_bytes(M, D, H, *which)
+        assert (tiles <= 512) == (kind == "small")
+        if kind != "small":
+            assert need == (0 if kind == "whole" else lib.momoe_wgrad_workspace_bytes(1, X, Y, M)) and lib.momoe_wgrad_stage_rows(1, X, Y, M, layout) == 64
+        if need:  # pieces of 64 stages of 32 tokens or more, so that the scratch holds them
+            stages, parts = -(-X // 256) * -(-Y // 256) * (M // 32 + 1), need // (256 * 256 * 4)
+            assert (-(-M // 32) >= 2 * max(64, -(-stages // max(parts, 1)))) == (kind == "cut") or kind == "small"
+    ins = _inputs(M, D, H)
+    for save in (0, 100):
+        _check_on_gpu(_step(_block(ins[1], ins[2], save), ins[0].to(DEV), ins[3].to(DEV)), ins)
+
+
+@pytest.mark.parametrize("M,D,H", [(33, 288, 96), (1025, 320, 576), (1100, 96, 64), (5000, 64, 160), (17000, 128, 96), (300, 2048, 5632), (4133, 1056, 4256), (4133, 2080, 4224)])
+def test_gradients_of_few_rows_among_many(M, D, H):
+    """G_y of zeros but for a few rows: the last ones, or 20 either side of where a slice or a piece of the tokens may end.  What they add
+    to the gradients of the weights is all there is, and the bounds are as small."""
+    ins = [t.to(DEV) for t in _inputs(M, D, H)]
+    block, zeros = _block(ins[1], ins[2]), torch.zeros_like(ins[3])
+    ends = list(range(64, M, 64)) if D * H < 1 << 20 else list(range(64, M, 64 * 7))
+    for lo, hi in [(M - 1, M), (M - M % 32, M), (M - 5, M), (max(0, M - 40), M)] + [(max(0, e - 20), min(M, e + 20)) for e in ends]:
+        Gy = zeros.clone()
+        Gy[lo:hi] = ins[3][lo:hi]
+        some = ins[0][lo:hi], ins[1], ins[2], Gy[lo:hi]
+        x, W1, W2, g = [t.double() for t in some]
+        got = _step(block, ins[0], Gy)
+        for name, t, (v, off) in zip(("GW1", "GW2"), got[2:], _bounds(*some)[2:]):
+            assert ((t.double() - v).abs() <= off).all(), (name, lo, hi, ((t.double() - v).abs() / off).max())
+            if hi - lo == 1:  # (that it were lost would be seen)
+                assert (v.abs() > 2 * off).any()
