@@ -464,3 +464,40 @@ def test_gradients_of_few_rows_among_many(M, D, H):
             assert ((t.double() - v).abs() <= off).all(), (name, lo, hi, ((t.double() - v).abs() / off).max())
             if hi - lo == 1:  # (that it were lost would be seen)
                 assert (v.abs() > 2 * off).any()
+
+
+def _pitches(D):
+    """[M, D] views of wider buffers: pitches that are no multiple of 8, of 4 GiB of rows and more, of 2^22 elements and more; with the rows
+    at the start, in the middle and at the end of the buffer's."""
+    for M, width, at in ((70, D + 4, 0), (70, D + 30, 6), (1 << 20, 2080, 0), (1 << 20, 2080, 2080 - D), (3, (1 << 22) + 8, 8)):
+        yield M, torch.zeros(M, width, device=DEV, dtype=torch.bfloat16)[:, at:at + D]
+
+
+def test_pitches_that_are_copied():
+    D, H = 32, 64
+    _, W1, W2, _ = _inputs(1, D, H)
+    block = _block(W1, W2)
+    for M, view in _pitches(D):
+        x, Gy = [torch.randn(M, D, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+        want = _step(block, x, Gy)
+        view.copy_(x)
+        assert all(torch.equal(a, b) for a, b in zip(_step(block, view, Gy), want))
+        view.copy_(Gy)
+        assert all(torch.equal(a, b) for a, b in zip(_step(block, x, view), want))
+
+
+@pytest.mark.parametrize("save", [0, 100])
+@pytest.mark.parametrize("D,H", [(4096, 32), (32, 4096)])
+def test_tokens_past_32_bit_offsets(D, H, save):
+    """x, y and Gx, or h, gz and what is kept, of more than 4 GiB: rows at the start, at the end and where offsets pass 2^31 and 2^32."""
+    M = (1 << 19) + 45
+    _, W1, W2, _ = _inputs(1, D, H)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, Gy = [torch.randn(M, D, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    block = _block(W1, W2, save).requires_grad_(False)
+    y, Gx = _step(block, x, Gy)[:2]
+    edge = [e // (w * p) for w in {D, H, 2 * H} for p in (2, 4) for e in (1 << 31, 1 << 32, 1 << 33)]
+    rows = torch.cat([torch.arange(max(0, e - 20), min(M, e + 20)) for e in [0, M] + [e for e in edge if e < M]]).unique().to(DEV)
+    _check((y[rows], Gx[rows]), _bounds(x[rows].cpu(), W1, W2, Gy[rows].cpu())[:2])
+    with torch.no_grad():
+        assert torch.equal(block(x)[rows], y[rows])

@@ -342,3 +342,44 @@ def test_weights_of_nan_and_infinity_reach_the_results(M):
                 hit[:] = first
                 hit[33] = True
                 assert not y[..., hit].isfinite().any() and y[..., ~hit].isfinite().all()
+
+
+def test_pitches_that_are_copied():
+    """Rows of x at pitches that the kernels do not take: no multiple of 8, 4 GiB of rows and more, 2^22 elements and more."""
+    D, H, N, group = 32, 64, 2, 32
+    w = _weights((N,), D, H, group)
+    layer = momoe_amd.MoMoEInt4(D, H, N, 1, *_on(w), group_size=group)
+    block = momoe_amd.FeedForwardInt4(D, H, *[t[0] for t in _on(w)], group_size=group)
+    for M, width, at in ((70, D + 4, 0), (70, D + 30, 6), (1 << 20, 2080, 2080 - D), (3, (1 << 22) + 8, 8)):
+        x = torch.randn(M, D, device=DEV, dtype=torch.bfloat16)
+        view = torch.zeros(M, width, device=DEV, dtype=torch.bfloat16)[:, at:at + D]
+        view.copy_(x)
+        mask = torch.zeros(N, M, dtype=torch.int32, device=DEV)
+        mask[torch.arange(M, device=DEV) % N, torch.arange(M, device=DEV)] = 1
+        s = torch.rand(N, M, device=DEV)
+        assert torch.equal(layer(view.unsqueeze(0), mask, s)[0], layer(x.unsqueeze(0), mask, s)[0]) and torch.equal(block(view), block(x))
+
+
+@pytest.mark.parametrize("D,H", [(4096, 32), (32, 4096)])
+def test_tokens_past_32_bit_offsets(D, H):
+    """x, y and ys, or h, of more than 4 GiB: rows at the start, at the end and where offsets pass 2^31 and 2^32.  Experts of such an x take
+    tiles of 32 rows."""
+    M, N, group = (1 << 19) + 45, 2, 64
+    w = _weights((N,), D, H, group)
+    layer = momoe_amd.MoMoEInt4(D, H, N, 1, *_on(w), group_size=group)
+    block = momoe_amd.FeedForwardInt4(D, H, *[t[0] for t in _on(w)], group_size=group)
+    assert momoe_amd._hip._lib.momoe_int4_tile_rows(M, D, H, N) == 64
+    x = torch.randn(1, M, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV, dtype=torch.bfloat16)
+    at = torch.arange(M, device=DEV)
+    mask, s = torch.zeros(N, M, dtype=torch.int32, device=DEV), torch.rand(N, M, device=DEV) + 0.5
+    mask[at % N, at] = 1
+    edge = [e // (c * p) for c in {D, H} for p in (2, 4) for e in (1 << 31, 1 << 32, 1 << 33)]
+    rows = torch.cat([torch.arange(max(0, e - 20), min(M, e + 20)) for e in [0, M] + [e for k in (1, 2) for e in (v * k for v in edge) if e < M]]).unique()
+    y, sizes = layer(x, mask, s)
+    assert torch.equal(sizes, mask.sum(1)) and y.isfinite().all()
+    for i in range(N):
+        mine = rows[rows % N == i]
+        want, off = _block(x[0, mine].cpu().double(), [t[i] for t in w], group)
+        sr = s[i, mine].cpu().double()[:, None]
+        _check(y[0, mine], sr * want, sr * off + (sr * want).abs() * 8 * E)
+    _check(block(x)[0, rows], *_block(x[0, rows].cpu().double(), [t[0] for t in w], group))
