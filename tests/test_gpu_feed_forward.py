@@ -501,3 +501,20 @@ def test_tokens_past_32_bit_offsets(D, H, save):
     _check((y[rows], Gx[rows]), _bounds(x[rows].cpu(), W1, W2, Gy[rows].cpu())[:2])
     with torch.no_grad():
         assert torch.equal(block(x)[rows], y[rows])
+
+
+@pytest.mark.parametrize("M,D,H", [(1, 96, 64), (16, 2080, 64), (17, 96, 64), (31, 288, 96), (100, 96, 2080), (1250, 224, 2048)])
+def test_the_forward_leaves_what_lies_behind(M, D, H):
+    """The entry points of the forward on buffers with room behind them, and h of more rows than there are."""
+    lib, st = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream
+    x, W1, W2, _ = [t.to(DEV) for t in _inputs(M, D, H)]
+    held, kept = lib.momoe_ffn_h_rows(M), (M + 15) // 16 * 16
+    ldm, need = held + 40, lib.momoe_ffn_workspace_bytes(M, D, H)
+    h, y = [torch.full((n + 4096,), 7.0, device=DEV, dtype=torch.bfloat16) for n in (H * ldm, M * D)]
+    ab = torch.full((lib.momoe_ffn_fragment_floats(M, 2 * H) + 4096,), 7.0, device=DEV)
+    ws = torch.full((need + 4096,), 7, device=DEV, dtype=torch.uint8)
+    assert lib.momoe_ffn_lin1_fwd(x.data_ptr(), D, W1.data_ptr(), h.data_ptr(), ab.data_ptr(), (M + 31) // 32 * 32, M, ldm, D, H, st) == 0
+    assert lib.momoe_ffn_lin2_fwd(h.data_ptr(), W2.data_ptr(), y.data_ptr(), M, ldm, D, H, ws.data_ptr() if need else None, need, st) == 0
+    torch.cuda.synchronize()
+    assert (h[H * ldm:] == 7).all() and (h[:H * ldm].view(-1, ldm, 32)[:, held:] == 7).all() and (ab[kept * 2 * H:] == 7).all()
+    assert (y[M * D:] == 7).all() and (ws[need:] == 7).all() and torch.equal(y[:M * D].view(M, D), _block(W1, W2)(x))

@@ -383,3 +383,69 @@ def test_tokens_past_32_bit_offsets(D, H):
         sr = s[i, mine].cpu().double()[:, None]
         _check(y[0, mine], sr * want, sr * off + (sr * want).abs() * 8 * E)
     _check(block(x)[0, rows], *_block(x[0, rows].cpu().double(), [t[0] for t in w], group))
+
+
+def _with_room(n, dtype, value=7):
+    """n values and room behind them; how to tell that it keeps its bits."""
+    t = torch.full((n + 4096,), value, device=DEV, dtype=dtype)
+    return t, lambda: bool((t[n:] == value).all())
+
+
+def test_laying_weights_out_leaves_what_lies_behind():
+    lib, st = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream
+    for N, R, C, halves, group in ((1, 32, 32, 2, 32), (3, 160, 96, 2, 64), (2, 288, 80, 1, 128), (5, 128, 16, 1, 32)):
+        codes, scale, _, _, zero, _ = _on(_weights((N,), R, C // 2, group))
+        nb, nw = lib.momoe_int4_weight_bytes(N, R, C), lib.momoe_int4_scale_words(N, R, C, group)
+        (packed, same), (words, same_words) = _with_room(nb, torch.uint8), _with_room(nw, torch.int32)
+        assert lib.momoe_int4_pack_weights(codes.data_ptr(), scale.data_ptr(), momoe_amd._hip._TYPES[scale.dtype], zero.data_ptr(), N, R, C, halves, group,
+                                           packed.data_ptr(), words.data_ptr(), st) == 0
+        torch.cuda.synchronize()
+        assert same() and same_words()
+        want = momoe_amd._hip.int4_pack_weights(codes, scale, zero, halves, group)
+        assert torch.equal(packed[:nb], want[0]) and torch.equal(words[:nw], want[1])
+
+
+@pytest.mark.parametrize("M,D,H", [(1, 96, 64), (16, 160, 2080), (17, 288, 96), (50, 2080, 160), (16, 4096, 1120), (300, 1056, 160), (1000, 288, 160), (2100, 160, 96)])
+def test_the_dense_block_leaves_what_lies_behind(M, D, H):
+    lib, st, group = momoe_amd._hip._lib, torch.cuda.current_stream().cuda_stream, 64
+    w = _weights((), D, H, group)
+    block, x = momoe_amd.FeedForwardInt4(D, H, *_on(w), group_size=group), _x(M, D).to(DEV)
+    need = lib.momoe_int4_ffn_workspace_bytes(M, D, H)
+    (h, h_same), (y, y_same), (ws, ws_same) = _with_room(lib.momoe_int4_h_rows(M, 1) * H, torch.bfloat16), _with_room(M * D, torch.bfloat16), _with_room(need, torch.uint8)
+    P = [t.data_ptr() for t in (block.Wl1_packed, block.Wl1_words, block.Wl2_packed, block.Wl2_words)]
+    assert lib.momoe_int4_ffn_fwd(x.data_ptr(), D, *P, group, h.data_ptr(), y.data_ptr(), ws.data_ptr() if need else None, need, M, D, H, st) == 0
+    torch.cuda.synchronize()
+    assert h_same() and y_same() and ws_same() and torch.equal(y[:M * D].view(M, D), block(x))
+
+
+@pytest.mark.parametrize("M,D,H,N,K,rows", [(1, 96, 64, 4, 2, 32), (7, 288, 160, 8, 2, 32), (40, 96, 160, 2, 1, 32), (7, 288, 160, 8, 2, 64), (100, 1056, 352, 8, 2, 64),
+                                            (300, 288, 416, 5, 2, 64), (3000, 160, 96, 3, 1, 64), (20, 1056, 352, 8, 2, 64), (20, 96, 1056, 8, 2, 64)])
+def test_the_experts_leave_what_lies_behind(M, D, H, N, K, rows):
+    """h with its second half, sums of slices, ys and y; of either height of tiles, whatever suits the sizes."""
+    hip, st, group = momoe_amd._hip, torch.cuda.current_stream().cuda_stream, 32
+    lib, msum = hip._lib, M * K
+    w = _weights((N,), D, H, group)
+    layer, x = momoe_amd.MoMoEInt4(D, H, N, K, *_on(w), group_size=group), _x(M, D).to(DEV)
+    mask, s = [t.to(DEV) for t in make_routing(M, N, K, seed=2)]
+    ib = hip.index_build(mask, K, tile_rows=rows)
+    n1, n2 = lib.momoe_int4_slices(msum, N, 2 * H, D, rows), lib.momoe_int4_slices(msum, N, D, H, rows)
+    need = n1 * msum * 2 * H * 4 if n1 > 1 else 0
+    (h, h_same), (ys, ys_same) = _with_room(lib.momoe_int4_h_rows(msum, N) * H, torch.bfloat16), _with_room(n2 * msum * D, torch.float32)
+    (ws, ws_same), (y, y_same) = _with_room(need, torch.uint8), _with_room(M * D, torch.bfloat16)
+    P = [t.data_ptr() for t in (layer.Wl1_packed, layer.Wl1_words, layer.Wl2_packed, layer.Wl2_words, ib["idx_Msum"], ib["tile_table"])]
+    assert lib.momoe_int4_lin1_swiglu_fwd(x.data_ptr(), D, P[0], P[1], group, P[4], P[5], rows, h.data_ptr(), ws.data_ptr() if need else None, need, M, D, H, N,
+                                          msum, st) == 0
+    assert lib.momoe_int4_lin2_scale_fwd(h.data_ptr(), P[2], P[3], group, s.data_ptr(), s.stride(0), s.stride(1), P[4], P[5], rows, ys.data_ptr(), M, D, H, N,
+                                         msum, st) == 0
+    assert lib.momoe_int4_combine(ys.data_ptr(), n2, ib["inv_MK"].data_ptr(), y.data_ptr(), M, D, K, msum, st) == 0
+    torch.cuda.synchronize()
+    assert h_same() and ys_same() and ws_same() and y_same()
+    want, off = torch.zeros(M, D, dtype=torch.float64), torch.zeros(M, D, dtype=torch.float64)
+    for i in range(N):
+        at = mask[i].cpu().nonzero().flatten()
+        if len(at):
+            out, d = _block(x[at].cpu().double(), [t[i] for t in w], group, len(at) <= 16 and msum <= 16 * N)
+            sr = s[i, at].cpu().double()[:, None]
+            want.index_add_(0, at, sr * out)
+            off.index_add_(0, at, sr * d + (sr * out).abs() * (K + 2) * 2 * E)
+    _check(y[:M * D], want, off)
