@@ -1,15 +1,17 @@
 // A dense SwiGLU block, forward and backward: the layers beside the mixture that have no router.
 //
 //   a | b = x W1,  h = a b sig(b),  y = h W2
-//   u = G_y W2^T,  G_a = u b sig(b),  G_b = u a sig(b) (1 + b (1 - sig(b))),  G_x = (G_a | G_b) W1^T,  G_W1 = x^T (G_a | G_b),  G_W2 = h^T G_y
+//   u = G_y W2^T,  G_a = u b sig(b),  G_b = u a sig(b) (1 + b (1 - sig(b))),
+//   G_x = (G_a | G_b) W1^T,  G_W1 = x^T (G_a | G_b),  G_W2 = h^T G_y
 //
 // Rows are tokens as they come: no routing index, no gather, no gate weights, no sum over experts.  The products' operands are bf16;
 // what meets in an epilogue is not rounded before: a | b that are kept for the backward, and u where a | b are made again, go through
 // memory in fp32, as whole accumulator fragments ([row / 16][column / 16][64 lanes][4]: 1 KiB a store).  (In bf16 they cost half as much
 // traffic and a rounding each, which doubles the error of the weight gradients.)
-//   h       [H / 32][ldm][32]    k-blocked, as the second product contracts over it; of up to kTwiceRows rows each of them is two, bf16 of
-//                                it and of what that leaves, as a tile has room for both: rounded, the h of one token, few of which are large,
-//                                can be more of y's error than y's own rounding (0.0023 to 0.0024 of the norm against 64 bits, then 0.0017)
+//   h       [H / 32][ldm][32]    k-blocked, as the second product contracts over it; of up to kTwiceRows rows each of them is two, bf16
+//                                of it and of what that leaves, as a tile has room for both: rounded, the h of one token, few of which
+//                                are large, can be more of y's error than y's own rounding (0.0023 to 0.0024 of the norm against 64
+//                                bits, then 0.0017)
 //   gz      [2H / 32][ldm][32]   G_a | G_b, k-blocked, for G_x and the gradient of W1; zeros behind the last row up to a multiple of 32
 //   hT      [rows / 32][H][32]   h once more, feature-major in groups of 32 rows, zeros behind the last row: for the gradient of W2
 // The weights' gradients are momoe_wgrad of one expert where their launches are large, and tiles of 128 x 128 where they are small.
@@ -331,8 +333,8 @@ int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   sums.add(a);
   return sum_slices(sums, st);
 }
-// The three products that need gz or hT and no more, in one launch, as none of them fills the CUs; x, w1, w2: null, or what is wanted.  1000 tokens,
-// 2176 x 1152: 15.5 + 23.6 + 25.3 us apart, 40 so (0.75 PFLOP/s); 128, 96 x 64: 4.5 + 4.9 + 3.5 and 5.
+// The three products that need gz or hT and no more, in one launch, as none of them fills the CUs; x, w1, w2: null, or what is wanted.
+// 1000 tokens, 2176 x 1152: 15.5 + 23.6 + 25.3 us apart, 40 so (0.75 PFLOP/s); 128, 96 x 64: 4.5 + 4.9 + 3.5 and 5.
 template <class Dx, int STAGES>
 __global__ __launch_bounds__(kSpanThreads, 2) void ffn_gradients_kernel(FfnArgs x, FfnArgs w1, FfnArgs w2, int x_blocks, int w1_blocks) {
   const int block = blockIdx.x;
@@ -355,13 +357,21 @@ int launch_gradients(const FfnArgs* x, const FfnArgs* w1, const FfnArgs* w2, hip
     if (a) sums.add(*a);
   return sum_slices(sums, st);
 }
-// Tiles of 32 rows as long as no CU has more than two of them, else of 64; a contraction is cut, where there is somewhere to leave its
-// sums, until every CU has two, into slices of at least 8 stages and not past 10 MB of sums.  (One CU pulls some 45 GB/s, so a
-// launch of few tiles takes as long as they are few.)  Us, contraction whole | cut in 2 | 4 | 8: 1 token, h W2 of 2048 x 8192 47 | 26 | 16 | 12;
-// 24 tokens, 4096 x 11264 64 | 34 | 22 | 21; 128, 4096 x 4096 25 | 18 | 17 | 21; 300, 2048 x 5632 40 | 26 | 23 | 24; 1000, 1024 x 2816 21 | 17 | 19 | 25;
-// 1000, 2176 x 1152 16 | 23 | 27 | 36.  32 rows | 64: 64 tokens, x W1 of 2048 x 5632 13.9 | 16.1; 128, 4096 x 4096 24.9 | 29.3, gz W1^T 41.7 | 52.0; 24, x W1
-// of 4096 x 11264 32.5 | 30.7.  128 rows a tile, or a deeper ring and one workgroup a CU, were faster nowhere but for 8 % of one launch
-// (1000 tokens, x W1 of 1024 x 2816).
+// Rule: tiles of 32 rows as long as no CU has more than two of them, else of 64.  A contraction is cut, where there is somewhere to
+// leave its sums, until every CU has two tiles, into slices of at least 8 stages and not past 10 MB of sums: a stage takes as long
+// however few tiles there are (ffn_tile.hpp), so that a launch of few takes as long as their contraction is.
+// Record, us.  Contraction whole | cut in 2 | 4 | 8:
+//   h W2, 1 token, 2048 x 8192     47 | 26 | 16 | 12        h W2, 300 tokens, 2048 x 5632    40 | 26 | 23 | 24
+//         24, 4096 x 11264         64 | 34 | 22 | 21              1000, 1024 x 2816          21 | 17 | 19 | 25
+//         128, 4096 x 4096         25 | 18 | 17 | 21              1000, 2176 x 1152          16 | 23 | 27 | 36
+// 32 rows | 64, weights from memory (in brackets one matrix again and again, of which the cache holds a part or all):
+//   x W1, 16 tokens, 2048 x 5632   20.9 | 21.4 (13.3 | 15.7)      x W1, 64, 2048 x 5632      20.8 | 23.9 (13.7 | 15.9)
+//         24, 2048 x 8192          21.1 | 21.8 (14.7 | 16.2)            500, 2048 x 512      15.7 | 18.1 (13.1 | 15.8)
+//         24, 4096 x 11264         43.5 | 43.7 (32.6 | 30.7)            1000, 2048 x 512     15.8 | 17.8 (13.5 | 15.9)
+//   past two of 32 rows a CU: 1000 tokens, 2176 x 1152 32.6 | 22.8; 2000, 2048 x 2048 70.3 | 49.5.  Between one and two the line is too
+//   high for 48 tokens, 4096 x 11264 (352 tiles): 71.1 | 46.0.
+// 128 rows a tile, or a deeper ring and one workgroup a CU, were faster nowhere but for 8 % of one launch (1000 tokens, x W1 of
+// 1024 x 2816).
 struct FfnPlan {
   int fm, slices;
 };
@@ -680,11 +690,16 @@ __global__ __launch_bounds__(kSpanThreads, 1) void ffn_span_kernel(FfnArgs p, in
 }
 
 // ---- which of the two -----------------------------------------------------------------------------------------------------------
-// 256 x 256 tiles where the results are three tenths of a round of one a CU at least (and there are two stages of k-values).  Us, small tiles | these,
-// by the number of these: x W1 of 2048 x 2816 for 700 tokens, 66 of them, 25.4 | 27.5; 1250, 2048 x 2048, 80, 35.4 | 27.0; 1200, 1024 x 2176, 85,
-// 19.9 | 16.9; 2000, 2048 x 2048, 128, 44.5 | 31.8; 4000, 256, 93.0 | 51.6; h W2, 2000, 2048 x 2048, 64, 26.3 | 26.5; 1250, 1024 x 4096, 80, 22.0 | 17.3;
-// 1000, 4096 x 2048, 32, 34.4 | 48.5; 24 tokens, x W1 of 4096 x 11264, 88, hardly filled, 36.5 | 58.  8192 tokens through 2048 x 8192: 414 (1.33 PFLOP/s) and 199 (1.38), 16384 through 4096 x 11264: 2329 (1.30)
-// and 1064 (1.42): what a large library product of these sizes reaches; bound by the matrix instructions at the clock that the card holds.
+// Rule: 256 x 256 tiles where the results are three tenths of a round of one a CU at least (and there are two stages of k-values).
+// Record, us, small tiles | these, and the number of these:
+//   x W1, 700 tokens, 2048 x 2816    25.4 | 27.5   66       h W2, 1000 tokens, 4096 x 2048    34.4 | 48.5   32
+//         1250, 2048 x 2048          35.4 | 27.0   80             1250, 1024 x 4096           22.0 | 17.3   80
+//         1200, 1024 x 2176          19.9 | 16.9   85             2000, 2048 x 2048           26.3 | 26.5   64
+//         2000, 2048 x 2048          44.5 | 31.8   128
+//         4000, 2048 x 2048          93.0 | 51.6   256
+//         24, 4096 x 11264           36.5 | 58     88, hardly filled
+// 8192 tokens through 2048 x 8192 take 414 (1.33 PFLOP/s) and 199 (1.38), 16384 through 4096 x 11264 2329 (1.30) and 1064 (1.42): what a
+// large library product of these sizes reaches; bound by the matrix instructions at the clock that the card holds.
 inline bool takes_span(int64_t rows, int64_t cols, int64_t contraction) {
   return rows > 2 * kTwiceRows && contraction >= WideSpan::AHEAD * kSpan && 10 * rows * cols >= 3 * persistent_grid() * (int64_t)(WideSpan::MAX_ROWS * WideSpan::COLS);
 }
@@ -721,11 +736,13 @@ int check_ffn(int64_t rows, int64_t ldm, int64_t D, int64_t H) {
     return MOMOE_ERR_UNSUPPORTED;
   return MOMOE_OK;
 }
-// Gradients of the weights in tiles of 128 x 128 as long as no CU has more than two of them and none contracts over more than 8192 tokens; where
-// the tiles are fewer, the tokens are cut, into slices of at least 512, and past 10 MB of sums of at least 2048.  Us, W2 and W1, momoe_wgrad |
-// these: 31 tokens, 64 x 96 6.9, 7.1 | 4.1, 4.3; 512, 512 x 512 17.8, 18.5 | 8.7, 9.2; 1000, 1024 x 2816 28.3, 30.8 | 16.6, 23.2; 4096, 512 x 512
-// 87.5, 95.6 | 15.8, 19.1; 8192, 1024 x 2816 79.7, 164 | 69.2, 118; 65536, 1024 x 2816 476, 751 | 952, 933; more tiles than two a CU: 300, 2048 x 5632
-// 17.1, 32.6 | 18.1, 31.4; 2048, 2048 x 8192 56.7, 116 | 84.8, 159.
+// Rule: gradients of the weights in tiles of 128 x 128 as long as no CU has more than two of them and none contracts over more than 8192
+// tokens; where the tiles are fewer, the tokens are cut, into slices of at least 512, and past 10 MB of sums of at least 2048.
+// Record, us, W2 and W1, momoe_wgrad | these:
+//   31 tokens, 64 x 96       6.9, 7.1 | 4.1, 4.3            8192, 1024 x 2816     79.7, 164 | 69.2, 118
+//   512, 512 x 512           17.8, 18.5 | 8.7, 9.2          65536, 1024 x 2816    476, 751 | 952, 933
+//   1000, 1024 x 2816        28.3, 30.8 | 16.6, 23.2        more tiles than two a CU: 300, 2048 x 5632    17.1, 32.6 | 18.1, 31.4
+//   4096, 512 x 512          87.5, 95.6 | 15.8, 19.1                                  2048, 2048 x 8192   56.7, 116 | 84.8, 159
 int wgrad_slices(int64_t rows, int64_t X, int64_t Y) {
   const int64_t tiles = cdiv64(X, kFfnCols) * cdiv64(Y, kFfnCols), room = 2 * persistent_grid();
   return (int)std::max<int64_t>(1, std::min({room / tiles, cdiv64(rows, kSpan) / 8, std::max((10 << 20) / (X * Y * 4), rows / 2048), (int64_t)16}));
@@ -733,9 +750,9 @@ int wgrad_slices(int64_t rows, int64_t X, int64_t Y) {
 bool wgrad_in_small_tiles(int64_t rows, int64_t X, int64_t Y) {
   return cdiv64(X, kFfnCols) * cdiv64(Y, kFfnCols) <= 2 * persistent_grid() && rows <= 8192 * (int64_t)wgrad_slices(rows, X, Y);
 }
-// An expert of all rows is cut along them, through the workspace, where its tiles leave CUs idle in their last round; tiles that fill 5 of 6
-// are done whole, which saves the partial sums' way through memory.  Us, 8192 tokens, D = 2048, H = 8192 (256 and 512 tiles of 256 x 256), cut |
-// whole: W2 335 | 256, W1 640 | 470.
+// An expert of all rows is cut along them, through the workspace, where its tiles leave CUs idle in their last round; tiles that fill 5
+// of 6 are done whole, which saves the partial sums' way through memory.  Us, 8192 tokens, D = 2048, H = 8192 (256 and 512 tiles of 256 x
+// 256), cut | whole: W2 335 | 256, W1 640 | 470.
 int64_t large_wgrad_bytes(int64_t rows, int64_t X, int64_t Y) {
   const int64_t bytes = momoe_wgrad_workspace_bytes(1, X, Y, rows);
   if (bytes <= 0) return bytes;

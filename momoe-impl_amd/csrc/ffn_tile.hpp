@@ -5,8 +5,12 @@
 // columns).  4 waves, 2 x 2.  STAGES stages in LDS; the fragments of one half of a stage are read while
 // the other is multiplied (read and then multiplied, one after the other, a stage took 0.36 to 0.75 us whatever was on the way).  A
 // contraction may be cut into `slices`, each a tile of its own that leaves fp32 sums for another kernel.
-// Bound by what a CU pulls, some 30 GB/s by one workgroup and 45 by two: 24 tokens through 4096 x 11264, x W1 36.5 us (5.1 TB/s, 176 workgroups),
-// h W2 17.6 (5.2 TB/s, 512); 1000 through 2176 x 1152, 26 and 16 (0.38 and 0.31 PFLOP/s).
+// Bound by a stage's chain of fragment reads, products, wait and barrier.  Of 64 x 128 a stage takes 0.39 us where one workgroup is on
+// a CU, whether 64 CUs have one or all, and 0.64 where two are; of 32 x 128 0.31 and 0.45 (63 to 92 GB/s a CU; slopes of x W1 over
+// contractions of 2048 to 8192).  The matrix instructions are 0.11 of the 0.39; of a wavefront's time 30 % is waits for transfers and
+// at the barrier, another 30 % for its turn to issue, and LDS banks do not conflict.  1000 tokens through 2176 x 1152: x W1 26 us (0.38
+// PFLOP/s; 288 tiles of 34 stages, of which the 32 CUs that have two take 22), h W2 16 (0.31).  24 through 4096 x 11264: x W1 36.5 (176
+// workgroups; 43.5 with weights of which the cache holds nothing), h W2 17.6 (5.2 TB/s, 512).
 #pragma once
 #include "gemm_span.hpp"
 
@@ -157,8 +161,8 @@ __device__ __forceinline__ void wait_for_stage(int after) {
   }
 }
 
-// A tile program P: P::Rows, P::Weights, FM; K, slices, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column of a
-// wave's fragments in the tile; epilogue(row0, rows, tn, slice, wm, wn, acc).  block: of this program's, from a multiple of 8 on.
+// A tile program P: P::Rows, P::Weights, FM; K, slices, rows, row_tiles, col_tiles; setup(row0, rows, tn, A, W), n_org(wn): first column
+// of a wave's fragments in the tile; epilogue(row0, rows, tn, slice, wm, wn, acc).  block: of this program's, from a multiple of 8 on.
 template <class P, int STAGES>
 __device__ __forceinline__ void run_ffn_tile(const P& prog, int block) {
   using Rows = typename P::Rows;

@@ -3,8 +3,8 @@
 // A weight is (code - zero) * scale: a code of 4 bits, a zero (0 to 15) and a 16-bit scale for each `group` (32, 64, 128) consecutive
 // k-values of a column.  A product over a group is
 //   sum_k x_k (code_k - zero) scale = scale * (sum_k x_k (128 + code_k) - (128 + zero) * sum_k x_k)
-// 128 + code is a bf16 whose low bits are the code: bits 0x4300 | code, one instruction for two of them and no conversion.  The sum of
-// x_k is a product with ones by the same matrix instruction, whose rate a call of few rows does not use up; it comes in the same lanes.  All
+// 128 + code is a bf16 whose low bits are the code: bits 0x4300 | code, one instruction for two of them and no conversion.  The sum
+// of x_k is a product with ones by the same matrix instruction, whose rate a call of few rows does not use up, in the same lanes.  All
 // of it in fp32: what is subtracted is up to 143 / 8 times as large as what is left, so that four bits of 24 go.  The scale, fp32 again,
 // meets the sum: a weight itself is never rounded.
 //
@@ -14,7 +14,8 @@
 //           column lane % 16; k-value 2 i in bits 4 i .. +3, 2 i + 1 in bits 16 + 4 i .. +3, so that a shift and a mask give a pair
 //   scales  [expert][16 columns][128 k-values][16][128 / group] words: the scale's fp32 bits (of a 16-bit type: the low 13 are zero) and,
 //           in the low four, the zero
-// Past the last k-value the codes are the zero of their group, or the scales are zero.  The columns of the first product are those of its two halves in turn, 16 a and 16 b.
+// Past the last k-value the codes are the zero of their group, or the scales are zero.  The columns of the first product are those of its
+// two halves in turn, 16 a and 16 b.
 #include <algorithm>
 
 #include "gemm_span.hpp"
@@ -264,15 +265,18 @@ __global__ __launch_bounds__(kFewThreads, 2) void int4_few_rows_kernel(Int4Args 
 
 // Tiles of 64 rows x 256 columns, for more rows than that: a wavefront owns 64 columns of them, two pairs of groups.  The rows come to LDS by
 // direct transfers, 128 k-values a stage, the codes and scales straight into registers; both are requested a stage ahead, and two
-// workgroups share a CU, so that one's products stand beside the other's vector work: for each 64 matrix instructions of a wavefront's stage
-// there are 112 instructions that make bf16 of codes and 64 that bring the sums of a group to the others (groups of 32: 256).
-// acc += scale * sum_k x_k (128 + code_k) as each group ends; what that is too much by, (128 + zero) scale * sum_k x_k, is a product of fp32
-// itself, contracted over the groups, and taken away four of them at a time by v_mfma_f32_16x16x4_f32.  (All at the end would let sums of
-// thousands of 128 x_k meet.)  Each of the first wavefronts sums one fragment of rows, for all of them, in LDS; two sets in turn, as a barrier a stage
-// lies between the writing of one and its use.  4096 tokens, 4096 x 11264: 1333 us with sums and differences of their own in each
-// wavefront, 1243 this way, 0.91 PFLOP/s.  It is bound by issue, the matrix instructions being busy half of the time and the vector ones two thirds.
-// Not faster: 128 rows a tile; wavefronts of 32 columns, eight a workgroup (1672) or four, of 64 rows and three workgroups a CU (1391; 1000 tokens to
-// 8 of 128 experts, groups of 64, 224 | 227) or of 96 and two (1439; 232); all fragments without a branch between them, which spills (1566).
+// workgroups share a CU, so that one's products stand beside the other's vector work: for each 64 matrix instructions of a wavefront's
+// stage there are 112 instructions that make bf16 of codes and 64 that bring the sums of a group to the others (groups of 32: 256).
+// acc += scale * sum_k x_k (128 + code_k) as each group ends; what that is too much by, (128 + zero) scale * sum_k x_k, is a product
+// of fp32 itself, contracted over the groups, and taken away four of them at a time by v_mfma_f32_16x16x4_f32.  (All at the end would
+// let sums of thousands of 128 x_k meet.)  Each of the first wavefronts sums one fragment of rows, for all of them, in LDS; two sets in
+// turn, as a barrier a stage lies between the writing of one and its use.  4096 tokens, 4096 x 11264: 1333 us with sums and differences
+// of their own in each wavefront, 1243 this way, 0.91 PFLOP/s.  It is bound by issue, the matrix instructions being busy half of the
+// time and the vector ones two thirds.  8 of 128 experts of 2048 x 768, groups of 128, whole calls: 0.35 PFLOP/s at 1000 tokens, 0.46 at
+// 2000, 0.53 at 4096, 0.57 at 16384.
+// Not faster: 128 rows a tile; wavefronts of 32 columns, eight a workgroup (1672) or four, of 64 rows and three workgroups a CU (1391;
+// 1000 tokens to 8 of 128 experts, groups of 64, 224 | 227) or of 96 and two (1439; 232); all fragments without a branch between
+// them, which spills (1566).
 // Fragments of rows that the tile does not have are left out.  A launch of few tiles has its contraction cut into slices,
 // whose sums int4_h_of_slices_kernel or the last kernel adds up.
 struct Int4Rows {
@@ -634,17 +638,20 @@ int launch(const Int4Args& a, int64_t tiles, int tile_rows, int group, hipStream
 // row tiles that a launch has about: one for each expert that may hold a row; more where the rows fill more than that
 int64_t row_tiles_of(int64_t Msum, int64_t N, int tile_rows) { return std::max(std::min(N, Msum), cdiv64(Msum, tile_rows)); }
 // Which tiles.  Those of 32 rows bring their rows to LDS for few columns at a time, but cut a contraction among the wavefronts of a
-// workgroup: they are the better ones for few rows and small weights, where the taller ones leave sums to another launch.  By what
-// all rows together read of codes, or of one block by its size.  Us, 32 | 64: 8 of 128 experts of 2048 x 768, 1 token 20 | 25, 16 tokens 71 | 63,
-// 131 128 | 85; a dense block of 1024 x 2816, 4 tokens 14 | 19, 16 18 | 19, 32 29 | 23, 200 42 | 41; 512 x 1024, 200 tokens 17 | 27; 2048 x 5632, 4
-// tokens 19 | 21, 16 31 | 24; 4096 x 11264, 1 token 30 | 28; groups of 32, 2176 x 1152, 50 tokens 27 | 37.
+// workgroup: they are the better ones for few rows and small weights, where the taller ones leave sums to another launch.
+// Rule: by what all rows together read of codes, or of one block by its size.
+// Record, us, 32 rows | 64:
+//   8 of 128 experts of 2048 x 768, 1 token 20 | 25, 16 tokens 71 | 63, 131 128 | 85
+//   dense, 1024 x 2816, 4 tokens 14 | 19, 16 18 | 19, 32 29 | 23, 200 42 | 41;  512 x 1024, 200 17 | 27;  2048 x 5632, 4 19 | 21, 16 31 | 24
+//          4096 x 11264, 1 token 30 | 28;  groups of 32, 2176 x 1152, 50 27 | 37
 int tile_rows_of(int64_t Msum, int64_t D, int64_t H, int64_t N) {
   const int64_t codes = 3 * D * H / 2;
   return Msum * codes <= (64 << 20) || (N == 1 && Msum <= 256 && codes <= (4 << 20)) ? 32 : 64;
 }
-// Slices of a contraction of K in 64-row tiles over `cols` columns (of both halves): as many as give every CU two tiles, of two stages at
-// least, up to 64 MiB of sums.  Us, a dense block with both contractions whole | cut: 4096 x 11264, 1 token 105 | 30, 64 194 | 62; 2048 x 5632, 300
-// 106 | 66, 1000 137 | 113; 1024 x 2816, 600 62 | 55.
+// Rule: slices of a contraction of K in 64-row tiles over `cols` columns (of both halves): as many as give every CU two tiles, of two
+// stages at least, up to 64 MiB of sums.
+// Record, us, a dense block with both contractions whole | cut:
+//   4096 x 11264, 1 token 105 | 30, 64 194 | 62;  2048 x 5632, 300 106 | 66, 1000 137 | 113;  1024 x 2816, 600 62 | 55
 int slices_of(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
   if (tile_rows != 64) return 1;
   const int64_t tiles = row_tiles_of(Msum, N, tile_rows) * cdiv64(cols, 256);
@@ -653,9 +660,10 @@ int slices_of(int64_t Msum, int64_t N, int64_t cols, int64_t K, int tile_rows) {
   return (int)n;
 }
 
-// What bf16 leaves of h is kept, too, of up to 16 rows an expert on average, and meets the weights as rows of their tiles' second fragments: of
-// so few results the error depends on the few large values of h (one token against 64 bits 0.0017 to 0.0024 of the norm, 0.0017 this way).  It costs the second product of 16 tokens
-// through 8 of 128 experts, 64-row tiles, 25.6 us instead of 21.3, of one token 6.5 instead of 5.7.
+// Rule: what bf16 leaves of h is kept, too, of up to 16 rows an expert on average, and meets the weights as rows of their tiles' second
+// fragments: of so few results the error depends on the few large values of h (one token against 64 bits 0.0017 to 0.0024 of the norm,
+// 0.0017 this way).  It costs the second product of 16 tokens through 8 of 128 experts, 64-row tiles, 25.6 us instead of 21.3, of one
+// token 6.5 instead of 5.7.
 bool keeps_rest(int64_t Msum, int64_t N) { return Msum <= 16 * N; }
 
 // the first product, of experts or of a dense block, with the sums of its slices in the workspace
