@@ -528,30 +528,33 @@ __global__ __launch_bounds__(256) void int4_sum_slices_kernel(const float* __res
 // out[m] = the sum of the rows of its experts, slice by slice, fp32, rounded once.  The row numbers and then the rows with unconditional
 // loads, as in combine_kernel.
 __global__ __launch_bounds__(256) void int4_combine_kernel(const float* __restrict__ rows, int slices, const int32_t* __restrict__ inv,
-                                                           bf16* __restrict__ out, int D, int K, int64_t msum) {
-  const int64_t m = blockIdx.x;
-  for (int c = threadIdx.x; c < D / 4; c += blockDim.x) {
-    f32x4 sum = {};
-    for (int k0 = 0; k0 < K; k0 += 8) {
-      int32_t r[8];
+                                                           bf16* __restrict__ out, int64_t M, int D, int K, int64_t msum) {
+  for (int64_t m = blockIdx.x; m < M; m += gridDim.x)
+    for (int c = threadIdx.x; c < D / 4; c += blockDim.x) {
+      f32x4 sum = {};
+      for (int k0 = 0; k0 < K; k0 += 8) {
+        int32_t r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = inv[m * K + min(k0 + j, K - 1)];
-      for (int s = 0; s < slices; ++s) {
-        const float* const from = rows + s * msum * D + c * 4;
-        f32x4 v[8];
+        for (int j = 0; j < 8; ++j) r[j] = inv[m * K + min(k0 + j, K - 1)];
+        for (int s = 0; s < slices; ++s) {
+          const float* const from = rows + s * msum * D + c * 4;
+          f32x4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool ok = k0 + j < K && (uint32_t)r[j] < (uint64_t)msum;
-          v[j] = *(const f32x4*)(from + (int64_t)(ok ? r[j] : 0) * D);
-          if (!ok) v[j] = f32x4{};
+          for (int j = 0; j < 8; ++j) {
+            const bool ok = k0 + j < K && (uint32_t)r[j] < (uint64_t)msum;
+            v[j] = *(const f32x4*)(from + (int64_t)(ok ? r[j] : 0) * D);
+            if (!ok) v[j] = f32x4{};
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum += v[j];
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += v[j];
       }
+      *(bf16x4*)(out + m * D + c * 4) = pack_bf16x4(sum[0], sum[1], sum[2], sum[3]);
     }
-    *(bf16x4*)(out + m * D + c * 4) = pack_bf16x4(sum[0], sum[1], sum[2], sum[3]);
-  }
 }
+
+// Workgroups of 256 of a launch that has `n` of them to do: a launch has fewer than 2^32 threads, and what is left they do in turn.
+unsigned workgroups_for(int64_t n) { return (unsigned)std::min<int64_t>(n, 1 << 23); }
 
 // ---- laying weights out ---------------------------------------------------------------------------------------------------
 struct Int4PackArgs {
@@ -567,40 +570,42 @@ __device__ __forceinline__ int column_of(const Int4PackArgs& p, int g, int c) { 
 
 __global__ __launch_bounds__(256) void int4_pack_codes_kernel(Int4PackArgs p) {
   const int KB = (int)int4_blocks(p.R), C = p.cols * p.halves, groups = C / 16;
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;  // [N][groups][KB][64][4]
-  if (q >= p.N * groups * KB * 256) return;
-  const int m = q & 3, l = (int)(q >> 2) & 63;
-  const int64_t f = q >> 8;
-  const int kb = (int)(f % KB), g = (int)(f / KB % groups);
-  const int64_t e = f / KB / groups;
-  const int k = kb * kInt4Block + 32 * m + 8 * (l >> 4), col = column_of(p, g, l & 15);
-  const int KG = (p.R + p.group - 1) / p.group, kg = k / p.group;
-  uint32_t word = 0;
+  const int64_t all = p.N * groups * KB * 256;  // [N][groups][KB][64][4]
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+    const int m = q & 3, l = (int)(q >> 2) & 63;
+    const int64_t f = q >> 8;
+    const int kb = (int)(f % KB), g = (int)(f / KB % groups);
+    const int64_t e = f / KB / groups;
+    const int k = kb * kInt4Block + 32 * m + 8 * (l >> 4), col = column_of(p, g, l & 15);
+    const int KG = (p.R + p.group - 1) / p.group, kg = k / p.group;
+    uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t b = 0;
-    if (k + 2 * i < p.R) b = p.w[(e * (p.R / 2) + k / 2 + i) * C + col];
-    else if (kg < KG) b = (p.zero ? p.zero[(e * KG + kg) * C + col] & 15u : 8u) * 17u;  // the zero of its group
-    word |= (b & 15u) << (4 * i) | (b >> 4) << (16 + 4 * i);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t b = 0;
+      if (k + 2 * i < p.R) b = p.w[(e * (p.R / 2) + k / 2 + i) * C + col];
+      else if (kg < KG) b = (p.zero ? p.zero[(e * KG + kg) * C + col] & 15u : 8u) * 17u;  // the zero of its group
+      word |= (b & 15u) << (4 * i) | (b >> 4) << (16 + 4 * i);
+    }
+    p.codes[q] = word;
   }
-  p.codes[q] = word;
 }
 
 __global__ __launch_bounds__(256) void int4_pack_scales_kernel(Int4PackArgs p) {
   const int KB = (int)int4_blocks(p.R), C = p.cols * p.halves, groups = C / 16, SG = kInt4Block / p.group;
   const int KG = (p.R + p.group - 1) / p.group;
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;  // [N][groups][KB][16][SG]
-  if (q >= p.N * groups * KB * 16 * SG) return;
-  const int sg = (int)(q % SG), c = (int)(q / SG) & 15;
-  const int64_t f = q / SG >> 4;
-  const int kb = (int)(f % KB), g = (int)(f / KB % groups), kg = kb * SG + sg;
-  uint32_t word = 0;
-  if (kg < KG) {
-    const int64_t at = (f / KB / groups * KG + kg) * C + column_of(p, g, c);
-    const float s = p.f16 ? (float)((const _Float16*)p.scale)[at] : (float)((const bf16*)p.scale)[at];
-    word = (__float_as_uint(s) & ~15u) | (p.zero ? p.zero[at] & 15u : 8u);
+  const int64_t all = p.N * groups * KB * 16 * SG;  // [N][groups][KB][16][SG]
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+    const int sg = (int)(q % SG), c = (int)(q / SG) & 15;
+    const int64_t f = q / SG >> 4;
+    const int kb = (int)(f % KB), g = (int)(f / KB % groups), kg = kb * SG + sg;
+    uint32_t word = 0;
+    if (kg < KG) {
+      const int64_t at = (f / KB / groups * KG + kg) * C + column_of(p, g, c);
+      const float s = p.f16 ? (float)((const _Float16*)p.scale)[at] : (float)((const bf16*)p.scale)[at];
+      word = (__float_as_uint(s) & ~15u) | (p.zero ? p.zero[at] & 15u : 8u);
+    }
+    p.words[q] = word;
   }
-  p.words[q] = word;
 }
 
 int check_int4(int64_t M, int64_t D, int64_t H, int64_t N, int64_t Msum, int group) {
@@ -701,11 +706,11 @@ extern "C" int momoe_int4_pack_weights(const void* codes_NRC, const void* scale,
   if (unaligned16(packed) || unaligned16(words) || ((uintptr_t)scale & 1)) return MOMOE_ERR_BAD_ARG;
   if (R % 32 != 0 || C % (16 * halves) != 0 || R >= (1 << 22) || C >= (1 << 24)) return MOMOE_ERR_UNSUPPORTED;
   const int64_t bytes = momoe_int4_weight_bytes(N, R, C), nwords = momoe_int4_scale_words(N, R, C, group);
-  if (nwords < 0 || bytes / 1024 >= (1ll << 31) || nwords / 256 >= (1ll << 31) - 1) return MOMOE_ERR_UNSUPPORTED;
+  if (nwords < 0) return MOMOE_ERR_UNSUPPORTED;
   const Int4PackArgs a{(const uint8_t*)codes_NRC, scale, (const uint8_t*)zero, N, (int)R, (int)(C / halves), halves, group,
                        scale_type == MOMOE_TYPE_F16, (uint32_t*)packed, (uint32_t*)words};
-  int4_pack_codes_kernel<<<(unsigned)(bytes / 1024), 256, 0, (hipStream_t)stream>>>(a);
-  int4_pack_scales_kernel<<<(unsigned)cdiv64(nwords, 256), 256, 0, (hipStream_t)stream>>>(a);
+  int4_pack_codes_kernel<<<workgroups_for(bytes / 1024), 256, 0, (hipStream_t)stream>>>(a);
+  int4_pack_scales_kernel<<<workgroups_for(cdiv64(nwords, 256)), 256, 0, (hipStream_t)stream>>>(a);
   return launch_status();
 }
 
@@ -763,7 +768,7 @@ extern "C" int momoe_int4_combine(const float* ys_MsumD, int slices, const int32
   if (!ys_MsumD || !inv_MK || !out_MD || M <= 0 || D <= 0 || K <= 0 || Msum <= 0 || slices <= 0) return MOMOE_ERR_BAD_ARG;
   if (D % 32 != 0 || M >= (1ll << 31) || Msum >= (1ll << 31)) return MOMOE_ERR_UNSUPPORTED;
   if (unaligned16(ys_MsumD) || unaligned16(out_MD)) return MOMOE_ERR_BAD_ARG;
-  int4_combine_kernel<<<(unsigned)M, 256, 0, (hipStream_t)stream>>>(ys_MsumD, slices, inv_MK, (bf16*)out_MD, (int)D, (int)K, Msum);
+  int4_combine_kernel<<<workgroups_for(M), 256, 0, (hipStream_t)stream>>>(ys_MsumD, slices, inv_MK, (bf16*)out_MD, M, (int)D, (int)K, Msum);
   return launch_status();
 }
 

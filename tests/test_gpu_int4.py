@@ -449,3 +449,36 @@ def test_the_experts_leave_what_lies_behind(M, D, H, N, K, rows):
             want.index_add_(0, at, sr * out)
             off.index_add_(0, at, sr * d + (sr * out).abs() * (K + 2) * 2 * E)
     _check(y[:M * D], want, off)
+
+
+def test_more_tokens_than_a_launch_has_workgroups():
+    """2^24 tokens and more: with a workgroup of 256 for each of them, a launch would have 2^32 threads."""
+    M, D, H, N, group = (1 << 24) + 77, 32, 32, 2, 32
+    w = _weights((N,), D, H, group)
+    layer = momoe_amd.MoMoEInt4(D, H, N, 1, *_on(w), group_size=group)
+    x = torch.randn(1, M, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV, dtype=torch.bfloat16)
+    at = torch.arange(M, device=DEV)
+    mask, s = torch.zeros(N, M, dtype=torch.int32, device=DEV), torch.rand(N, M, device=DEV) + 0.5
+    mask[at % N, at] = 1
+    y, _ = layer(x, mask, s)
+    assert y.isfinite().all() and (y != 0).any(-1).all()
+    rows = torch.cat([torch.arange(e - 40, e + 40) for e in (40, 1 << 22, 1 << 23, 1 << 24, M - 40)])
+    for i in range(N):
+        mine = rows[rows % N == i]
+        want, off = _block(x[0, mine].cpu().double(), [t[i] for t in w], group)
+        sr = s[i, mine].cpu().double()[:, None]
+        _check(y[0, mine], sr * want, sr * off + (sr * want).abs() * 8 * E)
+
+
+def test_laying_out_16_gib_of_codes():
+    """As many words that 2^32 threads would take one each: the last expert as by itself."""
+    N, R, C, group = 520, 4096, 16384, 128
+    codes, scale, _, _, zero, _ = _on(_weights((1,), R, C // 2, group))
+    many = [torch.zeros(N, *t.shape[1:], dtype=t.dtype, device=DEV) for t in (codes, scale, zero)]
+    for big, t in zip(many, (codes, scale, zero)):
+        big[0], big[-1] = t[0], t[0]
+    assert many[0].numel() > 1 << 34
+    packed, words = momoe_amd._hip.int4_pack_weights(*many, 2, group)
+    want = momoe_amd._hip.int4_pack_weights(codes, scale, zero, 2, group)
+    for got, one in ((packed, want[0]), (words, want[1])):
+        assert torch.equal(got.view(N, -1)[0], one) and torch.equal(got.view(N, -1)[-1], one) and not got.view(N, -1)[N // 2].any()
