@@ -318,6 +318,7 @@ int sum_slices(const FfnSums& sums, hipStream_t st) {
   return launch_status();
 }
 
+constexpr int64_t kMostTiles = (1ll << 32) / kSpanThreads - 8;  // a launch has fewer than 2^32 threads
 template <class P>
 int64_t blocks_of(const FfnArgs& a) {
   return cdiv64(cdiv64(a.rows, 32 * P::FM) * cdiv64(a.D, kFfnCols) * a.slices, 8) * 8;
@@ -326,7 +327,7 @@ template <class P, int STAGES>
 int launch_tiles(const FfnArgs& a, int64_t col_tiles, hipStream_t st) {
   static LdsLimit lds;
   const int64_t tiles = cdiv64(a.rows, 32 * P::FM) * col_tiles * a.slices;
-  if (tiles >= (1ll << 31) - 8) return MOMOE_ERR_UNSUPPORTED;
+  if (tiles > kMostTiles) return MOMOE_ERR_UNSUPPORTED;
   if (!allow_lds(ffn_tile_kernel<P, STAGES>, kFfnLds<P, STAGES>, lds)) return MOMOE_ERR_LAUNCH;
   ffn_tile_kernel<P, STAGES><<<(unsigned)(cdiv64(tiles, 8) * 8), kSpanThreads, kFfnLds<P, STAGES>, st>>>(a);
   FfnSums sums;
@@ -348,7 +349,7 @@ int launch_gradients(const FfnArgs* x, const FfnArgs* w1, const FfnArgs* w2, hip
   constexpr size_t bytes = std::max(kFfnLds<Dx, STAGES>, std::max(kFfnLds<FfnWgrad<false>, 2>, kFfnLds<FfnWgrad<true>, 2>));
   const int64_t bx = x ? blocks_of<Dx>(*x) : 0, b1 = w1 ? blocks_of<FfnWgrad<false>>(*w1) : 0, b2 = w2 ? blocks_of<FfnWgrad<true>>(*w2) : 0;
   if (bx + b1 + b2 == 0) return MOMOE_OK;
-  if (bx + b1 + b2 >= (1ll << 31)) return MOMOE_ERR_UNSUPPORTED;
+  if (bx + b1 + b2 > kMostTiles) return MOMOE_ERR_UNSUPPORTED;
   if (!allow_lds(ffn_gradients_kernel<Dx, STAGES>, bytes, lds)) return MOMOE_ERR_LAUNCH;
   const FfnArgs none{};
   ffn_gradients_kernel<Dx, STAGES><<<(unsigned)(bx + b1 + b2), kSpanThreads, bytes, st>>>(x ? *x : none, w1 ? *w1 : none, w2 ? *w2 : none, (int)bx, (int)b1);

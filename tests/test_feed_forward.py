@@ -77,3 +77,11 @@ def test_gradients_of_weights_that_are_too_wide_are_refused_before_any_is_comput
     take, most = lib.momoe_ffn_gradients_take, 1 << 20
     assert take(most, most // 2, 1, 1) == take(most, most, 0, 1) == take(2 * most, 2 * most, 0, 0) == 1
     assert take(most + 32, 32, 1, 0) == take(most + 32, 32, 0, 1) == take(32, most // 2 + 32, 1, 0) == take(32, most + 32, 0, 1) == take(0, 32, 0, 0) == 0
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    n = 1 << 30
+    assert lib.momoe_ffn_lin1_fwd(P, 32, P, P, None, 0, n, n, 32, 32, None) == lib.momoe_ffn_lin2_fwd(P, P, P, n, n, 32, 32, None, 0, None) == 2
+    assert lib.momoe_ffn_dgrad_h(P, 32, P, P, n, 32, 32, None) == lib.momoe_ffn_swiglu_bwd(P, 32, P, P, P, None, None, n, n, n, 32, 32, None) == 2
+    assert lib.momoe_ffn_dgrad_h_saved(P, 32, P, P, P, None, None, n, n, n, 32, 32, None) == 2
+    assert lib.momoe_ffn_gradients(None, 0, None, 0, P, None, P, None, P, None, None, None, 0, n, n, 32, 32, None) == 2
